@@ -79,7 +79,7 @@ def draw(rng):
         T = _log(rng, 1, min(16384, 4096 * 7168 // H))
         c = _norm(op, "", T, H, y=rng.choice(["bf16", "bf16", "fp16"]), r=rng.choice(["bf16", "fp32"]),
                   x="e4m3" if op == "norm" and rng.random() < 0.4 else "bf16", post=rng.random() < 0.5,
-                  gate=rng.choice(["none", "channel", "token", "full"]), scale=rng.choice([1.0, 0.5]),
+                  gate=rng.choice(["none", "channel", "token", "full" if T > 1 else "channel"]), scale=rng.choice([1.0, 0.5]),
                   pad=rng.choice([0, 0, 8, 24]))
     elif op in ("select", "select_bwd"):
         G = rng.choice([1, 1, 4, 8])

@@ -238,6 +238,168 @@ MOE_B200_API int moe_b200_forward_timed(const moe_b200_args* args, void* workspa
 MOE_B200_API int moe_b200_timer_read(moe_b200_timer* timer, float* stage_ms, int32_t* calls,
                                      int32_t reset);
 
+/*
+ * ---------------------------------------------------------------------------
+ * Operators around the layer, for a transformer block that holds it.  They
+ * take row-major tensors whose rows may be further apart than their length
+ * (strides in elements; elements of a row are adjacent), enqueue on `stream`
+ * without a host synchronisation, and return the status codes above.
+ */
+
+/* Element types. */
+#define MOE_B200_BF16 0
+#define MOE_B200_FP16 1
+#define MOE_B200_FP32 2
+#define MOE_B200_E4M3 3
+#define MOE_B200_INT8 4
+
+/*
+ * The norms around a block with its gate and residual sum, rows x cols (cols <= 16384):
+ *   n  = y, or y * s(y) * (post_weight + weight_offset) with post_weight
+ *   r' = residual + scale * gate * n            -> residual_out
+ *   x  = r' * s(r') * (pre_weight + weight_offset)   -> x (if pre_weight)
+ *   s(v) = 1 / sqrt(mean over the row of v^2 + eps)
+ * y may be null (x is the norm of residual; residual_out is not written), residual may be null
+ * (taken as 0).  post_weight, gate, pre_weight may be null.  The gate's element of (t, c) is
+ * gate[t * gate_row_stride + (gate_per_column ? c : 0)], so gate_row_stride 0 broadcasts it over
+ * rows.  residual and residual_out have residual_type, which is y_type or fp32; weights, gate
+ * and x have types of their own.  x computes from the unrounded r'.  With x_type e4m3, x_scale
+ * receives [ceil(cols / 128)][rows] scales max(amax, 1e-12) / 448, and x the codes: the layer's
+ * hidden_states_scale and hidden_states.  residual_out may be residual.
+ */
+typedef struct moe_b200_norm_args {
+  const void* y;
+  const void* residual;
+  const void* post_weight;
+  const void* pre_weight;
+  const void* gate;
+  void* residual_out;
+  void* x;
+  float* x_scale;
+  int64_t y_stride, residual_stride, residual_out_stride, x_stride, gate_row_stride;
+  int32_t rows, cols;
+  int32_t y_type, residual_type, post_weight_type, pre_weight_type, gate_type, x_type;
+  int32_t gate_per_column;
+  float scale, eps, weight_offset;
+} moe_b200_norm_args;
+MOE_B200_API int moe_b200_block_norm(const moe_b200_norm_args* args, void* stream);
+
+/*
+ * Gradients of block_norm from dx (of x, y_type) and dresidual (of residual_out), either null:
+ *   G = dresidual + s (w dx - r^ mean(w dx r^)),  r^ = residual * s(residual)  -> dresidual_in
+ * `residual` is the stored residual_out, y the forward's y; with no y only G and dpre_weight are
+ * computed.  dpre_weight, dpost_weight are fp32 [cols].  dgate is summed over what the gate is
+ * broadcast over: fp32 [cols] (row stride 0, per column), fp32 [rows] (per row), one fp32 (both
+ * broadcast); for a gate per element it has the gate's type and dgate_stride.  dy has y_type,
+ * dresidual_in residual_type; either may be null.  All sums are in a fixed order.
+ */
+typedef struct moe_b200_norm_backward_args {
+  const void* dx;
+  const void* dresidual;
+  const void* residual;
+  const void* y;
+  const void* post_weight;
+  const void* pre_weight;
+  const void* gate;
+  void* dresidual_in;
+  void* dy;
+  float* dpre_weight;
+  float* dpost_weight;
+  void* dgate;
+  int64_t dx_stride, dresidual_stride, residual_stride, y_stride, gate_row_stride;
+  int64_t dresidual_in_stride, dy_stride, dgate_stride;
+  int32_t rows, cols;
+  int32_t y_type, residual_type, post_weight_type, pre_weight_type, gate_type;
+  int32_t gate_per_column;
+  float scale, eps, weight_offset;
+} moe_b200_norm_backward_args;
+MOE_B200_API size_t moe_b200_block_norm_backward_workspace_size(int32_t rows, int32_t cols);
+MOE_B200_API int moe_b200_block_norm_backward(const moe_b200_norm_backward_args* args, void* workspace,
+                                              size_t workspace_bytes, void* stream);
+
+/*
+ * Choice of experts from router logits [num_tokens, num_experts] (up to 512 experts):
+ *   s = sigmoid or softmax of the logits;  sel = s + bias (bias [num_experts] or null)
+ *   with n_group > 1: the topk_group groups of consecutive experts with the highest score (the
+ *   sum of a group's two highest sel, or its highest) stay
+ *   idx [num_tokens, top_k]: the top_k (<= 32) highest sel, listed by ascending id; equal values
+ *   go to the lower id (groups likewise)
+ *   weight [num_tokens, top_k] = s of the chosen, / (their sum + 1e-20) if renormalize, * scale
+ *   counts [num_experts] (or null): tokens that chose each expert
+ * s is a 32-bit value with its exponential rounded once, as in the layer's routing; with
+ * sigmoid, 256 experts, 8 groups of which 4 stay, top_k 8 and renormalize, idx is
+ * moe_b200_route's and weight equals its weights up to the rounding of their sum.  A logit of -inf or of its type's lowest value switches its expert off; where
+ * no expert is left a slot holds id -1 and weight 0 (moe_b200_forward_routed skips it).  A row
+ * with a NaN score has ids -1 and NaN weights.
+ */
+#define MOE_B200_SCORE_SIGMOID 0
+#define MOE_B200_SCORE_SOFTMAX 1
+#define MOE_B200_GROUP_TOP2 0
+#define MOE_B200_GROUP_MAX 1
+typedef struct moe_b200_select_args {
+  const void* logits;
+  const void* bias;
+  int32_t* idx;
+  float* weight;
+  int32_t* counts;
+  int64_t logits_stride;
+  int32_t num_tokens, num_experts, top_k;
+  int32_t logits_type, bias_type;
+  int32_t score, n_group, topk_group, group_score, renormalize;
+  float scale;
+} moe_b200_select_args;
+MOE_B200_API int moe_b200_select_experts(const moe_b200_select_args* args, void* stream);
+
+/* The gradient of `weight` of moe_b200_select_experts with respect to the logits: dlogits (the
+ * logits' type) from dweight fp32 [num_tokens, top_k] and the chosen ids (distinct; -1 none).
+ * The choice itself, and with it the bias, has no gradient. */
+typedef struct moe_b200_select_backward_args {
+  const void* logits;
+  const int32_t* idx;
+  const float* dweight;
+  void* dlogits;
+  int64_t logits_stride, dlogits_stride;
+  int32_t num_tokens, num_experts, top_k;
+  int32_t logits_type;
+  int32_t score, renormalize;
+  float scale;
+} moe_b200_select_backward_args;
+MOE_B200_API int moe_b200_select_experts_backward(const moe_b200_select_backward_args* args, void* stream);
+
+/* 8-bit codes and scales of the rows of x (cols <= 32768): scale = max(amax / 127, 2^-126),
+ * q = rint(v / scale), v = x or, with swiglu, silu(x[:, cols:]) * x[:, :cols] of x [rows, 2 cols].
+ * A row with a NaN or an infinity gets a NaN scale and zero codes. */
+typedef struct moe_b200_quantize_args {
+  const void* x;
+  int8_t* q;
+  float* scale;
+  int64_t x_stride, q_stride;
+  int32_t rows, cols, x_type, swiglu;
+} moe_b200_quantize_args;
+MOE_B200_API int moe_b200_quantize_int8(const moe_b200_quantize_args* args, void* stream);
+
+/*
+ * y [num_tokens, out_features] = x_scale[t] * weight_scale[n] * sum_k q[t, k] weight[n, k] + bias[n]
+ * with exact integer sums.  x is int8 with x_scale, or bf16 / fp16 / fp32 and quantised in the
+ * call as moe_b200_quantize_int8 does (in_features <= 32768 then).  in_features is a multiple of
+ * 16; weight rows (and int8 x rows) start on 16-byte boundaries.
+ */
+typedef struct moe_b200_linear_args {
+  const void* x;
+  const float* x_scale;
+  const int8_t* weight;
+  const float* weight_scale;
+  const void* bias;
+  void* y;
+  int64_t x_stride, weight_stride, y_stride;
+  int32_t num_tokens, out_features, in_features;
+  int32_t x_type, y_type, bias_type, swiglu;
+} moe_b200_linear_args;
+MOE_B200_API size_t moe_b200_int8_linear_workspace_size(int32_t num_tokens, int32_t out_features,
+                                                        int32_t in_features, int32_t x_type);
+MOE_B200_API int moe_b200_int8_linear(const moe_b200_linear_args* args, void* workspace, size_t workspace_bytes,
+                                      void* stream);
+
 /* Text of the last host-side error of this thread ("" if none). */
 MOE_B200_API const char* moe_b200_last_error(void);
 

@@ -8,6 +8,9 @@
 hand-written CUDA of ``libmoe_b200.so`` (``include/moe_b200.h``); when that library
 is missing the call raises -- there is no CPU or PyTorch fallback.
 
+``block_norm``, ``select_experts`` and ``int8_linear`` (and their backward passes) are the
+operators around the layer in a transformer block (``ops.py``).
+
 Shape/dtype violations raise :class:`MoEArgumentError`, which is an
 ``AssertionError`` like the reference's own ``assert`` checks
 (``spec/reference_official.py:43-58``).
@@ -21,6 +24,9 @@ import threading
 import torch
 
 from . import _native
+from .ops import (BlockNormGrads, BlockNormOut, MoEArgumentError, Selection, _check, block_norm,
+                  block_norm_backward, int8_linear, quantize_int8, select_experts,
+                  select_experts_backward)
 
 H = 7168
 I = 2048
@@ -30,16 +36,8 @@ NIB = I // 128
 NG1B = 2 * I // 128
 
 __all__ = ["run", "kernel", "run_routed", "route", "device_status", "MoEArgumentError", "Workspace",
-           "GraphRunner"]
-
-
-class MoEArgumentError(AssertionError, ValueError):
-    """An input violates the layer definition (spec/definition.json)."""
-
-
-def _check(cond: bool, msg: str):
-    if not cond:
-        raise MoEArgumentError(msg)
+           "GraphRunner", "block_norm", "block_norm_backward", "BlockNormOut", "BlockNormGrads",
+           "select_experts", "select_experts_backward", "Selection", "int8_linear", "quantize_int8"]
 
 
 class Workspace:

@@ -36,7 +36,18 @@ EXPORTED = (
     "moe_b200_forward_timed",
     "moe_b200_timer_read",
     "moe_b200_route_noalloc",
+    "moe_b200_block_norm",
+    "moe_b200_block_norm_backward",
+    "moe_b200_block_norm_backward_workspace_size",
+    "moe_b200_select_experts",
+    "moe_b200_select_experts_backward",
+    "moe_b200_quantize_int8",
+    "moe_b200_int8_linear",
+    "moe_b200_int8_linear_workspace_size",
 )
+
+# element types of the operators around the layer
+BF16, FP16, FP32, E4M3, INT8 = range(5)
 
 
 class MoeArgs(ctypes.Structure):
@@ -78,6 +89,44 @@ class MoeLayout(ctypes.Structure):
     _fields_ = [(name, ctypes.c_size_t) for name in (
         "plan", "topk_idx", "topk_w", "tok_nloc", "tok_rows", "e_count", "e_start", "row_token",
         "row_weight", "c_hi", "c_lo", "c_scale", "status", "trace", "r_max", "r_pad", "total")]
+
+
+def _struct(name: str, doc: str, **fields):
+    """A ctypes structure whose members are given as type=names, in the header's order."""
+    kinds = {"ptr": ctypes.c_void_p, "i64": ctypes.c_int64, "i32": ctypes.c_int32, "f32": ctypes.c_float}
+    members = [(n, kinds[kind.rstrip("_")]) for kind, names in fields.items() for n in names.split()]
+    return type(name, (ctypes.Structure,), {"_fields_": members, "__doc__": doc})
+
+
+NormArgs = _struct(
+    "NormArgs", "moe_b200_norm_args (include/moe_b200.h)",
+    ptr="y residual post_weight pre_weight gate residual_out x x_scale",
+    i64="y_stride residual_stride residual_out_stride x_stride gate_row_stride",
+    i32="rows cols y_type residual_type post_weight_type pre_weight_type gate_type x_type gate_per_column",
+    f32="scale eps weight_offset")
+NormBackwardArgs = _struct(
+    "NormBackwardArgs", "moe_b200_norm_backward_args",
+    ptr="dx dresidual residual y post_weight pre_weight gate dresidual_in dy dpre_weight dpost_weight dgate",
+    i64="dx_stride dresidual_stride residual_stride y_stride gate_row_stride dresidual_in_stride dy_stride "
+        "dgate_stride",
+    i32="rows cols y_type residual_type post_weight_type pre_weight_type gate_type gate_per_column",
+    f32="scale eps weight_offset")
+SelectArgs = _struct(
+    "SelectArgs", "moe_b200_select_args",
+    ptr="logits bias idx weight counts", i64="logits_stride",
+    i32="num_tokens num_experts top_k logits_type bias_type score n_group topk_group group_score renormalize",
+    f32="scale")
+SelectBackwardArgs = _struct(
+    "SelectBackwardArgs", "moe_b200_select_backward_args",
+    ptr="logits idx dweight dlogits", i64="logits_stride dlogits_stride",
+    i32="num_tokens num_experts top_k logits_type score renormalize", f32="scale")
+QuantizeArgs = _struct(
+    "QuantizeArgs", "moe_b200_quantize_args",
+    ptr="x q scale", i64="x_stride q_stride", i32="rows cols x_type swiglu")
+LinearArgs = _struct(
+    "LinearArgs", "moe_b200_linear_args",
+    ptr="x x_scale weight weight_scale bias y", i64="x_stride weight_stride y_stride",
+    i32="num_tokens out_features in_features x_type y_type bias_type swiglu")
 
 
 _lib = None
@@ -124,6 +173,17 @@ def lib() -> ctypes.CDLL:
     l.moe_b200_timer_read.restype = ctypes.c_int
     l.moe_b200_route_noalloc.argtypes = [ctypes.POINTER(MoeArgs), vp, vp, vp, vp, vp, vp]
     l.moe_b200_route_noalloc.restype = ctypes.c_int
+    for fn, args, ws in (("block_norm", NormArgs, False), ("block_norm_backward", NormBackwardArgs, True),
+                         ("select_experts", SelectArgs, False),
+                         ("select_experts_backward", SelectBackwardArgs, False),
+                         ("quantize_int8", QuantizeArgs, False), ("int8_linear", LinearArgs, True)):
+        f = getattr(l, "moe_b200_" + fn)
+        f.argtypes = [ctypes.POINTER(args)] + ([vp, sz] if ws else []) + [vp]
+        f.restype = ctypes.c_int
+    l.moe_b200_block_norm_backward_workspace_size.argtypes = [i32, i32]
+    l.moe_b200_block_norm_backward_workspace_size.restype = sz
+    l.moe_b200_int8_linear_workspace_size.argtypes = [i32, i32, i32, i32]
+    l.moe_b200_int8_linear_workspace_size.restype = sz
     _lib = l
     return l
 

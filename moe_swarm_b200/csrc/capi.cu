@@ -13,6 +13,7 @@
 #include "../../include/moe_b200.h"
 #include "launch_args.cuh"
 #include "moe_internal.cuh"
+#include "op_common.cuh"
 
 namespace moe {
 
@@ -191,6 +192,19 @@ int launch_route(const moe_b200_args* a, uint8_t* ws, const moe::Layout& L, int 
 }  // namespace
 
 int moe::report_error(int code, const char* msg) { return fail(code, msg); }
+
+// What the operators around the layer share with it (op_common.cuh).
+int moe::report_cuda(cudaError_t e, const char* what) { return cuda_fail(e, what); }
+
+int moe::op_device(int* sms) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
+  const DeviceInfo& d = device_info(dev);
+  if (d.major != 10) return fail(MOE_B200_ERR_DEVICE, "an sm_100 (B200-class) device is required");
+  *sms = d.sms;
+  return MOE_B200_OK;
+}
 
 extern "C" {
 

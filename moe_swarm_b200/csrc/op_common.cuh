@@ -1,0 +1,174 @@
+// What the operators around the expert layer (norm.cu, select.cu, int8.cu) share: element types,
+// eight-element row chunks, warp and row reductions, host-side checks.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "../../include/moe_b200.h"
+#include "launch_args.cuh"
+#include "ptx.cuh"
+
+namespace moe {
+
+// Host helpers of the C entries (capi.cu).
+int report_cuda(cudaError_t e, const char* what);
+int op_device(int* sms);   // the current device must be sm_100; *sms = its SM count
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+inline int type_bytes(int t) { return t == MOE_B200_FP32 ? 4 : t == MOE_B200_E4M3 ? 1 : 2; }
+inline bool is_float_type(int t) { return t == MOE_B200_BF16 || t == MOE_B200_FP16 || t == MOE_B200_FP32; }
+// Whether every row of the tensor starts on a 16-byte boundary.
+inline bool rows_aligned(const void* p, int64_t stride, int type) {
+  return !p || (aligned16(p) && (stride * type_bytes(type)) % 16 == 0);
+}
+
+using bf16 = __nv_bfloat16;
+using fp16 = __half;
+
+__device__ __forceinline__ float to_f(bf16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f(fp16 v) { return __half2float(v); }
+__device__ __forceinline__ float to_f(float v) { return v; }
+template <class T> __device__ __forceinline__ T from_f(float v);
+template <> __device__ __forceinline__ bf16 from_f<bf16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ fp16 from_f<fp16>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ float from_f<float>(float v) { return v; }
+
+__device__ __forceinline__ void unpack2(uint32_t u, float* v, bf16) {
+  v[0] = __uint_as_float(u << 16);
+  v[1] = __uint_as_float(u & 0xffff0000u);
+}
+__device__ __forceinline__ void unpack2(uint32_t u, float* v, fp16) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u));
+  v[0] = f.x;
+  v[1] = f.y;
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, bf16) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, fp16) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Plain loads, not the read-only path: a tensor may be written by the kernel that this one waits
+// for (pdl_wait), and a read-only load may be moved above that wait.
+//
+// Eight consecutive elements from p.  VEC: p is 16-byte aligned and all eight exist; otherwise
+// the first n exist (n <= 0: none) and the rest read as 0.
+template <class T, bool VEC>
+__device__ __forceinline__ void load8(const T* p, int n, float* v) {
+  if constexpr (VEC) {
+    if (n <= 0) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = 0.f;
+    } else if constexpr (sizeof(T) == 4) {
+      const float4 a = reinterpret_cast<const float4*>(p)[0];
+      const float4 b = reinterpret_cast<const float4*>(p)[1];
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+      const uint4 u = *reinterpret_cast<const uint4*>(p);
+      unpack2(u.x, v, T{});
+      unpack2(u.y, v + 2, T{});
+      unpack2(u.z, v + 4, T{});
+      unpack2(u.w, v + 6, T{});
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = j < n ? to_f(p[j]) : 0.f;
+  }
+}
+
+template <class T, bool VEC>
+__device__ __forceinline__ void store8(T* p, int n, const float* v) {
+  if constexpr (VEC) {
+    if (n <= 0) return;
+    if constexpr (sizeof(T) == 4) {
+      reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+      *reinterpret_cast<uint4*>(p) = make_uint4(pack2(v[0], v[1], T{}), pack2(v[2], v[3], T{}),
+                                                pack2(v[4], v[5], T{}), pack2(v[6], v[7], T{}));
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < n) p[j] = from_f<T>(v[j]);
+  }
+}
+
+// The same with the element type known at run time (uniform over the grid): element `off` of p.
+template <bool VEC>
+__device__ __forceinline__ void load8_dyn(const void* p, int type, int64_t off, int n, float* v) {
+  if (type == MOE_B200_BF16) load8<bf16, VEC>(static_cast<const bf16*>(p) + off, n, v);
+  else if (type == MOE_B200_FP16) load8<fp16, VEC>(static_cast<const fp16*>(p) + off, n, v);
+  else load8<float, VEC>(static_cast<const float*>(p) + off, n, v);
+}
+template <bool VEC>
+__device__ __forceinline__ void store8_dyn(void* p, int type, int64_t off, int n, const float* v) {
+  if (type == MOE_B200_BF16) store8<bf16, VEC>(static_cast<bf16*>(p) + off, n, v);
+  else if (type == MOE_B200_FP16) store8<fp16, VEC>(static_cast<fp16*>(p) + off, n, v);
+  else store8<float, VEC>(static_cast<float*>(p) + off, n, v);
+}
+__device__ __forceinline__ float load1_dyn(const void* p, int type, int64_t off) {
+  if (type == MOE_B200_BF16) return to_f(static_cast<const bf16*>(p)[off]);
+  if (type == MOE_B200_FP16) return to_f(static_cast<const fp16*>(p)[off]);
+  return static_cast<const float*>(p)[off];
+}
+
+// max that keeps a NaN
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int d = 16; d >= 1; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  return v;
+}
+
+// Sums of N values over the `warps` warps of each row of a CTA whose blockDim is (32 * warps,
+// rows).  `buf` holds [rows][N][32] floats and may be reused after the next CTA barrier only.
+// Every thread of the CTA calls it (one barrier, none when a row is one warp); the order of the
+// additions is fixed.
+template <int N>
+__device__ __forceinline__ void row_sum(float (&v)[N], int warps, float* buf) {
+#pragma unroll
+  for (int k = 0; k < N; ++k) v[k] = warp_sum(v[k]);
+  if (warps == 1) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float* b = buf + threadIdx.y * N * 32;
+  if (lane == 0) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) b[k * 32 + warp] = v[k];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < N; ++k) v[k] = warp_sum(lane < warps ? b[k * 32 + lane] : 0.f);
+}
+
+// A programmatic dependent launch on `st`: the kernel may become resident while its predecessor
+// drains, and starts with pdl_wait().
+template <class... P, class... A>
+cudaError_t launch_pdl(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, A... args) {
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t c{};
+  c.gridDim = grid;
+  c.blockDim = block;
+  c.dynamicSmemBytes = smem;
+  c.stream = st;
+  c.attrs = at;
+  c.numAttrs = 1;
+  return cudaLaunchKernelEx(&c, kernel, args...);
+}
+
+}  // namespace moe

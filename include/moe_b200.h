@@ -400,6 +400,11 @@ MOE_B200_API size_t moe_b200_int8_linear_workspace_size(int32_t num_tokens, int3
 MOE_B200_API int moe_b200_int8_linear(const moe_b200_linear_args* args, void* workspace, size_t workspace_bytes,
                                       void* stream);
 
+/* Synchronises the stream and returns the status word of the operators above on the current
+ * device: 0, or the code of the first bounded device-side wait of moe_b200_int8_linear that
+ * timed out (its result is then not valid); reset if `clear`.  Negative: a status code, negated. */
+MOE_B200_API int moe_b200_operator_status(void* stream, int32_t clear);
+
 /* Text of the last host-side error of this thread ("" if none). */
 MOE_B200_API const char* moe_b200_last_error(void);
 

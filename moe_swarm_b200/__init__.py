@@ -25,8 +25,8 @@ import torch
 
 from . import _native
 from .ops import (BlockNormGrads, BlockNormOut, MoEArgumentError, Selection, _check, block_norm,
-                  block_norm_backward, int8_linear, quantize_int8, select_experts,
-                  select_experts_backward)
+                  block_norm_backward, int8_linear, operator_status, quantize_int8,
+                  select_experts, select_experts_backward)
 
 H = 7168
 I = 2048
@@ -37,7 +37,8 @@ NG1B = 2 * I // 128
 
 __all__ = ["run", "kernel", "run_routed", "route", "device_status", "MoEArgumentError", "Workspace",
            "GraphRunner", "block_norm", "block_norm_backward", "BlockNormOut", "BlockNormGrads",
-           "select_experts", "select_experts_backward", "Selection", "int8_linear", "quantize_int8"]
+           "select_experts", "select_experts_backward", "Selection", "int8_linear", "quantize_int8",
+           "operator_status"]
 
 
 class Workspace:

@@ -44,6 +44,7 @@ EXPORTED = (
     "moe_b200_quantize_int8",
     "moe_b200_int8_linear",
     "moe_b200_int8_linear_workspace_size",
+    "moe_b200_operator_status",
 )
 
 # element types of the operators around the layer
@@ -184,6 +185,8 @@ def lib() -> ctypes.CDLL:
     l.moe_b200_block_norm_backward_workspace_size.restype = sz
     l.moe_b200_int8_linear_workspace_size.argtypes = [i32, i32, i32, i32]
     l.moe_b200_int8_linear_workspace_size.restype = sz
+    l.moe_b200_operator_status.argtypes = [vp, i32]
+    l.moe_b200_operator_status.restype = ctypes.c_int
     _lib = l
     return l
 

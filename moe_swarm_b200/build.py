@@ -21,8 +21,8 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libmoe_b200.so"
 TRACE_LIB = PKG / "libmoe_b200_trace.so"   # MOE_TRACE build: per-CTA role counters
-SOURCES = ["route.cu", "wide.cu", "stream.cu", "combine.cu", "ep.cu", "norm.cu", "select.cu", "int8.cu", "capi.cu"]
-HEADERS = ["ptx.cuh", "moe_internal.cuh", "launch_args.cuh", "sched.cuh", "exp64.cuh", "op_common.cuh"]
+SOURCES = ["route.cu", "wide.cu", "stream.cu", "combine.cu", "ep.cu", "norm.cu", "select.cu", "int8.cu", "int8_gemm.cu", "capi.cu"]
+HEADERS = ["ptx.cuh", "moe_internal.cuh", "launch_args.cuh", "sched.cuh", "exp64.cuh", "op_common.cuh", "int8_gemm.cuh"]
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC",

@@ -63,17 +63,24 @@ EncodeTiledFn encode_fn() {
   return fn;
 }
 
-// Byte matrix [rows, cols] (row stride = cols bytes) read as 128x128-byte tiles, SWIZZLE_128B.
-bool encode_u8_2d(CUtensorMap* m, const void* base, uint64_t cols, uint64_t rows, uint32_t box_rows = 128) {
+// Byte matrix [rows, cols] (rows `pitch` bytes apart) read as tiles of 128 bytes x box_rows rows,
+// SWIZZLE_128B; what a tile has outside the matrix reads as 0.
+bool encode_u8_pitched(CUtensorMap* m, const void* base, uint64_t cols, uint64_t rows, uint64_t pitch,
+                       uint32_t box_rows) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return false;
   const cuuint64_t dims[2] = {cols, rows};
-  const cuuint64_t strides[1] = {cols};
+  const cuuint64_t strides[1] = {pitch};
   const cuuint32_t box[2] = {128, box_rows};
   const cuuint32_t estr[2] = {1, 1};
   return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Rows without a gap, 128 x 128-byte tiles unless box_rows says otherwise.
+bool encode_u8_2d(CUtensorMap* m, const void* base, uint64_t cols, uint64_t rows, uint32_t box_rows = 128) {
+  return encode_u8_pitched(m, base, cols, rows, cols, box_rows);
 }
 
 struct DeviceInfo {
@@ -195,6 +202,11 @@ int moe::report_error(int code, const char* msg) { return fail(code, msg); }
 
 // What the operators around the layer share with it (op_common.cuh).
 int moe::report_cuda(cudaError_t e, const char* what) { return cuda_fail(e, what); }
+
+bool moe::encode_rows_u8(CUtensorMap* m, const void* base, uint64_t cols, uint64_t rows, uint64_t pitch,
+                         uint32_t box_rows) {
+  return encode_u8_pitched(m, base, cols, rows, pitch, box_rows);
+}
 
 int moe::op_device(int* sms) {
   int dev = 0;

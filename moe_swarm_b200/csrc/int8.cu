@@ -8,13 +8,14 @@
 // or an infinity gets a NaN scale, so its outputs are NaN.
 #include <type_traits>
 
-#include "op_common.cuh"
+#include "int8_gemm.cuh"
 
 namespace moe {
 
 constexpr int kQuantPerThread = 32;                      // four 8-element chunks
 constexpr int kQuantMaxCols = 1024 * kQuantPerThread;
 constexpr int kInt8MaxK = 131056;
+constexpr int kInt8StreamMaxT = 256;
 
 struct QuantArgs {
   const void* x;
@@ -22,17 +23,6 @@ struct QuantArgs {
   float* scale;
   int64_t x_ld, q_ld;
   int rows, cols, warps, type, swiglu;
-};
-
-struct LinearArgs {
-  const int8_t* q;
-  const int8_t* w;
-  const float* sx;
-  const float* sw;
-  const void* bias;
-  void* y;
-  int64_t q_ld, w_ld, y_ld;
-  int T, N, K, y_type, bias_type;
 };
 
 // One row in the registers of a group of warps: maximum, then codes.
@@ -92,44 +82,6 @@ __global__ void __launch_bounds__(1024, 1) quant_kernel(QuantArgs a) {
         if (j < n) dst[e0 + j] = static_cast<int8_t>(b[j >> 2] >> (8 * (j & 3)));
     }
   }
-}
-
-// 64 x 64 outputs per CTA of 256 threads, 64 bytes of K at a time through shared memory.
-__global__ void __launch_bounds__(256) linear_simple_kernel(LinearArgs a) {
-  __shared__ int sa[64][17], sb[64][17];
-  pdl_wait();
-  pdl_launch_dependents();
-  const int t0 = blockIdx.y * 64, n0 = blockIdx.x * 64;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  int acc[4][4] = {};
-  for (int k0 = 0; k0 < a.K; k0 += 64) {
-    const int r = threadIdx.x >> 2, c = (threadIdx.x & 3) * 16;   // K is a multiple of 16
-    int4 va = make_int4(0, 0, 0, 0), vb = va;
-    if (t0 + r < a.T && k0 + c < a.K) va = *reinterpret_cast<const int4*>(a.q + (t0 + r) * a.q_ld + k0 + c);
-    if (n0 + r < a.N && k0 + c < a.K) vb = *reinterpret_cast<const int4*>(a.w + (n0 + r) * a.w_ld + k0 + c);
-    __syncthreads();
-    int* da = &sa[r][c / 4];
-    int* db = &sb[r][c / 4];
-    da[0] = va.x; da[1] = va.y; da[2] = va.z; da[3] = va.w;
-    db[0] = vb.x; db[1] = vb.y; db[2] = vb.z; db[3] = vb.w;
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 16; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(sa[ty + 16 * i][k], sb[tx + 16 * j][k], acc[i][j]);
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int t = t0 + ty + 16 * i, n = n0 + tx + 16 * j;
-      if (t >= a.T || n >= a.N) continue;
-      float v = static_cast<float>(acc[i][j]) * (a.sx[t] * a.sw[n]);
-      if (a.bias) v += load1_dyn(a.bias, a.bias_type, n);
-      store8_dyn<false>(a.y, a.y_type, t * a.y_ld + n, 1, &v);
-    }
 }
 
 namespace {
@@ -224,10 +176,10 @@ MOE_B200_API int moe_b200_int8_linear(const moe_b200_linear_args* a, void* works
   int sms = 0;
   if (int rc = op_device(&sms)) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int8_t* q_rows = static_cast<const int8_t*>(a->x);
+  int64_t q_ld = a->x_stride;
   LinearArgs l{};
-  l.q = static_cast<const int8_t*>(a->x);
   l.sx = a->x_scale;
-  l.q_ld = a->x_stride;
   cudaError_t e = cudaSuccess;
   if (quantise) {
     uint8_t* ws = static_cast<uint8_t*>(workspace);
@@ -243,22 +195,22 @@ MOE_B200_API int moe_b200_int8_linear(const moe_b200_linear_args* a, void* works
     q.swiglu = a->swiglu;
     e = quant_launch(q, st);
     if (e != cudaSuccess) return report_cuda(e, "int8_linear quantisation launch");
-    l.q = q.q;
+    q_rows = q.q;
+    q_ld = q.q_ld;
     l.sx = q.scale;
-    l.q_ld = q.q_ld;
+    l.early_w = 1;   // the quantisation waited for everything before it, and writes no weights
   }
-  l.w = a->weight;
   l.sw = a->weight_scale;
   l.bias = a->bias;
   l.y = a->y;
-  l.w_ld = a->weight_stride;
   l.y_ld = a->y_stride;
   l.T = a->num_tokens;
   l.N = a->out_features;
   l.K = a->in_features;
   l.y_type = a->y_type;
   l.bias_type = a->bias_type;
-  e = launch_pdl(linear_simple_kernel, dim3((l.N + 63) / 64, (l.T + 63) / 64), dim3(256), 0, st, l);
+  e = a->num_tokens <= kInt8StreamMaxT ? int8_stream_launch(q_rows, q_ld, a->weight, a->weight_stride, l, sms, st)
+                                       : int8_wide_launch(q_rows, q_ld, a->weight, a->weight_stride, l, sms, st);
   return e == cudaSuccess ? MOE_B200_OK : report_cuda(e, "int8_linear launch");
 }
 

@@ -1,0 +1,478 @@
+// Products of 8-bit integers with one scale per token and one per output channel, on tcgen05
+// (kind::i8: exact 32-bit integer sums in TMEM).
+//
+//   y[t][n] = (sx[t] * sw[n]) * sum_k q[t][k] * w[n][k]  (+ bias[n])
+//
+// stream: few tokens, bound by reading the weights once.  The weights are the MMA's M side (128
+//   rows), up to 256 tokens its N side; K is split over the CTAs of a cluster, whose integer
+//   partial sums meet in distributed shared memory (exact in any order).
+// wide: many tokens, bound by the tensor cores.  Persistent pairs of CTAs, each pair one 256 x 256
+//   output tile at a time (cta_group::2: each CTA loads half of either operand, 32 KB per 128
+//   bytes of K for 256 x 256 x 128 products), two TMEM accumulators so that one tile's epilogue
+//   runs under the next tile's products.
+//
+// Every wait is bounded (2 s); one that runs out is recorded in g_op_status.
+#include "int8_gemm.cuh"
+
+namespace moe {
+
+__device__ int g_op_status;
+
+// float(sum) * (sx * sw) + bias of a tile's column, rounded once to the output's type
+template <class YT>
+__device__ __forceinline__ void store_cols32(YT* dst, int n, bool vec, const float* v) {
+  if (vec && n >= 32) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 32 / static_cast<int>(sizeof(YT))) {
+      if constexpr (sizeof(YT) == 4) {
+        st_global_v8(reinterpret_cast<float*>(dst) + i, v + i);
+      } else {
+        uint32_t p[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) p[j] = pack2(v[i + 2 * j], v[i + 2 * j + 1], YT{});
+        st_global_v8_b32(dst + i, p);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (i < n) dst[i] = from_f<YT>(v[i]);
+  }
+}
+
+// 32 lanes x 32 consecutive columns, complete on return.
+__device__ __forceinline__ void tmem_ld32_wait(uint32_t ta, int* v) {
+  uint32_t r[32];
+  tmem_ld16x2_issue(ta, ta + 16, r);
+  tmem_wait_ld32(r);
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = static_cast<int>(r[i]);
+}
+
+// ---------------------------------------------------------------- wide
+constexpr int kIWStages = 6;
+constexpr int kIWStageBytes = 32768;     // 128 token rows | 128 weight rows of 128 bytes
+constexpr int kIWThreads = 320;          // producer, MMA, 8 epilogue warps
+constexpr int kIWEpiThreads = 256;
+constexpr int kIWGroup = 8;              // token tiles whose weight tiles run together (L2 reuse)
+
+struct IntWideSmem {
+  uint8_t stage[kIWStages][kIWStageBytes];
+  uint64_t full[kIWStages], empty[kIWStages];
+  uint64_t tfull[2], tempty[2];
+  uint32_t tmem_base;
+  int abort;
+  float sw[2][256], bias[2][256];
+};
+constexpr size_t kIWSmemBytes = sizeof(IntWideSmem) + 1024;
+static_assert(kIWSmemBytes <= 232448, "wide int8 kernel shared memory");
+
+// Tile order: blocks of kIWGroup token tiles, all weight tiles of a block before the next, token
+// tiles fastest, so that the tiles in flight share few rows of either operand.
+__device__ __forceinline__ void iw_tile(int tile, int mt, int nt, int* m, int* n) {
+  const int per = kIWGroup * nt, g = tile / per, r = tile - g * per;
+  const int rows = min(kIWGroup, mt - g * kIWGroup);
+  *n = r / rows;
+  *m = g * kIWGroup + r - *n * rows;
+}
+
+template <class YT>
+__global__ void __launch_bounds__(kIWThreads, 1)
+    int8_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmW, LinearArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  IntWideSmem& sm =
+      *reinterpret_cast<IntWideSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int mt = (a.T + 255) / 256, nt = (a.N + 255) / 256, tiles = mt * nt, kbs = (a.K + 127) / 128;
+  if (threadIdx.x == 0) {
+    sm.abort = 0;
+    for (int i = 0; i < kIWStages; ++i) {
+      mbar_init(&sm.full[i], 1);
+      mbar_init(&sm.empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sm.tfull[i], 1);
+      mbar_init(&sm.tempty[i], 16);   // 8 epilogue warps of each CTA
+    }
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(&sm.tmem_base, 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();   // both CTAs' barriers and TMEM exist before either touches the other's
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem_base;
+  pdl_launch_dependents();
+
+  if (warp == 0) {
+    // producer: this CTA's 128 rows of either operand; the bytes of both CTAs complete on the
+    // even CTA's barrier, whose thread issues the pair's products
+    uint32_t stage = 0, phase = 0, last = 0;   // last: bit s = parity of stage s's latest load
+    int issued = 0;
+    bool waited = false, ok = true;
+    for (int tile = pair; ok && tile < tiles; tile += pairs) {
+      int m, n;
+      iw_tile(tile, mt, nt, &m, &n);
+      const int y0 = m * 256 + 128 * rank, y1 = n * 256 + 128 * rank;
+      for (int kb = 0; kb < kbs; ++kb) {
+        ok = __all_sync(0xffffffffu,
+                        mbar_wait(&sm.empty[stage], phase ^ 1u, &sm.abort, &g_op_status, kStWaitProducer));
+        if (!ok) break;
+        if (!waited) {
+          pdl_wait();
+          waited = true;
+        }
+        if (rank == 0 && lane == 0) mbar_arrive_expect_tx(&sm.full[stage], 2 * kIWStageBytes);
+        __syncwarp();
+        const uint32_t bar = cluster_addr(smem_u32(&sm.full[stage]), 0);
+        if (lane == 0) tma_load_2d_pair(sm.stage[stage], &tmQ, bar, kb * 128, y0);
+        if (lane == 1) tma_load_2d_pair(sm.stage[stage] + 16384, &tmW, bar, kb * 128, y1);
+        last = (last & ~(1u << stage)) | (phase << stage);
+        issued = max(issued, static_cast<int>(stage) + 1);
+        if (++stage == kIWStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+    // given up: the pair's loads in flight, of which the even CTA's barriers know, land first
+    if (!ok && rank == 0 && lane == 0)
+      for (int i = 0; i < issued; ++i) {
+        int none = 0;
+        mbar_wait<true>(&sm.full[i], (last >> i) & 1u, &none, &g_op_status, kStWaitDrain);
+      }
+  } else if (warp == 1) {
+    if (rank == 0 && lane == 0) {
+      constexpr uint32_t idesc = idesc_s8_s32(256, 256);
+      uint32_t stage = 0, phase = 0;
+      int it = 0;
+      bool ok = true;
+      for (int tile = pair; ok && tile < tiles; tile += pairs, ++it) {
+        const int buf = it & 1;
+        if (!mbar_wait<true>(&sm.tempty[buf], ((it >> 1) & 1) ^ 1, &sm.abort, &g_op_status, kStWaitMmaTmem)) break;
+        tc_fence_after();
+        for (int kb = 0; kb < kbs; ++kb) {
+          ok = mbar_wait<true>(&sm.full[stage], phase, &sm.abort, &g_op_status, kStWaitMma);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t st = smem_u32(sm.stage[stage]);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            mma_i8_pair(tmem + buf * 256u, sdesc_k128_sw128(st + 32 * k), sdesc_k128_sw128(st + 16384 + 32 * k), idesc,
+                        (kb | k) > 0);
+          mma_commit_pair(&sm.empty[stage]);
+          if (++stage == kIWStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        mma_commit_pair(&sm.tfull[buf]);
+      }
+    }
+  } else {
+    // epilogue: lane quarter warp & 3 (32 token rows), column half (warp - 2) / 4
+    const int q = warp & 3, h = (warp - 2) >> 2, et = threadIdx.x - 64;
+    const bool vec = (reinterpret_cast<uintptr_t>(a.y) & 31u) == 0 && (a.y_ld * sizeof(YT)) % 32 == 0;
+    pdl_wait();
+    bool dead = false;
+    int it = 0;
+    for (int tile = pair; tile < tiles; tile += pairs, ++it) {
+      const int buf = it & 1;
+      int m, n;
+      iw_tile(tile, mt, nt, &m, &n);
+      const int t = m * 256 + 128 * rank + 32 * q + lane;
+      {
+        const int c = n * 256 + et;
+        sm.sw[buf][et] = c < a.N ? a.sw[c] : 0.f;
+        sm.bias[buf][et] = a.bias && c < a.N ? load1_dyn(a.bias, a.bias_type, c) : 0.f;
+      }
+      const float sx = t < a.T ? a.sx[t] : 0.f;
+      named_bar_sync(1, kIWEpiThreads);
+      // after an abort the warps still meet at every tile's barrier
+      if (!dead) {
+        const bool ok = mbar_wait(&sm.tfull[buf], (it >> 1) & 1, &sm.abort, &g_op_status, kStWaitEpilogue);
+        dead = !__all_sync(0xffffffffu, ok);
+      }
+      if (dead) continue;
+      tc_fence_after();
+      const uint32_t ta = tmem + (static_cast<uint32_t>(32 * q) << 16) + buf * 256u + 128u * h;
+#pragma unroll
+      for (int c0 = 0; c0 < 128; c0 += 32) {
+        int acc[32];
+        tmem_ld32_wait(ta + c0, acc);
+        if (c0 == 96) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(cluster_addr(smem_u32(&sm.tempty[buf]), 0));
+        }
+        const float* swp = &sm.sw[buf][128 * h + c0];
+        const float* bp = &sm.bias[buf][128 * h + c0];
+        float v[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = fmaf(static_cast<float>(acc[i]), sx * swp[i], bp[i]);
+        const int col = n * 256 + 128 * h + c0;
+        if (t < a.T) store_cols32(static_cast<YT*>(a.y) + t * a.y_ld + col, a.N - col, vec, v);
+      }
+    }
+  }
+  // no CTA leaves while the other's products still read its shared memory: the epilogue warps
+  // have seen every tile's products complete
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  if (warp == 1) tmem_dealloc_pair(tmem, 512);
+}
+
+// ---------------------------------------------------------------- stream
+constexpr int kISThreads = 192;          // producer, MMA, 4 epilogue warps
+constexpr int kISMaxStages = 8;
+
+struct IntStreamCtl {
+  uint64_t full[kISMaxStages], empty[kISMaxStages];
+  uint64_t tfull;
+  uint32_t tmem_base;
+  int abort;
+};
+
+// grid (splits * weight tiles, token tiles), clusters of `splits` CTAs along x.  Token tile: tn
+// rows (a multiple of 16, at most 256); stages of 16 KB of weights and tn x 128 bytes of tokens.
+// The integer partial sums [tn][128] of a split CTA reuse the stages.
+template <class YT>
+__global__ void __launch_bounds__(kISThreads) int8_stream_kernel(const __grid_constant__ CUtensorMap tmQ,
+                                                                 const __grid_constant__ CUtensorMap tmW, LinearArgs a,
+                                                                 int splits, int tn, int stages, uint32_t tmem_cols) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ IntStreamCtl sm;
+  uint8_t* base =
+      reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int split = splits > 1 ? static_cast<int>(cluster_rank()) : 0;
+  const int n0 = static_cast<int>(blockIdx.x) / splits * 128, t0 = blockIdx.y * tn;
+  const int kbs = (a.K + 127) / 128;
+  const int k0 = kbs * split / splits, k1 = kbs * (split + 1) / splits;
+  const int stage_bytes = 16384 + tn * 128;
+  if (threadIdx.x == 0) {
+    sm.abort = 0;
+    for (int i = 0; i < stages; ++i) {
+      mbar_init(&sm.full[i], 1);
+      mbar_init(&sm.empty[i], 1);
+    }
+    mbar_init(&sm.tfull, 1);
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&sm.tmem_base, tmem_cols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem_base;
+  pdl_launch_dependents();
+
+  bool ok = true;
+  if (warp == 0) {
+    // weights of the first stages start before the wait for the kernel that writes q and sx
+    if (!a.early_w) pdl_wait();
+    const int ahead = min(stages, k1 - k0);
+    for (int i = 0; i < ahead; ++i) {
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&sm.full[i], stage_bytes);
+        tma_load_2d(base + i * stage_bytes, &tmW, &sm.full[i], (k0 + i) * 128, n0);
+      }
+    }
+    if (a.early_w) pdl_wait();
+    for (int i = 0; i < ahead; ++i)
+      if (lane == 0) tma_load_2d(base + i * stage_bytes + 16384, &tmQ, &sm.full[i], (k0 + i) * 128, t0);
+    uint32_t stage = 0, phase = 0, last = 0;   // last: bit s = parity of stage s's latest load
+    for (int kb = k0 + ahead; kb < k1; ++kb) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&sm.empty[stage], phase, &sm.abort, &g_op_status, kStWaitProducer));
+      if (!ok) break;
+      if (lane == 0) mbar_arrive_expect_tx(&sm.full[stage], stage_bytes);
+      __syncwarp();
+      if (lane == 0) tma_load_2d(base + stage * stage_bytes, &tmW, &sm.full[stage], kb * 128, n0);
+      if (lane == 1) tma_load_2d(base + stage * stage_bytes + 16384, &tmQ, &sm.full[stage], kb * 128, t0);
+      last = (last & ~(1u << stage)) | ((phase ^ 1u) << stage);
+      if (++stage == static_cast<uint32_t>(stages)) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    }
+    if (!ok && lane == 0)   // given up: the loads in flight land first
+      for (int i = 0; i < ahead; ++i) {
+        int none = 0;
+        mbar_wait(&sm.full[i], (last >> i) & 1u, &none, &g_op_status, kStWaitDrain);
+      }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t idesc = idesc_s8_s32(128, tn);
+      uint32_t stage = 0, phase = 0;
+      for (int kb = k0; kb < k1; ++kb) {
+        if (!mbar_wait(&sm.full[stage], phase, &sm.abort, &g_op_status, kStWaitMma)) break;
+        tc_fence_after();
+        const uint32_t st = smem_u32(base + stage * stage_bytes);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          mma_i8(tmem, sdesc_k128_sw128(st + 32 * k), sdesc_k128_sw128(st + 16384 + 32 * k), idesc,
+                 (kb - k0) | k);
+        mma_commit(&sm.empty[stage]);
+        if (++stage == static_cast<uint32_t>(stages)) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      mma_commit(&sm.tfull);
+    }
+  }
+  __syncwarp();
+  const int q = warp & 3, r = 32 * q + lane;   // this thread's weight row of the tile
+  const int n = n0 + r;
+  const int live = min(tn, a.T - t0);
+  int* part = reinterpret_cast<int*>(base);    // [tn][128]
+  if (warp >= 2) {
+    pdl_wait();
+    const float sw = n < a.N ? a.sw[n] : 0.f;
+    const float bias = a.bias && n < a.N ? load1_dyn(a.bias, a.bias_type, n) : 0.f;
+    ok = mbar_wait(&sm.tfull, 0, &sm.abort, &g_op_status, kStWaitEpilogue);
+    if (__all_sync(0xffffffffu, ok)) {
+      tc_fence_after();
+      // every load and product of this CTA is complete: the stages are free
+      for (int c0 = 0; c0 < live; c0 += 32) {
+        int acc[32];
+        const uint32_t ta = tmem + (static_cast<uint32_t>(32 * q) << 16) + c0;
+        tmem_ld32_wait(ta, acc);
+        if (splits > 1) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (c0 + i < live) part[(c0 + i) * 128 + r] = acc[i];
+        } else if (n < a.N) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (c0 + i < live)
+              static_cast<YT*>(a.y)[(t0 + c0 + i) * a.y_ld + n] =
+                  from_f<YT>(fmaf(static_cast<float>(acc[i]), a.sx[t0 + c0 + i] * sw, bias));
+        }
+      }
+    }
+    if (splits > 1) {
+      cluster_sync();
+      // CTA `split` finishes its share of the token columns
+      const int c1 = live * (split + 1) / splits;
+      for (int c = live * split / splits; c < c1; ++c) {
+        int v[8];
+        const uint32_t at = smem_u32(part + c * 128 + r);
+#pragma unroll
+        for (int s = 0; s < 8; ++s) v[s] = s < splits ? ld_cluster_s32(cluster_addr(at, s)) : 0;
+        const int sum = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+        if (n < a.N)
+          static_cast<YT*>(a.y)[(t0 + c) * a.y_ld + n] =
+              from_f<YT>(fmaf(static_cast<float>(sum), a.sx[t0 + c] * sw, bias));
+      }
+      cluster_sync();   // the others have read this CTA's partial sums
+    }
+  } else if (splits > 1) {
+    cluster_sync();
+    cluster_sync();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem, tmem_cols);
+}
+
+namespace {
+
+template <class F>
+cudaError_t with_y_type(int type, F&& f) {
+  return type == MOE_B200_BF16 ? f(bf16{}) : type == MOE_B200_FP16 ? f(fp16{}) : f(float{});
+}
+
+cudaError_t launch_cluster(const void* kernel, dim3 grid, int threads, size_t smem, int cluster, cudaStream_t st,
+                           void** args) {
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = cluster;
+  at[1].val.clusterDim.y = 1;
+  at[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t c{};
+  c.gridDim = grid;
+  c.blockDim = dim3(threads);
+  c.dynamicSmemBytes = smem;
+  c.stream = st;
+  c.attrs = at;
+  c.numAttrs = 2;
+  return cudaLaunchKernelExC(&c, kernel, args);
+}
+
+}  // namespace
+
+cudaError_t int8_wide_launch(const int8_t* q, int64_t q_ld, const int8_t* w, int64_t w_ld, const LinearArgs& a,
+                             int sms, cudaStream_t st) {
+  CUtensorMap mq, mw;
+  if (!encode_rows_u8(&mq, q, a.K, a.T, q_ld, 128) || !encode_rows_u8(&mw, w, a.K, a.N, w_ld, 128))
+    return cudaErrorInvalidValue;
+  const int tiles = ((a.T + 255) / 256) * ((a.N + 255) / 256);
+  const int pairs = tiles < sms / 2 ? tiles : sms / 2;
+  return with_y_type(a.y_type, [&](auto yt) {
+    auto kernel = int8_wide_kernel<decltype(yt)>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kIWSmemBytes);
+    if (e != cudaSuccess) return e;
+    LinearArgs la = a;
+    void* args[] = {&mq, &mw, &la};
+    return launch_cluster(reinterpret_cast<const void*>(kernel), dim3(2 * pairs), kIWThreads, kIWSmemBytes, 2, st, args);
+  });
+}
+
+cudaError_t int8_stream_launch(const int8_t* q, int64_t q_ld, const int8_t* w, int64_t w_ld, const LinearArgs& a,
+                               int sms, cudaStream_t st) {
+  const int tt = (a.T + 255) / 256;
+  int tn = ((a.T + tt - 1) / tt + 15) / 16 * 16;
+  const int kbs = (a.K + 127) / 128, nt = (a.N + 127) / 128;
+  // split K until the CTAs fill the GPU about once (twice where two fit an SM), at least two
+  // 128-byte steps each
+  const int slots = tn <= 64 ? 2 * sms : sms;
+  int splits = 1;
+  while (splits < 8 && nt * tt * splits * 2 <= slots && kbs >= 4 * splits) splits *= 2;
+  const int stage_bytes = 16384 + tn * 128;
+  const int room = tn <= 64 ? 100 * 1024 : 200 * 1024;
+  int stages = room / stage_bytes;
+  if (stages > kISMaxStages) stages = kISMaxStages;
+  uint32_t cols = 32;
+  while (cols < static_cast<uint32_t>(tn)) cols *= 2;
+  const size_t smem = static_cast<size_t>(stages) * stage_bytes + 1024;
+  CUtensorMap mq, mw;
+  if (!encode_rows_u8(&mq, q, a.K, a.T, q_ld, tn) || !encode_rows_u8(&mw, w, a.K, a.N, w_ld, 128))
+    return cudaErrorInvalidValue;
+  return with_y_type(a.y_type, [&](auto yt) {
+    auto kernel = int8_stream_kernel<decltype(yt)>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 210 * 1024);
+    if (e != cudaSuccess) return e;
+    LinearArgs la = a;
+    void* args[] = {&mq, &mw, &la, &splits, &tn, &stages, &cols};
+    return launch_cluster(reinterpret_cast<const void*>(kernel), dim3(nt * splits, tt), kISThreads, smem, splits, st, args);
+  });
+}
+
+}  // namespace moe
+
+extern "C" MOE_B200_API int moe_b200_operator_status(void* stream, int32_t clear) {
+  using namespace moe;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  int v = 0;
+  cudaError_t e = cudaMemcpyFromSymbolAsync(&v, g_op_status, sizeof(int), 0, cudaMemcpyDeviceToHost, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  if (e == cudaSuccess && clear && v) {
+    const int zero = 0;
+    e = cudaMemcpyToSymbolAsync(g_op_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  }
+  if (e != cudaSuccess) return -report_cuda(e, "operator status");
+  return v;
+}

@@ -17,6 +17,9 @@ namespace moe {
 // Host helpers of the C entries (capi.cu).
 int report_cuda(cudaError_t e, const char* what);
 int op_device(int* sms);   // the current device must be sm_100; *sms = its SM count
+// A byte matrix with rows `pitch` bytes apart as TMA tiles of 128 bytes x box_rows rows (SWIZZLE_128B).
+bool encode_rows_u8(CUtensorMap* m, const void* base, uint64_t cols, uint64_t rows, uint64_t pitch,
+                    uint32_t box_rows);
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline int type_bytes(int t) { return t == MOE_B200_FP32 ? 4 : t == MOE_B200_E4M3 ? 1 : 2; }

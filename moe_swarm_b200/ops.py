@@ -337,3 +337,14 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
                            _ld(weight), _ld(out), T, N, K, _type(x), _type(out), _type(bias), bool(swiglu))
     _done(lib.moe_b200_int8_linear(ctypes.byref(a), ws.data_ptr(), ws.numel(), _stream(dev)), "int8_linear")
     return out
+
+
+def operator_status(device=None, clear: bool = True) -> int:
+    """Synchronises and returns the status word of this module's operators on the device: 0, or
+    the code of a bounded device-side wait that gave up (the call's result is then not valid)."""
+    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    with torch.cuda.device(dev):
+        rc = int(_native.lib().moe_b200_operator_status(_stream(dev), 1 if clear else 0))
+    if rc < 0:
+        raise RuntimeError(f"operator_status failed ({-rc}): {_native.last_error()}")
+    return rc

@@ -88,6 +88,7 @@ namespace {
 
 cudaError_t quant_launch(const QuantArgs& q0, cudaStream_t st) {
   QuantArgs q = q0;
+  if (q.rows == 1) q.x_ld = q.q_ld = 0;   // a single row has no pitch
   q.warps = (q.cols + 32 * kQuantPerThread - 1) / (32 * kQuantPerThread);
   const int rpc = q.warps >= 8 ? 1 : 8 / q.warps;
   const dim3 block(q.warps * 32, rpc), grid((q.rows + rpc - 1) / rpc);
@@ -164,9 +165,12 @@ MOE_B200_API int moe_b200_int8_linear(const moe_b200_linear_args* a, void* works
   if (a->num_tokens == 0) return MOE_B200_OK;
   if (!a->x || !a->weight || !a->weight_scale || !a->y || (!quantise && !a->x_scale))
     return report_error(MOE_B200_ERR_ARG, "null tensor pointer");
-  if (!aligned16(a->weight) || a->weight_stride % 16 || a->weight_stride < a->in_features)
+  // a single row has no pitch
+  const int64_t w_ld = a->out_features == 1 ? a->in_features : a->weight_stride;
+  const int64_t x_ld = a->num_tokens == 1 && !quantise ? a->in_features : a->x_stride;
+  if (!aligned16(a->weight) || w_ld % 16 || w_ld < a->in_features)
     return report_error(MOE_B200_ERR_ARG, "int8_linear: weight rows must start on 16-byte boundaries");
-  if (!quantise && (!aligned16(a->x) || a->x_stride % 16 || a->x_stride < a->in_features))
+  if (!quantise && (!aligned16(a->x) || x_ld % 16 || x_ld < a->in_features))
     return report_error(MOE_B200_ERR_ARG, "int8_linear: int8 x rows must start on 16-byte boundaries");
   const size_t need = moe_b200_int8_linear_workspace_size(a->num_tokens, a->out_features, a->in_features, a->x_type);
   if (!workspace || workspace_bytes < need)
@@ -177,7 +181,7 @@ MOE_B200_API int moe_b200_int8_linear(const moe_b200_linear_args* a, void* works
   if (int rc = op_device(&sms)) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int8_t* q_rows = static_cast<const int8_t*>(a->x);
-  int64_t q_ld = a->x_stride;
+  int64_t q_ld = x_ld;
   LinearArgs l{};
   l.sx = a->x_scale;
   cudaError_t e = cudaSuccess;
@@ -203,14 +207,14 @@ MOE_B200_API int moe_b200_int8_linear(const moe_b200_linear_args* a, void* works
   l.sw = a->weight_scale;
   l.bias = a->bias;
   l.y = a->y;
-  l.y_ld = a->y_stride;
+  l.y_ld = a->num_tokens == 1 ? 0 : a->y_stride;
   l.T = a->num_tokens;
   l.N = a->out_features;
   l.K = a->in_features;
   l.y_type = a->y_type;
   l.bias_type = a->bias_type;
-  e = a->num_tokens <= kInt8StreamMaxT ? int8_stream_launch(q_rows, q_ld, a->weight, a->weight_stride, l, sms, st)
-                                       : int8_wide_launch(q_rows, q_ld, a->weight, a->weight_stride, l, sms, st);
+  e = a->num_tokens <= kInt8StreamMaxT ? int8_stream_launch(q_rows, q_ld, a->weight, w_ld, l, sms, st)
+                                       : int8_wide_launch(q_rows, q_ld, a->weight, w_ld, l, sms, st);
   return e == cudaSuccess ? MOE_B200_OK : report_cuda(e, "int8_linear launch");
 }
 

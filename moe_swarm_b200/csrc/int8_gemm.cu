@@ -392,25 +392,6 @@ cudaError_t with_y_type(int type, F&& f) {
   return type == MOE_B200_BF16 ? f(bf16{}) : type == MOE_B200_FP16 ? f(fp16{}) : f(float{});
 }
 
-cudaError_t launch_cluster(const void* kernel, dim3 grid, int threads, size_t smem, int cluster, cudaStream_t st,
-                           void** args) {
-  cudaLaunchAttribute at[2];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  at[1].id = cudaLaunchAttributeClusterDimension;
-  at[1].val.clusterDim.x = cluster;
-  at[1].val.clusterDim.y = 1;
-  at[1].val.clusterDim.z = 1;
-  cudaLaunchConfig_t c{};
-  c.gridDim = grid;
-  c.blockDim = dim3(threads);
-  c.dynamicSmemBytes = smem;
-  c.stream = st;
-  c.attrs = at;
-  c.numAttrs = 2;
-  return cudaLaunchKernelExC(&c, kernel, args);
-}
-
 }  // namespace
 
 cudaError_t int8_wide_launch(const int8_t* q, int64_t q_ld, const int8_t* w, int64_t w_ld, const LinearArgs& a,
@@ -424,9 +405,7 @@ cudaError_t int8_wide_launch(const int8_t* q, int64_t q_ld, const int8_t* w, int
     auto kernel = int8_wide_kernel<decltype(yt)>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kIWSmemBytes);
     if (e != cudaSuccess) return e;
-    LinearArgs la = a;
-    void* args[] = {&mq, &mw, &la};
-    return launch_cluster(reinterpret_cast<const void*>(kernel), dim3(2 * pairs), kIWThreads, kIWSmemBytes, 2, st, args);
+    return launch_cluster_pdl(kernel, dim3(2 * pairs), dim3(kIWThreads), kIWSmemBytes, 2, st, mq, mw, a);
   });
 }
 
@@ -454,9 +433,8 @@ cudaError_t int8_stream_launch(const int8_t* q, int64_t q_ld, const int8_t* w, i
     auto kernel = int8_stream_kernel<decltype(yt)>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 210 * 1024);
     if (e != cudaSuccess) return e;
-    LinearArgs la = a;
-    void* args[] = {&mq, &mw, &la, &splits, &tn, &stages, &cols};
-    return launch_cluster(reinterpret_cast<const void*>(kernel), dim3(nt * splits, tt), kISThreads, smem, splits, st, args);
+    return launch_cluster_pdl(kernel, dim3(nt * splits, tt), dim3(kISThreads), smem, splits, st, mq, mw, a, splits, tn,
+                              stages, cols);
   });
 }
 

@@ -375,6 +375,7 @@ MOE_B200_API int moe_b200_block_norm(const moe_b200_norm_args* a, void* stream) 
   n.ro_ld = a->residual_out_stride;
   n.x_ld = a->x_stride;
   n.g_ld = a->gate_row_stride;
+  if (a->rows == 1) n.y_ld = n.r_ld = n.ro_ld = n.x_ld = n.g_ld = 0;   // a single row has no pitch
   n.rows = a->rows;
   n.cols = a->cols;
   n.post_type = a->post_weight_type;
@@ -388,14 +389,13 @@ MOE_B200_API int moe_b200_block_norm(const moe_b200_norm_args* a, void* stream) 
   int rpc;
   norm_shape(a->cols, &n.warps, &rpc);
   // whole 16-byte accesses need every row of every tensor on a 16-byte boundary (8 for e4m3)
-  const bool vec = a->cols % 8 == 0 && rows_aligned(a->y, a->y_stride, a->y_type) &&
-                   rows_aligned(a->residual, a->residual_stride, a->residual_type) &&
-                   rows_aligned(a->residual_out, a->residual_out_stride, a->residual_type) &&
-                   aligned16(a->post_weight) && aligned16(a->pre_weight) &&
-                   (!a->gate_per_column || rows_aligned(a->gate, a->gate_row_stride, a->gate_type)) &&
-                   (a->x_type == MOE_B200_E4M3
-                        ? (reinterpret_cast<uintptr_t>(a->x) & 7u) == 0 && a->x_stride % 8 == 0
-                        : rows_aligned(a->x, a->x_stride, a->x_type));
+  const bool vec = a->cols % 8 == 0 && rows_aligned(a->y, n.y_ld, a->y_type) &&
+                   rows_aligned(a->residual, n.r_ld, a->residual_type) &&
+                   rows_aligned(a->residual_out, n.ro_ld, a->residual_type) && aligned16(a->post_weight) &&
+                   aligned16(a->pre_weight) &&
+                   (!a->gate_per_column || rows_aligned(a->gate, n.g_ld, a->gate_type)) &&
+                   (a->x_type == MOE_B200_E4M3 ? (reinterpret_cast<uintptr_t>(a->x) & 7u) == 0 && n.x_ld % 8 == 0
+                                               : rows_aligned(a->x, n.x_ld, a->x_type));
   const dim3 block(n.warps * 32, rpc), grid((a->rows + rpc - 1) / rpc);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaSuccess;
@@ -465,6 +465,7 @@ MOE_B200_API int moe_b200_block_norm_backward(const moe_b200_norm_backward_args*
   n.dres_ld = a->dresidual_in_stride;
   n.dy_ld = a->dy_stride;
   n.dg_ld = a->dgate_stride;
+  if (a->rows == 1) n.dx_ld = n.dr_ld = n.r_ld = n.y_ld = n.g_ld = n.dres_ld = n.dy_ld = n.dg_ld = 0;
   n.rows = a->rows;
   n.cols = a->cols;
   n.post_type = a->post_weight_type;
@@ -494,14 +495,13 @@ MOE_B200_API int moe_b200_block_norm_backward(const moe_b200_norm_backward_args*
   n.dgate = n.gate_grad == 3 ? a->dgate : n.gate_grad == 2 ? (g_rows ? a->dgate : row_dots) : nullptr;
   int rpc;
   norm_shape(a->cols, &n.warps, &rpc);
-  const bool vec = a->cols % 8 == 0 && rows_aligned(a->y, a->y_stride, a->y_type) &&
-                   rows_aligned(a->dx, a->dx_stride, a->y_type) &&
-                   rows_aligned(a->dresidual, a->dresidual_stride, a->residual_type) &&
-                   rows_aligned(n.r, a->residual_stride, a->residual_type) &&
-                   rows_aligned(a->dresidual_in, a->dresidual_in_stride, a->residual_type) &&
-                   rows_aligned(a->dy, a->dy_stride, a->y_type) && aligned16(a->post_weight) &&
-                   aligned16(a->pre_weight) && (!a->gate || !g_cols || rows_aligned(a->gate, a->gate_row_stride, a->gate_type)) &&
-                   (n.gate_grad != 3 || rows_aligned(a->dgate, a->dgate_stride, a->gate_type));
+  const bool vec = a->cols % 8 == 0 && rows_aligned(a->y, n.y_ld, a->y_type) &&
+                   rows_aligned(a->dx, n.dx_ld, a->y_type) && rows_aligned(a->dresidual, n.dr_ld, a->residual_type) &&
+                   rows_aligned(n.r, n.r_ld, a->residual_type) &&
+                   rows_aligned(a->dresidual_in, n.dres_ld, a->residual_type) &&
+                   rows_aligned(a->dy, n.dy_ld, a->y_type) && aligned16(a->post_weight) && aligned16(a->pre_weight) &&
+                   (!g_cols || rows_aligned(a->gate, n.g_ld, a->gate_type)) &&
+                   (n.gate_grad != 3 || rows_aligned(a->dgate, n.dg_ld, a->gate_type));
   const dim3 block(n.warps * 32, rpc), grid(n.parts / rpc);
   dispatch_norm(a->y_type, a->residual_type, vec, block.x * block.y, [&](auto yt, auto rt, auto v, auto t) {
     e = launch_pdl(norm_bwd_kernel<decltype(yt), decltype(rt), decltype(v)::value, decltype(t)::value>, grid, block, 0,

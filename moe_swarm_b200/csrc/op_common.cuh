@@ -157,21 +157,31 @@ __device__ __forceinline__ void row_sum(float (&v)[N], int warps, float* buf) {
   for (int k = 0; k < N; ++k) v[k] = warp_sum(lane < warps ? b[k * 32 + lane] : 0.f);
 }
 
-// A programmatic dependent launch on `st`: the kernel may become resident while its predecessor
-// drains, and starts with pdl_wait().
+// A programmatic dependent launch on `st` in clusters of `cluster` CTAs along x: the kernel may
+// become resident while its predecessor drains, and calls pdl_wait() before it touches anything
+// that an earlier kernel wrote or reads.
 template <class... P, class... A>
-cudaError_t launch_pdl(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, A... args) {
-  cudaLaunchAttribute at[1];
+cudaError_t launch_cluster_pdl(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, int cluster, cudaStream_t st,
+                               const A&... args) {
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = cluster;
+  at[1].val.clusterDim.y = 1;
+  at[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t c{};
   c.gridDim = grid;
   c.blockDim = block;
   c.dynamicSmemBytes = smem;
   c.stream = st;
   c.attrs = at;
-  c.numAttrs = 1;
-  return cudaLaunchKernelEx(&c, kernel, args...);
+  c.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&c, kernel, static_cast<P>(args)...);
+}
+template <class... P, class... A>
+cudaError_t launch_pdl(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, const A&... args) {
+  return launch_cluster_pdl(kernel, grid, block, smem, 1, st, args...);
 }
 
 }  // namespace moe

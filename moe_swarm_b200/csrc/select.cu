@@ -15,7 +15,12 @@
 // routing kernel's own form; softmax: the quotient) rounded to 32 bits once from a double
 // evaluation, so a choice depends on no order of summation and on no approximation.
 //
-// One warp per token; lane l holds experts l, l + 32, ...
+// One warp per token; lane l holds experts V l .. V l + V - 1.  A double exponential per logit would
+// be most of the work, so a token is first chosen for with 32-bit scores whose error is bounded,
+// and the choice stands if every decision (the last group kept against the best one dropped, the
+// last expert chosen against the best one left) is further apart than that allows for; otherwise,
+// which for continuous logits is one token in some hundreds, the scores
+// are computed as defined and the choice is made again from those.
 #include <type_traits>
 
 #include "exp64.cuh"
@@ -35,6 +40,8 @@ struct SelectArgs {
   int* counts;
   int64_t ld;
   int T, E, K, type, bias_type, n_group, topk_group, top2, renorm;
+  int vec;       // rows start on 16 (32-bit logits) or 8 bytes
+  int cluster;   // the grid is one cluster, which adds up the counts by itself
   float scale;
 };
 
@@ -69,6 +76,251 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
+// Sorts v[0..N-1] descending (odd-even merge network).
+template <int N>
+__device__ __forceinline__ void sort_desc(uint32_t (&v)[N]) {
+#pragma unroll
+  for (int p = 1; p < N; p *= 2)
+#pragma unroll
+    for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+      for (int j = k % p; j + k < N; j += 2 * k)
+#pragma unroll
+        for (int i = 0; i < k; ++i)
+          if (i + j + k < N && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+            const uint32_t hi = max(v[i + j], v[i + j + k]), lo = min(v[i + j], v[i + j + k]);
+            v[i + j] = hi;
+            v[i + j + k] = lo;
+          }
+}
+
+// Loads this lane's V logits (experts first.. of E; the rest as -inf).
+template <int V>
+__device__ __forceinline__ void load_logits(const void* p, int type, int64_t off, int first, int E, bool vec, float* x) {
+  if (V >= 4 && vec && first + V <= E) {
+    if (type == MOE_B200_FP32) {
+#pragma unroll
+      for (int i = 0; i + 4 <= V; i += 4) {
+        const float4 f = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + off + first + i);
+        x[i] = f.x; x[i + 1] = f.y; x[i + 2] = f.z; x[i + 3] = f.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i + 4 <= V; i += 4) {
+        const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + off + first + i);
+        if (type == MOE_B200_BF16) {
+          unpack2(u.x, x + i, bf16{});
+          unpack2(u.y, x + i + 2, bf16{});
+        } else {
+          unpack2(u.x, x + i, fp16{});
+          unpack2(u.y, x + i + 2, fp16{});
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = first + i < E ? load1_dyn(p, type, off + first + i) : -INFINITY;
+  }
+}
+
+// The scores as defined (EXACT), or 32-bit ones.  Returns the largest score of the row that is
+// known without looking (sigmoid: 1; softmax: that of the largest logit): the size that errors
+// are measured by.  A 32-bit score is off by less than 2^-19 of it:
+//   sigmoid: __expf(-x) is off by |x| 2^-24 + 2^-22 of itself, which moves s by s (1 - s) times as
+//     much, at most 2^-24 and 2^-24; the sum and the quotient add 2^-22.
+//   softmax: x - m rounds by |x - m| 2^-24, which moves a score by at most 0.37 * 2^-24 of the
+//     largest; expf, the quotient and its product add 5 units, a sum of 16 terms in a lane and
+//     5 over the lanes 21 of 2^-24.
+template <int V, bool SOFTMAX, bool EXACT>
+__device__ __forceinline__ float scores(const float* x, float lowest, float* s) {
+  if constexpr (!SOFTMAX) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      if constexpr (EXACT) s[i] = x[i] <= lowest ? 0.f : __frcp_rn(1.0f + exp_to_f32(-static_cast<double>(x[i])));
+      else s[i] = x[i] <= lowest ? 0.f : __fdividef(1.0f, 1.0f + __expf(-fmaxf(x[i], -80.f)));
+    }
+    return 1.f;
+  } else {
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < V; ++i) m = fmaxf(m, x[i] <= lowest ? -INFINITY : x[i]);
+    m = warp_max(m);
+    if constexpr (EXACT) {
+      double ex[V], sum = 0.0;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const double d = static_cast<double>(x[i]) - static_cast<double>(m);
+        ex[i] = x[i] <= lowest ? 0.0 : d != d ? d : d < -700.0 ? 0.0 : exp_series(d);
+        sum += ex[i];
+      }
+      const double inv = 1.0 / warp_sum_d(sum);
+#pragma unroll
+      for (int i = 0; i < V; ++i) s[i] = x[i] <= lowest ? 0.f : static_cast<float>(ex[i] * inv);
+      return static_cast<float>(inv);
+    } else {
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        s[i] = x[i] <= lowest ? 0.f : expf(x[i] - m);
+        sum += s[i];
+      }
+      const float inv = 1.f / fmaxf(warp_sum(sum), 1e-30f);
+#pragma unroll
+      for (int i = 0; i < V; ++i) s[i] *= inv;
+      return inv;
+    }
+  }
+}
+
+// Two sides of a decision are told apart by the 32-bit scores if they differ by more than this
+// share of the sizes involved.  Each side is off by 2^-19 of the row's size for a score, twice that
+// for a group's two, and by 2^-20 of its own for the slot in a key's low bits and 2^-23 for the
+// sums' rounding: together less than 2^-17 + 2^-18.
+constexpr float kMargin = 1.52587890625e-05f;   // 2^-16
+
+// Whether `in` (the weakest taken) is above `out` (the strongest left) for certain.  -inf for
+// either: nothing was taken or left, no decision.
+__device__ __forceinline__ bool apart(float in, float out, float size) {
+  return out == -INFINITY || in == -INFINITY || in - out > kMargin * fmaxf(size, fmaxf(fabsf(in), fabsf(out)));
+}
+
+// Keys of the fast choice: order_key without its low 4 bits, in which the slot is kept; 0: not to be chosen.
+constexpr uint32_t kSlotMask = 15u;
+__device__ __forceinline__ float key_value(uint32_t k) {
+  if (k == 0) return -INFINITY;
+  k &= ~kSlotMask;
+  return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
+}
+
+// Group scores in the lanes of shared memory's scan: lane g < n_group scans group g.
+__device__ __forceinline__ void scan_group(const float* sel, int lane, int n_group, int gs, float* m1, float* m2) {
+  *m1 = *m2 = -INFINITY;
+  if (lane < n_group)
+    for (int j = 0; j < gs; ++j) {
+      // each lane starts elsewhere in its group, so that they do not meet in one bank
+      const int k = j + lane;
+      const float v = sel[lane * gs + (k < gs ? k : k % gs)];
+      *m2 = fmaxf(*m2, fminf(*m1, v));
+      *m1 = fmaxf(*m1, v);
+    }
+}
+
+// Bit mask of the groups that stay; *sure: no decision within the margin (fast scores).
+__device__ __forceinline__ uint32_t keep_groups(float score, int g, bool leader, int n_group, int per_group_lanes,
+                                                int topk_group, float size, bool* sure) {
+  int rank = 0;
+  for (int h = 0; h < n_group; ++h) {
+    const float o = __shfl_sync(0xffffffffu, score, h * per_group_lanes);
+    rank += (o > score || (o == score && h < g)) ? 1 : 0;
+  }
+  const bool kept = leader && rank < topk_group;
+  const float in = key_value(__reduce_min_sync(0xffffffffu, kept && score != -INFINITY ? order_key(score) | kSlotMask : ~0u));
+  const float out = key_value(__reduce_max_sync(0xffffffffu, leader && !kept && score != -INFINITY ? order_key(score) : 0u));
+  *sure = apart(in, out, size);
+  uint32_t mask = __ballot_sync(0xffffffffu, kept);
+  if (per_group_lanes > 1) {   // from lanes h * per_group_lanes to bits h
+    uint32_t m = 0;
+    for (int h = 0; h < n_group; ++h) m |= ((mask >> (h * per_group_lanes)) & 1u) << h;
+    mask = m;
+  }
+  return mask;
+}
+
+// The choice: bit i of the result says that this lane's expert i is chosen.  EXACT: by the
+// defined scores.  Otherwise *sure tells whether the 32-bit scores decide it.
+template <int V, bool EXACT>
+__device__ __forceinline__ uint32_t choose(const SelectArgs& a, const float* sel0, float* s_sel, int lane, float size,
+                                           bool* sure) {
+  float sel[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) sel[i] = sel0[i];
+  const int first = lane * V, gs = a.E / a.n_group;
+  *sure = true;
+  if (a.n_group > 1) {
+    uint32_t kept;
+    const int lanes = gs / V;
+    if (gs % V == 0 && (lanes & (lanes - 1)) == 0) {   // a group is `lanes` neighbouring lanes
+      float m1 = -INFINITY, m2 = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        m2 = fmaxf(m2, fminf(m1, sel[i]));
+        m1 = fmaxf(m1, sel[i]);
+      }
+      for (int d = 1; d < lanes; d <<= 1) {
+        const float o1 = __shfl_xor_sync(0xffffffffu, m1, d), o2 = __shfl_xor_sync(0xffffffffu, m2, d);
+        m2 = fmaxf(fminf(m1, o1), fmaxf(m2, o2));
+        m1 = fmaxf(m1, o1);
+      }
+      const float score = a.top2 ? m1 + (m2 == -INFINITY ? 0.f : m2) : m1;
+      const int g = lane / lanes;
+      kept = keep_groups(score, g, lane % lanes == 0 && g < a.n_group, a.n_group, lanes, a.topk_group, size,
+                         sure);
+      if (!((kept >> (g & 31)) & 1u)) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) sel[i] = -INFINITY;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (first + i < a.E) s_sel[first + i] = sel[i];
+      __syncwarp();
+      float m1, m2;
+      scan_group(s_sel, lane, a.n_group, gs, &m1, &m2);
+      const float score = a.top2 ? m1 + (m2 == -INFINITY ? 0.f : m2) : m1;
+      kept = keep_groups(score, lane, lane < a.n_group, a.n_group, 1, a.topk_group, size, sure);
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (first + i < a.E && !((kept >> ((first + i) / gs)) & 1u)) sel[i] = -INFINITY;
+      __syncwarp();
+    }
+  }
+  uint32_t taken = 0;
+  if constexpr (EXACT) {
+    uint32_t key[V];   // 0: not to be chosen
+#pragma unroll
+    for (int i = 0; i < V; ++i) key[i] = sel[i] == -INFINITY ? 0u : order_key(sel[i]);
+    for (int r = 0; r < a.K; ++r) {
+      uint32_t best = 0;
+      int at = 0;
+#pragma unroll
+      for (int i = V - 1; i >= 0; --i)
+        if (key[i] >= best) {
+          best = key[i];
+          at = i;
+        }
+      const uint32_t m = __reduce_max_sync(0xffffffffu, best);
+      if (m == 0) break;
+      if (lane == __ffs(__ballot_sync(0xffffffffu, best == m)) - 1) {
+        taken |= 1u << at;
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if (i == at) key[i] = 0;
+      }
+    }
+  } else {
+    uint32_t key[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      key[i] = sel[i] == -INFINITY ? 0u : (order_key(sel[i]) & ~kSlotMask) | static_cast<uint32_t>(V - 1 - i);
+    sort_desc(key);
+    uint32_t weakest = 0;
+    for (int r = 0; r < a.K; ++r) {
+      const uint32_t m = __reduce_max_sync(0xffffffffu, key[0]);
+      if (m == 0) break;
+      weakest = m;
+      // equal keys of several lanes: within the margin, so any order will do here
+      if (lane == __ffs(__ballot_sync(0xffffffffu, key[0] == m)) - 1) {
+        taken |= 1u << (V - 1 - static_cast<int>(key[0] & kSlotMask));
+#pragma unroll
+        for (int i = 0; i + 1 < V; ++i) key[i] = key[i + 1];
+        key[V - 1] = 0;
+      }
+    }
+    *sure = *sure && apart(key_value(weakest), key_value(__reduce_max_sync(0xffffffffu, key[0])), size);
+  }
+  return taken;
+}
+
 template <int V, bool SOFTMAX>
 __global__ void __launch_bounds__(kSelWarps * 32) select_kernel(SelectArgs a) {
   extern __shared__ float s_dyn[];   // [warps][E] sel of a token (groups only), then [E] counts
@@ -82,127 +334,84 @@ __global__ void __launch_bounds__(kSelWarps * 32) select_kernel(SelectArgs a) {
     __syncthreads();
   }
   const float lowest = lowest_of(a.type);
-  const int gs = a.E / a.n_group;
+  const int first = lane * V;
   float bias[V];
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int e = i * 32 + lane;
-    bias[i] = a.bias && e < a.E ? load1_dyn(a.bias, a.bias_type, e) : 0.f;
-  }
+  for (int i = 0; i < V; ++i) bias[i] = a.bias && first + i < a.E ? load1_dyn(a.bias, a.bias_type, first + i) : 0.f;
   for (int t = blockIdx.x * kSelWarps + warp; t < a.T; t += gridDim.x * kSelWarps) {
     float x[V], s[V], sel[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int e = i * 32 + lane;
-      x[i] = e < a.E ? load1_dyn(a.logits, a.type, t * a.ld + e) : -INFINITY;
-    }
-    if constexpr (SOFTMAX) {
-      float m = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < V; ++i) m = fmaxf(m, x[i] <= lowest ? -INFINITY : x[i]);
-      m = warp_max(m);
-      double ex[V], sum = 0.0;
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const double d = static_cast<double>(x[i]) - static_cast<double>(m);
-        ex[i] = x[i] <= lowest ? 0.0 : d != d ? d : d < -700.0 ? 0.0 : exp_series(d);
-        sum += ex[i];
-      }
-      sum = warp_sum_d(sum);
-      const double inv = 1.0 / sum;
-#pragma unroll
-      for (int i = 0; i < V; ++i) s[i] = x[i] <= lowest ? 0.f : static_cast<float>(ex[i] * inv);
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        s[i] = x[i] <= lowest ? 0.f : __frcp_rn(1.0f + exp_to_f32(-static_cast<double>(x[i])));
-    }
-    bool bad = false;
+    load_logits<V>(a.logits, a.type, t * a.ld, first, a.E, a.vec, x);
+    const float size = scores<V, SOFTMAX, false>(x, lowest, s);
+    bool bad = false, sure = true;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       sel[i] = x[i] <= lowest ? -INFINITY : s[i] + bias[i];
-      bad |= sel[i] != sel[i];
+      // the bounded sigmoid hides a NaN; an infinite logit makes a softmax NaN
+      bad |= sel[i] != sel[i] || x[i] != x[i];
     }
     bad = __any_sync(0xffffffffu, bad);
-    if (a.n_group > 1) {
+    uint32_t taken = 0;
+    if (!bad) taken = choose<V, false>(a, sel, s_sel, lane, size, &sure);
+    if (!sure) {
+      scores<V, SOFTMAX, true>(x, lowest, s);
+#pragma unroll
+      for (int i = 0; i < V; ++i) sel[i] = x[i] <= lowest ? -INFINITY : s[i] + bias[i];
+      taken = choose<V, true>(a, sel, s_sel, lane, size, &sure);
+    } else if constexpr (!SOFTMAX) {
+      // the chosen scores as defined (about one per lane that has any)
 #pragma unroll
       for (int i = 0; i < V; ++i)
-        if (i * 32 + lane < a.E) s_sel[i * 32 + lane] = sel[i];
-      __syncwarp();
-      float m1 = -INFINITY, m2 = -INFINITY;
-      if (lane < a.n_group)
-        for (int j = 0; j < gs; ++j) {
-          const float v = s_sel[lane * gs + j];
-          m2 = fmaxf(m2, fminf(m1, v));
-          m1 = fmaxf(m1, v);
-        }
-      const float score = a.top2 ? m1 + (m2 == -INFINITY ? 0.f : m2) : m1;
-      int rank = 0;
-      for (int h = 0; h < a.n_group; ++h) {
-        const float o = __shfl_sync(0xffffffffu, score, h);
-        rank += (o > score || (o == score && h < lane)) ? 1 : 0;
-      }
-      const uint32_t kept = __ballot_sync(0xffffffffu, lane < a.n_group && rank < a.topk_group);
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int e = i * 32 + lane;
-        if (e < a.E && !((kept >> (e / gs)) & 1u)) sel[i] = -INFINITY;
-      }
-      __syncwarp();
-    }
-    // key 0: not to be chosen (order_key(-inf) is above it, so -inf is mapped here)
-    uint32_t key[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) key[i] = bad || sel[i] == -INFINITY ? 0u : order_key(sel[i]);
-    uint32_t taken = 0;
-    for (int r = 0; r < a.K; ++r) {
-      uint32_t best = 0;
-      int at = 0;
-#pragma unroll
-      for (int i = V - 1; i >= 0; --i)
-        if (key[i] >= best) {
-          best = key[i];
-          at = i;
-        }
-      const uint32_t m = __reduce_max_sync(0xffffffffu, best);
-      if (m == 0) break;
-      const uint32_t e = __reduce_min_sync(0xffffffffu, best == m ? static_cast<uint32_t>(at * 32 + lane) : ~0u);
-      if ((e & 31u) == static_cast<uint32_t>(lane)) {
-        taken |= 1u << (e >> 5);
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-          if (i == static_cast<int>(e >> 5)) key[i] = 0;
-      }
+        if ((taken >> i) & 1u) s[i] = __frcp_rn(1.0f + exp_to_f32(-static_cast<double>(x[i])));
     }
     float part = 0.f;
 #pragma unroll
     for (int i = 0; i < V; ++i)
       if ((taken >> i) & 1u) part += s[i];
     const float denom = warp_sum(part) + 1e-20f;
-    int pos = 0;
+    const int mine = __popc(taken);
+    int pos = mine;   // exclusive prefix over the lanes
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, pos, d);
+      if (lane >= d) pos += o;
+    }
+    const int total = __shfl_sync(0xffffffffu, pos, 31);
+    pos -= mine;
     const int64_t base = static_cast<int64_t>(t) * a.K;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const bool mine = (taken >> i) & 1u;
-      const uint32_t b = __ballot_sync(0xffffffffu, mine);
-      if (mine) {
-        const int p = pos + __popc(b & ((1u << lane) - 1u));
-        a.idx[base + p] = i * 32 + lane;
-        a.w[base + p] = (a.renorm ? s[i] / denom : s[i]) * a.scale;
-        if (a.counts) atomicAdd(s_cnt + i * 32 + lane, 1);
+    for (int i = 0; i < V; ++i)
+      if ((taken >> i) & 1u) {
+        a.idx[base + pos] = first + i;
+        a.w[base + pos] = (a.renorm ? s[i] / denom : s[i]) * a.scale;
+        ++pos;
+        if (a.counts) atomicAdd(s_cnt + first + i, 1);
       }
-      pos += __popc(b);
-    }
-    if (lane >= pos && lane < a.K) {
+    if (lane >= total && lane < a.K) {
       a.idx[base + lane] = -1;
       a.w[base + lane] = bad ? __uint_as_float(0x7fc00000u) : 0.f;
     }
   }
-  if (a.counts) {
+  if (!a.counts) return;
+  if (a.cluster) {   // the CTAs of one cluster are the whole grid: the first adds up their counts
+    cluster_sync();
+    if (blockIdx.x == 0)
+      for (int e = threadIdx.x; e < a.E; e += blockDim.x) {
+        int n = 0;
+        for (uint32_t c = 0; c < gridDim.x; ++c) n += ld_cluster_s32(cluster_addr(smem_u32(s_cnt + e), c));
+        a.counts[e] = n;
+      }
+    cluster_sync();
+  } else {
     __syncthreads();
     for (int e = threadIdx.x; e < a.E; e += blockDim.x)
       if (s_cnt[e]) atomicAdd(a.counts + e, s_cnt[e]);   // integers: the order does not matter
   }
+}
+
+__global__ void __launch_bounds__(kSelMaxE) select_zero_kernel(int* counts, int E) {
+  pdl_wait();
+  pdl_launch_dependents();
+  if (threadIdx.x < E) counts[threadIdx.x] = 0;
 }
 
 // dlogits of a token, from the gradients dw of its chosen weights (ids distinct, -1: no expert).
@@ -342,9 +551,13 @@ MOE_B200_API int moe_b200_select_experts(const moe_b200_select_args* a, void* st
   if (int rc = op_device(&sms)) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaSuccess;
-  if (a->counts) {
-    e = cudaMemsetAsync(a->counts, 0, sizeof(int) * a->num_experts, st);
-    if (e != cudaSuccess) return report_cuda(e, "cudaMemsetAsync");
+  // Counts: up to 64 tokens are one cluster's, which adds up its CTAs' histograms; beyond that
+  // the CTAs add theirs to counts zeroed first.
+  const int ctas = select_grid(a->num_tokens, sms);
+  const bool cluster = a->counts && a->num_tokens > 0 && ctas <= 8;
+  if (a->counts && !cluster) {
+    e = launch_pdl(select_zero_kernel, dim3(1), dim3(kSelMaxE), 0, st, a->counts, a->num_experts);
+    if (e != cudaSuccess) return report_cuda(e, "select_experts launch");
   }
   if (a->num_tokens == 0) return MOE_B200_OK;
   SelectArgs s{};
@@ -365,11 +578,14 @@ MOE_B200_API int moe_b200_select_experts(const moe_b200_select_args* a, void* st
   s.renorm = a->renormalize;
   s.scale = a->scale;
   const size_t smem = ((s.n_group > 1 ? kSelWarps * s.E : 0) + (s.counts ? s.E : 0)) * sizeof(float);
-  const dim3 grid(select_grid(s.T, sms)), block(kSelWarps * 32);
+  const int bytes = 4 * type_bytes(s.type);
+  s.vec = reinterpret_cast<uintptr_t>(s.logits) % bytes == 0 && (s.T == 1 || s.ld % 4 == 0);
+  s.cluster = cluster;
+  const dim3 grid(ctas), block(kSelWarps * 32);
   dispatch_select(s.E, [&](auto v) {
     constexpr int V = decltype(v)::value;
-    e = a->score == MOE_B200_SCORE_SOFTMAX ? launch_pdl(select_kernel<V, true>, grid, block, smem, st, s)
-                                           : launch_pdl(select_kernel<V, false>, grid, block, smem, st, s);
+    auto kernel = a->score == MOE_B200_SCORE_SOFTMAX ? select_kernel<V, true> : select_kernel<V, false>;
+    e = cluster ? launch_cluster_pdl(kernel, grid, block, smem, ctas, st, s) : launch_pdl(kernel, grid, block, smem, st, s);
   });
   return e == cudaSuccess ? MOE_B200_OK : report_cuda(e, "select_experts launch");
 }

@@ -21,6 +21,7 @@ from . import _native
 _TYPES = {torch.bfloat16: _native.BF16, torch.float16: _native.FP16, torch.float32: _native.FP32,
           torch.float8_e4m3fn: _native.E4M3, torch.int8: _native.INT8}
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
+_FP32, _INT8, _LINEAR_IN = (torch.float32,), (torch.int8,), (*_FLOATS, torch.int8)
 
 
 class MoEArgumentError(AssertionError, ValueError):
@@ -52,33 +53,46 @@ class Selection(NamedTuple):
     counts: torch.Tensor | None       # int32 [E]
 
 
+# The checks run on every call, and a decode step's kernels take a few microseconds: each is one
+# expression, messages are put together only on refusal, devices are compared by index.
+
 def _rows(t, name: str, shape=None, dtypes=_FLOATS, dev=None):
-    """Checks a [rows, cols] tensor of the call; returns it."""
-    _check(t.dim() == 2 and (t.shape[1] < 2 or t.stride(1) == 1),
-           f"{name} must be [rows, cols] with adjacent elements in a row")
-    _check(t.shape[0] < 2 or t.stride(0) >= 0, f"{name}: negative row stride")
-    if shape is not None:
-        _check(t.shape == shape, f"{name} must be {list(shape)}")
-    _check(t.dtype in dtypes, f"{name} has an unsupported type {t.dtype}")
-    _check(t.is_cuda, "all tensors must be CUDA tensors (there is no CPU path)")
-    if dev is not None:
-        _check(t.device == dev, "all tensors must be on one device")
-    return t
+    """Checks a [rows, cols] CUDA tensor of the call; returns its row pitch in elements (which
+    says nothing for a single row)."""
+    st = t.stride()
+    if (len(st) != 2 or (st[1] != 1 and t.shape[1] > 1) or t.dtype not in dtypes
+            or (not t.is_cuda if dev is None else t.get_device() != dev)
+            or (shape is not None and t.shape != shape)):
+        _check(len(st) == 2 and (st[1] == 1 or t.shape[1] < 2),
+               f"{name} must be [rows, cols] with adjacent elements in a row")
+        _check(shape is None or t.shape == shape, f"{name} must be {list(shape or ())}")
+        _check(t.dtype in dtypes, f"{name} has an unsupported type {t.dtype}")
+        _check(t.is_cuda, "all tensors must be CUDA tensors (there is no CPU path)")
+        raise MoEArgumentError("all tensors must be on one device")
+    return st[0]
 
 
 def _result(t, name: str, shape, dtypes, dev):
-    """Checks a tensor that receives a result: rows may not overlap."""
-    _rows(t, name, shape, dtypes, dev)
-    _check(shape[0] < 2 or t.stride(0) >= shape[1], f"{name}: rows overlap")
-    return t
+    """Checks a tensor that receives a result: rows may not overlap.  Returns its row pitch."""
+    ld = _rows(t, name, shape, dtypes, dev)
+    if shape[0] > 1 and ld < shape[1]:
+        raise MoEArgumentError(f"{name}: rows overlap")
+    return ld
 
 
 def _vector(t, name: str, n: int, dtypes, dev):
-    if t is not None:
+    if t is None:
+        raise MoEArgumentError(f"{name} is required")
+    if t.shape != (n,) or (n > 1 and t.stride(0) != 1) or t.dtype not in dtypes or t.get_device() != dev:
         _check(t.dim() == 1 and t.shape[0] == n and t.is_contiguous(), f"{name} must be a contiguous [{n}] tensor")
         _check(t.dtype in dtypes, f"{name} has an unsupported type {t.dtype}")
-        _check(t.device == dev, "all tensors must be on one device")
-    return t
+        raise MoEArgumentError("all tensors must be on one device")
+
+
+def _matrix(t, name: str, shape, dtype, dev):
+    """Checks a contiguous matrix (the tensors that the layer's routing results are made of)."""
+    if t.shape != shape or t.dtype != dtype or not t.is_contiguous() or t.get_device() != dev:
+        raise MoEArgumentError(f"{name} must be a contiguous {dtype} {list(shape)} tensor on the device")
 
 
 def _ptr(t):
@@ -89,29 +103,50 @@ def _type(t) -> int:
     return 0 if t is None else _TYPES[t.dtype]
 
 
-def _ld(t) -> int:
-    """Row pitch in elements (a single row's stride is arbitrary and says nothing)."""
-    return 0 if t is None else t.stride(0) if t.shape[0] > 1 else t.shape[1]
+_functions: dict = {}   # operator -> its C entry, looked up once
 
 
-def _stream(dev) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
+def _call(fn: str, dev: int, args, *workspace):
+    """Calls moe_b200_<fn> on the device's current stream, with that device current."""
+    f = _functions.get(fn)
+    if f is None:
+        f = _functions[fn] = getattr(_native.lib(), "moe_b200_" + fn)
+    if torch._C._cuda_getDevice() == dev:
+        rc = f(args, *workspace, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = f(args, *workspace, torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        raise _failure(rc, fn)
 
 
-def _done(rc: int, what: str):
-    if rc == _native.OK:
-        return
+_SCRATCH_KEPT = 4 << 20   # bytes kept per (device, stream)
+_scratch: dict[tuple[int, int], torch.Tensor] = {}
+
+
+def _workspace(n: int, dev: int) -> torch.Tensor:
+    """Scratch of n bytes for a call on the device's current stream.  Small ones are kept per
+    (device, stream): the calls of one stream run one after another.  Large ones, and those of a
+    graph capture (whose replays would share them with later calls), are allocated per call."""
+    if n > _SCRATCH_KEPT or torch.cuda.is_current_stream_capturing():
+        return torch.empty(n, dtype=torch.uint8, device=dev)
+    key = (dev, torch._C._cuda_getCurrentRawStream(dev))
+    ws = _scratch.get(key)
+    if ws is None:
+        ws = _scratch[key] = torch.empty(_SCRATCH_KEPT, dtype=torch.uint8, device=dev)
+    return ws
+
+
+def _failure(rc: int, what: str) -> Exception:
     if rc == _native.ERR_ARG:
-        raise MoEArgumentError(f"{what}: {_native.last_error()}")
-    raise RuntimeError(f"{what} failed ({rc}): {_native.last_error()}")
+        return MoEArgumentError(f"{what}: {_native.last_error()}")
+    return RuntimeError(f"{what} failed ({rc}): {_native.last_error()}")
 
 
-def _gate_layout(gate, rows: int, cols: int, dev):
+def _gate_layout(gate, rows: int, cols: int, dev: int):
     """(row stride, varies along a row) of a gate [cols], [1, cols], [rows, 1], [1, 1] or [rows, cols]."""
-    if gate is None:
-        return 0, 0
-    _check(gate.dtype in _FLOATS, f"gate has an unsupported type {gate.dtype}")
-    _check(gate.device == dev, "all tensors must be on one device")
+    _check(gate.dtype in _FLOATS, "gate has an unsupported type")
+    _check(gate.get_device() == dev, "all tensors must be on one device")
     g = gate.unsqueeze(0) if gate.dim() == 1 else gate
     _check(g.dim() == 2 and g.shape[0] in (1, rows) and g.shape[1] in (1, cols),
            "gate must be broadcastable to [rows, cols]")
@@ -122,7 +157,6 @@ def _gate_layout(gate, rows: int, cols: int, dev):
     return g.stride(0) if per_row else 0, int(per_column)
 
 
-@torch.no_grad()
 def block_norm(y: torch.Tensor | None, residual: torch.Tensor | None, *, post_weight: torch.Tensor | None = None,
                gate: torch.Tensor | None = None, scale: float = 1.0, pre_weight: torch.Tensor | None = None,
                eps: float = 1e-6, weight_offset: float = 0.0, x_dtype: torch.dtype | None = None,
@@ -140,40 +174,46 @@ def block_norm(y: torch.Tensor | None, residual: torch.Tensor | None, *, post_we
     ``hidden_states_scale`` of :func:`moe_swarm_b200.run`.  ``residual_out`` (may be ``residual``)
     and ``out`` receive r' and x instead of new tensors.
     """
-    first = y if y is not None else residual
+    first = residual if y is None else y
     _check(first is not None, "y or residual is required")
-    _rows(first, "y" if y is not None else "residual")
-    shape, dev = first.shape, first.device
+    shape, dev = first.shape, first.get_device()
+    y_ld = r_ld = ro_ld = x_ld = 0
+    if y is not None:
+        y_ld = _rows(y, "y")
+        if residual is not None:
+            r_ld = _rows(residual, "residual", shape, (y.dtype, torch.float32), dev)
+    else:
+        r_ld = _rows(residual, "residual")
     rows, cols = shape
-    if y is not None and residual is not None:
-        _rows(residual, "residual", shape, (y.dtype, torch.float32), dev)
-    _vector(post_weight, "post_weight", cols, _FLOATS, dev)
-    _vector(pre_weight, "pre_weight", cols, _FLOATS, dev)
-    gate_ld, gate_cols = _gate_layout(gate, rows, cols, dev)
-    r_dtype = residual.dtype if residual is not None else y.dtype
+    if post_weight is not None:
+        _vector(post_weight, "post_weight", cols, _FLOATS, dev)
+    gate_ld, gate_cols = (0, 0) if gate is None else _gate_layout(gate, rows, cols, dev)
+    stream = y if residual is None else residual   # the tensor that r' is like
     if y is None:
         _check(residual_out is None, "residual_out is the residual itself without y")
     elif residual_out is None:
-        residual_out = torch.empty(shape, dtype=r_dtype, device=dev)
+        residual_out, ro_ld = torch.empty_like(stream), cols
     else:
-        _result(residual_out, "residual_out", shape, (r_dtype,), dev)
+        ro_ld = _result(residual_out, "residual_out", shape, (stream.dtype,), dev)
     x = x_scale = None
     if pre_weight is not None:
-        x_dtype = (out.dtype if out is not None else first.dtype) if x_dtype is None else x_dtype
-        _check(x_dtype in _TYPES and x_dtype != torch.int8, f"unsupported x_dtype {x_dtype}")
-        x = torch.empty(shape, dtype=x_dtype, device=dev) if out is None else _result(out, "out", shape, (x_dtype,), dev)
+        _vector(pre_weight, "pre_weight", cols, _FLOATS, dev)
+        if x_dtype is None:
+            x_dtype = first.dtype if out is None else out.dtype
+        _check(x_dtype in _TYPES and x_dtype != torch.int8, "unsupported x_dtype")
+        if out is None:
+            x, x_ld = torch.empty_like(first, dtype=x_dtype), cols
+        else:
+            x, x_ld = out, _result(out, "out", shape, (x_dtype,), dev)
         if x_dtype == torch.float8_e4m3fn:
-            x_scale = torch.empty(((cols + 127) // 128, rows), dtype=torch.float32, device=dev)
-    a = _native.NormArgs(
+            x_scale = torch.empty(((cols + 127) // 128, rows), dtype=torch.float32, device=first.device)
+    _call("block_norm", dev, _native.NormArgs(
         _ptr(y), _ptr(residual), _ptr(post_weight), _ptr(pre_weight), _ptr(gate), _ptr(residual_out), _ptr(x),
-        _ptr(x_scale), _ld(y), _ld(residual), _ld(residual_out), _ld(x), gate_ld, rows, cols, _type(first),
-        _TYPES[r_dtype], _type(post_weight), _type(pre_weight), _type(gate), _type(x), gate_cols, scale, eps,
-        weight_offset)
-    _done(_native.lib().moe_b200_block_norm(ctypes.byref(a), _stream(dev)), "block_norm")
+        _ptr(x_scale), y_ld, r_ld, ro_ld, x_ld, gate_ld, rows, cols, _TYPES[first.dtype], _TYPES[stream.dtype],
+        _type(post_weight), _type(pre_weight), _type(gate), _type(x), gate_cols, scale, eps, weight_offset))
     return BlockNormOut(residual if y is None else residual_out, x, x_scale)
 
 
-@torch.no_grad()
 def block_norm_backward(dx: torch.Tensor | None, dresidual: torch.Tensor | None, residual: torch.Tensor,
                         y: torch.Tensor | None, *, post_weight: torch.Tensor | None = None,
                         gate: torch.Tensor | None = None, scale: float = 1.0,
@@ -186,38 +226,40 @@ def block_norm_backward(dx: torch.Tensor | None, dresidual: torch.Tensor | None,
     Weight gradients are fp32.  The gate's gradient has the gate's shape, summed over what it is
     broadcast over: fp32 where it is summed, the gate's type for a [rows, cols] gate.
     """
-    _rows(residual, "residual")
-    shape, dev = residual.shape, residual.device
+    r_ld = _rows(residual, "residual")
+    shape, dev, r_dtype = residual.shape, residual.get_device(), residual.dtype
     rows, cols = shape
-    given = y if y is not None else dx if dx is not None else residual
-    _check(residual.dtype in (given.dtype, torch.float32), "residual must have y's type or fp32")
+    y_dtype = (residual if y is None and dx is None else dx if y is None else y).dtype
+    _check(r_dtype is y_dtype or r_dtype is torch.float32, "residual must have y's type or fp32")
     _check(dx is not None or dresidual is not None, "dx or dresidual is required")
     _check(dx is None or pre_weight is not None, "dx needs pre_weight")
     _check(y is not None or (post_weight is None and gate is None), "post_weight and gate need y")
-    for t, name, dtype in ((y, "y", given.dtype), (dx, "dx", given.dtype), (dresidual, "dresidual", residual.dtype)):
-        if t is not None:
-            _rows(t, name, shape, (dtype,), dev)
-    _vector(post_weight, "post_weight", cols, _FLOATS, dev)
-    _vector(pre_weight, "pre_weight", cols, _FLOATS, dev)
-    gate_ld, gate_cols = _gate_layout(gate, rows, cols, dev)
-
-    def new(like, dtype=None):
-        return None if like is None else torch.empty(like.shape, dtype=dtype or like.dtype, device=dev)
-
-    dres, dy = new(residual), new(y)
-    dpre = new(pre_weight, torch.float32) if dx is not None else None
-    dpost = new(post_weight, torch.float32)
-    dgate = new(gate, None if gate_ld and gate_cols else torch.float32)
-    lib = _native.lib()
-    n = lib.moe_b200_block_norm_backward_workspace_size(rows, cols)
-    ws = torch.empty(max(n, 256), dtype=torch.uint8, device=dev)
-    a = _native.NormBackwardArgs(
+    y_ld = 0 if y is None else _rows(y, "y", shape, (y_dtype,), dev)
+    dx_ld = 0 if dx is None else _rows(dx, "dx", shape, (y_dtype,), dev)
+    dr_ld = 0 if dresidual is None else _rows(dresidual, "dresidual", shape, (r_dtype,), dev)
+    dy = dpre = dpost = dgate = None
+    gate_ld = gate_cols = 0
+    dres = torch.empty_like(residual)
+    if y is not None:
+        dy = torch.empty_like(y)
+    if dx is not None:
+        _vector(pre_weight, "pre_weight", cols, _FLOATS, dev)
+        dpre = torch.empty_like(pre_weight, dtype=torch.float32)
+    if post_weight is not None:
+        _vector(post_weight, "post_weight", cols, _FLOATS, dev)
+        dpost = torch.empty_like(post_weight, dtype=torch.float32)
+    if gate is not None:
+        gate_ld, gate_cols = _gate_layout(gate, rows, cols, dev)
+        dgate = torch.empty_like(gate, dtype=gate.dtype if gate_ld and gate_cols else torch.float32,
+                                 memory_format=torch.contiguous_format)
+    n = _native.lib().moe_b200_block_norm_backward_workspace_size(rows, cols)
+    _check(n > 0, "unsupported sizes")
+    ws = _workspace(n, dev)
+    _call("block_norm_backward", dev, _native.NormBackwardArgs(
         _ptr(dx), _ptr(dresidual), _ptr(residual), _ptr(y), _ptr(post_weight), _ptr(pre_weight), _ptr(gate),
-        _ptr(dres), _ptr(dy), _ptr(dpre), _ptr(dpost), _ptr(dgate), _ld(dx), _ld(dresidual), _ld(residual), _ld(y),
-        gate_ld, _ld(dres), _ld(dy), cols, rows, cols, _TYPES[given.dtype], _type(residual), _type(post_weight),
-        _type(pre_weight), _type(gate), gate_cols, scale, eps, weight_offset)
-    _done(lib.moe_b200_block_norm_backward(ctypes.byref(a), ws.data_ptr(), ws.numel(), _stream(dev)),
-          "block_norm_backward")
+        _ptr(dres), _ptr(dy), _ptr(dpre), _ptr(dpost), _ptr(dgate), dx_ld, dr_ld, r_ld, y_ld, gate_ld, cols, cols,
+        cols, rows, cols, _TYPES[y_dtype], _TYPES[r_dtype], _type(post_weight), _type(pre_weight), _type(gate),
+        gate_cols, scale, eps, weight_offset), ws.data_ptr(), ws.numel())
     return BlockNormGrads(dres, dy, dpre, dpost, dgate)
 
 
@@ -225,7 +267,6 @@ _SCORES = {"sigmoid": 0, "softmax": 1}
 _GROUP_SCORES = {"top2": 0, "max": 1}
 
 
-@torch.no_grad()
 def select_experts(logits: torch.Tensor, top_k: int, *, score: str = "sigmoid", bias: torch.Tensor | None = None,
                    n_group: int = 1, topk_group: int = 1, group_score: str = "top2", renormalize: bool = True,
                    scale: float = 1.0, counts: bool = False) -> Selection:
@@ -240,62 +281,58 @@ def select_experts(logits: torch.Tensor, top_k: int, *, score: str = "sigmoid", 
     weight 0.  A row with a NaN score has ids -1 and NaN weights.  ``counts`` also returns how many
     tokens chose each expert.  idx and w are what :func:`moe_swarm_b200.run_routed` takes.
     """
-    _rows(logits, "logits")
+    ld = _rows(logits, "logits")
     T, E = logits.shape
-    dev = logits.device
+    dev, device = logits.get_device(), logits.device
     _check(score in _SCORES, "score must be 'sigmoid' or 'softmax'")
     _check(group_score in _GROUP_SCORES, "group_score must be 'top2' or 'max'")
     _check(1 <= top_k <= E, "top_k must be in [1, number of experts]")
-    _vector(bias, "bias", E, _FLOATS, dev)
-    idx = torch.empty((T, top_k), dtype=torch.int32, device=dev)
-    w = torch.empty((T, top_k), dtype=torch.float32, device=dev)
-    n = torch.empty(E, dtype=torch.int32, device=dev) if counts else None
-    a = _native.SelectArgs(_ptr(logits), _ptr(bias), _ptr(idx), _ptr(w), _ptr(n), _ld(logits), T, E, top_k,
-                           _type(logits), _type(bias), _SCORES[score], n_group, topk_group,
-                           _GROUP_SCORES[group_score], bool(renormalize), scale)
-    _done(_native.lib().moe_b200_select_experts(ctypes.byref(a), _stream(dev)), "select_experts")
+    if bias is not None:
+        _vector(bias, "bias", E, _FLOATS, dev)
+    idx = torch.empty((T, top_k), dtype=torch.int32, device=device)
+    w = torch.empty_like(idx, dtype=torch.float32)
+    n = torch.empty(E, dtype=torch.int32, device=device) if counts else None
+    _call("select_experts", dev, _native.SelectArgs(
+        logits.data_ptr(), _ptr(bias), idx.data_ptr(), w.data_ptr(), _ptr(n), ld, T, E, top_k, _TYPES[logits.dtype],
+        _type(bias), _SCORES[score], n_group, topk_group, _GROUP_SCORES[group_score], bool(renormalize), scale))
     return Selection(idx, w, n)
 
 
-@torch.no_grad()
 def select_experts_backward(dw: torch.Tensor, logits: torch.Tensor, idx: torch.Tensor, *, score: str = "sigmoid",
                             renormalize: bool = True, scale: float = 1.0) -> torch.Tensor:
     """The gradient of :func:`select_experts`' weights with respect to the logits, from ``dw``
     (float32 [T, top_k]) and the ids it chose.  The choice itself has no gradient."""
-    _rows(logits, "logits")
+    ld = _rows(logits, "logits")
     T, E = logits.shape
-    dev = logits.device
+    dev = logits.get_device()
     _check(score in _SCORES, "score must be 'sigmoid' or 'softmax'")
-    _check(idx.dim() == 2 and idx.shape[0] == T and idx.dtype == torch.int32 and idx.is_contiguous()
-           and idx.device == dev, "idx must be a contiguous int32 [T, top_k] tensor on the device")
-    _check(dw.shape == idx.shape and dw.dtype == torch.float32 and dw.is_contiguous() and dw.device == dev,
-           "dw must be a contiguous float32 [T, top_k] tensor on the device")
-    out = torch.empty((T, E), dtype=logits.dtype, device=dev)
-    a = _native.SelectBackwardArgs(_ptr(logits), _ptr(idx), _ptr(dw), _ptr(out), _ld(logits), E, T, E, idx.shape[1],
-                                   _type(logits), _SCORES[score], bool(renormalize), scale)
-    _done(_native.lib().moe_b200_select_experts_backward(ctypes.byref(a), _stream(dev)), "select_experts_backward")
+    _check(idx.dim() == 2, "idx must be [T, top_k]")
+    _matrix(idx, "idx", (T, idx.shape[1]), torch.int32, dev)
+    _matrix(dw, "dw", idx.shape, torch.float32, dev)
+    out = torch.empty_like(logits)
+    _call("select_experts_backward", dev, _native.SelectBackwardArgs(
+        logits.data_ptr(), idx.data_ptr(), dw.data_ptr(), out.data_ptr(), ld, E, T, E, idx.shape[1],
+        _TYPES[logits.dtype], _SCORES[score], bool(renormalize), scale))
     return out
 
 
-@torch.no_grad()
 def quantize_int8(x: torch.Tensor, *, swiglu: bool = False):
     """8-bit codes and scales of the rows of ``x``: (int8 [rows, cols], float32 [rows]) with
     scale = max(amax / 127, 2**-126).  With ``swiglu``, of silu(x[:, cols:]) * x[:, :cols] (the
     expert layer's order of the two halves).  For weights [out, in] the rows are the channels."""
-    _rows(x, "x")
-    dev = x.device
+    ld = _rows(x, "x")
+    dev, device = x.get_device(), x.device
     rows, cols = x.shape
     if swiglu:
         _check(cols % 2 == 0, "swiglu needs an even number of columns")
         cols //= 2
-    q = torch.empty((rows, cols), dtype=torch.int8, device=dev)
-    scale = torch.empty(rows, dtype=torch.float32, device=dev)
-    a = _native.QuantizeArgs(_ptr(x), _ptr(q), _ptr(scale), _ld(x), cols, rows, cols, _type(x), bool(swiglu))
-    _done(_native.lib().moe_b200_quantize_int8(ctypes.byref(a), _stream(dev)), "quantize_int8")
+    q = torch.empty((rows, cols), dtype=torch.int8, device=device)
+    scale = torch.empty(rows, dtype=torch.float32, device=device)
+    _call("quantize_int8", dev, _native.QuantizeArgs(x.data_ptr(), q.data_ptr(), scale.data_ptr(), ld, cols, rows, cols,
+                                                     _TYPES[x.dtype], bool(swiglu)))
     return q, scale
 
 
-@torch.no_grad()
 def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, *,
                 x_scale: torch.Tensor | None = None, bias: torch.Tensor | None = None, swiglu: bool = False,
                 out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -307,35 +344,35 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     multiple of 16 and rows of int8 tensors start on 16-byte boundaries.  ``out_dtype``: bf16 by
     default (x's type if that is fp16 or fp32).
     """
-    _rows(x, "x", dtypes=(*_FLOATS, torch.int8))
-    dev = x.device
-    _rows(weight, "weight", dtypes=(torch.int8,), dev=dev)
-    T, N, K = x.shape[0], weight.shape[0], weight.shape[1]
+    x_ld = _rows(x, "x", None, _LINEAR_IN)
+    dev = x.get_device()
+    w_ld = _rows(weight, "weight", None, _INT8, dev)
+    T, (N, K) = x.shape[0], weight.shape
     _check(x.shape[1] == (2 * K if swiglu else K), "x and weight do not fit")
-    _vector(weight_scale, "weight_scale", N, (torch.float32,), dev)
-    _check(weight_scale is not None, "weight_scale is required")
-    if x.dtype == torch.int8:
+    _vector(weight_scale, "weight_scale", N, _FP32, dev)
+    x_type = _TYPES[x.dtype]
+    if x_type == _native.INT8:
         _check(x_scale is not None, "an int8 x needs x_scale")
-        _vector(x_scale, "x_scale", T, (torch.float32,), dev)
+        _vector(x_scale, "x_scale", T, _FP32, dev)
     else:
         _check(x_scale is None, "x_scale is computed for a floating-point x")
-    _vector(bias, "bias", N, _FLOATS, dev)
+    if bias is not None:
+        _vector(bias, "bias", N, _FLOATS, dev)
     if out is None:
         if out_dtype is None:
-            out_dtype = torch.bfloat16 if x.dtype == torch.int8 else x.dtype
-        _check(out_dtype in _FLOATS, f"unsupported out_dtype {out_dtype}")
-        out = torch.empty((T, N), dtype=out_dtype, device=dev)
+            out_dtype = torch.bfloat16 if x_type == _native.INT8 else x.dtype
+        _check(out_dtype in _FLOATS, "unsupported out_dtype")
+        out, out_ld = torch.empty((T, N), dtype=out_dtype, device=x.device), N
     else:
-        _result(out, "out", (T, N), _FLOATS if out_dtype is None else (out_dtype,), dev)
+        out_ld = _result(out, "out", (T, N), _FLOATS if out_dtype is None else (out_dtype,), dev)
     if T == 0 or N == 0:
         return out
-    lib = _native.lib()
-    n = lib.moe_b200_int8_linear_workspace_size(T, N, K, _type(x))
+    n = _native.lib().moe_b200_int8_linear_workspace_size(T, N, K, x_type)
     _check(n > 0, "unsupported sizes")
-    ws = torch.empty(n, dtype=torch.uint8, device=dev)
-    a = _native.LinearArgs(_ptr(x), _ptr(x_scale), _ptr(weight), _ptr(weight_scale), _ptr(bias), _ptr(out), _ld(x),
-                           _ld(weight), _ld(out), T, N, K, _type(x), _type(out), _type(bias), bool(swiglu))
-    _done(lib.moe_b200_int8_linear(ctypes.byref(a), ws.data_ptr(), ws.numel(), _stream(dev)), "int8_linear")
+    ws = _workspace(n, dev)
+    _call("int8_linear", dev, _native.LinearArgs(
+        x.data_ptr(), _ptr(x_scale), weight.data_ptr(), weight_scale.data_ptr(), _ptr(bias), out.data_ptr(), x_ld, w_ld,
+        out_ld, T, N, K, x_type, _TYPES[out.dtype], _type(bias), bool(swiglu)), ws.data_ptr(), ws.numel())
     return out
 
 
@@ -344,7 +381,8 @@ def operator_status(device=None, clear: bool = True) -> int:
     the code of a bounded device-side wait that gave up (the call's result is then not valid)."""
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     with torch.cuda.device(dev):
-        rc = int(_native.lib().moe_b200_operator_status(_stream(dev), 1 if clear else 0))
+        stream = torch.cuda.current_stream(dev).cuda_stream
+        rc = int(_native.lib().moe_b200_operator_status(stream, 1 if clear else 0))
     if rc < 0:
         raise RuntimeError(f"operator_status failed ({-rc}): {_native.last_error()}")
     return rc

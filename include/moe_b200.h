@@ -401,8 +401,8 @@ MOE_B200_API int moe_b200_int8_linear(const moe_b200_linear_args* args, void* wo
                                       void* stream);
 
 /* Synchronises the stream and returns the status word of the operators above on the current
- * device: 0, or the code of the first bounded device-side wait of moe_b200_int8_linear that
- * timed out (its result is then not valid); reset if `clear`.  Negative: a status code, negated. */
+ * device: 0, or the code of the first of their bounded device-side waits that timed out (that
+ * call's result is then not valid); reset if `clear`.  Negative: a status code, negated. */
 MOE_B200_API int moe_b200_operator_status(void* stream, int32_t clear);
 
 /* Text of the last host-side error of this thread ("" if none). */

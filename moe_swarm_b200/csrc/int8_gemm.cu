@@ -16,8 +16,6 @@
 
 namespace moe {
 
-__device__ int g_op_status;
-
 // float(sum) * (sx * sw) + bias of a tile's column, rounded once to the output's type
 template <class YT>
 __device__ __forceinline__ void store_cols32(YT* dst, int n, bool vec, const float* v) {
@@ -438,19 +436,16 @@ cudaError_t int8_stream_launch(const int8_t* q, int64_t q_ld, const int8_t* w, i
   });
 }
 
+cudaError_t int8_status(cudaStream_t st, bool clear, int* v) { return take_status(st, clear, v); }
+
 }  // namespace moe
 
 extern "C" MOE_B200_API int moe_b200_operator_status(void* stream, int32_t clear) {
   using namespace moe;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  int v = 0;
-  cudaError_t e = cudaMemcpyFromSymbolAsync(&v, g_op_status, sizeof(int), 0, cudaMemcpyDeviceToHost, st);
-  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
-  if (e == cudaSuccess && clear && v) {
-    const int zero = 0;
-    e = cudaMemcpyToSymbolAsync(g_op_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st);
-    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
-  }
+  int norm = 0, int8 = 0;
+  cudaError_t e = norm_status(st, clear, &norm);
+  if (e == cudaSuccess) e = int8_status(st, clear, &int8);
   if (e != cudaSuccess) return -report_cuda(e, "operator status");
-  return v;
+  return norm ? norm : int8;
 }

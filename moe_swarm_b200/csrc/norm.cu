@@ -57,74 +57,18 @@ __device__ __forceinline__ void load_gate(const void* g, int type, int cols_vary
   }
 }
 
-// blockDim = (32 * warps, rows per CTA); a thread holds chunks threadIdx.x and
-// threadIdx.x + blockDim.x of its row.  Rows beyond the last run with no elements.
-template <class YT, class RT, bool VEC, int MAXT>
-__global__ void __launch_bounds__(MAXT, 1) norm_fwd_kernel(NormArgs a) {
-  __shared__ float buf[2][8 * 32];
-  pdl_wait();
-  pdl_launch_dependents();
-  const int row = blockIdx.x * blockDim.y + threadIdx.y;
-  const int cols = row < a.rows ? a.cols : 0;
-  float r[2][8];
-  int n[2], e0[2];
+// x = r * rstd * w of this thread's two chunks (w already holds pre_weight + off), stored in the
+// type asked for.  Whole half warps call it: a 128-column block is the 16 chunks of one.
+template <bool VEC>
+__device__ __forceinline__ void store_x(const NormArgs& a, int row, const int* e0, const int* n, float (&r)[2][8],
+                                        const float (&w)[2][8], float rstd) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    e0[i] = (threadIdx.x + i * blockDim.x) * 8;
-    n[i] = min(8, cols - e0[i]);
-  }
-  if (a.residual) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) load8<RT, VEC>(static_cast<const RT*>(a.residual) + row * a.r_ld + e0[i], n[i], r[i]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 16; ++j) r[j >> 3][j & 7] = 0.f;
-  }
-  if (a.y) {
-    float y[2][8];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) load8<YT, VEC>(static_cast<const YT*>(a.y) + row * a.y_ld + e0[i], n[i], y[i]);
-    if (a.post_w) {
-      float w[2][8];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) load8_dyn<VEC>(a.post_w, a.post_type, e0[i], n[i], w[i]);
-      float ss[1] = {0.f};
-#pragma unroll
-      for (int j = 0; j < 16; ++j) ss[0] += y[j >> 3][j & 7] * y[j >> 3][j & 7];
-      row_sum(ss, a.warps, buf[0]);
-      const float rstd = rsqrtf(ss[0] / a.cols + a.eps);
-#pragma unroll
-      for (int j = 0; j < 16; ++j) y[j >> 3][j & 7] *= rstd * (w[j >> 3][j & 7] + a.off);
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      float g[8];
-      load_gate<VEC>(a.gate, a.gate_type, a.gate_cols, row * a.g_ld, e0[i], n[i], g);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) r[i][j] += a.scale * (g[j] * y[i][j]);
-    }
-    if (a.residual_out) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) store8<RT, VEC>(static_cast<RT*>(a.residual_out) + row * a.ro_ld + e0[i], n[i], r[i]);
-    }
-  }
-  if (!a.pre_w) return;
-  float w[2][8];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) load8_dyn<VEC>(a.pre_w, a.pre_type, e0[i], n[i], w[i]);
-  float ss[1] = {0.f};
-#pragma unroll
-  for (int j = 0; j < 16; ++j) ss[0] += n[j >> 3] > (j & 7) ? r[j >> 3][j & 7] * r[j >> 3][j & 7] : 0.f;
-  row_sum(ss, a.warps, buf[1]);
-  const float rstd = rsqrtf(ss[0] / a.cols + a.eps);
-#pragma unroll
-  for (int j = 0; j < 16; ++j) r[j >> 3][j & 7] *= rstd * (w[j >> 3][j & 7] + a.off);
+  for (int j = 0; j < 16; ++j) r[j >> 3][j & 7] *= rstd * w[j >> 3][j & 7];
   if (a.x_type != MOE_B200_E4M3) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) store8_dyn<VEC>(a.x, a.x_type, row * a.x_ld + e0[i], n[i], r[i]);
     return;
   }
-  // a 128-column block is the 16 chunks of a half warp
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     float m = 0.f;
@@ -149,6 +93,201 @@ __global__ void __launch_bounds__(MAXT, 1) norm_fwd_kernel(NormArgs a) {
         if (j < n[i]) dst[j] = static_cast<uint8_t>(q[j >> 1] >> (8 * (j & 1)));
     }
   }
+}
+
+// One row per group of warps.  blockDim = (32 * warps, rows per CTA); a thread holds chunks
+// threadIdx.x and threadIdx.x + blockDim.x of its row.  Rows beyond the last run with no elements.
+template <class YT, class RT, bool VEC, int MAXT>
+__global__ void __launch_bounds__(MAXT, 1) norm_fwd_kernel(NormArgs a) {
+  __shared__ float buf[2][8 * 32];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int row = blockIdx.x * blockDim.y + threadIdx.y;
+  const int cols = row < a.rows ? a.cols : 0;
+  float r[2][8], w[2][8];
+  int n[2], e0[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    e0[i] = (threadIdx.x + i * blockDim.x) * 8;
+    n[i] = min(8, cols - e0[i]);
+  }
+  if (a.residual) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) load8<RT, VEC>(static_cast<const RT*>(a.residual) + row * a.r_ld + e0[i], n[i], r[i]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) r[j >> 3][j & 7] = 0.f;
+  }
+  if (a.y) {
+    float y[2][8];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) load8<YT, VEC>(static_cast<const YT*>(a.y) + row * a.y_ld + e0[i], n[i], y[i]);
+    if (a.post_w) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) load8_dyn<VEC>(a.post_w, a.post_type, e0[i], n[i], w[i]);
+      float ss[1] = {0.f};
+#pragma unroll
+      for (int j = 0; j < 16; ++j) ss[0] += y[j >> 3][j & 7] * y[j >> 3][j & 7];
+      row_sum(ss, a.warps, buf[0]);
+      const float rstd = rsqrtf(ss[0] / a.cols + a.eps);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) y[j >> 3][j & 7] *= rstd * (w[j >> 3][j & 7] + a.off);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float g[8];
+      load_gate<VEC>(a.gate, a.gate_type, a.gate_cols, row * a.g_ld, e0[i], n[i], g);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) r[i][j] += a.scale * (g[j] * y[i][j]);
+    }
+    if (a.residual_out) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) store8<RT, VEC>(static_cast<RT*>(a.residual_out) + row * a.ro_ld + e0[i], n[i], r[i]);
+    }
+  }
+  if (!a.pre_w) return;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) load8_dyn<VEC>(a.pre_w, a.pre_type, e0[i], n[i], w[i]);
+  float ss[1] = {0.f};
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    ss[0] += n[j >> 3] > (j & 7) ? r[j >> 3][j & 7] * r[j >> 3][j & 7] : 0.f;
+    w[j >> 3][j & 7] += a.off;
+  }
+  row_sum(ss, a.warps, buf[1]);
+  store_x<VEC>(a, row, e0, n, r, w, rsqrtf(ss[0] / a.cols + a.eps));
+}
+
+// Many rows: persistent CTAs, whose next rows (y | residual | gate per element) are on their way
+// to shared memory as bulk copies while a row is computed, so that the row's barriers and latencies
+// leave the memory busy.  Row tensors are 16-byte aligned; weights and a gate per column come
+// from L1.  A stage is refilled after the row's first barrier, when every thread holds its part.
+struct RingArgs {
+  int stages, y_bytes, r_bytes, g_bytes;   // bytes of a row of each tensor in a stage (0: not read)
+};
+constexpr int kRingMaxStages = 8;
+constexpr int kRingSmem = 200 * 1024;   // of an SM, shared by its CTAs
+
+template <class YT, class RT, bool POST>
+__global__ void __launch_bounds__(512, 2) norm_ring_kernel(NormArgs a, RingArgs g) {
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ float buf[3][32];   // sums of y^2; of r'^2 of even and odd rows
+  __shared__ uint64_t full[kRingMaxStages];
+  __shared__ int abort;
+  const int stage_bytes = g.y_bytes + g.r_bytes + g.g_bytes;
+  if (threadIdx.x == 0) {
+    abort = 0;
+    for (int i = 0; i < g.stages; ++i) mbar_init(&full[i], 1);
+    fence_mbar_init();
+  }
+  __syncthreads();
+  pdl_wait();
+  pdl_launch_dependents();
+  auto fetch = [&](int row, int stage) {   // one thread
+    uint8_t* dst = ring + stage * stage_bytes;
+    mbar_arrive_expect_tx(&full[stage], stage_bytes);
+    bulk_load(dst, static_cast<const YT*>(a.y) + row * a.y_ld, g.y_bytes, &full[stage]);
+    if (g.r_bytes)
+      bulk_load(dst + g.y_bytes, static_cast<const RT*>(a.residual) + row * a.r_ld, g.r_bytes, &full[stage]);
+    if (g.g_bytes)
+      bulk_load(dst + g.y_bytes + g.r_bytes,
+                static_cast<const uint8_t*>(a.gate) + row * a.g_ld * (g.g_bytes / a.cols), g.g_bytes, &full[stage]);
+  };
+  const int step = gridDim.x;
+  if (threadIdx.x == 0)
+    for (int i = 0; i < g.stages; ++i) {
+      const int64_t row = blockIdx.x + static_cast<int64_t>(i) * step;
+      if (row < a.rows) fetch(static_cast<int>(row), i);
+    }
+  int n[2], e0[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    e0[i] = (threadIdx.x + i * blockDim.x) * 8;
+    n[i] = min(8, a.cols - e0[i]);
+  }
+  const float inv_cols = 1.f / a.cols;
+  int stage = 0, parity = 0;
+  uint32_t phase = 0;
+  bool ok = true;
+  for (int row = blockIdx.x; row < a.rows; row += step) {
+    // after a wait that ran out the CTA still goes through its rows, without their contents
+    if (ok) ok = mbar_wait(&full[stage], phase, &abort, &g_op_status, kStWaitProducer);
+    const uint8_t* src = ring + stage * stage_bytes;
+    float r[2][8], y[2][8];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      load8<YT, true>(reinterpret_cast<const YT*>(src) + e0[i], n[i], y[i]);
+      if (g.r_bytes) load8<RT, true>(reinterpret_cast<const RT*>(src + g.y_bytes) + e0[i], n[i], r[i]);
+      else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) r[i][j] = 0.f;
+      }
+    }
+    float k = a.scale;
+    if (POST) {
+      float ss[1] = {0.f};
+#pragma unroll
+      for (int j = 0; j < 16; ++j) ss[0] += y[j >> 3][j & 7] * y[j >> 3][j & 7];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float pw[8];
+        load8_dyn<true>(a.post_w, a.post_type, e0[i], n[i], pw);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[i][j] *= pw[j] + a.off;
+      }
+      row_sum(ss, a.warps, buf[0]);
+      k *= rsqrtf(ss[0] * inv_cols + a.eps);
+    }
+    if (a.gate && !a.gate_cols) {
+      k *= load1_dyn(a.gate, a.gate_type, row * a.g_ld);
+    } else if (a.gate) {
+      const void* ge = g.g_bytes ? static_cast<const void*>(src + g.y_bytes + g.r_bytes) : a.gate;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float v[8];
+        load8_dyn<true>(ge, a.gate_type, e0[i], n[i], v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[i][j] *= v[j];
+      }
+    }
+    float ss[1] = {0.f};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float p = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        r[i][j] = fmaf(k, y[i][j], r[i][j]);
+        p = fmaf(r[i][j], r[i][j], p);
+      }
+      if (n[i] > 0) ss[0] += p;   // (k may be infinite)
+      store8<RT, true>(static_cast<RT*>(a.residual_out) + row * a.ro_ld + e0[i], n[i], r[i]);
+    }
+    float w[2][8];
+    if (a.pre_w) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        load8_dyn<true>(a.pre_w, a.pre_type, e0[i], n[i], w[i]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[i][j] += a.off;
+      }
+    }
+    row_sum(ss, a.warps, buf[1 + parity]);
+    parity ^= 1;
+    // every thread has its part of the stage (row_sum's barrier)
+    const int64_t next = row + static_cast<int64_t>(g.stages) * step;
+    if (threadIdx.x == 0 && ok && next < a.rows) fetch(static_cast<int>(next), stage);
+    if (ok && ++stage == g.stages) {
+      stage = 0;
+      phase ^= 1u;
+    }
+    if (a.pre_w) store_x<true>(a, row, e0, n, r, w, rsqrtf(ss[0] * inv_cols + a.eps));
+  }
+  if (!ok && threadIdx.x == 0)   // given up: the loads in flight land first
+    for (int i = 0; i < g.stages; ++i) {
+      int none = 0;
+      if (blockIdx.x + static_cast<int64_t>(i) * step < a.rows)
+        mbar_wait(&full[i], i >= stage ? phase : phase ^ 1u, &none, &g_op_status, kStWaitDrain);
+    }
 }
 
 // Persistent over rows; per-column sums stay in registers and go to `partial`, one slice per
@@ -335,6 +474,9 @@ bool type_pair_ok(int y, int r) { return is_float_type(y) && is_float_type(r) &&
 int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
 
 }  // namespace
+
+cudaError_t norm_status(cudaStream_t st, bool clear, int* v) { return take_status(st, clear, v); }
+
 }  // namespace moe
 
 extern "C" {
@@ -396,9 +538,30 @@ MOE_B200_API int moe_b200_block_norm(const moe_b200_norm_args* a, void* stream) 
                    (!a->gate_per_column || rows_aligned(a->gate, n.g_ld, a->gate_type)) &&
                    (a->x_type == MOE_B200_E4M3 ? (reinterpret_cast<uintptr_t>(a->x) & 7u) == 0 && n.x_ld % 8 == 0
                                                : rows_aligned(a->x, n.x_ld, a->x_type));
-  const dim3 block(n.warps * 32, rpc), grid((a->rows + rpc - 1) / rpc);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaSuccess;
+  // The ring: rows of two warps or more whose row tensors are 16-byte aligned, at least four per
+  // SM, and two or more of them in a CTA's share of shared memory.
+  RingArgs g{};
+  g.y_bytes = a->cols * type_bytes(a->y_type);
+  g.r_bytes = a->residual ? a->cols * type_bytes(a->residual_type) : 0;
+  g.g_bytes = a->gate && n.gate_cols && n.g_ld ? a->cols * type_bytes(a->gate_type) : 0;
+  const int stage_bytes = g.y_bytes + g.r_bytes + g.g_bytes;
+  const int ctas = n.warps >= 2 && n.warps <= 16 ? 32 / n.warps : 0;   // 1024 threads of an SM
+  g.stages = ctas ? kRingSmem / ctas / stage_bytes : 0;
+  if (g.stages > kRingMaxStages) g.stages = kRingMaxStages;
+  if (vec && a->y && a->rows >= 4 * sms && g.stages >= 2) {
+    const dim3 grid(a->rows < ctas * sms ? a->rows : ctas * sms), block(n.warps * 32);
+    const size_t smem = static_cast<size_t>(g.stages) * stage_bytes;
+    dispatch_norm(a->y_type, a->residual_type, true, 0, [&](auto yt, auto rt, auto, auto) {
+      auto kernel = a->post_weight ? norm_ring_kernel<decltype(yt), decltype(rt), true>
+                                   : norm_ring_kernel<decltype(yt), decltype(rt), false>;
+      e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem);
+      if (e == cudaSuccess) e = launch_pdl(kernel, grid, block, smem, st, n, g);
+    });
+    return e == cudaSuccess ? MOE_B200_OK : report_cuda(e, "block_norm launch");
+  }
+  const dim3 block(n.warps * 32, rpc), grid((a->rows + rpc - 1) / rpc);
   dispatch_norm(a->y_type, a->residual_type, vec, block.x * block.y, [&](auto yt, auto rt, auto v, auto t) {
     e = launch_pdl(norm_fwd_kernel<decltype(yt), decltype(rt), decltype(v)::value, decltype(t)::value>, grid, block, 0,
                    st, n);

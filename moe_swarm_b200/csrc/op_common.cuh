@@ -29,6 +29,22 @@ inline bool rows_aligned(const void* p, int64_t stride, int type) {
   return !p || (aligned16(p) && (stride * type_bytes(type)) % 16 == 0);
 }
 
+// First bounded wait of this file's kernels that ran out (0: none); one word per source file.
+static __device__ int g_op_status;
+// Reads (and with `clear` resets) it, synchronising the stream.
+static inline cudaError_t take_status(cudaStream_t st, bool clear, int* v) {
+  cudaError_t e = cudaMemcpyFromSymbolAsync(v, g_op_status, sizeof(int), 0, cudaMemcpyDeviceToHost, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  if (e == cudaSuccess && clear && *v) {
+    const int zero = 0;
+    e = cudaMemcpyToSymbolAsync(g_op_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  }
+  return e;
+}
+cudaError_t norm_status(cudaStream_t st, bool clear, int* v);   // norm.cu
+cudaError_t int8_status(cudaStream_t st, bool clear, int* v);   // int8_gemm.cu
+
 using bf16 = __nv_bfloat16;
 using fp16 = __half;
 
@@ -122,6 +138,14 @@ __device__ __forceinline__ float load1_dyn(const void* p, int type, int64_t off)
   if (type == MOE_B200_BF16) return to_f(static_cast<const bf16*>(p)[off]);
   if (type == MOE_B200_FP16) return to_f(static_cast<const fp16*>(p)[off]);
   return static_cast<const float*>(p)[off];
+}
+
+// Starts a copy of `bytes` (a multiple of 16, both addresses 16-byte aligned) from global to this
+// CTA's shared memory, completing on `bar`.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
 }
 
 // max that keeps a NaN

@@ -14,6 +14,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -21,8 +22,8 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libmoe_b200.so"
 TRACE_LIB = PKG / "libmoe_b200_trace.so"   # MOE_TRACE build: per-CTA role counters
-SOURCES = ["route.cu", "wide.cu", "stream.cu", "combine.cu", "ep.cu", "norm.cu", "select.cu", "int8.cu", "int8_gemm.cu", "capi.cu"]
-HEADERS = ["ptx.cuh", "moe_internal.cuh", "launch_args.cuh", "sched.cuh", "exp64.cuh", "op_common.cuh", "int8_gemm.cuh"]
+SOURCES = ["route.cu", "wide.cu", "stream.cu", "combine.cu", "ep.cu", "norm.cu", "norm_bwd.cu", "select.cu", "int8.cu", "int8_gemm.cu", "capi.cu"]
+HEADERS = ["ptx.cuh", "moe_internal.cuh", "launch_args.cuh", "sched.cuh", "exp64.cuh", "op_common.cuh", "norm_common.cuh", "int8_gemm.cuh"]
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC",
@@ -51,10 +52,10 @@ def build(verbose: bool = False, force: bool = False, ptxas_verbose: bool = Fals
     lib = TRACE_LIB if trace else LIB
     if not force and not trace and not needs_build():
         return LIB
-    objs = []
     build_dir = PKG / ("_build_trace" if trace else "_build")
     build_dir.mkdir(exist_ok=True)
-    for src in SOURCES:
+
+    def compile_one(src):
         obj = build_dir / (Path(src).stem + ".o")
         cmd = [nvcc(), *ARCH_FLAGS, *FLAGS, "-I", str(ROOT / "include"), "-c", str(CSRC / src), "-o", str(obj)]
         if trace:
@@ -64,7 +65,10 @@ def build(verbose: bool = False, force: bool = False, ptxas_verbose: bool = Fals
         if verbose:
             print(" ".join(cmd), flush=True)
         subprocess.run(cmd, check=True)
-        objs.append(str(obj))
+        return str(obj)
+
+    with ThreadPoolExecutor(max_workers=os.cpu_count() or 1) as pool:
+        objs = list(pool.map(compile_one, SOURCES))
     tmp = lib.with_suffix(".so.tmp")
     cmd = [nvcc(), *ARCH_FLAGS, "-shared", "-Xcompiler", "-fPIC", "-o", str(tmp), *objs]
     if verbose:

@@ -1,0 +1,477 @@
+// Gradients of the norms around a block (norm.cu), from dx of x and dr of r'.
+//
+//   G   = dr + s(r') (w dx - r^ mean(w dx r^)),  r^ = r' s(r')      gradient of the residual
+//   dw  = sum over rows of dx r^
+//   b   = (post_weight + off) * gate per column (1 where absent)
+//   dy  = scale gate s(y) (b G - y^ mean(b G y^)),  y^ = y s(y)     (scale gate b G without post_weight)
+//   dpost = scale gate sum over rows of G y^;  dgate = scale G y^ (post_weight + off), summed over what
+//   the gate is broadcast over.  A gate per column is a constant of the sum over rows, so one sum
+//   P = sum of G y^ serves dpost and dgate.
+//
+// s(r') and s(y) are computed again from the rows, whose elements stay in registers between the
+// row's sums.  Per-column sums are held in registers over a persistent CTA's rows (32-bit, fixed
+// order), written once per CTA and added up by norm_sum_kernel.
+#include "norm_common.cuh"
+
+namespace moe {
+
+enum : int { kGateNone = 0, kGateColumn = 1, kGateRow = 2, kGateElement = 3 };
+
+struct NormBwdArgs {
+  const void *dx, *dr, *r, *y, *post_w, *pre_w, *gate;
+  void *dres, *dy, *dgate;          // dgate: per element (gate type) or per row (fp32); null: none
+  float* partial;                   // [slots][parts][cols]: sums of dx r^ and of G y^
+  int64_t dx_ld, dr_ld, r_ld, y_ld, g_ld, dres_ld, dy_ld, dg_ld;
+  int rows, cols, warps, parts, vec;
+  int post_type, pre_type, gate_type, gate_cols;
+  int gate_grad, pre_slot, post_slot;
+  float scale, eps, off;
+};
+
+// What a row's computation keeps from row to row.
+struct NormBwdSums {
+  Row16 pre, post;
+};
+
+// One row whose tensors are loaded by `load(which, Row16&)`: 0 dx, 1 r, 2 y, 3 dr, 4 the gate.
+// POST, GATE (0 none or per column, 1 per row, 2 per element): -1 = known at run time only.
+template <class YT, class RT, bool VEC, int POST, int GATE, class Load>
+__device__ __forceinline__ void bwd_row(const NormBwdArgs& a, int row, int cols, float inv_cols, float* buf0, float* buf1,
+                                        NormBwdSums& sum, Load&& load) {
+  const bool post = POST < 0 ? a.post_w != nullptr : POST == 1;
+  const int gate = GATE < 0 ? (a.gate_grad == kGateElement ? 2 : a.gate_grad == kGateRow ? 1 : 0) : GATE;
+  const bool has_dx = GATE < 0 ? a.dx != nullptr : true, has_y = GATE < 0 ? a.y != nullptr : true;
+  Row16 r, dx, y, G;
+  float s[3] = {0.f, 0.f, 0.f};   // sum r'^2, sum w dx r', sum y^2
+  if (has_dx) {
+    load(1, r);
+    load(0, dx);
+    load_weight<VEC>(a.pre_w, a.pre_type, a.off, cols, G);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) G.v[i] = mul2(G.v[i], dx.v[i]);
+    s[0] = dot16(r, r);
+    s[1] = dot16(G, r);
+  }
+  if (has_y) {
+    load(2, y);
+    if (post) s[2] = dot16(y, y);
+  }
+  row_sum(s, a.warps, buf0);
+  // (rows beyond the last, which share a CTA with others, must leave the sums alone)
+  const float rstd = cols ? rsqrtf(s[0] * inv_cols + a.eps) : 0.f;
+  {
+    Row16 d;
+    if (a.dr) {
+      load(3, d);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) d.v[i] = dup2(0.f);
+    }
+    if (has_dx) {
+      const float k = -s[1] * inv_cols * rstd * rstd;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        sum.pre.v[i] = fma2(mul2(dx.v[i], r.v[i]), dup2(rstd), sum.pre.v[i]);
+        G.v[i] = fma2(dup2(rstd), fma2(r.v[i], dup2(k), G.v[i]), d.v[i]);
+      }
+    } else {
+      G = d;
+    }
+  }
+  if (a.dres) store_row<RT, VEC>(static_cast<RT*>(a.dres) + row * a.dres_ld, cols, G);
+  if (!has_y) return;
+  const float ystd = post ? (cols ? rsqrtf(s[2] * inv_cols + a.eps) : 0.f) : 1.f;
+  const float g_row = gate == 1 && cols ? load1_dyn(a.gate, a.gate_type, row * a.g_ld) : 1.f;
+  Row16 b;   // (post_weight + off) * gate per column
+  if (post) {
+    load_weight<VEC>(a.post_w, a.post_type, a.off, cols, b);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) b.v[i] = dup2(1.f);
+  }
+  const float q = g_row * ystd;
+  float t[1] = {0.f};   // sum of b G y
+  if (gate == 2) {
+    Row16 ge, dg;
+    load(4, ge);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float2 gy = mul2(G.v[i], y.v[i]);
+      sum.post.v[i] = fma2(mul2(gy, ge.v[i]), dup2(q), sum.post.v[i]);
+      dg.v[i] = mul2(mul2(gy, b.v[i]), dup2(a.scale * ystd));
+      G.v[i] = mul2(mul2(G.v[i], b.v[i]), ge.v[i]);
+    }
+    store_row_dyn<VEC>(a.dgate, a.gate_type, row * a.dg_ld, cols, dg);
+  } else {
+    if (gate == 0 && a.gate) {
+      Row16 gc;
+      load_row_dyn<VEC>(a.gate, a.gate_type, 0, cols, gc);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) b.v[i] = mul2(b.v[i], gc.v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      sum.post.v[i] = fma2(mul2(G.v[i], y.v[i]), dup2(q), sum.post.v[i]);
+      G.v[i] = mul2(G.v[i], b.v[i]);
+    }
+  }
+  float k = 0.f;
+  if (post || gate == 1) {
+    t[0] = dot16(G, y);
+    row_sum(t, a.warps, buf1);
+    if (gate == 1 && threadIdx.x == 0 && cols) static_cast<float*>(a.dgate)[row] = a.scale * ystd * t[0];
+    if (post) k = -t[0] * inv_cols * ystd * ystd;
+  }
+  if (!a.dy) return;
+  const float m = a.scale * q;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) G.v[i] = mul2(post ? fma2(y.v[i], dup2(k), G.v[i]) : G.v[i], dup2(m));
+  store_row<YT, VEC>(static_cast<YT*>(a.dy) + row * a.dy_ld, cols, G);
+}
+
+template <bool VEC>
+__device__ __forceinline__ void bwd_store_sums(const NormBwdArgs& a, int part, const NormBwdSums& sum) {
+  float* dst = a.partial + static_cast<int64_t>(part) * a.cols;
+  const int64_t slot = static_cast<int64_t>(a.parts) * a.cols;
+  if (a.pre_slot >= 0) store_row<float, VEC>(dst + a.pre_slot * slot, a.cols, sum.pre);
+  if (a.post_slot >= 0) store_row<float, VEC>(dst + a.post_slot * slot, a.cols, sum.post);
+}
+
+// Any alignment, any set of tensors: rows straight from global memory.  blockDim = (32 * warps,
+// rows per CTA); CTAs go through the rows in steps of the grid.
+template <class YT, class RT, bool VEC>
+__device__ __forceinline__ void bwd_direct(const NormBwdArgs& a, float (*buf)[8 * 3 * 32]) {
+  NormBwdSums sum;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sum.pre.v[i] = sum.post.v[i] = dup2(0.f);
+  const int step = gridDim.x * blockDim.y;
+  for (int row0 = blockIdx.x * blockDim.y; row0 < a.rows; row0 += step) {
+    const int row = row0 + threadIdx.y;
+    const int cols = row < a.rows ? a.cols : 0;
+    // a row without a second sum alternates the first one's buffer by itself
+    const bool two = a.y && (a.post_w || a.gate_grad == kGateRow);
+    const int first = two ? 0 : (row0 / step) & 1;
+    bwd_row<YT, RT, VEC, -1, -1>(a, row, cols, 1.f / a.cols, buf[first], buf[1], sum, [&](int which, Row16& v) {
+      if (which == 0) load_row<YT, VEC>(static_cast<const YT*>(a.dx) + row * a.dx_ld, cols, v);
+      else if (which == 1) load_row<RT, VEC>(static_cast<const RT*>(a.r) + row * a.r_ld, cols, v);
+      else if (which == 2) load_row<YT, VEC>(static_cast<const YT*>(a.y) + row * a.y_ld, cols, v);
+      else if (which == 3) load_row<RT, VEC>(static_cast<const RT*>(a.dr) + row * a.dr_ld, cols, v);
+      else load_row_dyn<VEC>(a.gate, a.gate_type, row * a.g_ld, cols, v);
+    });
+  }
+  bwd_store_sums<VEC>(a, blockIdx.x * blockDim.y + threadIdx.y, sum);
+}
+
+template <class YT, class RT, int MAXT>
+__global__ void __launch_bounds__(MAXT, 1) norm_bwd_kernel(NormBwdArgs a) {
+  __shared__ float buf[2][8 * 3 * 32];
+  pdl_wait();
+  pdl_launch_dependents();
+  if (a.vec) bwd_direct<YT, RT, true>(a, buf);
+  else bwd_direct<YT, RT, false>(a, buf);
+}
+
+// Aligned rows with all of dx, r', y: the next rows (dx | r' | y | dr | gate per element) are on
+// their way to shared memory as bulk copies while a row is computed.
+struct RingBwdArgs {
+  int stages, y_bytes, r_bytes, dr_bytes, g_bytes;   // bytes of a row of each (dx has y's type)
+};
+
+template <class YT, class RT, bool POST, int GATE>
+__global__ void __launch_bounds__(512, 1) norm_bwd_ring_kernel(NormBwdArgs a, RingBwdArgs g) {
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ float buf[2][3 * 32];
+  __shared__ uint64_t full[kRingMaxStages];
+  __shared__ int abort;
+  const int at_r = g.y_bytes, at_y = at_r + g.r_bytes, at_dr = at_y + g.y_bytes, at_g = at_dr + g.dr_bytes;
+  const int stage_bytes = at_g + g.g_bytes;
+  if (threadIdx.x == 0) {
+    abort = 0;
+    for (int i = 0; i < g.stages; ++i) mbar_init(&full[i], 1);
+    fence_mbar_init();
+  }
+  __syncthreads();
+  pdl_wait();
+  pdl_launch_dependents();
+  auto fetch = [&](int row, int stage) {   // one thread
+    uint8_t* dst = ring + stage * stage_bytes;
+    uint64_t* bar = &full[stage];
+    mbar_arrive_expect_tx(bar, stage_bytes);
+    bulk_load(dst, static_cast<const YT*>(a.dx) + row * a.dx_ld, g.y_bytes, bar);
+    bulk_load(dst + at_r, static_cast<const RT*>(a.r) + row * a.r_ld, g.r_bytes, bar);
+    bulk_load(dst + at_y, static_cast<const YT*>(a.y) + row * a.y_ld, g.y_bytes, bar);
+    if (g.dr_bytes) bulk_load(dst + at_dr, static_cast<const RT*>(a.dr) + row * a.dr_ld, g.dr_bytes, bar);
+    if (GATE == 2)
+      bulk_load(dst + at_g, static_cast<const uint8_t*>(a.gate) + row * a.g_ld * (g.g_bytes / a.cols), g.g_bytes, bar);
+  };
+  const int step = gridDim.x, cols = a.cols;
+  if (threadIdx.x == 0)
+    for (int i = 0; i < g.stages; ++i) {
+      const int64_t row = blockIdx.x + static_cast<int64_t>(i) * step;
+      if (row < a.rows) fetch(static_cast<int>(row), i);
+    }
+  NormBwdSums sum;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sum.pre.v[i] = sum.post.v[i] = dup2(0.f);
+  const float inv_cols = 1.f / cols;
+  int stage = 0, parity = 0;
+  uint32_t phase = 0;
+  bool ok = true;
+  for (int row = blockIdx.x; row < a.rows; row += step) {
+    // after a wait that ran out the CTA still goes through its rows, without their contents
+    if (ok) ok = mbar_wait(&full[stage], phase, &abort, &g_op_status, kStWaitProducer);
+    const uint8_t* src = ring + stage * stage_bytes;
+    constexpr bool two = POST || GATE == 1;   // a second sum over the row
+    bwd_row<YT, RT, true, POST ? 1 : 0, GATE>(
+        a, row, cols, inv_cols, buf[two ? 0 : parity], buf[1], sum, [&](int which, Row16& v) {
+          if (which == 0) load_row<YT, true>(reinterpret_cast<const YT*>(src), cols, v);
+          else if (which == 1) load_row<RT, true>(reinterpret_cast<const RT*>(src + at_r), cols, v);
+          else if (which == 2) load_row<YT, true>(reinterpret_cast<const YT*>(src + at_y), cols, v);
+          else if (which == 3) load_row<RT, true>(reinterpret_cast<const RT*>(src + at_dr), cols, v);
+          else load_row_dyn<true>(src + at_g, a.gate_type, 0, cols, v);
+        });
+    parity ^= 1;
+    // every thread has read the stage: the second sum's barrier, or one more
+    if (!two) __syncthreads();
+    const int64_t next = row + static_cast<int64_t>(g.stages) * step;
+    if (threadIdx.x == 0 && ok && next < a.rows) fetch(static_cast<int>(next), stage);
+    if (ok && ++stage == g.stages) {
+      stage = 0;
+      phase ^= 1u;
+    }
+  }
+  bwd_store_sums<true>(a, blockIdx.x, sum);
+  if (!ok && threadIdx.x == 0)   // given up: the loads in flight land first
+    for (int i = 0; i < g.stages; ++i) {
+      int none = 0;
+      if (blockIdx.x + static_cast<int64_t>(i) * step < a.rows)
+        mbar_wait(&full[i], i >= stage ? phase : phase ^ 1u, &none, &g_op_status, kStWaitDrain);
+    }
+}
+
+// Adds up the parts of a column, 32 columns per CTA, eight warps over the parts, their sums in
+// warp order.  blockIdx.y selects the sum: that of dx r^ is dpre_weight; that of G y^ gives
+// dpost_weight and the gradient of a gate per column.
+struct NormSumArgs {
+  const float* partial;
+  float *pre, *post, *gate;
+  const void *post_w, *chan;   // chan: the gate per column
+  int parts, cols, pre_slot, post_type, chan_type;
+  float scale, off;
+};
+__global__ void __launch_bounds__(256) norm_sum_kernel(NormSumArgs a) {
+  __shared__ float buf[8][32];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int c = blockIdx.x * 32 + threadIdx.x;
+  const float* p = a.partial + static_cast<int64_t>(blockIdx.y) * a.parts * a.cols + c;
+  float s = 0.f;
+  if (c < a.cols)
+    for (int i = threadIdx.y; i < a.parts; i += 8) s += p[static_cast<int64_t>(i) * a.cols];
+  buf[threadIdx.y][threadIdx.x] = s;
+  __syncthreads();
+  if (threadIdx.y != 0 || c >= a.cols) return;
+#pragma unroll
+  for (int w = 1; w < 8; ++w) s += buf[w][threadIdx.x];
+  if (static_cast<int>(blockIdx.y) == a.pre_slot) {
+    a.pre[c] = s;
+    return;
+  }
+  const float k = a.scale * s;
+  if (a.post) a.post[c] = a.chan ? k * load1_dyn(a.chan, a.chan_type, c) : k;
+  if (a.gate) a.gate[c] = a.post_w ? k * (load1_dyn(a.post_w, a.post_type, c) + a.off) : k;
+}
+
+// One value from `rows` of them (the gradient of a gate that is one number).
+__global__ void __launch_bounds__(1024) norm_total_kernel(const float* v, int rows, float* out) {
+  __shared__ float buf[32];
+  pdl_wait();
+  pdl_launch_dependents();
+  float s[1] = {0.f};
+  for (int i = threadIdx.x; i < rows; i += 1024) s[0] += v[i];
+  row_sum(s, 32, buf);
+  if (threadIdx.x == 0) *out = s[0];
+}
+
+namespace {
+
+// CTAs and with them the parts of the column sums, from the sizes alone (the workspace's size
+// goes by them): of 148 SMs, each with 512 threads' worth of registers.
+struct NormBwdShape {
+  int warps, rows_per_cta, direct_parts, ring_ctas, ring_parts;
+};
+NormBwdShape bwd_shape(int rows, int cols) {
+  NormBwdShape s{};
+  norm_shape(cols, &s.warps, &s.rows_per_cta);
+  const int need = (rows + s.rows_per_cta - 1) / s.rows_per_cta;
+  const int most = 148 * (s.warps > 8 ? 1 : 2);
+  s.direct_parts = (need < most ? need : most) * s.rows_per_cta;
+  if (s.warps >= 2 && s.warps <= 16) {
+    s.ring_ctas = 16 / s.warps;
+    s.ring_parts = rows < 148 * s.ring_ctas ? rows : 148 * s.ring_ctas;
+  }
+  return s;
+}
+
+int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
+
+}  // namespace
+
+cudaError_t norm_bwd_status(cudaStream_t st, bool clear, int* v) { return take_status(st, clear, v); }
+
+}  // namespace moe
+
+extern "C" {
+
+MOE_B200_API size_t moe_b200_block_norm_backward_workspace_size(int32_t rows, int32_t cols) {
+  using namespace moe;
+  if (rows < 0 || cols < 1 || cols > kNormMaxCols) return 0;
+  const NormBwdShape shape = bwd_shape(rows, cols);
+  const int parts = shape.direct_parts > shape.ring_parts ? shape.direct_parts : shape.ring_parts;
+  return static_cast<size_t>(align256(static_cast<int64_t>(2) * parts * cols * 4) + align256(static_cast<int64_t>(rows) * 4) +
+                             256);
+}
+
+MOE_B200_API int moe_b200_block_norm_backward(const moe_b200_norm_backward_args* a, void* workspace,
+                                              size_t workspace_bytes, void* stream) {
+  using namespace moe;
+  if (!a) return report_error(MOE_B200_ERR_ARG, "null args");
+  if (a->rows < 0 || a->cols < 1 || a->cols > kNormMaxCols)
+    return report_error(MOE_B200_ERR_ARG, "block_norm_backward: rows must be >= 0 and cols in [1, 16384]");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // what the gate varies over: columns only, rows only, both, neither
+  const bool g_rows = a->gate_row_stride != 0, g_cols = a->gate_per_column;
+  cudaError_t e = cudaSuccess;
+  if (a->rows == 0) {   // sums over no rows
+    if (a->dpre_weight) e = cudaMemsetAsync(a->dpre_weight, 0, sizeof(float) * a->cols, st);
+    if (e == cudaSuccess && a->dpost_weight) e = cudaMemsetAsync(a->dpost_weight, 0, sizeof(float) * a->cols, st);
+    if (e == cudaSuccess && a->dgate && !g_rows)
+      e = cudaMemsetAsync(a->dgate, 0, sizeof(float) * (g_cols ? a->cols : 1), st);
+    return e == cudaSuccess ? MOE_B200_OK : report_cuda(e, "cudaMemsetAsync");
+  }
+  if (!type_pair_ok(a->y_type, a->residual_type))
+    return report_error(MOE_B200_ERR_ARG, "block_norm_backward: the residual has y's type or fp32");
+  if (!a->dx && !a->dresidual) return report_error(MOE_B200_ERR_ARG, "block_norm_backward: dx or dresidual is required");
+  if (a->dx && (!a->residual || !a->pre_weight || !a->dpre_weight || !is_float_type(a->pre_weight_type)))
+    return report_error(MOE_B200_ERR_ARG, "block_norm_backward: dx needs residual, pre_weight and dpre_weight");
+  if (!a->y && (a->post_weight || a->gate || a->dy))
+    return report_error(MOE_B200_ERR_ARG, "block_norm_backward: post_weight, gate and dy need y");
+  if (a->post_weight && (!a->dpost_weight || !is_float_type(a->post_weight_type)))
+    return report_error(MOE_B200_ERR_ARG, "block_norm_backward: post_weight needs dpost_weight");
+  if (a->gate && (!a->dgate || !is_float_type(a->gate_type)))
+    return report_error(MOE_B200_ERR_ARG, "block_norm_backward: gate needs dgate");
+  if (!workspace || workspace_bytes < moe_b200_block_norm_backward_workspace_size(a->rows, a->cols))
+    return report_error(MOE_B200_ERR_WORKSPACE, "block_norm_backward: workspace too small");
+  if (reinterpret_cast<uintptr_t>(workspace) & 255u)
+    return report_error(MOE_B200_ERR_ARG, "workspace must be 256-byte aligned");
+  int sms = 0;
+  if (int rc = op_device(&sms)) return rc;
+  NormBwdArgs n{};
+  n.dx = a->dx;
+  n.dr = a->dresidual;
+  n.r = a->dx ? a->residual : nullptr;
+  n.y = a->y;
+  n.post_w = a->post_weight;
+  n.pre_w = a->pre_weight;
+  n.gate = a->gate;
+  n.dres = a->dresidual_in;
+  n.dy = a->dy;
+  n.dx_ld = a->dx_stride;
+  n.dr_ld = a->dresidual_stride;
+  n.r_ld = a->residual_stride;
+  n.y_ld = a->y_stride;
+  n.g_ld = a->gate_row_stride;
+  n.dres_ld = a->dresidual_in_stride;
+  n.dy_ld = a->dy_stride;
+  n.dg_ld = a->dgate_stride;
+  if (a->rows == 1) n.dx_ld = n.dr_ld = n.r_ld = n.y_ld = n.g_ld = n.dres_ld = n.dy_ld = n.dg_ld = 0;
+  n.rows = a->rows;
+  n.cols = a->cols;
+  n.post_type = a->post_weight_type;
+  n.pre_type = a->pre_weight_type;
+  n.gate_type = a->gate_type;
+  n.gate_cols = a->gate_per_column;
+  n.scale = a->scale;
+  n.eps = a->eps;
+  n.off = a->weight_offset;
+  n.partial = static_cast<float*>(workspace);
+  n.gate_grad = !a->gate ? kGateNone : g_rows && g_cols ? kGateElement : g_cols ? kGateColumn : kGateRow;
+  NormSumArgs s{};
+  int sums = 0;
+  n.pre_slot = n.post_slot = -1;
+  if (a->dx) {
+    n.pre_slot = sums;
+    s.pre = a->dpre_weight;
+    ++sums;
+  }
+  if (a->post_weight || n.gate_grad == kGateColumn) {
+    n.post_slot = sums;
+    s.post = a->post_weight ? a->dpost_weight : nullptr;
+    s.gate = n.gate_grad == kGateColumn ? static_cast<float*>(a->dgate) : nullptr;
+    ++sums;
+  }
+  const bool vec = a->cols % 8 == 0 && rows_aligned(a->y, n.y_ld, a->y_type) &&
+                   rows_aligned(a->dx, n.dx_ld, a->y_type) && rows_aligned(a->dresidual, n.dr_ld, a->residual_type) &&
+                   rows_aligned(n.r, n.r_ld, a->residual_type) &&
+                   rows_aligned(a->dresidual_in, n.dres_ld, a->residual_type) &&
+                   rows_aligned(a->dy, n.dy_ld, a->y_type) && aligned16(a->post_weight) && aligned16(a->pre_weight) &&
+                   (!g_cols || rows_aligned(a->gate, n.g_ld, a->gate_type)) &&
+                   (n.gate_grad != kGateElement || rows_aligned(a->dgate, n.dg_ld, a->gate_type));
+  const NormBwdShape shape = bwd_shape(a->rows, a->cols);
+  n.warps = shape.warps;
+  RingBwdArgs g{};
+  g.y_bytes = a->cols * type_bytes(a->y_type);
+  g.r_bytes = a->cols * type_bytes(a->residual_type);
+  g.dr_bytes = a->dresidual ? g.r_bytes : 0;
+  g.g_bytes = n.gate_grad == kGateElement ? a->cols * type_bytes(a->gate_type) : 0;
+  const int stage_bytes = 2 * g.y_bytes + g.r_bytes + g.dr_bytes + g.g_bytes;
+  g.stages = shape.ring_ctas ? kRingSmem / shape.ring_ctas / stage_bytes : 0;
+  if (g.stages > kRingMaxStages) g.stages = kRingMaxStages;
+  const bool ring = vec && a->dx && a->y && g.stages >= 2;
+  n.parts = ring ? shape.ring_parts : shape.direct_parts;
+  // the row sums of a gate that is one number go through the workspace
+  float* row_dots = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) +
+                                             align256(static_cast<int64_t>(2) * n.parts * a->cols * 4));
+  n.dgate = n.gate_grad == kGateElement ? a->dgate : n.gate_grad == kGateRow ? (g_rows ? a->dgate : row_dots) : nullptr;
+  dispatch_types(a->y_type, a->residual_type, [&](auto yt, auto rt) {
+    using YT = decltype(yt);
+    using RT = decltype(rt);
+    if (ring) {
+      const bool post = a->post_weight != nullptr;
+      auto kernel = n.gate_grad == kGateElement ? (post ? norm_bwd_ring_kernel<YT, RT, true, 2> : norm_bwd_ring_kernel<YT, RT, false, 2>)
+                    : n.gate_grad == kGateRow   ? (post ? norm_bwd_ring_kernel<YT, RT, true, 1> : norm_bwd_ring_kernel<YT, RT, false, 1>)
+                                                : (post ? norm_bwd_ring_kernel<YT, RT, true, 0> : norm_bwd_ring_kernel<YT, RT, false, 0>);
+      e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem);
+      if (e == cudaSuccess)
+        e = launch_pdl(kernel, dim3(n.parts), dim3(n.warps * 32), static_cast<size_t>(g.stages) * stage_bytes, st, n, g);
+    } else {
+      const dim3 block(n.warps * 32, shape.rows_per_cta), grid(n.parts / shape.rows_per_cta);
+      n.vec = vec;
+      auto kernel = block.x * block.y <= 512 ? norm_bwd_kernel<YT, RT, 512> : norm_bwd_kernel<YT, RT, 1024>;
+      e = launch_pdl(kernel, grid, block, 0, st, n);
+    }
+  });
+  if (e != cudaSuccess) return report_cuda(e, "block_norm_backward launch");
+  if (sums) {
+    s.partial = n.partial;
+    s.parts = n.parts;
+    s.cols = a->cols;
+    s.pre_slot = n.pre_slot;
+    s.post_w = a->post_weight;
+    s.post_type = a->post_weight_type;
+    s.chan = n.gate_grad == kGateColumn ? a->gate : nullptr;
+    s.chan_type = a->gate_type;
+    s.scale = a->scale;
+    s.off = a->weight_offset;
+    e = launch_pdl(norm_sum_kernel, dim3((a->cols + 31) / 32, sums), dim3(32, 8), 0, st, s);
+    if (e != cudaSuccess) return report_cuda(e, "block_norm_backward sum launch");
+  }
+  if (n.gate_grad == kGateRow && !g_rows) {
+    e = launch_pdl(norm_total_kernel, dim3(1), dim3(1024), 0, st, static_cast<const float*>(row_dots), a->rows,
+                   static_cast<float*>(a->dgate));
+    if (e != cudaSuccess) return report_cuda(e, "block_norm_backward total launch");
+  }
+  return MOE_B200_OK;
+}
+
+}  // extern "C"

@@ -42,8 +42,9 @@ static inline cudaError_t take_status(cudaStream_t st, bool clear, int* v) {
   }
   return e;
 }
-cudaError_t norm_status(cudaStream_t st, bool clear, int* v);   // norm.cu
-cudaError_t int8_status(cudaStream_t st, bool clear, int* v);   // int8_gemm.cu
+cudaError_t norm_status(cudaStream_t st, bool clear, int* v);       // norm.cu and norm_bwd.cu
+cudaError_t norm_bwd_status(cudaStream_t st, bool clear, int* v);
+cudaError_t int8_status(cudaStream_t st, bool clear, int* v);       // int8_gemm.cu
 
 using bf16 = __nv_bfloat16;
 using fp16 = __half;

@@ -26,48 +26,73 @@ struct NormArgs {
 };
 
 // x = r * rstd * w of this thread's elements, stored in the type asked for.  Whole warps call it:
-// a 128-column block's maximum is a shuffle over its half warp (VEC) or warp.
-template <bool VEC>
+// a 128-column block's maximum is a shuffle over its half warp (eight elements each, two blocks in
+// a thread) or warp (four each, four blocks).
+template <int LAY>
 __device__ __forceinline__ void store_x(const NormArgs& a, int row, int cols, Row16& r, const Row16& w, float rstd) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) r.v[i] = mul2(mul2(r.v[i], dup2(rstd)), w.v[i]);
   if (a.x_type != MOE_B200_E4M3) {
-    store_row_dyn<VEC>(a.x, a.x_type, row * a.x_ld, cols, r);
+    store_row_dyn<LAY>(a.x, a.x_type, row * a.x_ld, cols, r);
     return;
   }
-  constexpr int PER = VEC ? 8 : 4;   // this thread's elements of one block
+  uint8_t* dst = static_cast<uint8_t*>(a.x) + row * a.x_ld;
+  auto scale_of = [](float m) { return max_nan(m, 1e-12f) * (1.f / 448.f); };
+  if constexpr (LAY == kScattered) {
 #pragma unroll
-  for (int i = 0; i < 16; i += PER) {
-    float m = 0.f;
+    for (int i = 0; i < 16; i += 4) {
+      float m = 0.f;
 #pragma unroll
-    for (int j = i; j < i + PER; ++j)
-      if (col_of<VEC>(VEC ? i : j) < cols) m = max_nan(m, fabsf(r[j]));
+      for (int j = i; j < i + 4; ++j)
+        if (exists<LAY>(j, cols)) m = max_nan(m, fabsf(r[j]));
 #pragma unroll
-    for (int d = VEC ? 8 : 16; d >= 1; d >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
-    const int e0 = col_of<VEC>(i);
-    const float sc = max_nan(m, 1e-12f) / 448.f;
+      for (int d = 16; d >= 1; d >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
+      const float sc = scale_of(m), inv = __frcp_rn(sc);
+      const int e0 = col_of<LAY>(i) & ~127;
+      if ((threadIdx.x & 31) == 0 && e0 < cols) a.x_scale[static_cast<int64_t>(e0 >> 7) * a.rows + row] = sc;
+#pragma unroll
+      for (int j = i; j < i + 4; ++j)
+        if (exists<LAY>(j, cols)) dst[col_of<LAY>(j)] = static_cast<uint8_t>(cvt_e4m3x2(r[j] * inv, 0.f));
+    }
+  } else {
+    float m[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      m[i] = fabsf(r[8 * i]);
+#pragma unroll
+      for (int j = 1; j < 8; ++j) m[i] = max_nan(m[i], fabsf(r[8 * i + j]));
+      if (!exists<LAY>(8 * i, cols)) m[i] = 0.f;
+    }
+    // both maxima in one butterfly: the lower eight lanes of a half warp go on with the first
+    // block's, the upper with the second's
+    const bool upper = threadIdx.x & 8;
+    const float mine = upper ? m[1] : m[0];
+    float v = max_nan(mine, __shfl_xor_sync(0xffffffffu, upper ? m[0] : m[1], 8));
+#pragma unroll
+    for (int d = 4; d >= 1; d >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, d));
+    const float sc = scale_of(v);
     const float inv = __frcp_rn(sc);
-    if ((threadIdx.x & (VEC ? 15 : 31)) == 0 && e0 < cols)
-      a.x_scale[static_cast<int64_t>(e0 >> 7) * a.rows + row] = sc;
-    uint8_t* dst = static_cast<uint8_t*>(a.x) + row * a.x_ld;
-    uint32_t q[PER / 2];
+    const float other = __shfl_xor_sync(0xffffffffu, inv, 8);
+    const int block = col_of<LAY>(upper ? 8 : 0) >> 7;   // lane 0 or 8 of the half warp writes it
+    if ((threadIdx.x & 7) == 0 && block * 128 < cols) a.x_scale[static_cast<int64_t>(block) * a.rows + row] = sc;
 #pragma unroll
-    for (int j = 0; j < PER / 2; ++j) q[j] = cvt_e4m3x2(r[i + 2 * j] * inv, r[i + 2 * j + 1] * inv);
-    if constexpr (VEC) {
-      if (e0 < cols) *reinterpret_cast<uint2*>(dst + e0) = make_uint2(q[0] | (q[1] << 16), q[2] | (q[3] << 16));
-    } else {
+    for (int i = 0; i < 2; ++i) {
+      const float2 k = dup2((i == 1) == upper ? inv : other);
+      uint32_t q[4];
 #pragma unroll
-      for (int j = 0; j < PER; ++j) {
-        const int e = col_of<VEC>(i + j);
-        if (e < cols) dst[e] = static_cast<uint8_t>(q[j >> 1] >> (8 * (j & 1)));
+      for (int j = 0; j < 4; ++j) {
+        const float2 p = mul2(r.v[4 * i + j], k);
+        q[j] = cvt_e4m3x2(p.x, p.y);
       }
+      if (exists<LAY>(8 * i, cols))
+        *reinterpret_cast<uint2*>(dst + col_of<LAY>(8 * i)) = make_uint2(q[0] | (q[1] << 16), q[2] | (q[3] << 16));
     }
   }
 }
 
 // One row per group of warps.  blockDim = (32 * warps, rows per CTA).  Rows beyond the last run
 // with no elements.
-template <class YT, class RT, bool VEC, int MAXT>
+template <class YT, class RT, int LAY, int MAXT>
 __global__ void __launch_bounds__(MAXT, 1024 / MAXT) norm_fwd_kernel(NormArgs a) {
   __shared__ float buf[2][8 * 32];
   pdl_wait();
@@ -76,17 +101,17 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) norm_fwd_kernel(NormArgs a)
   const int cols = row < a.rows ? a.cols : 0;
   Row16 r, w;
   if (a.residual) {
-    load_row<RT, VEC>(static_cast<const RT*>(a.residual) + row * a.r_ld, cols, r);
+    load_row<RT, LAY>(static_cast<const RT*>(a.residual) + row * a.r_ld, cols, r);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) r.v[i] = dup2(0.f);
   }
   if (a.y) {
     Row16 y;
-    load_row<YT, VEC>(static_cast<const YT*>(a.y) + row * a.y_ld, cols, y);
+    load_row<YT, LAY>(static_cast<const YT*>(a.y) + row * a.y_ld, cols, y);
     float k = a.scale;
     if (a.post_w) {
-      load_weight<VEC>(a.post_w, a.post_type, a.off, cols, w);
+      load_weight<LAY>(a.post_w, a.post_type, a.off, cols, w);
       float ss[1] = {dot16(y, y)};
       row_sum(ss, a.warps, buf[0]);
       k *= rsqrtf(ss[0] / a.cols + a.eps);
@@ -94,7 +119,7 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) norm_fwd_kernel(NormArgs a)
       for (int i = 0; i < 8; ++i) y.v[i] = mul2(y.v[i], w.v[i]);
     }
     if (a.gate && a.gate_cols) {
-      load_row_dyn<VEC>(a.gate, a.gate_type, row * a.g_ld, cols, w);
+      load_row_dyn<LAY>(a.gate, a.gate_type, row * a.g_ld, cols, w);
 #pragma unroll
       for (int i = 0; i < 8; ++i) y.v[i] = mul2(y.v[i], w.v[i]);
     } else if (a.gate && cols) {
@@ -102,16 +127,13 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) norm_fwd_kernel(NormArgs a)
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) r.v[i] = fma2(dup2(k), y.v[i], r.v[i]);
-    if (a.residual_out) store_row<RT, VEC>(static_cast<RT*>(a.residual_out) + row * a.ro_ld, cols, r);
+    if (a.residual_out) store_row<RT, LAY>(static_cast<RT*>(a.residual_out) + row * a.ro_ld, cols, r);
   }
   if (!a.pre_w) return;
-  load_weight<VEC>(a.pre_w, a.pre_type, a.off, cols, w);
-  Row16 p;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) p.v[i] = mul2(r.v[i], r.v[i]);
-  float ss[1] = {sum_existing<VEC>(p, cols)};
+  load_weight<LAY>(a.pre_w, a.pre_type, a.off, cols, w);
+  float ss[1] = {squares_existing<LAY>(r, cols)};
   row_sum(ss, a.warps, buf[1]);
-  store_x<VEC>(a, row, cols, r, w, rsqrtf(ss[0] / a.cols + a.eps));
+  store_x<LAY>(a, row, cols, r, w, rsqrtf(ss[0] / a.cols + a.eps));
 }
 
 // Many rows: persistent CTAs, whose next rows (y | residual | gate per element) are on their way
@@ -122,7 +144,7 @@ struct RingArgs {
   int stages, y_bytes, r_bytes, g_bytes;   // bytes of a row of each tensor in a stage (0: not read)
 };
 
-template <class YT, class RT, bool POST>
+template <class YT, class RT, bool POST, int LAY>
 __global__ void __launch_bounds__(512, 2) norm_ring_kernel(NormArgs a, RingArgs g) {
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ float buf[3][32];   // sums of y^2; of r'^2 of even and odd rows
@@ -157,21 +179,22 @@ __global__ void __launch_bounds__(512, 2) norm_ring_kernel(NormArgs a, RingArgs 
   int stage = 0, parity = 0;
   uint32_t phase = 0;
   bool ok = true;
+  float g_next = a.gate && !a.gate_cols ? load1_dyn(a.gate, a.gate_type, blockIdx.x * a.g_ld) : 0.f;
   for (int row = blockIdx.x; row < a.rows; row += step) {
     // after a wait that ran out the CTA still goes through its rows, without their contents
     if (ok) ok = mbar_wait(&full[stage], phase, &abort, &g_op_status, kStWaitProducer);
     const uint8_t* src = ring + stage * stage_bytes;
     Row16 r, y, w;
-    load_row<YT, true>(reinterpret_cast<const YT*>(src), cols, y);
+    load_row<YT, LAY>(reinterpret_cast<const YT*>(src), cols, y);
     if (g.r_bytes) {
-      load_row<RT, true>(reinterpret_cast<const RT*>(src + g.y_bytes), cols, r);
+      load_row<RT, LAY>(reinterpret_cast<const RT*>(src + g.y_bytes), cols, r);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) r.v[i] = dup2(0.f);
     }
     float k = a.scale;
     if (POST) {
-      load_weight<true>(a.post_w, a.post_type, a.off, cols, w);
+      load_weight<LAY>(a.post_w, a.post_type, a.off, cols, w);
       float ss[1] = {dot16(y, y)};
       row_sum(ss, a.warps, buf[0]);
       k *= rsqrtf(ss[0] * inv_cols + a.eps);
@@ -179,22 +202,19 @@ __global__ void __launch_bounds__(512, 2) norm_ring_kernel(NormArgs a, RingArgs 
       for (int i = 0; i < 8; ++i) y.v[i] = mul2(y.v[i], w.v[i]);
     }
     if (a.gate && !a.gate_cols) {
-      k *= load1_dyn(a.gate, a.gate_type, row * a.g_ld);
+      k *= g_next;   // loaded a row ahead
+      if (row + static_cast<int64_t>(step) < a.rows) g_next = load1_dyn(a.gate, a.gate_type, (row + step) * a.g_ld);
     } else if (a.gate) {
-      load_row_dyn<true>(g.g_bytes ? static_cast<const void*>(src + g.y_bytes + g.r_bytes) : a.gate, a.gate_type, 0,
+      load_row_dyn<LAY>(g.g_bytes ? static_cast<const void*>(src + g.y_bytes + g.r_bytes) : a.gate, a.gate_type, 0,
                          cols, w);
 #pragma unroll
       for (int i = 0; i < 8; ++i) y.v[i] = mul2(y.v[i], w.v[i]);
     }
-    float2 p[2];   // squares of either chunk
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      r.v[i] = fma2(dup2(k), y.v[i], r.v[i]);
-      p[i >> 2] = (i & 3) ? fma2(r.v[i], r.v[i], p[i >> 2]) : mul2(r.v[i], r.v[i]);
-    }
-    store_row<RT, true>(static_cast<RT*>(a.residual_out) + row * a.ro_ld, cols, r);
-    float ss[1] = {(col_of<true>(0) < cols ? p[0].x + p[0].y : 0.f) + (col_of<true>(8) < cols ? p[1].x + p[1].y : 0.f)};
-    if (a.pre_w) load_weight<true>(a.pre_w, a.pre_type, a.off, cols, w);
+    for (int i = 0; i < 8; ++i) r.v[i] = fma2(dup2(k), y.v[i], r.v[i]);
+    store_row<RT, LAY>(static_cast<RT*>(a.residual_out) + row * a.ro_ld, cols, r);
+    float ss[1] = {squares_existing<LAY>(r, cols)};
+    if (a.pre_w) load_weight<LAY>(a.pre_w, a.pre_type, a.off, cols, w);
     row_sum(ss, a.warps, buf[1 + parity]);
     parity ^= 1;
     // every thread has its part of the stage (row_sum's barrier)
@@ -204,7 +224,7 @@ __global__ void __launch_bounds__(512, 2) norm_ring_kernel(NormArgs a, RingArgs 
       stage = 0;
       phase ^= 1u;
     }
-    if (a.pre_w) store_x<true>(a, row, cols, r, w, rsqrtf(ss[0] * inv_cols + a.eps));
+    if (a.pre_w) store_x<LAY>(a, row, cols, r, w, rsqrtf(ss[0] * inv_cols + a.eps));
   }
   if (!ok && threadIdx.x == 0)   // given up: the loads in flight land first
     for (int i = 0; i < g.stages; ++i) {
@@ -299,8 +319,11 @@ MOE_B200_API int moe_b200_block_norm(const moe_b200_norm_args* a, void* stream) 
     const dim3 grid(a->rows < ctas * sms ? a->rows : ctas * sms), block(n.warps * 32);
     const size_t smem = static_cast<size_t>(g.stages) * stage_bytes;
     dispatch_types(a->y_type, a->residual_type, [&](auto yt, auto rt) {
-      auto kernel = a->post_weight ? norm_ring_kernel<decltype(yt), decltype(rt), true>
-                                   : norm_ring_kernel<decltype(yt), decltype(rt), false>;
+      using YT = decltype(yt);
+      using RT = decltype(rt);
+      const bool full = a->cols == n.warps * 32 * kNormPerThread;
+      auto kernel = a->post_weight ? (full ? norm_ring_kernel<YT, RT, true, kFull> : norm_ring_kernel<YT, RT, true, kVec>)
+                                   : (full ? norm_ring_kernel<YT, RT, false, kFull> : norm_ring_kernel<YT, RT, false, kVec>);
       e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem);
       if (e == cudaSuccess) e = launch_pdl(kernel, grid, block, smem, st, n, g);
     });
@@ -311,8 +334,8 @@ MOE_B200_API int moe_b200_block_norm(const moe_b200_norm_args* a, void* stream) 
     using YT = decltype(yt);
     using RT = decltype(rt);
     // rows of up to 8192 columns take at most 512 threads, which may then use twice the registers
-    auto kernel = block.x * block.y <= 512 ? (vec ? norm_fwd_kernel<YT, RT, true, 512> : norm_fwd_kernel<YT, RT, false, 512>)
-                                           : (vec ? norm_fwd_kernel<YT, RT, true, 1024> : norm_fwd_kernel<YT, RT, false, 1024>);
+    auto kernel = block.x * block.y <= 512 ? (vec ? norm_fwd_kernel<YT, RT, kVec, 512> : norm_fwd_kernel<YT, RT, kScattered, 512>)
+                                           : (vec ? norm_fwd_kernel<YT, RT, kVec, 1024> : norm_fwd_kernel<YT, RT, kScattered, 1024>);
     e = launch_pdl(kernel, grid, block, 0, st, n);
   });
   return e == cudaSuccess ? MOE_B200_OK : report_cuda(e, "block_norm launch");

@@ -35,9 +35,9 @@ struct NormBwdSums {
 
 // One row whose tensors are loaded by `load(which, Row16&)`: 0 dx, 1 r, 2 y, 3 dr, 4 the gate.
 // POST, GATE (0 none or per column, 1 per row, 2 per element): -1 = known at run time only.
-template <class YT, class RT, bool VEC, int POST, int GATE, class Load>
+template <class YT, class RT, int LAY, int POST, int GATE, class Load>
 __device__ __forceinline__ void bwd_row(const NormBwdArgs& a, int row, int cols, float inv_cols, float* buf0, float* buf1,
-                                        NormBwdSums& sum, Load&& load) {
+                                        NormBwdSums& sum, float g_of_row, Load&& load) {
   const bool post = POST < 0 ? a.post_w != nullptr : POST == 1;
   const int gate = GATE < 0 ? (a.gate_grad == kGateElement ? 2 : a.gate_grad == kGateRow ? 1 : 0) : GATE;
   const bool has_dx = GATE < 0 ? a.dx != nullptr : true, has_y = GATE < 0 ? a.y != nullptr : true;
@@ -46,7 +46,7 @@ __device__ __forceinline__ void bwd_row(const NormBwdArgs& a, int row, int cols,
   if (has_dx) {
     load(1, r);
     load(0, dx);
-    load_weight<VEC>(a.pre_w, a.pre_type, a.off, cols, G);
+    load_weight<LAY>(a.pre_w, a.pre_type, a.off, cols, G);
 #pragma unroll
     for (int i = 0; i < 8; ++i) G.v[i] = mul2(G.v[i], dx.v[i]);
     s[0] = dot16(r, r);
@@ -78,13 +78,13 @@ __device__ __forceinline__ void bwd_row(const NormBwdArgs& a, int row, int cols,
       G = d;
     }
   }
-  if (a.dres) store_row<RT, VEC>(static_cast<RT*>(a.dres) + row * a.dres_ld, cols, G);
+  if (a.dres) store_row<RT, LAY>(static_cast<RT*>(a.dres) + row * a.dres_ld, cols, G);
   if (!has_y) return;
   const float ystd = post ? (cols ? rsqrtf(s[2] * inv_cols + a.eps) : 0.f) : 1.f;
-  const float g_row = gate == 1 && cols ? load1_dyn(a.gate, a.gate_type, row * a.g_ld) : 1.f;
+  const float g_row = gate == 1 ? g_of_row : 1.f;
   Row16 b;   // (post_weight + off) * gate per column
   if (post) {
-    load_weight<VEC>(a.post_w, a.post_type, a.off, cols, b);
+    load_weight<LAY>(a.post_w, a.post_type, a.off, cols, b);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) b.v[i] = dup2(1.f);
@@ -101,11 +101,11 @@ __device__ __forceinline__ void bwd_row(const NormBwdArgs& a, int row, int cols,
       dg.v[i] = mul2(mul2(gy, b.v[i]), dup2(a.scale * ystd));
       G.v[i] = mul2(mul2(G.v[i], b.v[i]), ge.v[i]);
     }
-    store_row_dyn<VEC>(a.dgate, a.gate_type, row * a.dg_ld, cols, dg);
+    store_row_dyn<LAY>(a.dgate, a.gate_type, row * a.dg_ld, cols, dg);
   } else {
     if (gate == 0 && a.gate) {
       Row16 gc;
-      load_row_dyn<VEC>(a.gate, a.gate_type, 0, cols, gc);
+      load_row_dyn<LAY>(a.gate, a.gate_type, 0, cols, gc);
 #pragma unroll
       for (int i = 0; i < 8; ++i) b.v[i] = mul2(b.v[i], gc.v[i]);
     }
@@ -126,20 +126,20 @@ __device__ __forceinline__ void bwd_row(const NormBwdArgs& a, int row, int cols,
   const float m = a.scale * q;
 #pragma unroll
   for (int i = 0; i < 8; ++i) G.v[i] = mul2(post ? fma2(y.v[i], dup2(k), G.v[i]) : G.v[i], dup2(m));
-  store_row<YT, VEC>(static_cast<YT*>(a.dy) + row * a.dy_ld, cols, G);
+  store_row<YT, LAY>(static_cast<YT*>(a.dy) + row * a.dy_ld, cols, G);
 }
 
-template <bool VEC>
+template <int LAY>
 __device__ __forceinline__ void bwd_store_sums(const NormBwdArgs& a, int part, const NormBwdSums& sum) {
   float* dst = a.partial + static_cast<int64_t>(part) * a.cols;
   const int64_t slot = static_cast<int64_t>(a.parts) * a.cols;
-  if (a.pre_slot >= 0) store_row<float, VEC>(dst + a.pre_slot * slot, a.cols, sum.pre);
-  if (a.post_slot >= 0) store_row<float, VEC>(dst + a.post_slot * slot, a.cols, sum.post);
+  if (a.pre_slot >= 0) store_row<float, LAY>(dst + a.pre_slot * slot, a.cols, sum.pre);
+  if (a.post_slot >= 0) store_row<float, LAY>(dst + a.post_slot * slot, a.cols, sum.post);
 }
 
 // Any alignment, any set of tensors: rows straight from global memory.  blockDim = (32 * warps,
 // rows per CTA); CTAs go through the rows in steps of the grid.
-template <class YT, class RT, bool VEC>
+template <class YT, class RT, int LAY>
 __device__ __forceinline__ void bwd_direct(const NormBwdArgs& a, float (*buf)[8 * 3 * 32]) {
   NormBwdSums sum;
 #pragma unroll
@@ -151,15 +151,16 @@ __device__ __forceinline__ void bwd_direct(const NormBwdArgs& a, float (*buf)[8 
     // a row without a second sum alternates the first one's buffer by itself
     const bool two = a.y && (a.post_w || a.gate_grad == kGateRow);
     const int first = two ? 0 : (row0 / step) & 1;
-    bwd_row<YT, RT, VEC, -1, -1>(a, row, cols, 1.f / a.cols, buf[first], buf[1], sum, [&](int which, Row16& v) {
-      if (which == 0) load_row<YT, VEC>(static_cast<const YT*>(a.dx) + row * a.dx_ld, cols, v);
-      else if (which == 1) load_row<RT, VEC>(static_cast<const RT*>(a.r) + row * a.r_ld, cols, v);
-      else if (which == 2) load_row<YT, VEC>(static_cast<const YT*>(a.y) + row * a.y_ld, cols, v);
-      else if (which == 3) load_row<RT, VEC>(static_cast<const RT*>(a.dr) + row * a.dr_ld, cols, v);
-      else load_row_dyn<VEC>(a.gate, a.gate_type, row * a.g_ld, cols, v);
+    const float g_row = a.gate_grad == kGateRow && cols ? load1_dyn(a.gate, a.gate_type, row * a.g_ld) : 0.f;
+    bwd_row<YT, RT, LAY, -1, -1>(a, row, cols, 1.f / a.cols, buf[first], buf[1], sum, g_row, [&](int which, Row16& v) {
+      if (which == 0) load_row<YT, LAY>(static_cast<const YT*>(a.dx) + row * a.dx_ld, cols, v);
+      else if (which == 1) load_row<RT, LAY>(static_cast<const RT*>(a.r) + row * a.r_ld, cols, v);
+      else if (which == 2) load_row<YT, LAY>(static_cast<const YT*>(a.y) + row * a.y_ld, cols, v);
+      else if (which == 3) load_row<RT, LAY>(static_cast<const RT*>(a.dr) + row * a.dr_ld, cols, v);
+      else load_row_dyn<LAY>(a.gate, a.gate_type, row * a.g_ld, cols, v);
     });
   }
-  bwd_store_sums<VEC>(a, blockIdx.x * blockDim.y + threadIdx.y, sum);
+  bwd_store_sums<LAY>(a, blockIdx.x * blockDim.y + threadIdx.y, sum);
 }
 
 template <class YT, class RT, int MAXT>
@@ -167,8 +168,8 @@ __global__ void __launch_bounds__(MAXT, 1) norm_bwd_kernel(NormBwdArgs a) {
   __shared__ float buf[2][8 * 3 * 32];
   pdl_wait();
   pdl_launch_dependents();
-  if (a.vec) bwd_direct<YT, RT, true>(a, buf);
-  else bwd_direct<YT, RT, false>(a, buf);
+  if (a.vec) bwd_direct<YT, RT, kVec>(a, buf);
+  else bwd_direct<YT, RT, kScattered>(a, buf);
 }
 
 // Aligned rows with all of dx, r', y: the next rows (dx | r' | y | dr | gate per element) are on
@@ -177,7 +178,7 @@ struct RingBwdArgs {
   int stages, y_bytes, r_bytes, dr_bytes, g_bytes;   // bytes of a row of each (dx has y's type)
 };
 
-template <class YT, class RT, bool POST, int GATE>
+template <class YT, class RT, int LAY, int POST, int GATE>
 __global__ void __launch_bounds__(512, 1) norm_bwd_ring_kernel(NormBwdArgs a, RingBwdArgs g) {
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ float buf[2][3 * 32];
@@ -201,7 +202,7 @@ __global__ void __launch_bounds__(512, 1) norm_bwd_ring_kernel(NormBwdArgs a, Ri
     bulk_load(dst + at_r, static_cast<const RT*>(a.r) + row * a.r_ld, g.r_bytes, bar);
     bulk_load(dst + at_y, static_cast<const YT*>(a.y) + row * a.y_ld, g.y_bytes, bar);
     if (g.dr_bytes) bulk_load(dst + at_dr, static_cast<const RT*>(a.dr) + row * a.dr_ld, g.dr_bytes, bar);
-    if (GATE == 2)
+    if (g.g_bytes)
       bulk_load(dst + at_g, static_cast<const uint8_t*>(a.gate) + row * a.g_ld * (g.g_bytes / a.cols), g.g_bytes, bar);
   };
   const int step = gridDim.x, cols = a.cols;
@@ -214,21 +215,27 @@ __global__ void __launch_bounds__(512, 1) norm_bwd_ring_kernel(NormBwdArgs a, Ri
 #pragma unroll
   for (int i = 0; i < 8; ++i) sum.pre.v[i] = sum.post.v[i] = dup2(0.f);
   const float inv_cols = 1.f / cols;
+  const bool two = (POST < 0 ? a.post_w != nullptr : POST == 1) ||   // a second sum over the row
+                   (GATE < 0 ? a.gate_grad == kGateRow : GATE == 1);
   int stage = 0, parity = 0;
   uint32_t phase = 0;
   bool ok = true;
+  float g_next = a.gate_grad == kGateRow ? load1_dyn(a.gate, a.gate_type, blockIdx.x * a.g_ld) : 0.f;
   for (int row = blockIdx.x; row < a.rows; row += step) {
     // after a wait that ran out the CTA still goes through its rows, without their contents
     if (ok) ok = mbar_wait(&full[stage], phase, &abort, &g_op_status, kStWaitProducer);
     const uint8_t* src = ring + stage * stage_bytes;
-    constexpr bool two = POST || GATE == 1;   // a second sum over the row
-    bwd_row<YT, RT, true, POST ? 1 : 0, GATE>(
-        a, row, cols, inv_cols, buf[two ? 0 : parity], buf[1], sum, [&](int which, Row16& v) {
-          if (which == 0) load_row<YT, true>(reinterpret_cast<const YT*>(src), cols, v);
-          else if (which == 1) load_row<RT, true>(reinterpret_cast<const RT*>(src + at_r), cols, v);
-          else if (which == 2) load_row<YT, true>(reinterpret_cast<const YT*>(src + at_y), cols, v);
-          else if (which == 3) load_row<RT, true>(reinterpret_cast<const RT*>(src + at_dr), cols, v);
-          else load_row_dyn<true>(src + at_g, a.gate_type, 0, cols, v);
+    const float g_row = g_next;   // the gate per row, loaded a row ahead
+    if (a.gate_grad == kGateRow && row + static_cast<int64_t>(step) < a.rows)
+      g_next = load1_dyn(a.gate, a.gate_type, (row + step) * a.g_ld);
+    
+    bwd_row<YT, RT, LAY, POST, GATE>(
+        a, row, cols, inv_cols, buf[two ? 0 : parity], buf[1], sum, g_row, [&](int which, Row16& v) {
+          if (which == 0) load_row<YT, LAY>(reinterpret_cast<const YT*>(src), cols, v);
+          else if (which == 1) load_row<RT, LAY>(reinterpret_cast<const RT*>(src + at_r), cols, v);
+          else if (which == 2) load_row<YT, LAY>(reinterpret_cast<const YT*>(src + at_y), cols, v);
+          else if (which == 3) load_row<RT, LAY>(reinterpret_cast<const RT*>(src + at_dr), cols, v);
+          else load_row_dyn<LAY>(src + at_g, a.gate_type, 0, cols, v);
         });
     parity ^= 1;
     // every thread has read the stage: the second sum's barrier, or one more
@@ -240,7 +247,7 @@ __global__ void __launch_bounds__(512, 1) norm_bwd_ring_kernel(NormBwdArgs a, Ri
       phase ^= 1u;
     }
   }
-  bwd_store_sums<true>(a, blockIdx.x, sum);
+  bwd_store_sums<LAY>(a, blockIdx.x, sum);
   if (!ok && threadIdx.x == 0)   // given up: the loads in flight land first
     for (int i = 0; i < g.stages; ++i) {
       int none = 0;
@@ -437,10 +444,16 @@ MOE_B200_API int moe_b200_block_norm_backward(const moe_b200_norm_backward_args*
     using YT = decltype(yt);
     using RT = decltype(rt);
     if (ring) {
-      const bool post = a->post_weight != nullptr;
-      auto kernel = n.gate_grad == kGateElement ? (post ? norm_bwd_ring_kernel<YT, RT, true, 2> : norm_bwd_ring_kernel<YT, RT, false, 2>)
-                    : n.gate_grad == kGateRow   ? (post ? norm_bwd_ring_kernel<YT, RT, true, 1> : norm_bwd_ring_kernel<YT, RT, false, 1>)
-                                                : (post ? norm_bwd_ring_kernel<YT, RT, true, 0> : norm_bwd_ring_kernel<YT, RT, false, 0>);
+      // every combination has its kernel where rows fill their threads; one for all elsewhere
+      auto of_gate = [&](auto post) {
+        constexpr int P = decltype(post)::value;
+        return n.gate_grad == kGateElement ? norm_bwd_ring_kernel<YT, RT, kFull, P, 2>
+               : n.gate_grad == kGateRow   ? norm_bwd_ring_kernel<YT, RT, kFull, P, 1>
+                                           : norm_bwd_ring_kernel<YT, RT, kFull, P, 0>;
+      };
+      auto kernel = a->cols != n.warps * 32 * kNormPerThread ? norm_bwd_ring_kernel<YT, RT, kVec, -1, -1>
+                    : a->post_weight                         ? of_gate(std::integral_constant<int, 1>{})
+                                                             : of_gate(std::integral_constant<int, 0>{});
       e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem);
       if (e == cudaSuccess)
         e = launch_pdl(kernel, dim3(n.parts), dim3(n.warps * 32), static_cast<size_t>(g.stages) * stage_bytes, st, n, g);

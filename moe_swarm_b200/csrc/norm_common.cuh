@@ -47,83 +47,127 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 }
 __device__ __forceinline__ float2 dup2(float a) { return make_float2(a, a); }
 
-// Where a thread's element q of its row is.  VEC: two chunks of eight neighbours, for 16-byte
-// accesses.  Otherwise 128-column blocks by warp, lane + 32 m within one, so that the accesses of
-// a warp are neighbours whatever the row's alignment.  Either way a 128-column block belongs to a
-// half warp (eight elements each) or to a warp (four each).
-template <bool VEC>
+// How a row lies in its threads.  kVec, kFull: two chunks of eight neighbours, for 16-byte accesses;
+// kFull: every chunk exists (the row is 16 x its threads long), so nothing is checked.
+// kScattered: 128-column blocks by warp, lane + 32 m within one, so that the accesses of a warp are
+// neighbours whatever the row's alignment.  In each a 128-column block belongs to a half warp
+// (eight elements each) or to a warp (four each).
+enum : int { kScattered = 0, kVec = 1, kFull = 2 };
+
+// The column of this thread's element q.
+template <int LAY>
 __device__ __forceinline__ int col_of(int q) {
-  if constexpr (VEC) return static_cast<int>(threadIdx.x + (q >> 3) * blockDim.x) * 8 + (q & 7);
+  if constexpr (LAY != kScattered) return static_cast<int>(threadIdx.x + (q >> 3) * blockDim.x) * 8 + (q & 7);
   return static_cast<int>((threadIdx.x >> 5) + (q >> 2) * (blockDim.x >> 5)) * 128 +
          static_cast<int>(threadIdx.x & 31) + 32 * (q & 3);
 }
+template <int LAY>
+__device__ __forceinline__ bool exists(int q, int cols) {
+  return LAY == kFull || col_of<LAY>(q) < cols;
+}
 
-template <class T, bool VEC>
-__device__ __forceinline__ void load_row(const T* row, int cols, Row16& r) {
-  if constexpr (VEC) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      float v[8];
-      const int e0 = col_of<true>(8 * i);
-      load8<T, true>(row + e0, cols - e0, v);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) r[8 * i + j] = v[j];
-    }
+template <class T>
+__device__ __forceinline__ void load_chunk(const T* p, float2* v) {
+  if constexpr (sizeof(T) == 4) {
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+    v[0] = make_float2(a.x, a.y);
+    v[1] = make_float2(a.z, a.w);
+    v[2] = make_float2(b.x, b.y);
+    v[3] = make_float2(b.z, b.w);
   } else {
-#pragma unroll
-    for (int q = 0; q < 16; ++q) {
-      const int e = col_of<false>(q);
-      r[q] = e < cols ? to_f(row[e]) : 0.f;
-    }
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    float f[2];
+    unpack2(u.x, f, T{});
+    v[0] = make_float2(f[0], f[1]);
+    unpack2(u.y, f, T{});
+    v[1] = make_float2(f[0], f[1]);
+    unpack2(u.z, f, T{});
+    v[2] = make_float2(f[0], f[1]);
+    unpack2(u.w, f, T{});
+    v[3] = make_float2(f[0], f[1]);
   }
 }
-template <class T, bool VEC>
-__device__ __forceinline__ void store_row(T* row, int cols, const Row16& r) {
-  if constexpr (VEC) {
+
+template <class T, int LAY>
+__device__ __forceinline__ void load_row(const T* row, int cols, Row16& r) {
+  if constexpr (LAY != kScattered) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      float v[8];
-      const int e0 = col_of<true>(8 * i);
+      if (exists<LAY>(8 * i, cols)) {
+        load_chunk(row + col_of<LAY>(8 * i), r.v + 4 * i);
+      } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = r[8 * i + j];
-      store8<T, true>(row + e0, cols - e0, v);
+        for (int j = 0; j < 4; ++j) r.v[4 * i + j] = dup2(0.f);
+      }
     }
   } else {
 #pragma unroll
-    for (int q = 0; q < 16; ++q) {
-      const int e = col_of<false>(q);
-      if (e < cols) row[e] = from_f<T>(r[q]);
+    for (int q = 0; q < 16; ++q) r[q] = exists<LAY>(q, cols) ? to_f(row[col_of<LAY>(q)]) : 0.f;
+  }
+}
+template <class T, int LAY>
+__device__ __forceinline__ void store_row(T* row, int cols, const Row16& r) {
+  if constexpr (LAY != kScattered) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (!exists<LAY>(8 * i, cols)) continue;
+      T* p = row + col_of<LAY>(8 * i);
+      const float2* v = r.v + 4 * i;
+      if constexpr (sizeof(T) == 4) {
+        reinterpret_cast<float4*>(p)[0] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+        reinterpret_cast<float4*>(p)[1] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
+      } else {
+        *reinterpret_cast<uint4*>(p) = make_uint4(pack2(v[0].x, v[0].y, T{}), pack2(v[1].x, v[1].y, T{}),
+                                                  pack2(v[2].x, v[2].y, T{}), pack2(v[3].x, v[3].y, T{}));
+      }
     }
+  } else {
+#pragma unroll
+    for (int q = 0; q < 16; ++q)
+      if (exists<LAY>(q, cols)) row[col_of<LAY>(q)] = from_f<T>(r[q]);
   }
 }
 // The same with the type known at run time; `off` in elements.
-template <bool VEC>
+template <int LAY>
 __device__ __forceinline__ void load_row_dyn(const void* p, int type, int64_t off, int cols, Row16& r) {
-  if (type == MOE_B200_BF16) load_row<bf16, VEC>(static_cast<const bf16*>(p) + off, cols, r);
-  else if (type == MOE_B200_FP16) load_row<fp16, VEC>(static_cast<const fp16*>(p) + off, cols, r);
-  else load_row<float, VEC>(static_cast<const float*>(p) + off, cols, r);
+  if (type == MOE_B200_BF16) load_row<bf16, LAY>(static_cast<const bf16*>(p) + off, cols, r);
+  else if (type == MOE_B200_FP16) load_row<fp16, LAY>(static_cast<const fp16*>(p) + off, cols, r);
+  else load_row<float, LAY>(static_cast<const float*>(p) + off, cols, r);
 }
-template <bool VEC>
+template <int LAY>
 __device__ __forceinline__ void store_row_dyn(void* p, int type, int64_t off, int cols, const Row16& r) {
-  if (type == MOE_B200_BF16) store_row<bf16, VEC>(static_cast<bf16*>(p) + off, cols, r);
-  else if (type == MOE_B200_FP16) store_row<fp16, VEC>(static_cast<fp16*>(p) + off, cols, r);
-  else store_row<float, VEC>(static_cast<float*>(p) + off, cols, r);
+  if (type == MOE_B200_BF16) store_row<bf16, LAY>(static_cast<bf16*>(p) + off, cols, r);
+  else if (type == MOE_B200_FP16) store_row<fp16, LAY>(static_cast<fp16*>(p) + off, cols, r);
+  else store_row<float, LAY>(static_cast<float*>(p) + off, cols, r);
 }
-template <bool VEC>
+template <int LAY>
 __device__ __forceinline__ void load_weight(const void* p, int type, float off, int cols, Row16& w) {
-  load_row_dyn<VEC>(p, type, 0, cols, w);
+  load_row_dyn<LAY>(p, type, 0, cols, w);
+  if (off == 0.f) return;
 #pragma unroll
   for (int i = 0; i < 8; ++i) w.v[i] = add2(w.v[i], dup2(off));
 }
 
-// Sums over a row, of elements that exist: those beyond the row are 0 in every tensor, but a
-// factor of the row may be infinite.  VEC: chunk-wise, with whole chunks in or out.
-template <bool VEC>
-__device__ __forceinline__ float sum_existing(const Row16& p, int cols) {
-  float s = 0.f;
+// Sum of squares of the elements that exist: those beyond the row are 0 in every tensor, but may
+// have met an infinite factor of the row since.
+template <int LAY>
+__device__ __forceinline__ float squares_existing(const Row16& r, int cols) {
+  if constexpr (LAY == kScattered) {
+    float s = 0.f;
 #pragma unroll
-  for (int q = 0; q < 16; ++q) s += col_of<VEC>(q) < cols ? p[q] : 0.f;
-  return s;
+    for (int q = 0; q < 16; ++q) s = exists<LAY>(q, cols) ? fmaf(r[q], r[q], s) : s;
+    return s;
+  } else {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float2 p = mul2(r.v[4 * i], r.v[4 * i]);
+#pragma unroll
+      for (int j = 1; j < 4; ++j) p = fma2(r.v[4 * i + j], r.v[4 * i + j], p);
+      if (exists<LAY>(8 * i, cols)) s += p.x + p.y;
+    }
+    return s;
+  }
 }
 __device__ __forceinline__ float dot16(const Row16& a, const Row16& b) {
   float2 s = mul2(a.v[0], b.v[0]);

@@ -38,7 +38,7 @@ __device__ __forceinline__ void store_x(const NormArgs& a, int row, int cols, Ro
   }
   uint8_t* dst = static_cast<uint8_t*>(a.x) + row * a.x_ld;
   auto scale_of = [](float m) { return max_nan(m, 1e-12f) * (1.f / 448.f); };
-  if constexpr (LAY == kScattered) {
+  if constexpr (!is_vec(LAY)) {
 #pragma unroll
     for (int i = 0; i < 16; i += 4) {
       float m = 0.f;
@@ -136,21 +136,16 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) norm_fwd_kernel(NormArgs a)
   store_x<LAY>(a, row, cols, r, w, rsqrtf(ss[0] / a.cols + a.eps));
 }
 
-// Many rows: persistent CTAs, whose next rows (y | residual | gate per element) are on their way
+// Many rows: persistent CTAs, whose next rows (y, residual, gate per element) are on their way
 // to shared memory as bulk copies while a row is computed, so that the row's barriers and latencies
-// leave the memory busy.  Row tensors are 16-byte aligned; weights and a gate per column come
-// from L1.  A stage is refilled after the row's last barrier, when every thread holds its part.
-struct RingArgs {
-  int stages, y_bytes, r_bytes, g_bytes;   // bytes of a row of each tensor in a stage (0: not read)
-};
-
+// leave the memory busy.  Weights and a gate per column come from L1.  A stage is refilled after
+// the row's last barrier, when every thread holds its part.
 template <class YT, class RT, bool POST, int LAY>
-__global__ void __launch_bounds__(512, 2) norm_ring_kernel(NormArgs a, RingArgs g) {
+__global__ void __launch_bounds__(512, 2) norm_ring_kernel(NormArgs a, RingPlan g) {
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ float buf[3][32];   // sums of y^2; of r'^2 of even and odd rows
   __shared__ uint64_t full[kRingMaxStages];
   __shared__ int abort;
-  const int stage_bytes = g.y_bytes + g.r_bytes + g.g_bytes;
   if (threadIdx.x == 0) {
     abort = 0;
     for (int i = 0; i < g.stages; ++i) mbar_init(&full[i], 1);
@@ -159,22 +154,13 @@ __global__ void __launch_bounds__(512, 2) norm_ring_kernel(NormArgs a, RingArgs 
   __syncthreads();
   pdl_wait();
   pdl_launch_dependents();
-  auto fetch = [&](int row, int stage) {   // one thread
-    uint8_t* dst = ring + stage * stage_bytes;
-    mbar_arrive_expect_tx(&full[stage], stage_bytes);
-    bulk_load(dst, static_cast<const YT*>(a.y) + row * a.y_ld, g.y_bytes, &full[stage]);
-    if (g.r_bytes)
-      bulk_load(dst + g.y_bytes, static_cast<const RT*>(a.residual) + row * a.r_ld, g.r_bytes, &full[stage]);
-    if (g.g_bytes)
-      bulk_load(dst + g.y_bytes + g.r_bytes,
-                static_cast<const uint8_t*>(a.gate) + row * a.g_ld * (g.g_bytes / a.cols), g.g_bytes, &full[stage]);
-  };
   const int step = gridDim.x, cols = a.cols;
   if (threadIdx.x == 0)
     for (int i = 0; i < g.stages; ++i) {
       const int64_t row = blockIdx.x + static_cast<int64_t>(i) * step;
-      if (row < a.rows) fetch(static_cast<int>(row), i);
+      if (row < a.rows) ring_fetch(g, static_cast<int>(row), ring + i * g.stage_bytes, &full[i]);
     }
+  const bool g_element = a.gate && a.gate_cols && a.g_ld;   // the ring's last tensor
   const float inv_cols = 1.f / cols;
   int stage = 0, parity = 0;
   uint32_t phase = 0;
@@ -183,11 +169,11 @@ __global__ void __launch_bounds__(512, 2) norm_ring_kernel(NormArgs a, RingArgs 
   for (int row = blockIdx.x; row < a.rows; row += step) {
     // after a wait that ran out the CTA still goes through its rows, without their contents
     if (ok) ok = mbar_wait(&full[stage], phase, &abort, &g_op_status, kStWaitProducer);
-    const uint8_t* src = ring + stage * stage_bytes;
+    uint8_t* src = ring + stage * g.stage_bytes;
     Row16 r, y, w;
-    load_row<YT, LAY>(reinterpret_cast<const YT*>(src), cols, y);
-    if (g.r_bytes) {
-      load_row<RT, LAY>(reinterpret_cast<const RT*>(src + g.y_bytes), cols, r);
+    load_row<YT, LAY>(reinterpret_cast<const YT*>(src + g.t[0].at), cols, y);
+    if (a.residual) {
+      load_row<RT, LAY>(reinterpret_cast<const RT*>(src + g.t[1].at), cols, r);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) r.v[i] = dup2(0.f);
@@ -205,8 +191,7 @@ __global__ void __launch_bounds__(512, 2) norm_ring_kernel(NormArgs a, RingArgs 
       k *= g_next;   // loaded a row ahead
       if (row + static_cast<int64_t>(step) < a.rows) g_next = load1_dyn(a.gate, a.gate_type, (row + step) * a.g_ld);
     } else if (a.gate) {
-      load_row_dyn<LAY>(g.g_bytes ? static_cast<const void*>(src + g.y_bytes + g.r_bytes) : a.gate, a.gate_type, 0,
-                         cols, w);
+      load_row_dyn<LAY>(g_element ? static_cast<const void*>(src + g.t[a.residual ? 2 : 1].at) : a.gate, a.gate_type, 0, cols, w);
 #pragma unroll
       for (int i = 0; i < 8; ++i) y.v[i] = mul2(y.v[i], w.v[i]);
     }
@@ -219,7 +204,7 @@ __global__ void __launch_bounds__(512, 2) norm_ring_kernel(NormArgs a, RingArgs 
     parity ^= 1;
     // every thread has its part of the stage (row_sum's barrier)
     const int64_t next = row + static_cast<int64_t>(g.stages) * step;
-    if (threadIdx.x == 0 && ok && next < a.rows) fetch(static_cast<int>(next), stage);
+    if (threadIdx.x == 0 && ok && next < a.rows) ring_fetch(g, static_cast<int>(next), src, &full[stage]);
     if (ok && ++stage == g.stages) {
       stage = 0;
       phase ^= 1u;
@@ -305,25 +290,27 @@ MOE_B200_API int moe_b200_block_norm(const moe_b200_norm_args* a, void* stream) 
                                                : rows_aligned(a->x, n.x_ld, a->x_type));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaSuccess;
-  // The ring: rows of two warps or more whose row tensors are 16-byte aligned, at least four per
-  // SM, and two or more of them in a CTA's share of shared memory.
-  RingArgs g{};
-  g.y_bytes = a->cols * type_bytes(a->y_type);
-  g.r_bytes = a->residual ? a->cols * type_bytes(a->residual_type) : 0;
-  g.g_bytes = a->gate && n.gate_cols && n.g_ld ? a->cols * type_bytes(a->gate_type) : 0;
-  const int stage_bytes = g.y_bytes + g.r_bytes + g.g_bytes;
+  // The ring: aligned rows of two warps or more, at least four per SM, and two or more of them in
+  // a CTA's share of shared memory.
+  RingPlan g{};
+  ring_add(&g, a->y, n.y_ld, a->cols, a->y_type);
+  ring_add(&g, a->residual, n.r_ld, a->cols, a->residual_type);
+  if (a->gate_per_column && n.g_ld) ring_add(&g, a->gate, n.g_ld, a->cols, a->gate_type);
   const int ctas = n.warps >= 2 && n.warps <= 16 ? 32 / n.warps : 0;   // 1024 threads of an SM
-  g.stages = ctas ? kRingSmem / ctas / stage_bytes : 0;
+  g.stages = ctas ? kRingSmem / ctas / g.stage_bytes : 0;
   if (g.stages > kRingMaxStages) g.stages = kRingMaxStages;
   if (vec && a->y && a->rows >= 4 * sms && g.stages >= 2) {
     const dim3 grid(a->rows < ctas * sms ? a->rows : ctas * sms), block(n.warps * 32);
-    const size_t smem = static_cast<size_t>(g.stages) * stage_bytes;
+    const size_t smem = static_cast<size_t>(g.stages) * g.stage_bytes;
     dispatch_types(a->y_type, a->residual_type, [&](auto yt, auto rt) {
       using YT = decltype(yt);
       using RT = decltype(rt);
-      const bool full = a->cols == n.warps * 32 * kNormPerThread;
-      auto kernel = a->post_weight ? (full ? norm_ring_kernel<YT, RT, true, kFull> : norm_ring_kernel<YT, RT, true, kVec>)
-                                   : (full ? norm_ring_kernel<YT, RT, false, kFull> : norm_ring_kernel<YT, RT, false, kVec>);
+      auto laid = [&](auto post) {
+        constexpr bool P = decltype(post)::value;
+        return a->cols == n.warps * 32 * kNormPerThread ? norm_ring_kernel<YT, RT, P, kFull>
+                                                        : norm_ring_kernel<YT, RT, P, kVec>;
+      };
+      auto kernel = a->post_weight ? laid(std::true_type{}) : laid(std::false_type{});
       e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem);
       if (e == cudaSuccess) e = launch_pdl(kernel, grid, block, smem, st, n, g);
     });
@@ -334,8 +321,14 @@ MOE_B200_API int moe_b200_block_norm(const moe_b200_norm_args* a, void* stream) 
     using YT = decltype(yt);
     using RT = decltype(rt);
     // rows of up to 8192 columns take at most 512 threads, which may then use twice the registers
-    auto kernel = block.x * block.y <= 512 ? (vec ? norm_fwd_kernel<YT, RT, kVec, 512> : norm_fwd_kernel<YT, RT, kScattered, 512>)
-                                           : (vec ? norm_fwd_kernel<YT, RT, kVec, 1024> : norm_fwd_kernel<YT, RT, kScattered, 1024>);
+    auto sized = [&](auto t) {
+      constexpr int MAXT = decltype(t)::value;
+      return vec                             ? norm_fwd_kernel<YT, RT, kVec, MAXT>
+             : a->cols >= 384 * n.warps ? norm_fwd_kernel<YT, RT, kTail, MAXT>
+                                        : norm_fwd_kernel<YT, RT, kScattered, MAXT>;
+    };
+    auto kernel = block.x * block.y <= 512 ? sized(std::integral_constant<int, 512>{})
+                                           : sized(std::integral_constant<int, 1024>{});
     e = launch_pdl(kernel, grid, block, 0, st, n);
   });
   return e == cudaSuccess ? MOE_B200_OK : report_cuda(e, "block_norm launch");

@@ -15,6 +15,7 @@
 
 namespace moe {
 
+constexpr int kFactorBytes = 2 * kNormPerThread * 4;   // per thread of a row
 enum : int { kGateNone = 0, kGateColumn = 1, kGateRow = 2, kGateElement = 3 };
 
 struct NormBwdArgs {
@@ -33,11 +34,32 @@ struct NormBwdSums {
   Row16 pre, post;
 };
 
-// One row whose tensors are loaded by `load(which, Row16&)`: 0 dx, 1 r, 2 y, 3 dr, 4 the gate.
-// POST, GATE (0 none or per column, 1 per row, 2 per element): -1 = known at run time only.
-template <class YT, class RT, int LAY, int POST, int GATE, class Load>
+// Factors per column: w = pre_weight + off, b = (post_weight + off) * gate per column.
+template <int LAY>
+__device__ __forceinline__ void factor_w(const NormBwdArgs& a, Row16& w) {
+  load_weight<LAY>(a.pre_w, a.pre_type, a.off, a.cols, w);
+}
+template <int LAY>
+__device__ __forceinline__ void factor_b(const NormBwdArgs& a, Row16& b) {
+  if (a.post_w) {
+    load_weight<LAY>(a.post_w, a.post_type, a.off, a.cols, b);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) b.v[i] = dup2(1.f);
+  }
+  if (a.gate_grad != kGateColumn) return;
+  Row16 g;
+  load_row_dyn<LAY>(a.gate, a.gate_type, 0, a.cols, g);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) b.v[i] = mul2(b.v[i], g.v[i]);
+}
+
+// One row.  load(which, v): which = 0 dx, 1 r', 2 y, 3 dr, 4 the gate per element, 5 w, 6 b; done()
+// is called when everything is loaded.  POST, GATE (0 none or per column, 1 per row, 2 per
+// element): -1 = known at run time only.
+template <class YT, class RT, int LAY, int POST, int GATE, class Load, class Done>
 __device__ __forceinline__ void bwd_row(const NormBwdArgs& a, int row, int cols, float inv_cols, float* buf0, float* buf1,
-                                        NormBwdSums& sum, float g_of_row, Load&& load) {
+                                        NormBwdSums& sum, float g_of_row, Load&& load, Done&& done) {
   const bool post = POST < 0 ? a.post_w != nullptr : POST == 1;
   const int gate = GATE < 0 ? (a.gate_grad == kGateElement ? 2 : a.gate_grad == kGateRow ? 1 : 0) : GATE;
   const bool has_dx = GATE < 0 ? a.dx != nullptr : true, has_y = GATE < 0 ? a.y != nullptr : true;
@@ -46,7 +68,7 @@ __device__ __forceinline__ void bwd_row(const NormBwdArgs& a, int row, int cols,
   if (has_dx) {
     load(1, r);
     load(0, dx);
-    load_weight<LAY>(a.pre_w, a.pre_type, a.off, cols, G);
+    load(5, G);
 #pragma unroll
     for (int i = 0; i < 8; ++i) G.v[i] = mul2(G.v[i], dx.v[i]);
     s[0] = dot16(r, r);
@@ -56,9 +78,9 @@ __device__ __forceinline__ void bwd_row(const NormBwdArgs& a, int row, int cols,
     load(2, y);
     if (post) s[2] = dot16(y, y);
   }
-  row_sum(s, a.warps, buf0);
-  // (rows beyond the last, which share a CTA with others, must leave the sums alone)
-  const float rstd = cols ? rsqrtf(s[0] * inv_cols + a.eps) : 0.f;
+  if (LAY == kFull || a.warps <= 16) row_sum3(s, a.warps, buf0);
+  else row_sum(s, a.warps, buf0);
+  const float rstd = rsqrtf(s[0] * inv_cols + a.eps);
   {
     Row16 d;
     if (a.dr) {
@@ -79,18 +101,16 @@ __device__ __forceinline__ void bwd_row(const NormBwdArgs& a, int row, int cols,
     }
   }
   if (a.dres) store_row<RT, LAY>(static_cast<RT*>(a.dres) + row * a.dres_ld, cols, G);
-  if (!has_y) return;
-  const float ystd = post ? (cols ? rsqrtf(s[2] * inv_cols + a.eps) : 0.f) : 1.f;
-  const float g_row = gate == 1 ? g_of_row : 1.f;
-  Row16 b;   // (post_weight + off) * gate per column
-  if (post) {
-    load_weight<LAY>(a.post_w, a.post_type, a.off, cols, b);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) b.v[i] = dup2(1.f);
+  if (!has_y) {
+    done();
+    return;
   }
+  const float ystd = post ? rsqrtf(s[2] * inv_cols + a.eps) : 1.f;
+  const float g_row = gate == 1 ? g_of_row : 1.f;
   const float q = g_row * ystd;
-  float t[1] = {0.f};   // sum of b G y
+  const bool has_b = post || a.gate_grad == kGateColumn;
+  Row16 b;
+  if (has_b) load(6, b);
   if (gate == 2) {
     Row16 ge, dg;
     load(4, ge);
@@ -98,29 +118,27 @@ __device__ __forceinline__ void bwd_row(const NormBwdArgs& a, int row, int cols,
     for (int i = 0; i < 8; ++i) {
       const float2 gy = mul2(G.v[i], y.v[i]);
       sum.post.v[i] = fma2(mul2(gy, ge.v[i]), dup2(q), sum.post.v[i]);
-      dg.v[i] = mul2(mul2(gy, b.v[i]), dup2(a.scale * ystd));
-      G.v[i] = mul2(mul2(G.v[i], b.v[i]), ge.v[i]);
+      dg.v[i] = mul2(has_b ? mul2(gy, b.v[i]) : gy, dup2(a.scale * ystd));
+      G.v[i] = mul2(G.v[i], ge.v[i]);
     }
     store_row_dyn<LAY>(a.dgate, a.gate_type, row * a.dg_ld, cols, dg);
   } else {
-    if (gate == 0 && a.gate) {
-      Row16 gc;
-      load_row_dyn<LAY>(a.gate, a.gate_type, 0, cols, gc);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) b.v[i] = mul2(b.v[i], gc.v[i]);
-    }
+    for (int i = 0; i < 8; ++i) sum.post.v[i] = fma2(mul2(G.v[i], y.v[i]), dup2(q), sum.post.v[i]);
+  }
+  if (has_b) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      sum.post.v[i] = fma2(mul2(G.v[i], y.v[i]), dup2(q), sum.post.v[i]);
-      G.v[i] = mul2(G.v[i], b.v[i]);
-    }
+    for (int i = 0; i < 8; ++i) G.v[i] = mul2(G.v[i], b.v[i]);
   }
   float k = 0.f;
   if (post || gate == 1) {
-    t[0] = dot16(G, y);
+    float t[1] = {dot16(G, y)};   // sum of b G y
     row_sum(t, a.warps, buf1);
-    if (gate == 1 && threadIdx.x == 0 && cols) static_cast<float*>(a.dgate)[row] = a.scale * ystd * t[0];
+    done();
+    if (gate == 1 && threadIdx.x == 0) static_cast<float*>(a.dgate)[row] = a.scale * ystd * t[0];
     if (post) k = -t[0] * inv_cols * ystd * ystd;
+  } else {
+    done();
   }
   if (!a.dy) return;
   const float m = a.scale * q;
@@ -129,88 +147,108 @@ __device__ __forceinline__ void bwd_row(const NormBwdArgs& a, int row, int cols,
   store_row<YT, LAY>(static_cast<YT*>(a.dy) + row * a.dy_ld, cols, G);
 }
 
+// Writes a CTA's part of the column sums.  Rows side by side in a CTA (threadIdx.y) are added up
+// first, in their order, through `shared` ([rows][cols] floats; null with one row).
 template <int LAY>
-__device__ __forceinline__ void bwd_store_sums(const NormBwdArgs& a, int part, const NormBwdSums& sum) {
-  float* dst = a.partial + static_cast<int64_t>(part) * a.cols;
+__device__ __forceinline__ void bwd_store_sums(const NormBwdArgs& a, const NormBwdSums& sum, float* shared) {
+  float* dst = a.partial + static_cast<int64_t>(blockIdx.x) * a.cols;
   const int64_t slot = static_cast<int64_t>(a.parts) * a.cols;
-  if (a.pre_slot >= 0) store_row<float, LAY>(dst + a.pre_slot * slot, a.cols, sum.pre);
-  if (a.post_slot >= 0) store_row<float, LAY>(dst + a.post_slot * slot, a.cols, sum.post);
+  auto put = [&](float* out, const Row16& v) {
+    if (blockDim.y == 1) {
+      store_row<float, LAY>(out, a.cols, v);
+      return;
+    }
+    __syncthreads();
+    store_row<float, LAY>(shared + threadIdx.y * a.cols, a.cols, v);
+    __syncthreads();
+    for (int c = threadIdx.y * blockDim.x + threadIdx.x; c < a.cols; c += blockDim.x * blockDim.y) {
+      float s = shared[c];
+      for (int y = 1; y < static_cast<int>(blockDim.y); ++y) s += shared[y * a.cols + c];
+      out[c] = s;
+    }
+  };
+  if (a.pre_slot >= 0) put(dst + a.pre_slot * slot, sum.pre);
+  if (a.post_slot >= 0) put(dst + a.post_slot * slot, sum.post);
 }
 
-// Any alignment, any set of tensors: rows straight from global memory.  blockDim = (32 * warps,
-// rows per CTA); CTAs go through the rows in steps of the grid.
+// Any alignment, any set of tensors: rows straight from global memory, one per CTA at a time.
 template <class YT, class RT, int LAY>
-__device__ __forceinline__ void bwd_direct(const NormBwdArgs& a, float (*buf)[8 * 3 * 32]) {
+__device__ __forceinline__ void bwd_direct(const NormBwdArgs& a, float (*buf)[3 * 32]) {
   NormBwdSums sum;
 #pragma unroll
   for (int i = 0; i < 8; ++i) sum.pre.v[i] = sum.post.v[i] = dup2(0.f);
-  const int step = gridDim.x * blockDim.y;
-  for (int row0 = blockIdx.x * blockDim.y; row0 < a.rows; row0 += step) {
-    const int row = row0 + threadIdx.y;
-    const int cols = row < a.rows ? a.cols : 0;
-    // a row without a second sum alternates the first one's buffer by itself
-    const bool two = a.y && (a.post_w || a.gate_grad == kGateRow);
-    const int first = two ? 0 : (row0 / step) & 1;
-    const float g_row = a.gate_grad == kGateRow && cols ? load1_dyn(a.gate, a.gate_type, row * a.g_ld) : 0.f;
-    bwd_row<YT, RT, LAY, -1, -1>(a, row, cols, 1.f / a.cols, buf[first], buf[1], sum, g_row, [&](int which, Row16& v) {
+  const int cols = a.cols;
+  // a row without a second sum alternates the first one's buffer by itself
+  const bool two = a.y && (a.post_w || a.gate_grad == kGateRow);
+  int first = 0;
+  for (int row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const float g_row = a.gate_grad == kGateRow ? load1_dyn(a.gate, a.gate_type, row * a.g_ld) : 0.f;
+    bwd_row<YT, RT, LAY, -1, -1>(a, row, cols, 1.f / cols, buf[first], buf[1], sum, g_row, [&](int which, Row16& v) {
       if (which == 0) load_row<YT, LAY>(static_cast<const YT*>(a.dx) + row * a.dx_ld, cols, v);
       else if (which == 1) load_row<RT, LAY>(static_cast<const RT*>(a.r) + row * a.r_ld, cols, v);
       else if (which == 2) load_row<YT, LAY>(static_cast<const YT*>(a.y) + row * a.y_ld, cols, v);
       else if (which == 3) load_row<RT, LAY>(static_cast<const RT*>(a.dr) + row * a.dr_ld, cols, v);
-      else load_row_dyn<LAY>(a.gate, a.gate_type, row * a.g_ld, cols, v);
-    });
+      else if (which == 4) load_row_dyn<LAY>(a.gate, a.gate_type, row * a.g_ld, cols, v);
+      else if (which == 5) factor_w<LAY>(a, v);
+      else factor_b<LAY>(a, v);
+    }, [] {});
+    if (!two) first ^= 1;
   }
-  bwd_store_sums<LAY>(a, blockIdx.x * blockDim.y + threadIdx.y, sum);
+  bwd_store_sums<LAY>(a, sum, nullptr);
 }
 
 template <class YT, class RT, int MAXT>
 __global__ void __launch_bounds__(MAXT, 1) norm_bwd_kernel(NormBwdArgs a) {
-  __shared__ float buf[2][8 * 3 * 32];
+  __shared__ float buf[2][3 * 32];
   pdl_wait();
   pdl_launch_dependents();
   if (a.vec) bwd_direct<YT, RT, kVec>(a, buf);
+  else if (a.cols >= 384 * a.warps) bwd_direct<YT, RT, kTail>(a, buf);
   else bwd_direct<YT, RT, kScattered>(a, buf);
 }
 
-// Aligned rows with all of dx, r', y: the next rows (dx | r' | y | dr | gate per element) are on
-// their way to shared memory as bulk copies while a row is computed.
-struct RingBwdArgs {
-  int stages, y_bytes, r_bytes, dr_bytes, g_bytes;   // bytes of a row of each (dx has y's type)
-};
-
+// Aligned rows with all of dx, r', y: the next rows (dx, r', y, dr, gate per element) are on their
+// way to shared memory as bulk copies while a row is computed.  The factors per column are put
+// into shared memory once, 32-bit, as each thread reads them.  Rows of one warp go eight to a CTA,
+// each warp with a ring of its own and no CTA barrier until the sums are written.
 template <class YT, class RT, int LAY, int POST, int GATE>
-__global__ void __launch_bounds__(512, 1) norm_bwd_ring_kernel(NormBwdArgs a, RingBwdArgs g) {
+__global__ void __launch_bounds__(512, 1) norm_bwd_ring_kernel(NormBwdArgs a, RingPlan g) {
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ float buf[2][3 * 32];
-  __shared__ uint64_t full[kRingMaxStages];
+  __shared__ uint64_t bars[8][kRingMaxStages];
   __shared__ int abort;
-  const int at_r = g.y_bytes, at_y = at_r + g.r_bytes, at_dr = at_y + g.y_bytes, at_g = at_dr + g.dr_bytes;
-  const int stage_bytes = at_g + g.g_bytes;
+  float4* factors = reinterpret_cast<float4*>(ring);   // [w | b][4][threads of a row]
+  uint8_t* my_ring = ring + kFactorBytes * blockDim.x + threadIdx.y * g.stages * g.stage_bytes;
+  uint64_t* full = bars[threadIdx.y];
   if (threadIdx.x == 0) {
-    abort = 0;
+    if (threadIdx.y == 0) abort = 0;
     for (int i = 0; i < g.stages; ++i) mbar_init(&full[i], 1);
     fence_mbar_init();
   }
   __syncthreads();
   pdl_wait();
   pdl_launch_dependents();
-  auto fetch = [&](int row, int stage) {   // one thread
-    uint8_t* dst = ring + stage * stage_bytes;
-    uint64_t* bar = &full[stage];
-    mbar_arrive_expect_tx(bar, stage_bytes);
-    bulk_load(dst, static_cast<const YT*>(a.dx) + row * a.dx_ld, g.y_bytes, bar);
-    bulk_load(dst + at_r, static_cast<const RT*>(a.r) + row * a.r_ld, g.r_bytes, bar);
-    bulk_load(dst + at_y, static_cast<const YT*>(a.y) + row * a.y_ld, g.y_bytes, bar);
-    if (g.dr_bytes) bulk_load(dst + at_dr, static_cast<const RT*>(a.dr) + row * a.dr_ld, g.dr_bytes, bar);
-    if (g.g_bytes)
-      bulk_load(dst + at_g, static_cast<const uint8_t*>(a.gate) + row * a.g_ld * (g.g_bytes / a.cols), g.g_bytes, bar);
-  };
-  const int step = gridDim.x, cols = a.cols;
+  const int step = gridDim.x * blockDim.y, cols = a.cols;
+  const int row0 = blockIdx.x * blockDim.y + threadIdx.y;
   if (threadIdx.x == 0)
     for (int i = 0; i < g.stages; ++i) {
-      const int64_t row = blockIdx.x + static_cast<int64_t>(i) * step;
-      if (row < a.rows) fetch(static_cast<int>(row), i);
+      const int64_t row = row0 + static_cast<int64_t>(i) * step;
+      if (row < a.rows) ring_fetch(g, static_cast<int>(row), my_ring + i * g.stage_bytes, &full[i]);
     }
+  if (threadIdx.y == 0) {
+    Row16 f;
+    auto put = [&](int at) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        factors[(at + i) * blockDim.x + threadIdx.x] =
+            make_float4(f.v[2 * i].x, f.v[2 * i].y, f.v[2 * i + 1].x, f.v[2 * i + 1].y);
+    };
+    factor_w<LAY>(a, f);
+    put(0);
+    factor_b<LAY>(a, f);
+    put(4);
+  }
+  if (blockDim.y > 1) __syncthreads();   // (a row's threads read what they wrote themselves)
   NormBwdSums sum;
 #pragma unroll
   for (int i = 0; i < 8; ++i) sum.pre.v[i] = sum.post.v[i] = dup2(0.f);
@@ -220,40 +258,51 @@ __global__ void __launch_bounds__(512, 1) norm_bwd_ring_kernel(NormBwdArgs a, Ri
   int stage = 0, parity = 0;
   uint32_t phase = 0;
   bool ok = true;
-  float g_next = a.gate_grad == kGateRow ? load1_dyn(a.gate, a.gate_type, blockIdx.x * a.g_ld) : 0.f;
-  for (int row = blockIdx.x; row < a.rows; row += step) {
+  float g_next = a.gate_grad == kGateRow && row0 < a.rows ? load1_dyn(a.gate, a.gate_type, row0 * a.g_ld) : 0.f;
+  for (int row = row0; row < a.rows; row += step) {
     // after a wait that ran out the CTA still goes through its rows, without their contents
     if (ok) ok = mbar_wait(&full[stage], phase, &abort, &g_op_status, kStWaitProducer);
-    const uint8_t* src = ring + stage * stage_bytes;
+    uint8_t* src = my_ring + stage * g.stage_bytes;
     const float g_row = g_next;   // the gate per row, loaded a row ahead
     if (a.gate_grad == kGateRow && row + static_cast<int64_t>(step) < a.rows)
       g_next = load1_dyn(a.gate, a.gate_type, (row + step) * a.g_ld);
-    
     bwd_row<YT, RT, LAY, POST, GATE>(
         a, row, cols, inv_cols, buf[two ? 0 : parity], buf[1], sum, g_row, [&](int which, Row16& v) {
-          if (which == 0) load_row<YT, LAY>(reinterpret_cast<const YT*>(src), cols, v);
-          else if (which == 1) load_row<RT, LAY>(reinterpret_cast<const RT*>(src + at_r), cols, v);
-          else if (which == 2) load_row<YT, LAY>(reinterpret_cast<const YT*>(src + at_y), cols, v);
-          else if (which == 3) load_row<RT, LAY>(reinterpret_cast<const RT*>(src + at_dr), cols, v);
-          else load_row_dyn<LAY>(src + at_g, a.gate_type, 0, cols, v);
+          if (which >= 5) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float4 f = factors[((which - 5) * 4 + i) * blockDim.x + threadIdx.x];
+              v.v[2 * i] = make_float2(f.x, f.y);
+              v.v[2 * i + 1] = make_float2(f.z, f.w);
+            }
+            return;
+          }
+          // the ring's order: dx, r', y, dr (if any), gate (if per element)
+          const uint8_t* p = src + (which == 4 ? (a.dr ? g.t[4].at : g.t[3].at) : g.t[which].at);
+          if (which == 0 || which == 2) load_row<YT, LAY>(reinterpret_cast<const YT*>(p), cols, v);
+          else if (which != 4) load_row<RT, LAY>(reinterpret_cast<const RT*>(p), cols, v);
+          else load_row_dyn<LAY>(p, a.gate_type, 0, cols, v);
+        },
+        [&] {
+          // every thread has read the stage: the second sum's barrier, or one more
+          if (a.warps == 1) __syncwarp();
+          else if (!two) __syncthreads();
+          const int64_t next = row + static_cast<int64_t>(g.stages) * step;
+          if (threadIdx.x == 0 && ok && next < a.rows) ring_fetch(g, static_cast<int>(next), src, &full[stage]);
         });
     parity ^= 1;
-    // every thread has read the stage: the second sum's barrier, or one more
-    if (!two) __syncthreads();
-    const int64_t next = row + static_cast<int64_t>(g.stages) * step;
-    if (threadIdx.x == 0 && ok && next < a.rows) fetch(static_cast<int>(next), stage);
     if (ok && ++stage == g.stages) {
       stage = 0;
       phase ^= 1u;
     }
   }
-  bwd_store_sums<LAY>(a, blockIdx.x, sum);
   if (!ok && threadIdx.x == 0)   // given up: the loads in flight land first
     for (int i = 0; i < g.stages; ++i) {
       int none = 0;
-      if (blockIdx.x + static_cast<int64_t>(i) * step < a.rows)
+      if (row0 + static_cast<int64_t>(i) * step < a.rows)
         mbar_wait(&full[i], i >= stage ? phase : phase ^ 1u, &none, &g_op_status, kStWaitDrain);
     }
+  bwd_store_sums<LAY>(a, sum, reinterpret_cast<float*>(ring + kFactorBytes * blockDim.x));
 }
 
 // Adds up the parts of a column, 32 columns per CTA, eight warps over the parts, their sums in
@@ -303,19 +352,27 @@ __global__ void __launch_bounds__(1024) norm_total_kernel(const float* v, int ro
 namespace {
 
 // CTAs and with them the parts of the column sums, from the sizes alone (the workspace's size
-// goes by them): of 148 SMs, each with 512 threads' worth of registers.
+// goes by them): 148 SMs, each with 512 threads' worth of registers.
 struct NormBwdShape {
-  int warps, rows_per_cta, direct_parts, ring_ctas, ring_parts;
+  int warps, direct_parts, ring_ctas, ring_rows, ring_parts;   // ring_rows: rows side by side in a CTA
 };
 NormBwdShape bwd_shape(int rows, int cols) {
   NormBwdShape s{};
-  norm_shape(cols, &s.warps, &s.rows_per_cta);
-  const int need = (rows + s.rows_per_cta - 1) / s.rows_per_cta;
-  const int most = 148 * (s.warps > 8 ? 1 : 2);
-  s.direct_parts = (need < most ? need : most) * s.rows_per_cta;
-  if (s.warps >= 2 && s.warps <= 16) {
-    s.ring_ctas = 16 / s.warps;
-    s.ring_parts = rows < 148 * s.ring_ctas ? rows : 148 * s.ring_ctas;
+  if (rows < 1) rows = 1;
+  int rpc;
+  norm_shape(cols, &s.warps, &rpc);
+  const int per_sm = s.warps > 16 ? 1 : 16 / s.warps > 8 ? 8 : 16 / s.warps;
+  s.direct_parts = rows < 148 * per_sm ? rows : 148 * per_sm;
+  if (s.warps <= 16) {
+    s.ring_rows = 1;
+    s.ring_ctas = per_sm;
+    if (s.warps == 1) {   // few rows spread over the SMs, many share a CTA's final sum
+      s.ring_ctas = 2;
+      const int even = (rows + 148 * 2 - 1) / (148 * 2);
+      s.ring_rows = even < 8 ? even : 8;
+    }
+    const int need = (rows + s.ring_rows - 1) / s.ring_rows;
+    s.ring_parts = need < 148 * s.ring_ctas ? need : 148 * s.ring_ctas;
   }
   return s;
 }
@@ -426,13 +483,14 @@ MOE_B200_API int moe_b200_block_norm_backward(const moe_b200_norm_backward_args*
                    (n.gate_grad != kGateElement || rows_aligned(a->dgate, n.dg_ld, a->gate_type));
   const NormBwdShape shape = bwd_shape(a->rows, a->cols);
   n.warps = shape.warps;
-  RingBwdArgs g{};
-  g.y_bytes = a->cols * type_bytes(a->y_type);
-  g.r_bytes = a->cols * type_bytes(a->residual_type);
-  g.dr_bytes = a->dresidual ? g.r_bytes : 0;
-  g.g_bytes = n.gate_grad == kGateElement ? a->cols * type_bytes(a->gate_type) : 0;
-  const int stage_bytes = 2 * g.y_bytes + g.r_bytes + g.dr_bytes + g.g_bytes;
-  g.stages = shape.ring_ctas ? kRingSmem / shape.ring_ctas / stage_bytes : 0;
+  RingPlan g{};
+  ring_add(&g, a->dx, n.dx_ld, a->cols, a->y_type);
+  ring_add(&g, n.r, n.r_ld, a->cols, a->residual_type);
+  ring_add(&g, a->y, n.y_ld, a->cols, a->y_type);
+  ring_add(&g, a->dresidual, n.dr_ld, a->cols, a->residual_type);
+  if (n.gate_grad == kGateElement) ring_add(&g, a->gate, n.g_ld, a->cols, a->gate_type);
+  const int factors = kFactorBytes * n.warps * 32;
+  g.stages = shape.ring_ctas ? (kRingSmem / shape.ring_ctas - factors) / shape.ring_rows / g.stage_bytes : 0;
   if (g.stages > kRingMaxStages) g.stages = kRingMaxStages;
   const bool ring = vec && a->dx && a->y && g.stages >= 2;
   n.parts = ring ? shape.ring_parts : shape.direct_parts;
@@ -456,12 +514,12 @@ MOE_B200_API int moe_b200_block_norm_backward(const moe_b200_norm_backward_args*
                                                              : of_gate(std::integral_constant<int, 0>{});
       e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem);
       if (e == cudaSuccess)
-        e = launch_pdl(kernel, dim3(n.parts), dim3(n.warps * 32), static_cast<size_t>(g.stages) * stage_bytes, st, n, g);
+        e = launch_pdl(kernel, dim3(n.parts), dim3(n.warps * 32, shape.ring_rows),
+                       factors + static_cast<size_t>(g.stages) * g.stage_bytes * shape.ring_rows, st, n, g);
     } else {
-      const dim3 block(n.warps * 32, shape.rows_per_cta), grid(n.parts / shape.rows_per_cta);
       n.vec = vec;
-      auto kernel = block.x * block.y <= 512 ? norm_bwd_kernel<YT, RT, 512> : norm_bwd_kernel<YT, RT, 1024>;
-      e = launch_pdl(kernel, grid, block, 0, st, n);
+      auto kernel = n.warps <= 16 ? norm_bwd_kernel<YT, RT, 512> : norm_bwd_kernel<YT, RT, 1024>;
+      e = launch_pdl(kernel, dim3(n.parts), dim3(n.warps * 32), 0, st, n);
     }
   });
   if (e != cudaSuccess) return report_cuda(e, "block_norm_backward launch");

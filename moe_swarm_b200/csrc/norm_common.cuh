@@ -11,7 +11,7 @@ namespace moe {
 constexpr int kNormPerThread = 16;            // elements of a row in a thread
 constexpr int kNormMaxCols = 1024 * kNormPerThread;
 constexpr int kRingMaxStages = 8;
-constexpr int kRingSmem = 200 * 1024;         // of an SM, shared by its CTAs
+constexpr int kRingSmem = 216 * 1024;         // of an SM, shared by its CTAs
 
 // Sixteen elements as eight pairs: two fused multiply-adds per instruction (f32x2).
 struct Row16 {
@@ -50,20 +50,22 @@ __device__ __forceinline__ float2 dup2(float a) { return make_float2(a, a); }
 // How a row lies in its threads.  kVec, kFull: two chunks of eight neighbours, for 16-byte accesses;
 // kFull: every chunk exists (the row is 16 x its threads long), so nothing is checked.
 // kScattered: 128-column blocks by warp, lane + 32 m within one, so that the accesses of a warp are
-// neighbours whatever the row's alignment.  In each a 128-column block belongs to a half warp
-// (eight elements each) or to a warp (four each).
-enum : int { kScattered = 0, kVec = 1, kFull = 2 };
+// neighbours whatever the row's alignment.  kTail: the same, where only the last four elements of a
+// thread may be missing (rows of at least 384 x their warps, so all of more than 1536 columns).
+// In each a 128-column block belongs to a half warp (eight elements each) or to a warp (four each).
+enum : int { kScattered = 0, kTail = 1, kVec = 2, kFull = 3 };
+constexpr bool is_vec(int lay) { return lay >= kVec; }
 
 // The column of this thread's element q.
 template <int LAY>
 __device__ __forceinline__ int col_of(int q) {
-  if constexpr (LAY != kScattered) return static_cast<int>(threadIdx.x + (q >> 3) * blockDim.x) * 8 + (q & 7);
+  if constexpr (is_vec(LAY)) return static_cast<int>(threadIdx.x + (q >> 3) * blockDim.x) * 8 + (q & 7);
   return static_cast<int>((threadIdx.x >> 5) + (q >> 2) * (blockDim.x >> 5)) * 128 +
          static_cast<int>(threadIdx.x & 31) + 32 * (q & 3);
 }
 template <int LAY>
 __device__ __forceinline__ bool exists(int q, int cols) {
-  return LAY == kFull || col_of<LAY>(q) < cols;
+  return LAY == kFull || (LAY == kTail && q < 12) || col_of<LAY>(q) < cols;
 }
 
 template <class T>
@@ -90,7 +92,7 @@ __device__ __forceinline__ void load_chunk(const T* p, float2* v) {
 
 template <class T, int LAY>
 __device__ __forceinline__ void load_row(const T* row, int cols, Row16& r) {
-  if constexpr (LAY != kScattered) {
+  if constexpr (is_vec(LAY)) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       if (exists<LAY>(8 * i, cols)) {
@@ -107,7 +109,7 @@ __device__ __forceinline__ void load_row(const T* row, int cols, Row16& r) {
 }
 template <class T, int LAY>
 __device__ __forceinline__ void store_row(T* row, int cols, const Row16& r) {
-  if constexpr (LAY != kScattered) {
+  if constexpr (is_vec(LAY)) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       if (!exists<LAY>(8 * i, cols)) continue;
@@ -152,7 +154,7 @@ __device__ __forceinline__ void load_weight(const void* p, int type, float off, 
 // have met an infinite factor of the row since.
 template <int LAY>
 __device__ __forceinline__ float squares_existing(const Row16& r, int cols) {
-  if constexpr (LAY == kScattered) {
+  if constexpr (!is_vec(LAY)) {
     float s = 0.f;
 #pragma unroll
     for (int q = 0; q < 16; ++q) s = exists<LAY>(q, cols) ? fmaf(r[q], r[q], s) : s;
@@ -174,6 +176,39 @@ __device__ __forceinline__ float dot16(const Row16& a, const Row16& b) {
 #pragma unroll
   for (int i = 1; i < 8; ++i) s = fma2(a.v[i], b.v[i], s);
   return s.x + s.y;
+}
+
+// ---------------------------------------------------------------- rings of rows
+// The row tensors that a persistent CTA streams through shared memory: rows of `bytes` bytes,
+// `pitch` bytes apart, each with its place in a stage.
+struct RingTensor {
+  const uint8_t* base;
+  int64_t pitch;
+  int bytes, at;
+};
+constexpr int kRingTensors = 5;
+struct RingPlan {
+  RingTensor t[kRingTensors];
+  int n, stages, stage_bytes;
+};
+
+// One thread: starts the copies of a row's tensors into a stage, completing on `bar`.
+__device__ __forceinline__ void ring_fetch(const RingPlan& g, int row, uint8_t* stage, uint64_t* bar) {
+  mbar_arrive_expect_tx(bar, g.stage_bytes);
+#pragma unroll
+  for (int i = 0; i < kRingTensors; ++i)
+    if (i < g.n) bulk_load(stage + g.t[i].at, g.t[i].base + row * g.t[i].pitch, g.t[i].bytes, bar);
+}
+
+// Host: adds a tensor of 16-byte aligned rows (not if p is null).
+inline void ring_add(RingPlan* g, const void* p, int64_t ld, int cols, int type) {
+  if (!p) return;
+  RingTensor& t = g->t[g->n++];
+  t.base = static_cast<const uint8_t*>(p);
+  t.pitch = ld * type_bytes(type);
+  t.bytes = cols * type_bytes(type);
+  t.at = g->stage_bytes;
+  g->stage_bytes += t.bytes;
 }
 
 // Warps of a row and rows of a CTA: a row takes as few warps as hold it; short rows share a CTA

@@ -182,6 +182,33 @@ __device__ __forceinline__ void row_sum(float (&v)[N], int warps, float* buf) {
   for (int k = 0; k < N; ++k) v[k] = warp_sum(lane < warps ? b[k * 32 + lane] : 0.f);
 }
 
+// The same for three values of a row of up to 16 warps, with less than half the shuffles: a warp's
+// butterfly leaves each of four groups of lanes (bits 3 and 4 of the lane) with one value.
+__device__ __forceinline__ void row_sum3(float (&v)[3], int warps, float* buf) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const bool hi = lane & 16, odd = lane & 8;
+  // lanes below 16 go on with v[0] and v[1], the others with v[2] (and nothing)
+  const float send0 = hi ? v[0] : v[2], send1 = hi ? v[1] : 0.f;
+  float p = (hi ? v[2] : v[0]) + __shfl_xor_sync(0xffffffffu, send0, 16);
+  float q = (hi ? 0.f : v[1]) + __shfl_xor_sync(0xffffffffu, send1, 16);
+  float s = (odd ? q : p) + __shfl_xor_sync(0xffffffffu, odd ? p : q, 8);
+#pragma unroll
+  for (int d = 4; d >= 1; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+  if (warps > 1) {
+    float* b = buf + threadIdx.y * 3 * 32;
+    const int k = lane >> 3;   // 0, 1, 2: this group's value
+    if ((lane & 7) == 0 && k < 3) b[k * 32 + warp] = s;
+    __syncthreads();
+    const int j = lane & 7;
+    s = k < 3 ? (j < warps ? b[k * 32 + j] : 0.f) + (j + 8 < warps ? b[k * 32 + j + 8] : 0.f) : 0.f;
+#pragma unroll
+    for (int d = 4; d >= 1; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+  }
+  v[0] = __shfl_sync(0xffffffffu, s, 0);
+  v[1] = __shfl_sync(0xffffffffu, s, 8);
+  v[2] = __shfl_sync(0xffffffffu, s, 16);
+}
+
 // A programmatic dependent launch on `st` in clusters of `cluster` CTAs along x: the kernel may
 // become resident while its predecessor drains, and calls pdl_wait() before it touches anything
 // that an earlier kernel wrote or reads.

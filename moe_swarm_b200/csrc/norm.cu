@@ -99,16 +99,17 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) norm_fwd_kernel(NormArgs a)
   pdl_launch_dependents();
   const int row = blockIdx.x * blockDim.y + threadIdx.y;
   const int cols = row < a.rows ? a.cols : 0;
+  const int from = min(row, a.rows - 1);   // a row that exists
   Row16 r, w;
   if (a.residual) {
-    load_row<RT, LAY>(static_cast<const RT*>(a.residual) + row * a.r_ld, cols, r);
+    load_row<RT, LAY>(static_cast<const RT*>(a.residual) + from * a.r_ld, cols, r);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) r.v[i] = dup2(0.f);
   }
   if (a.y) {
     Row16 y;
-    load_row<YT, LAY>(static_cast<const YT*>(a.y) + row * a.y_ld, cols, y);
+    load_row<YT, LAY>(static_cast<const YT*>(a.y) + from * a.y_ld, cols, y);
     float k = a.scale;
     if (a.post_w) {
       load_weight<LAY>(a.post_w, a.post_type, a.off, cols, w);
@@ -119,7 +120,7 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) norm_fwd_kernel(NormArgs a)
       for (int i = 0; i < 8; ++i) y.v[i] = mul2(y.v[i], w.v[i]);
     }
     if (a.gate && a.gate_cols) {
-      load_row_dyn<LAY>(a.gate, a.gate_type, row * a.g_ld, cols, w);
+      load_row_dyn<LAY>(a.gate, a.gate_type, from * a.g_ld, cols, w);
 #pragma unroll
       for (int i = 0; i < 8; ++i) y.v[i] = mul2(y.v[i], w.v[i]);
     } else if (a.gate && cols) {
@@ -308,7 +309,7 @@ MOE_B200_API int moe_b200_block_norm(const moe_b200_norm_args* a, void* stream) 
       auto laid = [&](auto post) {
         constexpr bool P = decltype(post)::value;
         return a->cols == n.warps * 32 * kNormPerThread ? norm_ring_kernel<YT, RT, P, kFull>
-                                                        : norm_ring_kernel<YT, RT, P, kVec>;
+                                                        : norm_ring_kernel<YT, RT, P, kHalf>;
       };
       auto kernel = a->post_weight ? laid(std::true_type{}) : laid(std::false_type{});
       e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem);

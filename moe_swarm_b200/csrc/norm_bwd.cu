@@ -23,7 +23,7 @@ struct NormBwdArgs {
   void *dres, *dy, *dgate;          // dgate: per element (gate type) or per row (fp32); null: none
   float* partial;                   // [slots][parts][cols]: sums of dx r^ and of G y^
   int64_t dx_ld, dr_ld, r_ld, y_ld, g_ld, dres_ld, dy_ld, dg_ld;
-  int rows, cols, warps, parts, vec;
+  int rows, cols, warps, parts;
   int post_type, pre_type, gate_type, gate_cols;
   int gate_grad, pre_slot, post_slot;
   float scale, eps, off;
@@ -197,19 +197,18 @@ __device__ __forceinline__ void bwd_direct(const NormBwdArgs& a, float (*buf)[3 
   bwd_store_sums<LAY>(a, sum, nullptr);
 }
 
-template <class YT, class RT, int MAXT>
+template <class YT, class RT, int LAY, int MAXT>
 __global__ void __launch_bounds__(MAXT, 1) norm_bwd_kernel(NormBwdArgs a) {
   __shared__ float buf[2][3 * 32];
   pdl_wait();
   pdl_launch_dependents();
-  if (a.vec) bwd_direct<YT, RT, kVec>(a, buf);
-  else if (a.cols >= 384 * a.warps) bwd_direct<YT, RT, kTail>(a, buf);
-  else bwd_direct<YT, RT, kScattered>(a, buf);
+  bwd_direct<YT, RT, LAY>(a, buf);
 }
 
 // Aligned rows with all of dx, r', y: the next rows (dx, r', y, dr, gate per element) are on their
 // way to shared memory as bulk copies while a row is computed.  The factors per column are put
-// into shared memory once, 32-bit, as each thread reads them.  Rows of one warp go eight to a CTA,
+// into shared memory once, 32-bit, as each thread reads them, beside a 16-bit residual; a 32-bit one
+// leaves its ring too little room, and they are read in place.  Rows of one warp go eight to a CTA,
 // each warp with a ring of its own and no CTA barrier until the sums are written.
 template <class YT, class RT, int LAY, int POST, int GATE>
 __global__ void __launch_bounds__(512, 1) norm_bwd_ring_kernel(NormBwdArgs a, RingPlan g) {
@@ -217,8 +216,10 @@ __global__ void __launch_bounds__(512, 1) norm_bwd_ring_kernel(NormBwdArgs a, Ri
   __shared__ float buf[2][3 * 32];
   __shared__ uint64_t bars[8][kRingMaxStages];
   __shared__ int abort;
+  constexpr bool kShared = sizeof(RT) == 2;
+  const int factor_bytes = kShared ? kFactorBytes * blockDim.x : 0;
   float4* factors = reinterpret_cast<float4*>(ring);   // [w | b][4][threads of a row]
-  uint8_t* my_ring = ring + kFactorBytes * blockDim.x + threadIdx.y * g.stages * g.stage_bytes;
+  uint8_t* my_ring = ring + factor_bytes + threadIdx.y * g.stages * g.stage_bytes;
   uint64_t* full = bars[threadIdx.y];
   if (threadIdx.x == 0) {
     if (threadIdx.y == 0) abort = 0;
@@ -235,7 +236,7 @@ __global__ void __launch_bounds__(512, 1) norm_bwd_ring_kernel(NormBwdArgs a, Ri
       const int64_t row = row0 + static_cast<int64_t>(i) * step;
       if (row < a.rows) ring_fetch(g, static_cast<int>(row), my_ring + i * g.stage_bytes, &full[i]);
     }
-  if (threadIdx.y == 0) {
+  if (kShared && threadIdx.y == 0) {
     Row16 f;
     auto put = [&](int at) {
 #pragma unroll
@@ -268,6 +269,11 @@ __global__ void __launch_bounds__(512, 1) norm_bwd_ring_kernel(NormBwdArgs a, Ri
       g_next = load1_dyn(a.gate, a.gate_type, (row + step) * a.g_ld);
     bwd_row<YT, RT, LAY, POST, GATE>(
         a, row, cols, inv_cols, buf[two ? 0 : parity], buf[1], sum, g_row, [&](int which, Row16& v) {
+          if (which >= 5 && !kShared) {
+            if (which == 5) factor_w<LAY>(a, v);
+            else factor_b<LAY>(a, v);
+            return;
+          }
           if (which >= 5) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -302,7 +308,7 @@ __global__ void __launch_bounds__(512, 1) norm_bwd_ring_kernel(NormBwdArgs a, Ri
       if (row0 + static_cast<int64_t>(i) * step < a.rows)
         mbar_wait(&full[i], i >= stage ? phase : phase ^ 1u, &none, &g_op_status, kStWaitDrain);
     }
-  bwd_store_sums<LAY>(a, sum, reinterpret_cast<float*>(ring + kFactorBytes * blockDim.x));
+  bwd_store_sums<LAY>(a, sum, reinterpret_cast<float*>(ring + factor_bytes));
 }
 
 // Adds up the parts of a column, 32 columns per CTA, eight warps over the parts, their sums in
@@ -361,7 +367,7 @@ NormBwdShape bwd_shape(int rows, int cols) {
   if (rows < 1) rows = 1;
   int rpc;
   norm_shape(cols, &s.warps, &rpc);
-  const int per_sm = s.warps > 16 ? 1 : 16 / s.warps > 8 ? 8 : 16 / s.warps;
+  const int per_sm = s.warps > 16 ? 1 : 16 / s.warps;
   s.direct_parts = rows < 148 * per_sm ? rows : 148 * per_sm;
   if (s.warps <= 16) {
     s.ring_rows = 1;
@@ -376,6 +382,8 @@ NormBwdShape bwd_shape(int rows, int cols) {
   }
   return s;
 }
+
+bool shared_factors(int residual_type) { return type_bytes(residual_type) == 2; }   // as the ring kernel has them
 
 int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
 
@@ -489,10 +497,10 @@ MOE_B200_API int moe_b200_block_norm_backward(const moe_b200_norm_backward_args*
   ring_add(&g, a->y, n.y_ld, a->cols, a->y_type);
   ring_add(&g, a->dresidual, n.dr_ld, a->cols, a->residual_type);
   if (n.gate_grad == kGateElement) ring_add(&g, a->gate, n.g_ld, a->cols, a->gate_type);
-  const int factors = kFactorBytes * n.warps * 32;
+  const int factors = shared_factors(a->residual_type) ? kFactorBytes * n.warps * 32 : 0;
   g.stages = shape.ring_ctas ? (kRingSmem / shape.ring_ctas - factors) / shape.ring_rows / g.stage_bytes : 0;
   if (g.stages > kRingMaxStages) g.stages = kRingMaxStages;
-  const bool ring = vec && a->dx && a->y && g.stages >= 2;
+  const bool ring = vec && a->dx && a->y && g.stages >= 1;
   n.parts = ring ? shape.ring_parts : shape.direct_parts;
   // the row sums of a gate that is one number go through the workspace
   float* row_dots = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) +
@@ -502,23 +510,30 @@ MOE_B200_API int moe_b200_block_norm_backward(const moe_b200_norm_backward_args*
     using YT = decltype(yt);
     using RT = decltype(rt);
     if (ring) {
-      // every combination has its kernel where rows fill their threads; one for all elsewhere
-      auto of_gate = [&](auto post) {
-        constexpr int P = decltype(post)::value;
-        return n.gate_grad == kGateElement ? norm_bwd_ring_kernel<YT, RT, kFull, P, 2>
-               : n.gate_grad == kGateRow   ? norm_bwd_ring_kernel<YT, RT, kFull, P, 1>
-                                           : norm_bwd_ring_kernel<YT, RT, kFull, P, 0>;
+      auto of_gate = [&](auto lay, auto post) {
+        constexpr int L = decltype(lay)::value, P = decltype(post)::value;
+        return n.gate_grad == kGateElement ? norm_bwd_ring_kernel<YT, RT, L, P, 2>
+               : n.gate_grad == kGateRow   ? norm_bwd_ring_kernel<YT, RT, L, P, 1>
+                                           : norm_bwd_ring_kernel<YT, RT, L, P, 0>;
       };
-      auto kernel = a->cols != n.warps * 32 * kNormPerThread ? norm_bwd_ring_kernel<YT, RT, kVec, -1, -1>
-                    : a->post_weight                         ? of_gate(std::integral_constant<int, 1>{})
-                                                             : of_gate(std::integral_constant<int, 0>{});
+      auto of_post = [&](auto lay) {
+        return a->post_weight ? of_gate(lay, std::integral_constant<int, 1>{}) : of_gate(lay, std::integral_constant<int, 0>{});
+      };
+      auto kernel = a->cols == n.warps * 32 * kNormPerThread ? of_post(std::integral_constant<int, kFull>{})
+                    : a->cols >= 256                         ? of_post(std::integral_constant<int, kHalf>{})
+                                                             : norm_bwd_ring_kernel<YT, RT, kVec, -1, -1>;
       e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem);
       if (e == cudaSuccess)
         e = launch_pdl(kernel, dim3(n.parts), dim3(n.warps * 32, shape.ring_rows),
                        factors + static_cast<size_t>(g.stages) * g.stage_bytes * shape.ring_rows, st, n, g);
     } else {
-      n.vec = vec;
-      auto kernel = n.warps <= 16 ? norm_bwd_kernel<YT, RT, 512> : norm_bwd_kernel<YT, RT, 1024>;
+      auto sized = [&](auto t) {
+        constexpr int MAXT = decltype(t)::value;
+        return vec                             ? norm_bwd_kernel<YT, RT, kVec, MAXT>
+               : a->cols >= 384 * n.warps ? norm_bwd_kernel<YT, RT, kTail, MAXT>
+                                          : norm_bwd_kernel<YT, RT, kScattered, MAXT>;
+      };
+      auto kernel = n.warps <= 16 ? sized(std::integral_constant<int, 512>{}) : sized(std::integral_constant<int, 1024>{});
       e = launch_pdl(kernel, dim3(n.parts), dim3(n.warps * 32), 0, st, n);
     }
   });

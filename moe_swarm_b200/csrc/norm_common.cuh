@@ -47,13 +47,14 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 }
 __device__ __forceinline__ float2 dup2(float a) { return make_float2(a, a); }
 
-// How a row lies in its threads.  kVec, kFull: two chunks of eight neighbours, for 16-byte accesses;
-// kFull: every chunk exists (the row is 16 x its threads long), so nothing is checked.
+// How a row lies in its threads.  kVec, kHalf, kFull: two chunks of eight neighbours, for 16-byte
+// accesses; kHalf: every first chunk exists (rows of at least 256 x their warps, so all of more than
+// 256 columns); kFull: every chunk exists (the row is 16 x its threads long), so nothing is checked.
 // kScattered: 128-column blocks by warp, lane + 32 m within one, so that the accesses of a warp are
 // neighbours whatever the row's alignment.  kTail: the same, where only the last four elements of a
 // thread may be missing (rows of at least 384 x their warps, so all of more than 1536 columns).
 // In each a 128-column block belongs to a half warp (eight elements each) or to a warp (four each).
-enum : int { kScattered = 0, kTail = 1, kVec = 2, kFull = 3 };
+enum : int { kScattered = 0, kTail = 1, kVec = 2, kHalf = 3, kFull = 4 };
 constexpr bool is_vec(int lay) { return lay >= kVec; }
 
 // The column of this thread's element q.
@@ -65,7 +66,7 @@ __device__ __forceinline__ int col_of(int q) {
 }
 template <int LAY>
 __device__ __forceinline__ bool exists(int q, int cols) {
-  return LAY == kFull || (LAY == kTail && q < 12) || col_of<LAY>(q) < cols;
+  return LAY == kFull || (LAY == kHalf && q < 8) || (LAY == kTail && q < 12) || col_of<LAY>(q) < cols;
 }
 
 template <class T>
@@ -90,6 +91,8 @@ __device__ __forceinline__ void load_chunk(const T* p, float2* v) {
   }
 }
 
+// (The row itself must exist: what lies beyond its end is not read, but where there is nothing to
+// read at all, its first element may be.)
 template <class T, int LAY>
 __device__ __forceinline__ void load_row(const T* row, int cols, Row16& r) {
   if constexpr (is_vec(LAY)) {
@@ -103,8 +106,19 @@ __device__ __forceinline__ void load_row(const T* row, int cols, Row16& r) {
       }
     }
   } else {
+    // kScattered: unconditional loads, so that all sixteen are in flight together; a branch around
+    // each would wait for it (backward of 5000 x 700: 74 -> 54 us).  The last four of kTail are
+    // better left out (forward of 4096 x 5001: 62 -> 57 us).
 #pragma unroll
-    for (int q = 0; q < 16; ++q) r[q] = exists<LAY>(q, cols) ? to_f(row[col_of<LAY>(q)]) : 0.f;
+    for (int q = 0; q < 16; ++q) {
+      const bool ok = exists<LAY>(q, cols);
+      if (LAY == kTail) {
+        r[q] = ok ? to_f(row[col_of<LAY>(q)]) : 0.f;
+      } else {
+        const float f = to_f(row[ok ? col_of<LAY>(q) : 0]);
+        r[q] = ok ? f : 0.f;
+      }
+    }
   }
 }
 template <class T, int LAY>

@@ -9,11 +9,11 @@
 #include <type_traits>
 
 #include "int8_gemm.cuh"
+#include "norm_common.cuh"
 
 namespace moe {
 
-constexpr int kQuantPerThread = 32;                      // four 8-element chunks
-constexpr int kQuantMaxCols = 1024 * kQuantPerThread;
+constexpr int kQuantMaxCols = 2 * kNormMaxCols;
 constexpr int kInt8MaxK = 131056;
 constexpr int kInt8StreamMaxT = 256;
 
@@ -25,81 +25,201 @@ struct QuantArgs {
   int rows, cols, warps, type, swiglu;
 };
 
-// One row in the registers of a group of warps: maximum, then codes.
-template <class XT, bool VEC>
-__global__ void __launch_bounds__(1024, 1) quant_kernel(QuantArgs a) {
+// silu(gate) * up.  The fast exponential is off by (|gate| + 4) 2^-24 of itself: a share of the
+// product that only counts where gate is far below 0 and the product next to nothing, and that is
+// small beside half a code, 2^-8 of the row's largest.
+__device__ __forceinline__ void swiglu16(Row16& up, const Row16& gate) {
+#pragma unroll
+  for (int j = 0; j < 16; ++j) up[j] *= silu_fast(gate[j]);
+}
+
+__device__ __forceinline__ float row_amax(const Row16& v) {
+  float m = fabsf(v[0]);
+#pragma unroll
+  for (int j = 1; j < 16; ++j) m = max_nan(m, fabsf(v[j]));
+  return m;
+}
+// Maximum over a row's warps (blockDim = (32 * warps, rows)); `buf` [rows][32] is free again after
+// the next CTA barrier.
+__device__ __forceinline__ float row_max(float m, int warps, float* buf) {
+#pragma unroll
+  for (int d = 16; d >= 1; d >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
+  if (warps == 1) return m;
+  const int lane = threadIdx.x & 31;
+  float* b = buf + threadIdx.y * 32;
+  if (lane == 0) b[threadIdx.x >> 5] = m;
+  __syncthreads();
+  m = lane < warps ? b[lane] : 0.f;
+#pragma unroll
+  for (int d = 16; d >= 1; d >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
+  return m;
+}
+
+// A row's scale and its reciprocal; a row with a NaN or an infinity: NaN, and 0 for zero codes.
+__device__ __forceinline__ float quant_scale(float m, float* inv) {
+  const bool finite = m <= 3.4028234663852886e38f;
+  const float sc = finite ? fmaxf(m / 127.f, 1.17549435082228751e-38f) : __uint_as_float(0x7fc00000u);
+  *inv = finite ? 1.f / sc : 0.f;
+  return sc;
+}
+
+// Codes: v * inv lies in [-127, 127] to 2 units, so adding 1.5 * 2^23 rounds it to an integer (ties
+// to even) whose two's complement is the sum's low byte; four bytes are picked out of four sums.
+// (Conversions run at an eighth of the rate.)
+__device__ __forceinline__ uint32_t codes4(float2 a, float2 b, float2 inv) {
+  const float2 magic = dup2(12582912.f);
+  a = fma2(a, inv, magic);
+  b = fma2(b, inv, magic);
+  const uint32_t lo = __byte_perm(__float_as_uint(a.x), __float_as_uint(a.y), 0x0040);
+  const uint32_t hi = __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0040);
+  return __byte_perm(lo, hi, 0x5410);
+}
+template <int LAY>
+__device__ __forceinline__ void store_codes(int8_t* row, int cols, const Row16& v, float inv) {
+  uint32_t c[4];
+  const float2 k = dup2(inv);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c[i] = inv != 0.f ? codes4(v.v[2 * i], v.v[2 * i + 1], k) : 0u;
+  if constexpr (is_vec(LAY)) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (exists<LAY>(8 * i, cols)) *reinterpret_cast<uint2*>(row + col_of<LAY>(8 * i)) = make_uint2(c[2 * i], c[2 * i + 1]);
+  } else {
+#pragma unroll
+    for (int q = 0; q < 16; ++q)
+      if (exists<LAY>(q, cols)) row[col_of<LAY>(q)] = static_cast<int8_t>(c[q >> 2] >> (8 * (q & 3)));
+  }
+}
+
+// One row in the registers of a group of warps, N times 16 elements per thread (N = 2: the second
+// 16 are those of the row's second half of threads x 16 columns).
+template <class XT, int LAY, int N>
+__global__ void __launch_bounds__(N == 1 ? 512 : 1024, 1) quant_kernel(QuantArgs a) {
   __shared__ float buf[8 * 32];
   pdl_wait();
   pdl_launch_dependents();
   const int row = blockIdx.x * blockDim.y + threadIdx.y;
-  const int cols = row < a.rows ? a.cols : 0;
-  const XT* src = static_cast<const XT*>(a.x) + row * a.x_ld;
-  float v[4][8], m = 0.f;
+  const XT* src = static_cast<const XT*>(a.x) + min(row, a.rows - 1) * a.x_ld;
+  Row16 v[N];
+  float m = 0.f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int e0 = (threadIdx.x + i * blockDim.x) * 8, n = min(8, cols - e0);
-    load8<XT, VEC>(src + e0, n, v[i]);
+  for (int n = 0; n < N; ++n) {
+    const int at = n * 16 * blockDim.x, cols = row < a.rows ? max(0, a.cols - at) : 0;
+    load_row<XT, LAY>(src + (cols ? at : 0), cols, v[n]);
     if (a.swiglu) {
-      float g[8];
-      load8<XT, VEC>(src + a.cols + e0, n, g);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] *= g[j] / (1.f + expf(-g[j]));
+      Row16 g;
+      load_row<XT, LAY>(src + (cols ? a.cols + at : 0), cols, g);
+      swiglu16(v[n], g);
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) m = max_nan(m, fabsf(v[i][j]));
+    m = max_nan(m, row_amax(v[n]));
   }
-#pragma unroll
-  for (int d = 16; d >= 1; d >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
-  if (a.warps > 1) {
-    const int lane = threadIdx.x & 31;
-    if (lane == 0) buf[threadIdx.y * 32 + (threadIdx.x >> 5)] = m;
-    __syncthreads();
-    m = lane < a.warps ? buf[threadIdx.y * 32 + lane] : 0.f;
-#pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
-  }
+  m = row_max(m, a.warps, buf);
   if (row >= a.rows) return;
-  const bool finite = m <= 3.4028234663852886e38f;
-  const float sc = finite ? fmaxf(m / 127.f, 1.17549435082228751e-38f) : __uint_as_float(0x7fc00000u);
-  const float inv = finite ? 1.f / sc : 0.f;
+  float inv;
+  const float sc = quant_scale(m, &inv);
   if (threadIdx.x == 0) a.scale[row] = sc;
-  int8_t* dst = a.q + row * a.q_ld;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int e0 = (threadIdx.x + i * blockDim.x) * 8, n = min(8, cols - e0);
-    if (n <= 0) continue;
-    uint32_t b[2] = {0, 0};
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int c = finite ? max(-127, min(127, __float2int_rn(v[i][j] * inv))) : 0;
-      b[j >> 2] |= static_cast<uint32_t>(c & 0xff) << (8 * (j & 3));
-    }
-    if constexpr (VEC) {
-      *reinterpret_cast<uint2*>(dst + e0) = make_uint2(b[0], b[1]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (j < n) dst[e0 + j] = static_cast<int8_t>(b[j >> 2] >> (8 * (j & 3)));
-    }
+  for (int n = 0; n < N; ++n) {
+    const int at = n * 16 * blockDim.x;
+    if (at < a.cols) store_codes<LAY>(a.q + row * a.q_ld + at, a.cols - at, v[n], inv);
   }
 }
 
+// Many aligned rows: persistent CTAs with their next rows on the way to shared memory, as the norm's.
+template <class XT, int LAY>
+__global__ void __launch_bounds__(512, 2) quant_ring_kernel(QuantArgs a, RingPlan g) {
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ float buf[2][32];   // of even and odd rows
+  __shared__ uint64_t full[kRingMaxStages];
+  __shared__ int abort;
+  if (threadIdx.x == 0) {
+    abort = 0;
+    for (int i = 0; i < g.stages; ++i) mbar_init(&full[i], 1);
+    fence_mbar_init();
+  }
+  __syncthreads();
+  pdl_wait();
+  pdl_launch_dependents();
+  const int step = gridDim.x, cols = a.cols;
+  if (threadIdx.x == 0)
+    for (int i = 0; i < g.stages; ++i) {
+      const int64_t row = blockIdx.x + static_cast<int64_t>(i) * step;
+      if (row < a.rows) ring_fetch(g, static_cast<int>(row), ring + i * g.stage_bytes, &full[i]);
+    }
+  int stage = 0, parity = 0;
+  uint32_t phase = 0;
+  bool ok = true;
+  for (int row = blockIdx.x; row < a.rows; row += step) {
+    // after a wait that ran out the CTA still goes through its rows, without their contents
+    if (ok) ok = mbar_wait(&full[stage], phase, &abort, &g_op_status, kStWaitProducer);
+    uint8_t* src = ring + stage * g.stage_bytes;
+    Row16 v;
+    load_row<XT, LAY>(reinterpret_cast<const XT*>(src), cols, v);
+    if (a.swiglu) {
+      Row16 gate;
+      load_row<XT, LAY>(reinterpret_cast<const XT*>(src + g.t[1].at), cols, gate);
+      swiglu16(v, gate);
+    }
+    const float m = row_max(row_amax(v), a.warps, buf[parity]);
+    parity ^= 1;
+    // every thread has its part of the stage (row_max's barrier)
+    const int64_t next = row + static_cast<int64_t>(g.stages) * step;
+    if (threadIdx.x == 0 && ok && next < a.rows) ring_fetch(g, static_cast<int>(next), src, &full[stage]);
+    if (ok && ++stage == g.stages) {
+      stage = 0;
+      phase ^= 1u;
+    }
+    float inv;
+    const float sc = quant_scale(m, &inv);
+    if (threadIdx.x == 0) a.scale[row] = sc;
+    store_codes<LAY>(a.q + row * a.q_ld, cols, v, inv);
+  }
+  if (!ok && threadIdx.x == 0)   // given up: the loads in flight land first
+    for (int i = 0; i < g.stages; ++i) {
+      int none = 0;
+      if (blockIdx.x + static_cast<int64_t>(i) * step < a.rows)
+        mbar_wait(&full[i], i >= stage ? phase : phase ^ 1u, &none, &g_op_status, kStWaitDrain);
+    }
+}
+
+cudaError_t quant_status(cudaStream_t st, bool clear, int* v) { return take_status(st, clear, v); }
+
 namespace {
 
-cudaError_t quant_launch(const QuantArgs& q0, cudaStream_t st) {
+cudaError_t quant_launch(const QuantArgs& q0, int sms, cudaStream_t st) {
   QuantArgs q = q0;
   if (q.rows == 1) q.x_ld = q.q_ld = 0;   // a single row has no pitch
-  q.warps = (q.cols + 32 * kQuantPerThread - 1) / (32 * kQuantPerThread);
-  const int rpc = q.warps >= 8 ? 1 : 8 / q.warps;
-  const dim3 block(q.warps * 32, rpc), grid((q.rows + rpc - 1) / rpc);
+  int rpc;
+  const bool twice = q.cols > kNormMaxCols / 2;   // 32 elements per thread
+  norm_shape(twice ? (q.cols + 1) / 2 : q.cols, &q.warps, &rpc);
   const bool vec = q.cols % 8 == 0 && rows_aligned(q.x, q.x_ld, q.type) &&
                    (reinterpret_cast<uintptr_t>(q.q) & 7u) == 0 && q.q_ld % 8 == 0;
+  cudaError_t e = cudaSuccess;
   auto go = [&](auto t) {
     using XT = decltype(t);
-    return vec ? launch_pdl(quant_kernel<XT, true>, grid, block, 0, st, q)
-               : launch_pdl(quant_kernel<XT, false>, grid, block, 0, st, q);
+    // the ring: aligned rows of two warps or more, at least four per SM
+    RingPlan g{};
+    ring_add(&g, q.x, q.x_ld, q.cols, q.type);
+    if (q.swiglu) ring_add(&g, static_cast<const XT*>(q.x) + q.cols, q.x_ld, q.cols, q.type);
+    const int ctas = q.warps >= 2 ? 32 / q.warps : 0;   // 1024 threads of an SM
+    g.stages = ctas ? kRingSmem / ctas / g.stage_bytes : 0;
+    if (g.stages > kRingMaxStages) g.stages = kRingMaxStages;
+    if (vec && !twice && q.rows >= 4 * sms && g.stages >= 2) {
+      const dim3 grid(q.rows < ctas * sms ? q.rows : ctas * sms), block(q.warps * 32);
+      auto kernel = q.cols == q.warps * 32 * kNormPerThread ? quant_ring_kernel<XT, kFull> : quant_ring_kernel<XT, kHalf>;
+      e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem);
+      if (e == cudaSuccess) e = launch_pdl(kernel, grid, block, static_cast<size_t>(g.stages) * g.stage_bytes, st, q, g);
+      return;
+    }
+    const dim3 block(q.warps * 32, rpc), grid((q.rows + rpc - 1) / rpc);
+    auto kernel = twice ? (vec ? quant_kernel<XT, kVec, 2> : quant_kernel<XT, kScattered, 2>)
+                        : (vec ? quant_kernel<XT, kVec, 1> : quant_kernel<XT, kScattered, 1>);
+    e = launch_pdl(kernel, grid, block, 0, st, q);
   };
-  return q.type == MOE_B200_BF16 ? go(bf16{}) : q.type == MOE_B200_FP16 ? go(fp16{}) : go(float{});
+  if (q.type == MOE_B200_BF16) go(bf16{});
+  else if (q.type == MOE_B200_FP16) go(fp16{});
+  else go(float{});
+  return e;
 }
 
 int quant_check(const void* x, int type, int rows, int cols, const char** why) {
@@ -136,7 +256,7 @@ MOE_B200_API int moe_b200_quantize_int8(const moe_b200_quantize_args* a, void* s
   q.cols = a->cols;
   q.type = a->x_type;
   q.swiglu = a->swiglu;
-  const cudaError_t e = quant_launch(q, static_cast<cudaStream_t>(stream));
+  const cudaError_t e = quant_launch(q, sms, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? MOE_B200_OK : report_cuda(e, "quantize_int8 launch");
 }
 
@@ -197,7 +317,7 @@ MOE_B200_API int moe_b200_int8_linear(const moe_b200_linear_args* a, void* works
     q.cols = a->in_features;
     q.type = a->x_type;
     q.swiglu = a->swiglu;
-    e = quant_launch(q, st);
+    e = quant_launch(q, sms, st);
     if (e != cudaSuccess) return report_cuda(e, "int8_linear quantisation launch");
     q_rows = q.q;
     q_ld = q.q_ld;

@@ -16,19 +16,24 @@
 
 namespace moe {
 
-// float(sum) * (sx * sw) + bias of a tile's column, rounded once to the output's type
+// 32 consecutive outputs of a row, n of which exist.  align: bytes that every such address is a
+// multiple of (32 or 16: whole vectors).
 template <class YT>
-__device__ __forceinline__ void store_cols32(YT* dst, int n, bool vec, const float* v) {
-  if (vec && n >= 32) {
+__device__ __forceinline__ void store_cols32(YT* dst, int n, int align, const float* v) {
+  if (n >= 32) {
 #pragma unroll
     for (int i = 0; i < 32; i += 32 / static_cast<int>(sizeof(YT))) {
-      if constexpr (sizeof(YT) == 4) {
-        st_global_v8(reinterpret_cast<float*>(dst) + i, v + i);
-      } else {
-        uint32_t p[8];
+      uint32_t p[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) p[j] = pack2(v[i + 2 * j], v[i + 2 * j + 1], YT{});
+      for (int j = 0; j < 8; ++j) {
+        if constexpr (sizeof(YT) == 4) p[j] = __float_as_uint(v[i + j]);
+        else p[j] = pack2(v[i + 2 * j], v[i + 2 * j + 1], YT{});
+      }
+      if (align == 32) {
         st_global_v8_b32(dst + i, p);
+      } else {
+        reinterpret_cast<uint4*>(dst + i)[0] = make_uint4(p[0], p[1], p[2], p[3]);
+        reinterpret_cast<uint4*>(dst + i)[1] = make_uint4(p[4], p[5], p[6], p[7]);
       }
     }
   } else {
@@ -54,16 +59,18 @@ constexpr int kIWThreads = 320;          // producer, MMA, 8 epilogue warps
 constexpr int kIWEpiThreads = 256;
 constexpr int kIWGroup = 8;              // token tiles whose weight tiles run together (L2 reuse)
 
+// Beside the stages, which are dynamic shared memory at a 1024-byte boundary.
 struct IntWideSmem {
-  uint8_t stage[kIWStages][kIWStageBytes];
   uint64_t full[kIWStages], empty[kIWStages];
   uint64_t tfull[2], tempty[2];
+  alignas(16) float sw[2][256];
+  float bias[2][256];
+  float turn[8][32][17];   // unaligned outputs: 16 columns of a warp's 32 rows, turned to whole rows
   uint32_t tmem_base;
   int abort;
-  float sw[2][256], bias[2][256];
 };
-constexpr size_t kIWSmemBytes = sizeof(IntWideSmem) + 1024;
-static_assert(kIWSmemBytes <= 232448, "wide int8 kernel shared memory");
+constexpr size_t kIWSmemBytes = kIWStages * kIWStageBytes + 1024;
+static_assert(kIWSmemBytes + sizeof(IntWideSmem) <= 232448, "wide int8 kernel shared memory");
 
 // Tile order: blocks of kIWGroup token tiles, all weight tiles of a block before the next, token
 // tiles fastest, so that the tiles in flight share few rows of either operand.
@@ -78,8 +85,8 @@ template <class YT>
 __global__ void __launch_bounds__(kIWThreads, 1)
     int8_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmW, LinearArgs a) {
   extern __shared__ uint8_t smem_raw[];
-  IntWideSmem& sm =
-      *reinterpret_cast<IntWideSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  __shared__ IntWideSmem sm;
+  const uint32_t stages = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
@@ -128,8 +135,8 @@ __global__ void __launch_bounds__(kIWThreads, 1)
         if (rank == 0 && lane == 0) mbar_arrive_expect_tx(&sm.full[stage], 2 * kIWStageBytes);
         __syncwarp();
         const uint32_t bar = cluster_addr(smem_u32(&sm.full[stage]), 0);
-        if (lane == 0) tma_load_2d_pair(sm.stage[stage], &tmQ, bar, kb * 128, y0);
-        if (lane == 1) tma_load_2d_pair(sm.stage[stage] + 16384, &tmW, bar, kb * 128, y1);
+        if (lane == 0) tma_load_2d_pair(stages + stage * kIWStageBytes, &tmQ, bar, kb * 128, y0);
+        if (lane == 1) tma_load_2d_pair(stages + stage * kIWStageBytes + 16384, &tmW, bar, kb * 128, y1);
         last = (last & ~(1u << stage)) | (phase << stage);
         issued = max(issued, static_cast<int>(stage) + 1);
         if (++stage == kIWStages) {
@@ -142,7 +149,7 @@ __global__ void __launch_bounds__(kIWThreads, 1)
     if (!ok && rank == 0 && lane == 0)
       for (int i = 0; i < issued; ++i) {
         int none = 0;
-        mbar_wait<true>(&sm.full[i], (last >> i) & 1u, &none, &g_op_status, kStWaitDrain);
+        mbar_wait(&sm.full[i], (last >> i) & 1u, &none, &g_op_status, kStWaitDrain);
       }
   } else if (warp == 1) {
     if (rank == 0 && lane == 0) {
@@ -152,13 +159,13 @@ __global__ void __launch_bounds__(kIWThreads, 1)
       bool ok = true;
       for (int tile = pair; ok && tile < tiles; tile += pairs, ++it) {
         const int buf = it & 1;
-        if (!mbar_wait<true>(&sm.tempty[buf], ((it >> 1) & 1) ^ 1, &sm.abort, &g_op_status, kStWaitMmaTmem)) break;
+        if (!mbar_wait(&sm.tempty[buf], ((it >> 1) & 1) ^ 1, &sm.abort, &g_op_status, kStWaitMmaTmem)) break;
         tc_fence_after();
         for (int kb = 0; kb < kbs; ++kb) {
-          ok = mbar_wait<true>(&sm.full[stage], phase, &sm.abort, &g_op_status, kStWaitMma);
+          ok = mbar_wait(&sm.full[stage], phase, &sm.abort, &g_op_status, kStWaitMma);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t st = smem_u32(sm.stage[stage]);
+          const uint32_t st = stages + stage * kIWStageBytes;
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             mma_i8_pair(tmem + buf * 256u, sdesc_k128_sw128(st + 32 * k), sdesc_k128_sw128(st + 16384 + 32 * k), idesc,
@@ -175,7 +182,11 @@ __global__ void __launch_bounds__(kIWThreads, 1)
   } else {
     // epilogue: lane quarter warp & 3 (32 token rows), column half (warp - 2) / 4
     const int q = warp & 3, h = (warp - 2) >> 2, et = threadIdx.x - 64;
-    const bool vec = (reinterpret_cast<uintptr_t>(a.y) & 31u) == 0 && (a.y_ld * sizeof(YT)) % 32 == 0;
+    // rows of outputs on 32- or 16-byte boundaries are stored by their thread as whole vectors;
+    // others go through shared memory, so that a warp stores neighbours (2 rows x 16 columns)
+    auto on = [&](uint64_t n) { return reinterpret_cast<uintptr_t>(a.y) % n == 0 && (a.y_ld * sizeof(YT)) % n == 0; };
+    const int align = on(32) ? 32 : on(16) ? 16 : 0;
+    float (*turn)[17] = sm.turn[warp - 2];
     pdl_wait();
     bool dead = false;
     int it = 0;
@@ -199,22 +210,50 @@ __global__ void __launch_bounds__(kIWThreads, 1)
       if (dead) continue;
       tc_fence_after();
       const uint32_t ta = tmem + (static_cast<uint32_t>(32 * q) << 16) + buf * 256u + 128u * h;
+      // the accumulator's next 32 columns are read while these are stored
+      uint32_t acc[2][32];
+      tmem_ld16x2_issue(ta, ta + 16, acc[0]);
 #pragma unroll
-      for (int c0 = 0; c0 < 128; c0 += 32) {
-        int acc[32];
-        tmem_ld32_wait(ta + c0, acc);
-        if (c0 == 96) {
+      for (int i = 0; i < 4; ++i) {
+        const int c0 = 32 * i;
+        tmem_wait_ld32(acc[i & 1]);
+        if (i < 3) {
+          tmem_ld16x2_issue(ta + c0 + 32, ta + c0 + 48, acc[(i + 1) & 1]);
+        } else {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(cluster_addr(smem_u32(&sm.tempty[buf]), 0));
         }
-        const float* swp = &sm.sw[buf][128 * h + c0];
-        const float* bp = &sm.bias[buf][128 * h + c0];
+        const float4* swp = reinterpret_cast<const float4*>(&sm.sw[buf][128 * h + c0]);
+        const float4* bp = reinterpret_cast<const float4*>(&sm.bias[buf][128 * h + c0]);
         float v[32];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = fmaf(static_cast<float>(acc[i]), sx * swp[i], bp[i]);
+        for (int j = 0; j < 8; ++j) {
+          const float4 w4 = swp[j], b4 = bp[j];
+          const uint32_t* u = acc[i & 1] + 4 * j;
+          v[4 * j] = fmaf(static_cast<float>(static_cast<int>(u[0])), sx * w4.x, b4.x);
+          v[4 * j + 1] = fmaf(static_cast<float>(static_cast<int>(u[1])), sx * w4.y, b4.y);
+          v[4 * j + 2] = fmaf(static_cast<float>(static_cast<int>(u[2])), sx * w4.z, b4.z);
+          v[4 * j + 3] = fmaf(static_cast<float>(static_cast<int>(u[3])), sx * w4.w, b4.w);
+        }
         const int col = n * 256 + 128 * h + c0;
-        if (t < a.T) store_cols32(static_cast<YT*>(a.y) + t * a.y_ld + col, a.N - col, vec, v);
+        if (align) {
+          if (t < a.T) store_cols32(static_cast<YT*>(a.y) + t * a.y_ld + col, a.N - col, align, v);
+        } else {
+          const int row0 = m * 256 + 128 * static_cast<int>(rank) + 32 * q;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) turn[lane][j] = v[16 * half + j];
+            __syncwarp();
+            const int cc = col + 16 * half + (lane & 15);
+            if (cc < a.N)
+#pragma unroll 4
+              for (int r = lane >> 4; r < 32; r += 2)
+                if (row0 + r < a.T) static_cast<YT*>(a.y)[(row0 + r) * a.y_ld + cc] = from_f<YT>(turn[r][lane & 15]);
+          }
+        }
       }
     }
   }
@@ -329,51 +368,77 @@ __global__ void __launch_bounds__(kISThreads) int8_stream_kernel(const __grid_co
     }
   }
   __syncwarp();
-  const int q = warp & 3, r = 32 * q + lane;   // this thread's weight row of the tile
-  const int n = n0 + r;
   const int live = min(tn, a.T - t0);
-  int* part = reinterpret_cast<int*>(base);    // [tn][128]
+  const uint32_t part = smem_u32(base);        // int [live][128] partial sums, in place of the stages
   if (warp >= 2) {
     pdl_wait();
-    const float sw = n < a.N ? a.sw[n] : 0.f;
-    const float bias = a.bias && n < a.N ? load1_dyn(a.bias, a.bias_type, n) : 0.f;
     ok = mbar_wait(&sm.tfull, 0, &sm.abort, &g_op_status, kStWaitEpilogue);
     if (__all_sync(0xffffffffu, ok)) {
       tc_fence_after();
       // every load and product of this CTA is complete: the stages are free
+      const int q = warp & 3, r = 32 * q + lane;   // this thread's weight row of the tile
       for (int c0 = 0; c0 < live; c0 += 32) {
         int acc[32];
-        const uint32_t ta = tmem + (static_cast<uint32_t>(32 * q) << 16) + c0;
-        tmem_ld32_wait(ta, acc);
-        if (splits > 1) {
+        tmem_ld32_wait(tmem + (static_cast<uint32_t>(32 * q) << 16) + c0, acc);
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (c0 + i < live) part[(c0 + i) * 128 + r] = acc[i];
-        } else if (n < a.N) {
+        for (int i = 0; i < 32; ++i)
+          if (c0 + i < live) st_shared_s32(part + ((c0 + i) * 128 + r) * 4, acc[i]);
+      }
+    }
+    if (splits > 1) cluster_sync();
+    else named_bar_sync(1, 128);
+    // CTA `split` finishes its share of the token columns, a warp one column at a time: a lane
+    // adds up four neighbouring outputs.  Two columns' loads are in flight together.
+    const int n = n0 + 4 * lane;
+    float sw[4], bias[4];
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (c0 + i < live)
-              static_cast<YT*>(a.y)[(t0 + c0 + i) * a.y_ld + n] =
-                  from_f<YT>(fmaf(static_cast<float>(acc[i]), a.sx[t0 + c0 + i] * sw, bias));
+    for (int j = 0; j < 4; ++j) {
+      sw[j] = n + j < a.N ? a.sw[n + j] : 0.f;
+      bias[j] = a.bias && n + j < a.N ? load1_dyn(a.bias, a.bias_type, n + j) : 0.f;
+    }
+    const int c1 = live * (split + 1) / splits;
+    const bool vec = n + 4 <= a.N && reinterpret_cast<uintptr_t>(a.y) % (4 * sizeof(YT)) == 0 && a.y_ld % 4 == 0;
+    for (int c = live * split / splits + warp - 2; c < c1; c += 8) {
+      const int two = c + 4 < c1 ? 2 : 1;
+      int4 v[2][8];
+      float sx[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        if (k >= two) break;
+        const uint32_t at = part + ((c + 4 * k) * 128 + 4 * lane) * 4;
+#pragma unroll
+        for (int s = 0; s < 8; ++s)
+          if (s < splits) v[k][s] = ld_cluster_v4(splits > 1 ? cluster_addr(at, s) : at);
+        sx[k] = a.sx[t0 + c + 4 * k];
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        if (k >= two) break;
+        int4 sum = v[k][0];
+#pragma unroll
+        for (int s = 1; s < 8; ++s)
+          if (s < splits) {
+            sum.x += v[k][s].x;
+            sum.y += v[k][s].y;
+            sum.z += v[k][s].z;
+            sum.w += v[k][s].w;
+          }
+        float o[4] = {static_cast<float>(sum.x), static_cast<float>(sum.y), static_cast<float>(sum.z),
+                      static_cast<float>(sum.w)};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = fmaf(o[j], sx[k] * sw[j], bias[j]);
+        YT* dst = static_cast<YT*>(a.y) + (t0 + c + 4 * k) * a.y_ld + n;
+        if (vec) {
+          if constexpr (sizeof(YT) == 4) *reinterpret_cast<float4*>(dst) = make_float4(o[0], o[1], o[2], o[3]);
+          else *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(o[0], o[1], YT{}), pack2(o[2], o[3], YT{}));
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (n + j < a.N) dst[j] = from_f<YT>(o[j]);
         }
       }
     }
-    if (splits > 1) {
-      cluster_sync();
-      // CTA `split` finishes its share of the token columns
-      const int c1 = live * (split + 1) / splits;
-      for (int c = live * split / splits; c < c1; ++c) {
-        int v[8];
-        const uint32_t at = smem_u32(part + c * 128 + r);
-#pragma unroll
-        for (int s = 0; s < 8; ++s) v[s] = s < splits ? ld_cluster_s32(cluster_addr(at, s)) : 0;
-        const int sum = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
-        if (n < a.N)
-          static_cast<YT*>(a.y)[(t0 + c) * a.y_ld + n] =
-              from_f<YT>(fmaf(static_cast<float>(sum), a.sx[t0 + c] * sw, bias));
-      }
-      cluster_sync();   // the others have read this CTA's partial sums
-    }
+    if (splits > 1) cluster_sync();   // the others have read this CTA's partial sums
   } else if (splits > 1) {
     cluster_sync();
     cluster_sync();
@@ -443,9 +508,10 @@ cudaError_t int8_status(cudaStream_t st, bool clear, int* v) { return take_statu
 extern "C" MOE_B200_API int moe_b200_operator_status(void* stream, int32_t clear) {
   using namespace moe;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  int norm = 0, int8 = 0;
+  int norm = 0, quant = 0, int8 = 0;
   cudaError_t e = norm_status(st, clear, &norm);
+  if (e == cudaSuccess) e = quant_status(st, clear, &quant);
   if (e == cudaSuccess) e = int8_status(st, clear, &int8);
   if (e != cudaSuccess) return -report_cuda(e, "operator status");
-  return norm ? norm : int8;
+  return norm ? norm : quant ? quant : int8;
 }

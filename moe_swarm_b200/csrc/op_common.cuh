@@ -44,6 +44,7 @@ static inline cudaError_t take_status(cudaStream_t st, bool clear, int* v) {
 }
 cudaError_t norm_status(cudaStream_t st, bool clear, int* v);       // norm.cu and norm_bwd.cu
 cudaError_t norm_bwd_status(cudaStream_t st, bool clear, int* v);
+cudaError_t quant_status(cudaStream_t st, bool clear, int* v);      // int8.cu
 cudaError_t int8_status(cudaStream_t st, bool clear, int* v);       // int8_gemm.cu
 
 using bf16 = __nv_bfloat16;

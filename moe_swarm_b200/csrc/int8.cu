@@ -15,7 +15,6 @@ namespace moe {
 
 constexpr int kQuantMaxCols = 2 * kNormMaxCols;
 constexpr int kInt8MaxK = 131056;
-constexpr int kInt8StreamMaxT = 256;
 
 struct QuantArgs {
   const void* x;
@@ -182,6 +181,138 @@ __global__ void __launch_bounds__(512, 2) quant_ring_kernel(QuantArgs a, RingPla
     }
 }
 
+// ---------------------------------------------------------------- one or two tokens
+// The whole layer in one launch: every CTA quantises the tokens for itself into shared memory (they
+// come from L2; 14 KB each at 7168), then each warp takes whole weight rows, 4 KB of them in
+// flight, and adds up four products per instruction (dp4a).  The weights cross HBM once; the warps
+// per SM are chosen so that the rows come out even.  One token 7168 -> 4096 from bf16: 5.1 us, 5.7
+// TB/s (the streaming kernel and its quantisation: 9.2).  From three tokens on the products take
+// longer than the weights: 11 us against 9.2.
+constexpr int kGemvMaxT = 2;
+
+struct GemvArgs {
+  const void* x;
+  const float* sx;
+  const int8_t* w;
+  const float* sw;
+  const void* bias;
+  void* y;
+  int64_t x_ld, w_ld, y_ld;
+  int T, N, K, vec, swiglu, y_type, bias_type;
+};
+
+// Eight elements of a row from column e on (what is quantised), as the row kernels compute them.
+template <class XT>
+__device__ __forceinline__ void gemv_load8(const GemvArgs& a, const XT* row, int e, float* v) {
+  auto load = [&](const XT* p, float* out) {
+    if (a.vec) load8<XT, true>(p, 8, out);
+    else load8<XT, false>(p, 8, out);
+  };
+  load(row + e, v);
+  if (!a.swiglu) return;
+  float g[8];
+  load(row + a.K + e, g);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] *= silu_fast(g[j]);
+}
+
+template <class XT, int TT>
+__global__ void __launch_bounds__(1024, 1) int8_gemv_kernel(GemvArgs a) {
+  extern __shared__ int4 xs[];   // [TT][K / 16] codes
+  __shared__ float s_max[TT][32], s_scale[TT];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int units = a.K / 16;
+  int n = blockIdx.x * warps + warp;
+  int4 w[8];
+  auto load_w = [&](int row, int u0) {
+    const int4* p = reinterpret_cast<const int4*>(a.w + row * a.w_ld) + u0 + lane;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      w[j] = u0 + lane + 32 * j < units ? p[32 * j] : make_int4(0, 0, 0, 0);
+  };
+  if (n < a.N) load_w(n, 0);   // on its way while the tokens are quantised
+  if constexpr (std::is_same<XT, int8_t>::value) {
+    for (int t = 0; t < TT; ++t)
+      for (int u = threadIdx.x; u < units; u += blockDim.x)
+        xs[t * units + u] = t < a.T ? reinterpret_cast<const int4*>(static_cast<const int8_t*>(a.x) + t * a.x_ld)[u]
+                                    : make_int4(0, 0, 0, 0);
+    if (threadIdx.x < TT) s_scale[threadIdx.x] = static_cast<int>(threadIdx.x) < a.T ? a.sx[threadIdx.x] : 0.f;
+  } else {
+    const XT* x = static_cast<const XT*>(a.x);
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+      float m = 0.f;
+      if (t < a.T)
+        for (int e = threadIdx.x * 8; e < a.K; e += blockDim.x * 8) {
+          float v[8];
+          gemv_load8(a, x + t * a.x_ld, e, v);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) m = max_nan(m, fabsf(v[j]));
+        }
+#pragma unroll
+      for (int d = 16; d >= 1; d >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
+      if (lane == 0) s_max[t][warp] = m;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+      float m = lane < warps ? s_max[t][lane] : 0.f;
+#pragma unroll
+      for (int d = 16; d >= 1; d >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
+      float inv;
+      const float sc = quant_scale(m, &inv);
+      if (threadIdx.x == 0) s_scale[t] = sc;
+      uint2* dst = reinterpret_cast<uint2*>(xs + t * units);
+      for (int e = threadIdx.x * 8; e < a.K; e += blockDim.x * 8) {
+        uint2 c = make_uint2(0, 0);
+        if (t < a.T && inv != 0.f) {
+          float v[8];
+          gemv_load8(a, x + t * a.x_ld, e, v);
+          const float2 k = dup2(inv);
+          c.x = codes4(make_float2(v[0], v[1]), make_float2(v[2], v[3]), k);
+          c.y = codes4(make_float2(v[4], v[5]), make_float2(v[6], v[7]), k);
+        }
+        dst[e / 8] = c;
+      }
+    }
+  }
+  __syncthreads();
+  for (; n < a.N; n += gridDim.x * warps) {
+    int acc[TT] = {};
+    for (int u0 = 0; u0 < units; u0 += 256) {
+      if (u0) load_w(n, u0);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int u = u0 + lane + 32 * j;
+        if (u >= units) break;
+#pragma unroll
+        for (int t = 0; t < TT; ++t) {
+          const int4 q = xs[t * units + u];
+          acc[t] = __dp4a(w[j].x, q.x, acc[t]);
+          acc[t] = __dp4a(w[j].y, q.y, acc[t]);
+          acc[t] = __dp4a(w[j].z, q.z, acc[t]);
+          acc[t] = __dp4a(w[j].w, q.w, acc[t]);
+        }
+      }
+    }
+    const int next = n + gridDim.x * warps;
+    if (next < a.N) load_w(next, 0);
+#pragma unroll
+    for (int t = 0; t < TT; ++t) acc[t] = __reduce_add_sync(0xffffffffu, acc[t]);
+    // lane t stores token t's output
+    int mine = acc[0];
+#pragma unroll
+    for (int t = 1; t < TT; ++t) mine = lane == t ? acc[t] : mine;
+    if (lane < a.T) {
+      const float b = a.bias ? load1_dyn(a.bias, a.bias_type, n) : 0.f;
+      const float v = fmaf(static_cast<float>(mine), s_scale[lane] * a.sw[n], b);
+      store8_dyn<false>(a.y, a.y_type, lane * a.y_ld + n, 1, &v);
+    }
+  }
+}
+
 cudaError_t quant_status(cudaStream_t st, bool clear, int* v) { return take_status(st, clear, v); }
 
 namespace {
@@ -220,6 +351,27 @@ cudaError_t quant_launch(const QuantArgs& q0, int sms, cudaStream_t st) {
   else if (q.type == MOE_B200_FP16) go(fp16{});
   else go(float{});
   return e;
+}
+
+cudaError_t gemv_launch(const GemvArgs& g, int x_type, int sms, cudaStream_t st) {
+  // rows per SM in as few rounds of at most 32 warps as it takes; the same number in each
+  const int rows = (g.N + sms - 1) / sms, rounds = (rows + 31) / 32;
+  int warps = (rows + rounds - 1) / rounds;
+  if (warps < 8) warps = 8;
+  const int need = (g.N + warps - 1) / warps;
+  const dim3 grid(need < sms ? need : sms), block(warps * 32);
+  auto sized = [&](auto t, auto tt) {
+    using XT = decltype(t);
+    constexpr int TT = decltype(tt)::value;
+    auto kernel = int8_gemv_kernel<XT, TT>;
+    static SmemOnce once;
+    const cudaError_t e = once.set(reinterpret_cast<const void*>(kernel), TT * kQuantMaxCols);
+    return e == cudaSuccess ? launch_pdl(kernel, grid, block, static_cast<size_t>(TT) * g.K, st, g) : e;
+  };
+  auto go = [&](auto t) {
+    return g.T == 1 ? sized(t, std::integral_constant<int, 1>{}) : sized(t, std::integral_constant<int, 2>{});
+  };
+  return x_type == MOE_B200_BF16 ? go(bf16{}) : x_type == MOE_B200_FP16 ? go(fp16{}) : x_type == MOE_B200_FP32 ? go(0.f) : go(int8_t{});
 }
 
 int quant_check(const void* x, int type, int rows, int cols, const char** why) {
@@ -300,6 +452,27 @@ MOE_B200_API int moe_b200_int8_linear(const moe_b200_linear_args* a, void* works
   int sms = 0;
   if (int rc = op_device(&sms)) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (a->num_tokens <= kGemvMaxT && a->in_features <= kQuantMaxCols) {
+    GemvArgs g{};
+    g.x = a->x;
+    g.sx = a->x_scale;
+    g.w = a->weight;
+    g.sw = a->weight_scale;
+    g.bias = a->bias;
+    g.y = a->y;
+    g.x_ld = a->num_tokens == 1 ? 0 : a->x_stride;
+    g.w_ld = w_ld;
+    g.y_ld = a->y_stride;
+    g.T = a->num_tokens;
+    g.N = a->out_features;
+    g.K = a->in_features;
+    g.vec = quantise && rows_aligned(a->x, g.x_ld, a->x_type);
+    g.swiglu = a->swiglu;
+    g.y_type = a->y_type;
+    g.bias_type = a->bias_type;
+    const cudaError_t e = gemv_launch(g, a->x_type, sms, st);
+    return e == cudaSuccess ? MOE_B200_OK : report_cuda(e, "int8_linear launch");
+  }
   const int8_t* q_rows = static_cast<const int8_t*>(a->x);
   int64_t q_ld = x_ld;
   LinearArgs l{};
@@ -333,8 +506,7 @@ MOE_B200_API int moe_b200_int8_linear(const moe_b200_linear_args* a, void* works
   l.K = a->in_features;
   l.y_type = a->y_type;
   l.bias_type = a->bias_type;
-  e = a->num_tokens <= kInt8StreamMaxT ? int8_stream_launch(q_rows, q_ld, a->weight, w_ld, l, sms, st)
-                                       : int8_wide_launch(q_rows, q_ld, a->weight, w_ld, l, sms, st);
+  e = int8_gemm_launch(q_rows, q_ld, a->weight, w_ld, l, sms, st);
   return e == cudaSuccess ? MOE_B200_OK : report_cuda(e, "int8_linear launch");
 }
 

@@ -55,6 +55,10 @@ __device__ __forceinline__ void tmem_ld32_wait(uint32_t ta, int* v) {
 // ---------------------------------------------------------------- wide
 constexpr int kIWStages = 6;
 constexpr int kIWStageBytes = 32768;     // 128 token rows | 128 weight rows of 128 bytes
+// Rows of one bulk copy.  A box's loads go through the copy unit one after another; two per operand
+// half keep it busier than one (8192 x 4096 x 7168: 152 us with 128 rows, 146 with 64), smaller ones
+// cost more in their number (176 with 32, 263 with 16).
+constexpr int kIWBox = 64;
 constexpr int kIWThreads = 320;          // producer, MMA, 8 epilogue warps
 constexpr int kIWEpiThreads = 256;
 constexpr int kIWGroup = 8;              // token tiles whose weight tiles run together (L2 reuse)
@@ -123,7 +127,7 @@ __global__ void __launch_bounds__(kIWThreads, 1)
     for (int tile = pair; ok && tile < tiles; tile += pairs) {
       int m, n;
       iw_tile(tile, mt, nt, &m, &n);
-      const int y0 = m * 256 + 128 * rank, y1 = n * 256 + 128 * rank;
+      const int y0 = m * 256 + 128 * rank, y1 = n * 256 + 128 * static_cast<int>(rank);
       for (int kb = 0; kb < kbs; ++kb) {
         ok = __all_sync(0xffffffffu,
                         mbar_wait(&sm.empty[stage], phase ^ 1u, &sm.abort, &g_op_status, kStWaitProducer));
@@ -135,8 +139,13 @@ __global__ void __launch_bounds__(kIWThreads, 1)
         if (rank == 0 && lane == 0) mbar_arrive_expect_tx(&sm.full[stage], 2 * kIWStageBytes);
         __syncwarp();
         const uint32_t bar = cluster_addr(smem_u32(&sm.full[stage]), 0);
-        if (lane == 0) tma_load_2d_pair(stages + stage * kIWStageBytes, &tmQ, bar, kb * 128, y0);
-        if (lane == 1) tma_load_2d_pair(stages + stage * kIWStageBytes + 16384, &tmW, bar, kb * 128, y1);
+        // lane l loads box l: token rows first, then weight rows
+        constexpr int kQBoxes = 128 / kIWBox, kBoxes = 2 * kQBoxes;
+        if (lane < kBoxes) {
+          const bool is_q = lane < kQBoxes;
+          tma_load_2d_pair(stages + stage * kIWStageBytes + lane * kIWBox * 128, is_q ? &tmQ : &tmW, bar, kb * 128,
+                           is_q ? y0 + lane * kIWBox : y1 + (lane - kQBoxes) * kIWBox);
+        }
         last = (last & ~(1u << stage)) | (phase << stage);
         issued = max(issued, static_cast<int>(stage) + 1);
         if (++stage == kIWStages) {
@@ -267,7 +276,8 @@ __global__ void __launch_bounds__(kIWThreads, 1)
 }
 
 // ---------------------------------------------------------------- stream
-constexpr int kISThreads = 192;          // producer, MMA, 4 epilogue warps
+constexpr int kISThreads = 320;          // producer, MMA, 8 epilogue warps
+constexpr int kISEpiThreads = 256;
 constexpr int kISMaxStages = 8;
 
 struct IntStreamCtl {
@@ -277,11 +287,66 @@ struct IntStreamCtl {
   int abort;
 };
 
+// Adds up the S partial sums of token columns c0, c0 + 8, ... < c1 of the tile (a warp one column at
+// a time, a lane four neighbouring outputs) and stores them; the loads of as many columns as make
+// 16 vectors are in flight together.
+template <class YT, int S>
+__device__ __forceinline__ void is_finish(const LinearArgs& a, uint32_t part, int n0, int t0, int c0, int c1, int lane) {
+  constexpr int C = S == 1 ? 8 : 16 / S;
+  const int n = n0 + 4 * lane;
+  float sw[4], bias[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    sw[j] = n + j < a.N ? a.sw[n + j] : 0.f;
+    bias[j] = a.bias && n + j < a.N ? load1_dyn(a.bias, a.bias_type, n + j) : 0.f;
+  }
+  const bool vec = n + 4 <= a.N && reinterpret_cast<uintptr_t>(a.y) % (4 * sizeof(YT)) == 0 && a.y_ld % 4 == 0;
+  uint32_t from[S];
+#pragma unroll
+  for (int s = 0; s < S; ++s) from[s] = (S > 1 ? cluster_addr(part, s) : part) + 16 * lane;
+  for (int c = c0; c < c1; c += 8 * C) {
+    int4 v[C][S];
+    float sx[C];
+#pragma unroll
+    for (int k = 0; k < C; ++k)
+      if (c + 8 * k < c1) {
+#pragma unroll
+        for (int s = 0; s < S; ++s) v[k][s] = ld_cluster_v4(from[s] + (c + 8 * k) * 512);
+        sx[k] = a.sx[t0 + c + 8 * k];
+      }
+#pragma unroll
+    for (int k = 0; k < C; ++k) {
+      if (c + 8 * k >= c1) break;
+      int4 sum = v[k][0];
+#pragma unroll
+      for (int s = 1; s < S; ++s) {
+        sum.x += v[k][s].x;
+        sum.y += v[k][s].y;
+        sum.z += v[k][s].z;
+        sum.w += v[k][s].w;
+      }
+      float o[4] = {static_cast<float>(sum.x), static_cast<float>(sum.y), static_cast<float>(sum.z),
+                    static_cast<float>(sum.w)};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = fmaf(o[j], sx[k] * sw[j], bias[j]);
+      YT* dst = static_cast<YT*>(a.y) + (t0 + c + 8 * k) * a.y_ld + n;
+      if (vec) {
+        if constexpr (sizeof(YT) == 4) *reinterpret_cast<float4*>(dst) = make_float4(o[0], o[1], o[2], o[3]);
+        else *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(o[0], o[1], YT{}), pack2(o[2], o[3], YT{}));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (n + j < a.N) dst[j] = from_f<YT>(o[j]);
+      }
+    }
+  }
+}
+
 // grid (splits * weight tiles, token tiles), clusters of `splits` CTAs along x.  Token tile: tn
 // rows (a multiple of 16, at most 256); stages of 16 KB of weights and tn x 128 bytes of tokens.
 // The integer partial sums [tn][128] of a split CTA reuse the stages.
 template <class YT>
-__global__ void __launch_bounds__(kISThreads) int8_stream_kernel(const __grid_constant__ CUtensorMap tmQ,
+__global__ void __launch_bounds__(kISThreads, 2) int8_stream_kernel(const __grid_constant__ CUtensorMap tmQ,
                                                                  const __grid_constant__ CUtensorMap tmW, LinearArgs a,
                                                                  int splits, int tn, int stages, uint32_t tmem_cols) {
   extern __shared__ uint8_t smem_raw[];
@@ -315,26 +380,30 @@ __global__ void __launch_bounds__(kISThreads) int8_stream_kernel(const __grid_co
 
   bool ok = true;
   if (warp == 0) {
+    auto load_w = [&](int stage, int kb) {
+      if (lane == 0) tma_load_2d(base + stage * stage_bytes, &tmW, &sm.full[stage], kb * 128, n0);
+    };
+    auto load_q = [&](int stage, int kb) {
+      if (lane == 1) tma_load_2d(base + stage * stage_bytes + 16384, &tmQ, &sm.full[stage], kb * 128, t0);
+    };
     // weights of the first stages start before the wait for the kernel that writes q and sx
     if (!a.early_w) pdl_wait();
     const int ahead = min(stages, k1 - k0);
     for (int i = 0; i < ahead; ++i) {
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&sm.full[i], stage_bytes);
-        tma_load_2d(base + i * stage_bytes, &tmW, &sm.full[i], (k0 + i) * 128, n0);
-      }
+      if (lane == 0) mbar_arrive_expect_tx(&sm.full[i], stage_bytes);
+      __syncwarp();
+      load_w(i, k0 + i);
     }
     if (a.early_w) pdl_wait();
-    for (int i = 0; i < ahead; ++i)
-      if (lane == 0) tma_load_2d(base + i * stage_bytes + 16384, &tmQ, &sm.full[i], (k0 + i) * 128, t0);
+    for (int i = 0; i < ahead; ++i) load_q(i, k0 + i);
     uint32_t stage = 0, phase = 0, last = 0;   // last: bit s = parity of stage s's latest load
     for (int kb = k0 + ahead; kb < k1; ++kb) {
       ok = __all_sync(0xffffffffu, mbar_wait(&sm.empty[stage], phase, &sm.abort, &g_op_status, kStWaitProducer));
       if (!ok) break;
       if (lane == 0) mbar_arrive_expect_tx(&sm.full[stage], stage_bytes);
       __syncwarp();
-      if (lane == 0) tma_load_2d(base + stage * stage_bytes, &tmW, &sm.full[stage], kb * 128, n0);
-      if (lane == 1) tma_load_2d(base + stage * stage_bytes + 16384, &tmQ, &sm.full[stage], kb * 128, t0);
+      load_w(stage, kb);
+      load_q(stage, kb);
       last = (last & ~(1u << stage)) | ((phase ^ 1u) << stage);
       if (++stage == static_cast<uint32_t>(stages)) {
         stage = 0;
@@ -377,7 +446,7 @@ __global__ void __launch_bounds__(kISThreads) int8_stream_kernel(const __grid_co
       tc_fence_after();
       // every load and product of this CTA is complete: the stages are free
       const int q = warp & 3, r = 32 * q + lane;   // this thread's weight row of the tile
-      for (int c0 = 0; c0 < live; c0 += 32) {
+      for (int c0 = warp < 6 ? 0 : 32; c0 < live; c0 += 64) {
         int acc[32];
         tmem_ld32_wait(tmem + (static_cast<uint32_t>(32 * q) << 16) + c0, acc);
 #pragma unroll
@@ -386,58 +455,13 @@ __global__ void __launch_bounds__(kISThreads) int8_stream_kernel(const __grid_co
       }
     }
     if (splits > 1) cluster_sync();
-    else named_bar_sync(1, 128);
-    // CTA `split` finishes its share of the token columns, a warp one column at a time: a lane
-    // adds up four neighbouring outputs.  Two columns' loads are in flight together.
-    const int n = n0 + 4 * lane;
-    float sw[4], bias[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      sw[j] = n + j < a.N ? a.sw[n + j] : 0.f;
-      bias[j] = a.bias && n + j < a.N ? load1_dyn(a.bias, a.bias_type, n + j) : 0.f;
-    }
-    const int c1 = live * (split + 1) / splits;
-    const bool vec = n + 4 <= a.N && reinterpret_cast<uintptr_t>(a.y) % (4 * sizeof(YT)) == 0 && a.y_ld % 4 == 0;
-    for (int c = live * split / splits + warp - 2; c < c1; c += 8) {
-      const int two = c + 4 < c1 ? 2 : 1;
-      int4 v[2][8];
-      float sx[2];
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        if (k >= two) break;
-        const uint32_t at = part + ((c + 4 * k) * 128 + 4 * lane) * 4;
-#pragma unroll
-        for (int s = 0; s < 8; ++s)
-          if (s < splits) v[k][s] = ld_cluster_v4(splits > 1 ? cluster_addr(at, s) : at);
-        sx[k] = a.sx[t0 + c + 4 * k];
-      }
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        if (k >= two) break;
-        int4 sum = v[k][0];
-#pragma unroll
-        for (int s = 1; s < 8; ++s)
-          if (s < splits) {
-            sum.x += v[k][s].x;
-            sum.y += v[k][s].y;
-            sum.z += v[k][s].z;
-            sum.w += v[k][s].w;
-          }
-        float o[4] = {static_cast<float>(sum.x), static_cast<float>(sum.y), static_cast<float>(sum.z),
-                      static_cast<float>(sum.w)};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] = fmaf(o[j], sx[k] * sw[j], bias[j]);
-        YT* dst = static_cast<YT*>(a.y) + (t0 + c + 4 * k) * a.y_ld + n;
-        if (vec) {
-          if constexpr (sizeof(YT) == 4) *reinterpret_cast<float4*>(dst) = make_float4(o[0], o[1], o[2], o[3]);
-          else *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(o[0], o[1], YT{}), pack2(o[2], o[3], YT{}));
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (n + j < a.N) dst[j] = from_f<YT>(o[j]);
-        }
-      }
-    }
+    else named_bar_sync(1, kISEpiThreads);
+    // CTA `split` finishes its share of the token columns
+    const int c0 = live * split / splits + warp - 2, c1 = live * (split + 1) / splits;
+    if (splits == 8) is_finish<YT, 8>(a, part, n0, t0, c0, c1, lane);
+    else if (splits == 4) is_finish<YT, 4>(a, part, n0, t0, c0, c1, lane);
+    else if (splits == 2) is_finish<YT, 2>(a, part, n0, t0, c0, c1, lane);
+    else is_finish<YT, 1>(a, part, n0, t0, c0, c1, lane);
     if (splits > 1) cluster_sync();   // the others have read this CTA's partial sums
   } else if (splits > 1) {
     cluster_sync();
@@ -455,20 +479,21 @@ cudaError_t with_y_type(int type, F&& f) {
   return type == MOE_B200_BF16 ? f(bf16{}) : type == MOE_B200_FP16 ? f(fp16{}) : f(float{});
 }
 
-}  // namespace
-
 cudaError_t int8_wide_launch(const int8_t* q, int64_t q_ld, const int8_t* w, int64_t w_ld, const LinearArgs& a,
                              int sms, cudaStream_t st) {
+  // (Tiles of 256 x 128 for twice the SMs at work gain nothing: an MMA of half the width takes nearly
+  // as long.  512 x 4096 x 7168: 21.9 us with 256 x 256, 20.5 with 256 x 128, 14 split over K.)
+  const int pairs = sms / 2, tiles = ((a.T + 255) / 256) * ((a.N + 255) / 256);
   CUtensorMap mq, mw;
-  if (!encode_rows_u8(&mq, q, a.K, a.T, q_ld, 128) || !encode_rows_u8(&mw, w, a.K, a.N, w_ld, 128))
+  if (!encode_rows_u8(&mq, q, a.K, a.T, q_ld, kIWBox) || !encode_rows_u8(&mw, w, a.K, a.N, w_ld, kIWBox))
     return cudaErrorInvalidValue;
-  const int tiles = ((a.T + 255) / 256) * ((a.N + 255) / 256);
-  const int pairs = tiles < sms / 2 ? tiles : sms / 2;
   return with_y_type(a.y_type, [&](auto yt) {
     auto kernel = int8_wide_kernel<decltype(yt)>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kIWSmemBytes);
+    static SmemOnce once;
+    const cudaError_t e = once.set(reinterpret_cast<const void*>(kernel), kIWSmemBytes);
     if (e != cudaSuccess) return e;
-    return launch_cluster_pdl(kernel, dim3(2 * pairs), dim3(kIWThreads), kIWSmemBytes, 2, st, mq, mw, a);
+    return launch_cluster_pdl(kernel, dim3(2 * (tiles < pairs ? tiles : pairs)), dim3(kIWThreads), kIWSmemBytes, 2, st, mq,
+                              mw, a);
   });
 }
 
@@ -477,11 +502,12 @@ cudaError_t int8_stream_launch(const int8_t* q, int64_t q_ld, const int8_t* w, i
   const int tt = (a.T + 255) / 256;
   int tn = ((a.T + tt - 1) / tt + 15) / 16 * 16;
   const int kbs = (a.K + 127) / 128, nt = (a.N + 127) / 128;
-  // split K until the CTAs fill the GPU about once (twice where two fit an SM), at least two
-  // 128-byte steps each
-  const int slots = tn <= 64 ? 2 * sms : sms;
+  // Split K until the CTAs fill the GPU about once (twice where two fit an SM), at least two
+  // 128-byte steps each.  Clusters of eight only where two CTAs fit an SM: of one-per-SM clusters a
+  // part of the GPU holds two and leaves SMs over (1000 x 512 x 4096: 18.6 us in eights).
+  const int slots = tn <= 64 ? 2 * sms : sms, most = tn <= 64 ? 8 : 4;
   int splits = 1;
-  while (splits < 8 && nt * tt * splits * 2 <= slots && kbs >= 4 * splits) splits *= 2;
+  while (splits < most && nt * tt * splits * 2 <= slots && kbs >= 4 * splits) splits *= 2;
   const int stage_bytes = 16384 + tn * 128;
   const int room = tn <= 64 ? 100 * 1024 : 200 * 1024;
   int stages = room / stage_bytes;
@@ -494,11 +520,24 @@ cudaError_t int8_stream_launch(const int8_t* q, int64_t q_ld, const int8_t* w, i
     return cudaErrorInvalidValue;
   return with_y_type(a.y_type, [&](auto yt) {
     auto kernel = int8_stream_kernel<decltype(yt)>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 210 * 1024);
+    static SmemOnce once;
+    const cudaError_t e = once.set(reinterpret_cast<const void*>(kernel), 210 * 1024);
     if (e != cudaSuccess) return e;
     return launch_cluster_pdl(kernel, dim3(nt * splits, tt), dim3(kISThreads), smem, splits, st, mq, mw, a, splits, tn,
                               stages, cols);
   });
+}
+
+}  // namespace
+
+// Up to 256 tokens: stream.  Beyond that, stream only where its tiles are few enough to be split over
+// K and K is long enough to gain by it: 512 x 4096 x 7168 18.9 us against 21.3 wide, 512 x 2048 x 2048
+// 10.3 against 9.2, 768 x 4096 x 7168 (unsplit) 27 against 22.
+cudaError_t int8_gemm_launch(const int8_t* q, int64_t q_ld, const int8_t* w, int64_t w_ld, const LinearArgs& a, int sms,
+                             cudaStream_t st) {
+  const int64_t tiles = static_cast<int64_t>((a.T + 255) / 256) * ((a.N + 127) / 128);
+  const bool stream = a.T <= 256 || (tiles * 2 <= sms && a.K >= 4096);
+  return stream ? int8_stream_launch(q, q_ld, w, w_ld, a, sms, st) : int8_wide_launch(q, q_ld, w, w_ld, a, sms, st);
 }
 
 cudaError_t int8_status(cudaStream_t st, bool clear, int* v) { return take_status(st, clear, v); }

@@ -15,9 +15,8 @@ struct LinearArgs {
   int early_w;          // the weights are not written by the kernel this one depends on
 };
 
-cudaError_t int8_stream_launch(const int8_t* q, int64_t q_ld, const int8_t* w, int64_t w_ld, const LinearArgs& a,
-                               int sms, cudaStream_t st);
-cudaError_t int8_wide_launch(const int8_t* q, int64_t q_ld, const int8_t* w, int64_t w_ld, const LinearArgs& a,
-                             int sms, cudaStream_t st);
+// q: int8 [T][K], rows q_ld apart; w: int8 [N][K], rows w_ld apart (both 16-byte aligned).
+cudaError_t int8_gemm_launch(const int8_t* q, int64_t q_ld, const int8_t* w, int64_t w_ld, const LinearArgs& a, int sms,
+                             cudaStream_t st);
 
 }  // namespace moe

@@ -6,6 +6,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 
 #include "../../include/moe_b200.h"
@@ -20,6 +21,24 @@ int op_device(int* sms);   // the current device must be sm_100; *sms = its SM c
 // A byte matrix with rows `pitch` bytes apart as TMA tiles of 128 bytes x box_rows rows (SWIZZLE_128B).
 bool encode_rows_u8(CUtensorMap* m, const void* base, uint64_t cols, uint64_t rows, uint64_t pitch,
                     uint32_t box_rows);
+
+// Raises a kernel's dynamic shared memory limit once per device (a static of the launching code,
+// which must use it for one kernel only).  Setting it twice in a race is harmless.
+class SmemOnce {
+ public:
+  cudaError_t set(const void* kernel, int bytes) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64 && (done_.load(std::memory_order_acquire) >> dev) & 1u) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && dev >= 0 && dev < 64) done_.fetch_or(1ull << dev, std::memory_order_release);
+    return e;
+  }
+
+ private:
+  std::atomic<uint64_t> done_{0};
+};
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline int type_bytes(int t) { return t == MOE_B200_FP32 ? 4 : t == MOE_B200_E4M3 ? 1 : 2; }

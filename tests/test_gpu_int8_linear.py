@@ -38,7 +38,7 @@ def run_exact(T, N, K, out=BF, bias=None, seed=0, full=False, w_pad=0, x_pad=0):
     R.close(y, ref, mag, steps=8)     # integer to 32 bits, three products, one sum
 
 
-@pytest.mark.parametrize("T", [1, 2, 15, 16, 17, 33, 64, 65, 127, 128, 129, 200, 257, 300, 513, 700])
+@pytest.mark.parametrize("T", [1, 2, 3, 15, 16, 17, 33, 64, 65, 127, 128, 129, 200, 257, 300, 513, 700])
 @pytest.mark.parametrize("N,K", [(1, 16), (64, 128), (100, 144), (129, 1040), (300, 272), (512, 2048), (1001, 640)])
 def test_int8_input(T, N, K):
     run_exact(T, N, K, out=F32, seed=T + N + K)
@@ -52,7 +52,7 @@ def test_types_and_bias(T, out, bias):
     run_exact(T, 263, 272, out=out, bias=bias, seed=6)
 
 
-@pytest.mark.parametrize("T", [1, 40, 300])
+@pytest.mark.parametrize("T", [1, 2, 40, 300])
 def test_extreme_codes_and_long_sums(T):
     run_exact(T, 96, 4096, out=F32, full=True, seed=3)
     # the largest sums that 32-bit integers hold: 131056 * 128 * 128 < 2^31
@@ -64,7 +64,7 @@ def test_extreme_codes_and_long_sums(T):
     assert (y == float(K * 128 * 128)).all()
 
 
-@pytest.mark.parametrize("T", [5, 150, 600])
+@pytest.mark.parametrize("T", [1, 2, 5, 150, 600])
 def test_row_pitch(T):
     run_exact(T, 130, 208, out=F32, w_pad=16, x_pad=48, seed=8)
     q, w = codes(T, 64, 1).cuda(), codes(50, 64, 2).cuda()
@@ -112,7 +112,7 @@ def test_quantize_special_rows():
     assert (y[1] == 0).all() and torch.isfinite(y[[0, 1, 4, 6, 7]]).all()
 
 
-@pytest.mark.parametrize("T", [1, 9, 64, 80, 150, 600])
+@pytest.mark.parametrize("T", [1, 2, 9, 64, 80, 150, 600])
 @pytest.mark.parametrize("N,K", [(96, 272), (1000, 1024)])
 @pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("swiglu", [False, True])

@@ -52,6 +52,7 @@ struct SelectBwdArgs {
   void* dlogits;
   int64_t ld, dld;
   int T, E, K, type, renorm;
+  int vec, dvec;   // rows start on 16 (32-bit logits) or 8 bytes
   float scale;
 };
 
@@ -78,7 +79,7 @@ __device__ __forceinline__ float warp_max(float v) {
 
 // Sorts v[0..N-1] descending (odd-even merge network).
 template <int N>
-__device__ __forceinline__ void sort_desc(uint32_t (&v)[N]) {
+__device__ __forceinline__ void sort_desc(float (&v)[N]) {
 #pragma unroll
   for (int p = 1; p < N; p *= 2)
 #pragma unroll
@@ -88,10 +89,21 @@ __device__ __forceinline__ void sort_desc(uint32_t (&v)[N]) {
 #pragma unroll
         for (int i = 0; i < k; ++i)
           if (i + j + k < N && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
-            const uint32_t hi = max(v[i + j], v[i + j + k]), lo = min(v[i + j], v[i + j + k]);
+            const float hi = fmaxf(v[i + j], v[i + j + k]), lo = fminf(v[i + j], v[i + j + k]);
             v[i + j] = hi;
             v[i + j + k] = lo;
           }
+}
+
+__device__ __forceinline__ float redux_max(float v) {
+  float m;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+  return m;
+}
+__device__ __forceinline__ float redux_min(float v) {
+  float m;
+  asm volatile("redux.sync.min.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+  return m;
 }
 
 // Loads this lane's V logits (experts first.. of E; the rest as -inf).
@@ -123,21 +135,42 @@ __device__ __forceinline__ void load_logits(const void* p, int type, int64_t off
   }
 }
 
+template <int V>
+__device__ __forceinline__ void store_logits(void* p, int type, int64_t off, int first, int E, bool vec, const float* x) {
+  if (V >= 4 && vec && first + V <= E) {
+#pragma unroll
+    for (int i = 0; i + 4 <= V; i += 4) {
+      if (type == MOE_B200_FP32)
+        *reinterpret_cast<float4*>(static_cast<float*>(p) + off + first + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+      else if (type == MOE_B200_BF16)
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + off + first + i) =
+            make_uint2(pack2(x[i], x[i + 1], bf16{}), pack2(x[i + 2], x[i + 3], bf16{}));
+      else
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + off + first + i) =
+            make_uint2(pack2(x[i], x[i + 1], fp16{}), pack2(x[i + 2], x[i + 3], fp16{}));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (first + i < E) store8_dyn<false>(p, type, off + first + i, 1, x + i);
+  }
+}
+
 // The scores as defined (EXACT), or 32-bit ones.  Returns the largest score of the row that is
 // known without looking (sigmoid: 1; softmax: that of the largest logit): the size that errors
 // are measured by.  A 32-bit score is off by less than 2^-19 of it:
 //   sigmoid: __expf(-x) is off by |x| 2^-24 + 2^-22 of itself, which moves s by s (1 - s) times as
 //     much, at most 2^-24 and 2^-24; the sum and the quotient add 2^-22.
-//   softmax: x - m rounds by |x - m| 2^-24, which moves a score by at most 0.37 * 2^-24 of the
-//     largest; expf, the quotient and its product add 5 units, a sum of 16 terms in a lane and
-//     5 over the lanes 21 of 2^-24.
+//   softmax: x - m and its product with log2(e) round by |x - m| 2^-24 each, which moves a score by
+//     at most 0.74 * 2^-24 of the largest; the exponential, the quotient and its product add 6
+//     units, a sum of 16 terms in a lane and 5 over the lanes 21 of 2^-24.
 template <int V, bool SOFTMAX, bool EXACT>
 __device__ __forceinline__ float scores(const float* x, float lowest, float* s) {
   if constexpr (!SOFTMAX) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       if constexpr (EXACT) s[i] = x[i] <= lowest ? 0.f : __frcp_rn(1.0f + exp_to_f32(-static_cast<double>(x[i])));
-      else s[i] = x[i] <= lowest ? 0.f : __fdividef(1.0f, 1.0f + __expf(-fmaxf(x[i], -80.f)));
+      else s[i] = x[i] <= lowest ? 0.f : __fdividef(1.0f, 1.0f + __expf(-max_nan(x[i], -80.f)));
     }
     return 1.f;
   } else {
@@ -161,10 +194,10 @@ __device__ __forceinline__ float scores(const float* x, float lowest, float* s) 
       float sum = 0.f;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        s[i] = x[i] <= lowest ? 0.f : expf(x[i] - m);
+        s[i] = x[i] <= lowest ? 0.f : __expf(x[i] - m);
         sum += s[i];
       }
-      const float inv = 1.f / fmaxf(warp_sum(sum), 1e-30f);
+      const float inv = 1.f / max_nan(warp_sum(sum), 1e-30f);
 #pragma unroll
       for (int i = 0; i < V; ++i) s[i] *= inv;
       return inv;
@@ -184,15 +217,15 @@ __device__ __forceinline__ bool apart(float in, float out, float size) {
   return out == -INFINITY || in == -INFINITY || in - out > kMargin * fmaxf(size, fmaxf(fabsf(in), fabsf(out)));
 }
 
-// Keys of the fast choice: order_key without its low 4 bits, in which the slot is kept; 0: not to be chosen.
-constexpr uint32_t kSlotMask = 15u;
-__device__ __forceinline__ float key_value(uint32_t k) {
-  if (k == 0) return -INFINITY;
-  k &= ~kSlotMask;
-  return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
+// Keys of the fast choice: sel (below kHuge in size) with its low 4 bits replaced by the slot;
+// kNone: not to be chosen.
+constexpr float kNone = -3.4e38f, kHuge = 1e30f;
+__device__ __forceinline__ float slot_key(float sel, int slot) {
+  return sel == -INFINITY ? kNone : __uint_as_float((__float_as_uint(sel) & ~15u) | slot);
 }
+__device__ __forceinline__ float or_none(float v) { return v <= kNone ? -INFINITY : v; }
 
-// Group scores in the lanes of shared memory's scan: lane g < n_group scans group g.
+// Group scores from shared memory: lane g < n_group scans group g.
 __device__ __forceinline__ void scan_group(const float* sel, int lane, int n_group, int gs, float* m1, float* m2) {
   *m1 = *m2 = -INFINITY;
   if (lane < n_group)
@@ -204,126 +237,143 @@ __device__ __forceinline__ void scan_group(const float* sel, int lane, int n_gro
       *m1 = fmaxf(*m1, v);
     }
 }
-
-// Bit mask of the groups that stay; *sure: no decision within the margin (fast scores).
-__device__ __forceinline__ uint32_t keep_groups(float score, int g, bool leader, int n_group, int per_group_lanes,
-                                                int topk_group, float size, bool* sure) {
-  int rank = 0;
-  for (int h = 0; h < n_group; ++h) {
-    const float o = __shfl_sync(0xffffffffu, score, h * per_group_lanes);
-    rank += (o > score || (o == score && h < g)) ? 1 : 0;
-  }
-  const bool kept = leader && rank < topk_group;
-  const float in = key_value(__reduce_min_sync(0xffffffffu, kept && score != -INFINITY ? order_key(score) | kSlotMask : ~0u));
-  const float out = key_value(__reduce_max_sync(0xffffffffu, leader && !kept && score != -INFINITY ? order_key(score) : 0u));
-  *sure = apart(in, out, size);
-  uint32_t mask = __ballot_sync(0xffffffffu, kept);
-  if (per_group_lanes > 1) {   // from lanes h * per_group_lanes to bits h
-    uint32_t m = 0;
-    for (int h = 0; h < n_group; ++h) m |= ((mask >> (h * per_group_lanes)) & 1u) << h;
-    mask = m;
-  }
-  return mask;
+__device__ __forceinline__ float group_score(const SelectArgs& a, float m1, float m2) {
+  return a.top2 ? m1 + (m2 == -INFINITY ? 0.f : m2) : m1;
 }
 
-// The choice: bit i of the result says that this lane's expert i is chosen.  EXACT: by the
-// defined scores.  Otherwise *sure tells whether the 32-bit scores decide it.
-template <int V, bool EXACT>
-__device__ __forceinline__ uint32_t choose(const SelectArgs& a, const float* sel0, float* s_sel, int lane, float size,
-                                           bool* sure) {
-  float sel[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) sel[i] = sel0[i];
+// Whether group g (its score in each of its lanes, lane h * lanes first) is among the topk_group
+// best; *sure: no decision within the margin.
+__device__ __forceinline__ bool keep_group(const SelectArgs& a, float score, int g, int lanes, float size, bool* sure) {
+  int rank = 0;
+  for (int h = 0; h < a.n_group; ++h) {
+    const float o = __shfl_sync(0xffffffffu, score, h * lanes);
+    rank += (o > score || (o == score && h < g)) ? 1 : 0;
+  }
+  const bool kept = g < a.n_group && rank < a.topk_group;
+  const float in = redux_min(kept && score != -INFINITY ? score : INFINITY);
+  const float out = redux_max(g < a.n_group && !kept ? score : -INFINITY);
+  *sure = in == INFINITY || apart(in, out, size);
+  return kept;
+}
+
+// Whether a group is a power of two of neighbouring lanes (*lanes); otherwise groups are scored
+// through shared memory.
+template <int V>
+__device__ __forceinline__ bool groups_by_lane(const SelectArgs& a, int* lanes) {
+  const int gs = a.E / a.n_group;
+  *lanes = gs / V;
+  return gs % V == 0 && (*lanes & (*lanes - 1)) == 0;
+}
+// A lane's part of its group, of which m1 >= m2 are its two highest, is it kept?
+__device__ __forceinline__ bool keep_by_lane(const SelectArgs& a, float m1, float m2, int lane, int lanes, float size,
+                                             bool* sure) {
+  for (int d = 1; d < lanes; d <<= 1) {
+    const float o1 = __shfl_xor_sync(0xffffffffu, m1, d), o2 = __shfl_xor_sync(0xffffffffu, m2, d);
+    m2 = fmaxf(fminf(m1, o1), fmaxf(m2, o2));
+    m1 = fmaxf(m1, o1);
+  }
+  return keep_group(a, group_score(a, m1, m2), lane / lanes, lanes, size, sure);
+}
+
+// Drops what is not in a kept group from sel, through shared memory: groups of any size.
+template <int V>
+__device__ __forceinline__ void drop_groups(const SelectArgs& a, float* sel, float* s_sel, int lane, float size, bool* sure) {
   const int first = lane * V, gs = a.E / a.n_group;
-  *sure = true;
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (first + i < a.E) s_sel[first + i] = sel[i];
+  __syncwarp();
+  float m1, m2;
+  scan_group(s_sel, lane, a.n_group, gs, &m1, &m2);
+  const uint32_t kept = __ballot_sync(0xffffffffu, keep_group(a, group_score(a, m1, m2), lane, 1, size, sure));
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (first + i < a.E && !((kept >> ((first + i) / gs)) & 1u)) sel[i] = -INFINITY;
+  __syncwarp();
+}
+
+// The choice by the defined scores: bit i of the result says that this lane's expert i is chosen.
+template <int V>
+__device__ __forceinline__ uint32_t choose_exact(const SelectArgs& a, float* sel, float* s_sel, int lane) {
+  bool sure, kept = true;
+  int lanes;
   if (a.n_group > 1) {
-    uint32_t kept;
-    const int lanes = gs / V;
-    if (gs % V == 0 && (lanes & (lanes - 1)) == 0) {   // a group is `lanes` neighbouring lanes
+    if (groups_by_lane<V>(a, &lanes)) {
       float m1 = -INFINITY, m2 = -INFINITY;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         m2 = fmaxf(m2, fminf(m1, sel[i]));
         m1 = fmaxf(m1, sel[i]);
       }
-      for (int d = 1; d < lanes; d <<= 1) {
-        const float o1 = __shfl_xor_sync(0xffffffffu, m1, d), o2 = __shfl_xor_sync(0xffffffffu, m2, d);
-        m2 = fmaxf(fminf(m1, o1), fmaxf(m2, o2));
-        m1 = fmaxf(m1, o1);
-      }
-      const float score = a.top2 ? m1 + (m2 == -INFINITY ? 0.f : m2) : m1;
-      const int g = lane / lanes;
-      kept = keep_groups(score, g, lane % lanes == 0 && g < a.n_group, a.n_group, lanes, a.topk_group, size,
-                         sure);
-      if (!((kept >> (g & 31)) & 1u)) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) sel[i] = -INFINITY;
-      }
+      kept = keep_by_lane(a, m1, m2, lane, lanes, 1.f, &sure);
     } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (first + i < a.E) s_sel[first + i] = sel[i];
-      __syncwarp();
-      float m1, m2;
-      scan_group(s_sel, lane, a.n_group, gs, &m1, &m2);
-      const float score = a.top2 ? m1 + (m2 == -INFINITY ? 0.f : m2) : m1;
-      kept = keep_groups(score, lane, lane < a.n_group, a.n_group, 1, a.topk_group, size, sure);
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (first + i < a.E && !((kept >> ((first + i) / gs)) & 1u)) sel[i] = -INFINITY;
-      __syncwarp();
+      drop_groups<V>(a, sel, s_sel, lane, 1.f, &sure);
     }
+  }
+  uint32_t key[V], taken = 0;   // key 0: not to be chosen
+#pragma unroll
+  for (int i = 0; i < V; ++i) key[i] = !kept || sel[i] == -INFINITY ? 0u : order_key(sel[i]);
+  for (int r = 0; r < a.K; ++r) {
+    uint32_t best = 0;
+    int at = 0;
+#pragma unroll
+    for (int i = V - 1; i >= 0; --i)
+      if (key[i] >= best) {
+        best = key[i];
+        at = i;
+      }
+    const uint32_t m = __reduce_max_sync(0xffffffffu, best);
+    if (m == 0) break;
+    if (lane == __ffs(__ballot_sync(0xffffffffu, best == m)) - 1) {
+      taken |= 1u << at;
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (i == at) key[i] = 0;
+    }
+  }
+  return taken;
+}
+
+// The choice by 32-bit scores; *sure tells whether they decide it.
+template <int V>
+__device__ __forceinline__ uint32_t choose_fast(const SelectArgs& a, float* sel, float* s_sel, int lane, float size,
+                                                bool* sure) {
+  int lanes;
+  const bool by_lane = groups_by_lane<V>(a, &lanes);
+  *sure = true;
+  if (a.n_group > 1 && !by_lane) drop_groups<V>(a, sel, s_sel, lane, size, sure);
+  float key[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) key[i] = slot_key(sel[i], i);
+  sort_desc(key);
+  if (a.n_group > 1 && by_lane &&
+      !keep_by_lane(a, or_none(key[0]), V > 1 ? or_none(key[V > 1 ? 1 : 0]) : -INFINITY, lane, lanes, size, sure)) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) key[i] = kNone;
   }
   uint32_t taken = 0;
-  if constexpr (EXACT) {
-    uint32_t key[V];   // 0: not to be chosen
+  float weakest = kNone;
+  for (int r = 0; r < a.K; ++r) {
+    const float m = redux_max(key[0]);
+    if (m <= kNone) break;
+    weakest = m;
+    // equal keys of several lanes: within the margin, so any order will do here
+    if (lane == __ffs(__ballot_sync(0xffffffffu, key[0] == m)) - 1) {
+      taken |= 1u << (__float_as_uint(m) & 15u);
 #pragma unroll
-    for (int i = 0; i < V; ++i) key[i] = sel[i] == -INFINITY ? 0u : order_key(sel[i]);
-    for (int r = 0; r < a.K; ++r) {
-      uint32_t best = 0;
-      int at = 0;
-#pragma unroll
-      for (int i = V - 1; i >= 0; --i)
-        if (key[i] >= best) {
-          best = key[i];
-          at = i;
-        }
-      const uint32_t m = __reduce_max_sync(0xffffffffu, best);
-      if (m == 0) break;
-      if (lane == __ffs(__ballot_sync(0xffffffffu, best == m)) - 1) {
-        taken |= 1u << at;
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-          if (i == at) key[i] = 0;
-      }
+      for (int i = 0; i + 1 < V; ++i) key[i] = key[i + 1];
+      key[V - 1] = kNone;
     }
-  } else {
-    uint32_t key[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-      key[i] = sel[i] == -INFINITY ? 0u : (order_key(sel[i]) & ~kSlotMask) | static_cast<uint32_t>(V - 1 - i);
-    sort_desc(key);
-    uint32_t weakest = 0;
-    for (int r = 0; r < a.K; ++r) {
-      const uint32_t m = __reduce_max_sync(0xffffffffu, key[0]);
-      if (m == 0) break;
-      weakest = m;
-      // equal keys of several lanes: within the margin, so any order will do here
-      if (lane == __ffs(__ballot_sync(0xffffffffu, key[0] == m)) - 1) {
-        taken |= 1u << (V - 1 - static_cast<int>(key[0] & kSlotMask));
-#pragma unroll
-        for (int i = 0; i + 1 < V; ++i) key[i] = key[i + 1];
-        key[V - 1] = 0;
-      }
-    }
-    *sure = *sure && apart(key_value(weakest), key_value(__reduce_max_sync(0xffffffffu, key[0])), size);
   }
+  *sure = *sure && apart(or_none(weakest), or_none(redux_max(key[0])), size);
   return taken;
 }
 
 template <int V, bool SOFTMAX>
 __global__ void __launch_bounds__(kSelWarps * 32) select_kernel(SelectArgs a) {
   extern __shared__ float s_dyn[];   // [warps][E] sel of a token (groups only), then [E] counts
+  __shared__ float s_val[kSelWarps][kSelMaxK];
+  __shared__ int s_id[kSelWarps][kSelMaxK];
   pdl_wait();
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -342,34 +392,27 @@ __global__ void __launch_bounds__(kSelWarps * 32) select_kernel(SelectArgs a) {
     float x[V], s[V], sel[V];
     load_logits<V>(a.logits, a.type, t * a.ld, first, a.E, a.vec, x);
     const float size = scores<V, SOFTMAX, false>(x, lowest, s);
-    bool bad = false, sure = true;
+    float largest = 0.f;   // in size, NaN if there is one
+    auto biased = [&](int i) { return x[i] <= lowest || bias[i] == -INFINITY ? -INFINITY : s[i] + bias[i]; };
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      sel[i] = x[i] <= lowest ? -INFINITY : s[i] + bias[i];
-      // the bounded sigmoid hides a NaN; an infinite logit makes a softmax NaN
-      bad |= sel[i] != sel[i] || x[i] != x[i];
+      sel[i] = biased(i);
+      largest = max_nan(largest, sel[i] == -INFINITY ? 0.f : fabsf(sel[i]));
     }
-    bad = __any_sync(0xffffffffu, bad);
+    const bool bad = __any_sync(0xffffffffu, largest != largest);
     uint32_t taken = 0;
-    if (!bad) taken = choose<V, false>(a, sel, s_sel, lane, size, &sure);
+    // (biases so large that sums of them overflow are left to the exact choice)
+    bool sure = bad || !__any_sync(0xffffffffu, largest >= kHuge);
+    if (!bad && sure) taken = choose_fast<V>(a, sel, s_sel, lane, size, &sure);
     if (!sure) {
       scores<V, SOFTMAX, true>(x, lowest, s);
 #pragma unroll
-      for (int i = 0; i < V; ++i) sel[i] = x[i] <= lowest ? -INFINITY : s[i] + bias[i];
-      taken = choose<V, true>(a, sel, s_sel, lane, size, &sure);
-    } else if constexpr (!SOFTMAX) {
-      // the chosen scores as defined (about one per lane that has any)
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        if ((taken >> i) & 1u) s[i] = __frcp_rn(1.0f + exp_to_f32(-static_cast<double>(x[i])));
+      for (int i = 0; i < V; ++i) sel[i] = biased(i);
+      taken = choose_exact<V>(a, sel, s_sel, lane);
     }
-    float part = 0.f;
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-      if ((taken >> i) & 1u) part += s[i];
-    const float denom = warp_sum(part) + 1e-20f;
+    // the chosen, by ascending id, to one lane each: those compute and store the weights
     const int mine = __popc(taken);
-    int pos = mine;   // exclusive prefix over the lanes
+    int pos = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const int o = __shfl_up_sync(0xffffffffu, pos, d);
@@ -377,19 +420,26 @@ __global__ void __launch_bounds__(kSelWarps * 32) select_kernel(SelectArgs a) {
     }
     const int total = __shfl_sync(0xffffffffu, pos, 31);
     pos -= mine;
-    const int64_t base = static_cast<int64_t>(t) * a.K;
 #pragma unroll
     for (int i = 0; i < V; ++i)
       if ((taken >> i) & 1u) {
-        a.idx[base + pos] = first + i;
-        a.w[base + pos] = (a.renorm ? s[i] / denom : s[i]) * a.scale;
+        s_val[warp][pos] = SOFTMAX ? s[i] : x[i];
+        s_id[warp][pos] = first + i;
         ++pos;
-        if (a.counts) atomicAdd(s_cnt + first + i, 1);
       }
-    if (lane >= total && lane < a.K) {
-      a.idx[base + lane] = -1;
-      a.w[base + lane] = bad ? __uint_as_float(0x7fc00000u) : 0.f;
+    __syncwarp();
+    const bool have = lane < total;
+    float w = have ? s_val[warp][lane] : 0.f;
+    const int id = have ? s_id[warp][lane] : -1;
+    __syncwarp();
+    if constexpr (!SOFTMAX) w = have ? __frcp_rn(1.0f + exp_to_f32(-static_cast<double>(w))) : 0.f;   // as defined
+    const float denom = warp_sum(w) + 1e-20f;
+    if (lane < a.K) {
+      const int64_t o = static_cast<int64_t>(t) * a.K + lane;
+      a.idx[o] = id;
+      a.w[o] = bad ? __uint_as_float(0x7fc00000u) : (a.renorm ? w / denom : w) * a.scale;
     }
+    if (a.counts && have) atomicAdd(s_cnt + id, 1);
   }
   if (!a.counts) return;
   if (a.cluster) {   // the CTAs of one cluster are the whole grid: the first adds up their counts
@@ -417,89 +467,83 @@ __global__ void __launch_bounds__(kSelMaxE) select_zero_kernel(int* counts, int 
 // dlogits of a token, from the gradients dw of its chosen weights (ids distinct, -1: no expert).
 //   renormalised, S = sum of the chosen s + 1e-20:  ds_k = scale * (dw_k - sum_j dw_j s_j / S) / S
 //   softmax: dx_e = s_e (ds_e - sum_j ds_j s_j);  sigmoid: dx_e = ds_e s_e (1 - s_e)
+// The scores go to shared memory, where a lane per chosen expert finds its own; those lanes work out
+// the sums and put their own results among what every lane stores.
 template <int V, bool SOFTMAX>
 __global__ void __launch_bounds__(kSelWarps * 32) select_bwd_kernel(SelectBwdArgs a) {
+  __shared__ __align__(16) float s_row[kSelWarps][32 * V];
   pdl_wait();
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const float lowest = lowest_of(a.type);
+  const int first = lane * V;
+  float* row = s_row[warp];
   for (int t = blockIdx.x * kSelWarps + warp; t < a.T; t += gridDim.x * kSelWarps) {
-    float x[V], s[V], d[V] = {};
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int e = i * 32 + lane;
-      x[i] = e < a.E ? load1_dyn(a.logits, a.type, t * a.ld + e) : -INFINITY;
-    }
-    const int64_t base = static_cast<int64_t>(t) * a.K;
-    const int my_id = lane < a.K ? a.idx[base + lane] : -1;
-    const float my_dw = lane < a.K ? a.dw[base + lane] * a.scale : 0.f;
+    float x[V], s[V];
+    load_logits<V>(a.logits, a.type, t * a.ld, first, a.E, a.vec, x);
+    const int64_t at = static_cast<int64_t>(t) * a.K + lane;
+    const int id = lane < a.K ? a.idx[at] : -1;
+    const bool have = id >= 0 && id < a.E;
+    float d = have ? a.dw[at] * a.scale : 0.f;
     if constexpr (SOFTMAX) {
       float m = -INFINITY;
 #pragma unroll
       for (int i = 0; i < V; ++i) m = fmaxf(m, x[i] <= lowest ? -INFINITY : x[i]);
-      m = warp_max(m);
+      m = redux_max(m);
       float sum = 0.f;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        s[i] = x[i] <= lowest ? 0.f : expf(x[i] - m);
+        s[i] = x[i] <= lowest ? 0.f : __expf(x[i] - m);
         sum += s[i];
       }
-      const float inv = 1.f / fmaxf(warp_sum(sum), 1e-30f);
+      const float inv = 1.f / max_nan(warp_sum(sum), 1e-30f);
 #pragma unroll
       for (int i = 0; i < V; ++i) s[i] *= inv;
     } else {
 #pragma unroll
-      for (int i = 0; i < V; ++i) s[i] = x[i] <= lowest ? 0.f : 1.f / (1.f + expf(-x[i]));
+      for (int i = 0; i < V; ++i) s[i] = x[i] <= lowest ? 0.f : x[i];
     }
-    bool bad = false;
-#pragma unroll
-    for (int i = 0; i < V; ++i) bad |= x[i] != x[i] || s[i] != s[i];
-    bad = __any_sync(0xffffffffu, bad);
-    uint32_t taken = 0;
-    for (int k = 0; k < a.K; ++k) {
-      const int id = __shfl_sync(0xffffffffu, my_id, k);
-      const float dw = __shfl_sync(0xffffffffu, my_dw, k);
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (id == i * 32 + lane) {
-          d[i] = dw;
-          taken |= 1u << i;
-        }
-    }
-    float chosen = 0.f, dot = 0.f;
+    float all = 0.f;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      if ((taken >> i) & 1u) chosen += s[i];
-      dot += d[i] * s[i];
+      row[first + i] = s[i];
+      all = max_nan(all, s[i]);
     }
+    const bool bad = __any_sync(0xffffffffu, all != all);   // a NaN logit, or an infinite one of a softmax
+    __syncwarp();
+    float sk = have ? row[id] : 0.f;
+    // sigmoid: from the logit that was put there (one that is switched off was not chosen)
+    float one_minus = 0.f;
+    if constexpr (!SOFTMAX) {
+      const float e = expf(-sk);
+      sk = have ? 1.f / (1.f + e) : 0.f;
+      one_minus = sk < 1.f ? 1.f - sk : 0.f;
+    }
+    float dot = d * sk;
     if (a.renorm) {
-      const float S = warp_sum(chosen) + 1e-20f;
+      const float S = warp_sum(sk) + 1e-20f;
       const float mean = warp_sum(dot) / S;
-      dot = 0.f;
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        d[i] = (taken >> i) & 1u ? (d[i] - mean) / S : 0.f;
-        dot += d[i] * s[i];
-      }
+      d = have ? (d - mean) / S : 0.f;
+      dot = d * sk;
     }
+    float mine;   // this lane's chosen expert's gradient
     if constexpr (SOFTMAX) {
       dot = warp_sum(dot);
-#pragma unroll
-      for (int i = 0; i < V; ++i) d[i] = s[i] * (d[i] - dot);
+      mine = sk * (d - dot);
     } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i) d[i] *= s[i] * (1.f - s[i]);
+      mine = d * sk * one_minus;
     }
+    __syncwarp();
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int e = i * 32 + lane;
-      if (e >= a.E) continue;
-      const float v = bad ? __uint_as_float(0x7fc00000u) : d[i];
-      const int64_t o = t * a.dld + e;
-      if (a.type == MOE_B200_BF16) static_cast<bf16*>(a.dlogits)[o] = from_f<bf16>(v);
-      else if (a.type == MOE_B200_FP16) static_cast<fp16*>(a.dlogits)[o] = from_f<fp16>(v);
-      else static_cast<float*>(a.dlogits)[o] = v;
-    }
+    for (int i = 0; i < V; ++i) row[first + i] = SOFTMAX ? -s[i] * dot : 0.f;
+    __syncwarp();
+    if (have) row[id] = mine;
+    __syncwarp();
+    float g[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) g[i] = bad ? __uint_as_float(0x7fc00000u) : row[first + i];
+    store_logits<V>(a.dlogits, a.type, t * a.dld, first, a.E, a.dvec, g);
+    __syncwarp();
   }
 }
 
@@ -618,6 +662,9 @@ MOE_B200_API int moe_b200_select_experts_backward(const moe_b200_select_backward
   s.type = a->logits_type;
   s.renorm = a->renormalize;
   s.scale = a->scale;
+  const int bytes = 4 * type_bytes(s.type);
+  s.vec = reinterpret_cast<uintptr_t>(s.logits) % bytes == 0 && (s.T == 1 || s.ld % 4 == 0);
+  s.dvec = reinterpret_cast<uintptr_t>(s.dlogits) % bytes == 0 && (s.T == 1 || s.dld % 4 == 0);
   cudaError_t e = cudaSuccess;
   const dim3 grid(select_grid(s.T, sms)), block(kSelWarps * 32);
   cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -128,6 +128,19 @@ def test_close_scores_are_told_apart():
     check(x, 8)
 
 
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+def test_biases_of_any_size(score):
+    """Biases from the tiny to the overflowing, and -inf: chosen by the defined 32-bit sums."""
+    g = torch.Generator().manual_seed(8)
+    x = torch.randn(40, 64, generator=g).cuda()
+    for size in (1e-30, 1e-7, 1.0, 1e4, 1e29, 1e32, 2.5e38):
+        b = (torch.randn(64, generator=g) * 0.3 + torch.randint(-1, 2, (64,), generator=g)).clamp(-1.3, 1.3) * size
+        b[5] = float("-inf")
+        for kw in (dict(), dict(n_group=8, topk_group=3), dict(n_group=8, topk_group=3, group_score="max"),
+                   dict(n_group=16, topk_group=5)):
+            check(x, 6, score=score, bias=b.cuda(), **kw)
+
+
 @pytest.mark.parametrize("T", [1, 255, 4096])
 def test_row_pitch_and_sizes(T):
     x = logits_of(T, 33, seed=7, pad=7)

@@ -71,12 +71,6 @@ __device__ __forceinline__ double warp_sum_d(double v) {
   for (int d = 16; d >= 1; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
   return v;
 }
-__device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-  for (int d = 16; d >= 1; d >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
-  return v;
-}
-
 // Sorts v[0..N-1] descending (odd-even merge network).
 template <int N>
 __device__ __forceinline__ void sort_desc(float (&v)[N]) {
@@ -176,8 +170,8 @@ __device__ __forceinline__ float scores(const float* x, float lowest, float* s) 
   } else {
     float m = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < V; ++i) m = fmaxf(m, x[i] <= lowest ? -INFINITY : x[i]);
-    m = warp_max(m);
+    for (int i = 0; i < V; ++i) m = fmaxf(m, x[i]);   // (switched off ones do no harm)
+    m = redux_max(m);
     if constexpr (EXACT) {
       double ex[V], sum = 0.0;
 #pragma unroll
@@ -206,10 +200,10 @@ __device__ __forceinline__ float scores(const float* x, float lowest, float* s) 
 }
 
 // Two sides of a decision are told apart by the 32-bit scores if they differ by more than this
-// share of the sizes involved.  Each side is off by 2^-19 of the row's size for a score, twice that
-// for a group's two, and by 2^-20 of its own for the slot in a key's low bits and 2^-23 for the
-// sums' rounding: together less than 2^-17 + 2^-18.
-constexpr float kMargin = 1.52587890625e-05f;   // 2^-16
+// share of the sizes involved.  An expert's score is off by 2^-19 of the row's size and its key by
+// 2^-19 of itself (the lane in the low bits), a group's by 2^-19 of the size for either of its two;
+// their sums round by 2^-23.  For both sides of a decision that is less than 2^-16.
+constexpr float kMargin = 1.52587890625e-05f;
 
 // Whether `in` (the weakest taken) is above `out` (the strongest left) for certain.  -inf for
 // either: nothing was taken or left, no decision.
@@ -217,11 +211,11 @@ __device__ __forceinline__ bool apart(float in, float out, float size) {
   return out == -INFINITY || in == -INFINITY || in - out > kMargin * fmaxf(size, fmaxf(fabsf(in), fabsf(out)));
 }
 
-// Keys of the fast choice: sel (below kHuge in size) with its low 4 bits replaced by the slot;
-// kNone: not to be chosen.
-constexpr float kNone = -3.4e38f, kHuge = 1e30f;
-__device__ __forceinline__ float slot_key(float sel, int slot) {
-  return sel == -INFINITY ? kNone : __uint_as_float((__float_as_uint(sel) & ~15u) | slot);
+// Keys of the fast choice: sel (below kHuge in size) with the lane in its low 5 bits, so that no two
+// lanes have equal ones; at most kNone: not to be chosen.
+constexpr float kNone = -3.39e38f, kHuge = 1e30f;
+__device__ __forceinline__ float lane_key(float sel, int lane) {
+  return __uint_as_float((__float_as_uint(fmaxf(sel, -3.4e38f)) & ~31u) | lane);
 }
 __device__ __forceinline__ float or_none(float v) { return v <= kNone ? -INFINITY : v; }
 
@@ -334,51 +328,68 @@ __device__ __forceinline__ uint32_t choose_exact(const SelectArgs& a, float* sel
   return taken;
 }
 
-// The choice by 32-bit scores; *sure tells whether they decide it.
+// The choice by 32-bit scores; *sure tells whether they decide it.  Each lane sorts its keys; a round
+// is then one maximum over the warp's first keys and a shift of the list that held it.  What is
+// chosen is what reaches the last round's maximum.
 template <int V>
 __device__ __forceinline__ uint32_t choose_fast(const SelectArgs& a, float* sel, float* s_sel, int lane, float size,
                                                 bool* sure) {
-  int lanes;
-  const bool by_lane = groups_by_lane<V>(a, &lanes);
   *sure = true;
-  if (a.n_group > 1 && !by_lane) drop_groups<V>(a, sel, s_sel, lane, size, sure);
-  float key[V];
+  if (a.n_group > 1) {
+    int lanes;
+    if (groups_by_lane<V>(a, &lanes)) {
+      float m1 = -INFINITY, m2 = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < V; ++i) key[i] = slot_key(sel[i], i);
-  sort_desc(key);
-  if (a.n_group > 1 && by_lane &&
-      !keep_by_lane(a, or_none(key[0]), V > 1 ? or_none(key[V > 1 ? 1 : 0]) : -INFINITY, lane, lanes, size, sure)) {
+      for (int i = 0; i < V; ++i) {
+        m2 = fmaxf(m2, fminf(m1, sel[i]));
+        m1 = fmaxf(m1, sel[i]);
+      }
+      if (!keep_by_lane(a, m1, m2, lane, lanes, size, sure)) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) key[i] = kNone;
-  }
-  uint32_t taken = 0;
-  float weakest = kNone;
-  for (int r = 0; r < a.K; ++r) {
-    const float m = redux_max(key[0]);
-    if (m <= kNone) break;
-    weakest = m;
-    // equal keys of several lanes: within the margin, so any order will do here
-    if (lane == __ffs(__ballot_sync(0xffffffffu, key[0] == m)) - 1) {
-      taken |= 1u << (__float_as_uint(m) & 15u);
-#pragma unroll
-      for (int i = 0; i + 1 < V; ++i) key[i] = key[i + 1];
-      key[V - 1] = kNone;
+        for (int i = 0; i < V; ++i) sel[i] = -INFINITY;
+      }
+    } else {
+      drop_groups<V>(a, sel, s_sel, lane, size, sure);
     }
   }
-  *sure = *sure && apart(or_none(weakest), or_none(redux_max(key[0])), size);
+  float key[V], list[V + 1];
+#pragma unroll
+  for (int i = 0; i < V; ++i) key[i] = lane_key(sel[i], lane);
+  {
+    float sorted[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) sorted[i] = key[i];
+    sort_desc(sorted);
+#pragma unroll
+    for (int i = 0; i < V; ++i) list[i] = sorted[i];
+    list[V] = -3.4e38f;
+  }
+  float last = INFINITY;
+  for (int r = 0; r < a.K; ++r) {
+    const float m = redux_max(list[0]);
+    if (m <= kNone) break;
+    last = m;
+    const bool mine = list[0] == m;
+#pragma unroll
+    for (int i = 0; i < V; ++i) list[i] = mine ? list[i + 1] : list[i];
+  }
+  // (equal keys of one lane on both sides of the end are not apart)
+  *sure = *sure && (last == INFINITY || apart(last, or_none(redux_max(list[0])), size));
+  uint32_t taken = 0;
+#pragma unroll
+  for (int i = 0; i < V; ++i) taken |= key[i] >= last ? 1u << i : 0u;
   return taken;
 }
 
 template <int V, bool SOFTMAX>
 __global__ void __launch_bounds__(kSelWarps * 32) select_kernel(SelectArgs a) {
-  extern __shared__ float s_dyn[];   // [warps][E] sel of a token (groups only), then [E] counts
-  __shared__ float s_val[kSelWarps][kSelMaxK];
+  extern __shared__ __align__(16) float s_dyn[];   // [warps][32 V] values of a token, then [E] counts
   __shared__ int s_id[kSelWarps][kSelMaxK];
   pdl_wait();
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float* s_sel = s_dyn + warp * a.E;
-  int* s_cnt = reinterpret_cast<int*>(s_dyn + (a.n_group > 1 ? kSelWarps * a.E : 0));
+  float* s_row = s_dyn + warp * 32 * V;
+  int* s_cnt = reinterpret_cast<int*>(s_dyn + kSelWarps * 32 * V);
   if (a.counts) {
     for (int e = threadIdx.x; e < a.E; e += blockDim.x) s_cnt[e] = 0;
     __syncthreads();
@@ -386,31 +397,37 @@ __global__ void __launch_bounds__(kSelWarps * 32) select_kernel(SelectArgs a) {
   const float lowest = lowest_of(a.type);
   const int first = lane * V;
   float bias[V];
+  bool wild = false;
 #pragma unroll
-  for (int i = 0; i < V; ++i) bias[i] = a.bias && first + i < a.E ? load1_dyn(a.bias, a.bias_type, first + i) : 0.f;
+  for (int i = 0; i < V; ++i) {
+    bias[i] = a.bias && first + i < a.E ? load1_dyn(a.bias, a.bias_type, first + i) : 0.f;
+    wild |= fabsf(bias[i]) >= kHuge && bias[i] != -INFINITY;
+  }
+  // biases so large that sums of two overflow: every choice by the defined scores
+  wild = __any_sync(0xffffffffu, wild);
   for (int t = blockIdx.x * kSelWarps + warp; t < a.T; t += gridDim.x * kSelWarps) {
     float x[V], s[V], sel[V];
     load_logits<V>(a.logits, a.type, t * a.ld, first, a.E, a.vec, x);
     const float size = scores<V, SOFTMAX, false>(x, lowest, s);
-    float largest = 0.f;   // in size, NaN if there is one
-    auto biased = [&](int i) { return x[i] <= lowest || bias[i] == -INFINITY ? -INFINITY : s[i] + bias[i]; };
+    float nan = 0.f;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      sel[i] = biased(i);
-      largest = max_nan(largest, sel[i] == -INFINITY ? 0.f : fabsf(sel[i]));
+      sel[i] = x[i] <= lowest ? -INFINITY : s[i] + bias[i];
+      nan = max_nan(nan, sel[i]);
     }
-    const bool bad = __any_sync(0xffffffffu, largest != largest);
+    const bool bad = __any_sync(0xffffffffu, nan != nan);
     uint32_t taken = 0;
-    // (biases so large that sums of them overflow are left to the exact choice)
-    bool sure = bad || !__any_sync(0xffffffffu, largest >= kHuge);
-    if (!bad && sure) taken = choose_fast<V>(a, sel, s_sel, lane, size, &sure);
+    bool sure = bad || !wild;
+    if (!bad && sure) taken = choose_fast<V>(a, sel, s_row, lane, size, &sure);
     if (!sure) {
       scores<V, SOFTMAX, true>(x, lowest, s);
 #pragma unroll
-      for (int i = 0; i < V; ++i) sel[i] = biased(i);
-      taken = choose_exact<V>(a, sel, s_sel, lane);
+      for (int i = 0; i < V; ++i) sel[i] = x[i] <= lowest ? -INFINITY : s[i] + bias[i];
+      taken = choose_exact<V>(a, sel, s_row, lane);
     }
     // the chosen, by ascending id, to one lane each: those compute and store the weights
+#pragma unroll
+    for (int i = 0; i < V; ++i) s_row[first + i] = SOFTMAX ? s[i] : x[i];
     const int mine = __popc(taken);
     int pos = mine;
 #pragma unroll
@@ -419,18 +436,11 @@ __global__ void __launch_bounds__(kSelWarps * 32) select_kernel(SelectArgs a) {
       if (lane >= d) pos += o;
     }
     const int total = __shfl_sync(0xffffffffu, pos, 31);
-    pos -= mine;
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-      if ((taken >> i) & 1u) {
-        s_val[warp][pos] = SOFTMAX ? s[i] : x[i];
-        s_id[warp][pos] = first + i;
-        ++pos;
-      }
+    for (pos -= mine; taken; taken &= taken - 1) s_id[warp][pos++] = first + __ffs(taken) - 1;
     __syncwarp();
     const bool have = lane < total;
-    float w = have ? s_val[warp][lane] : 0.f;
     const int id = have ? s_id[warp][lane] : -1;
+    float w = have ? s_row[id] : 0.f;
     __syncwarp();
     if constexpr (!SOFTMAX) w = have ? __frcp_rn(1.0f + exp_to_f32(-static_cast<double>(w))) : 0.f;   // as defined
     const float denom = warp_sum(w) + 1e-20f;
@@ -488,7 +498,7 @@ __global__ void __launch_bounds__(kSelWarps * 32) select_bwd_kernel(SelectBwdArg
     if constexpr (SOFTMAX) {
       float m = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < V; ++i) m = fmaxf(m, x[i] <= lowest ? -INFINITY : x[i]);
+      for (int i = 0; i < V; ++i) m = fmaxf(m, x[i]);
       m = redux_max(m);
       float sum = 0.f;
 #pragma unroll
@@ -621,13 +631,13 @@ MOE_B200_API int moe_b200_select_experts(const moe_b200_select_args* a, void* st
   s.top2 = a->group_score == MOE_B200_GROUP_TOP2;
   s.renorm = a->renormalize;
   s.scale = a->scale;
-  const size_t smem = ((s.n_group > 1 ? kSelWarps * s.E : 0) + (s.counts ? s.E : 0)) * sizeof(float);
   const int bytes = 4 * type_bytes(s.type);
   s.vec = reinterpret_cast<uintptr_t>(s.logits) % bytes == 0 && (s.T == 1 || s.ld % 4 == 0);
   s.cluster = cluster;
   const dim3 grid(ctas), block(kSelWarps * 32);
   dispatch_select(s.E, [&](auto v) {
     constexpr int V = decltype(v)::value;
+    const size_t smem = (kSelWarps * 32 * V + (s.counts ? s.E : 0)) * sizeof(float);
     auto kernel = a->score == MOE_B200_SCORE_SOFTMAX ? select_kernel<V, true> : select_kernel<V, false>;
     e = cluster ? launch_cluster_pdl(kernel, grid, block, smem, ctas, st, s) : launch_pdl(kernel, grid, block, smem, st, s);
   });

@@ -262,8 +262,8 @@ MOE_B200_API int moe_b200_timer_read(moe_b200_timer* timer, float* stage_ms, int
  * y may be null (x is the norm of residual; residual_out is not written), residual may be null
  * (taken as 0).  post_weight, gate, pre_weight may be null.  The gate's element of (t, c) is
  * gate[t * gate_row_stride + (gate_per_column ? c : 0)], so gate_row_stride 0 broadcasts it over
- * rows.  residual and residual_out have residual_type, which is y_type or fp32; weights, gate
- * and x have types of their own.  x computes from the unrounded r'.  With x_type e4m3, x_scale
+ * rows.  residual and residual_out have residual_type (fp32 if y is); weights, gate and x have
+ * types of their own.  x computes from the unrounded r'.  With x_type e4m3, x_scale
  * receives [ceil(cols / 128)][rows] scales max(amax, 1e-12) / 448, and x the codes: the layer's
  * hidden_states_scale and hidden_states.  residual_out may be residual.
  */

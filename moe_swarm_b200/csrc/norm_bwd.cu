@@ -422,7 +422,7 @@ MOE_B200_API int moe_b200_block_norm_backward(const moe_b200_norm_backward_args*
     return e == cudaSuccess ? MOE_B200_OK : report_cuda(e, "cudaMemsetAsync");
   }
   if (!type_pair_ok(a->y_type, a->residual_type))
-    return report_error(MOE_B200_ERR_ARG, "block_norm_backward: the residual has y's type or fp32");
+    return report_error(MOE_B200_ERR_ARG, "block_norm_backward: with a y of fp32 the residual is fp32 too (types bf16, fp16, fp32)");
   if (!a->dx && !a->dresidual) return report_error(MOE_B200_ERR_ARG, "block_norm_backward: dx or dresidual is required");
   if (a->dx && (!a->residual || !a->pre_weight || !a->dpre_weight || !is_float_type(a->pre_weight_type)))
     return report_error(MOE_B200_ERR_ARG, "block_norm_backward: dx needs residual, pre_weight and dpre_weight");

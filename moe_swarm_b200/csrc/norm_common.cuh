@@ -235,12 +235,18 @@ inline void norm_shape(int cols, int* warps, int* rows_per_cta) {
 // f(y type, residual type)
 template <class F>
 void dispatch_types(int y_type, int r_type, F&& f) {
-  if (y_type == MOE_B200_BF16) r_type == MOE_B200_FP32 ? f(bf16{}, float{}) : f(bf16{}, bf16{});
-  else if (y_type == MOE_B200_FP16) r_type == MOE_B200_FP32 ? f(fp16{}, float{}) : f(fp16{}, fp16{});
+  auto with = [&](auto yt) {
+    if (r_type == MOE_B200_BF16) f(yt, bf16{});
+    else if (r_type == MOE_B200_FP16) f(yt, fp16{});
+    else f(yt, float{});
+  };
+  if (y_type == MOE_B200_BF16) with(bf16{});
+  else if (y_type == MOE_B200_FP16) with(fp16{});
   else f(float{}, float{});
 }
+// A 32-bit y goes with a 32-bit residual.
 inline bool type_pair_ok(int y, int r) {
-  return is_float_type(y) && is_float_type(r) && (r == y || r == MOE_B200_FP32);
+  return is_float_type(y) && is_float_type(r) && (y != MOE_B200_FP32 || r == MOE_B200_FP32);
 }
 
 }  // namespace moe

@@ -11,7 +11,7 @@ results.
 
 from __future__ import annotations
 
-import ctypes
+import threading
 from typing import NamedTuple
 
 import torch
@@ -120,17 +120,18 @@ def _call(fn: str, dev: int, args, *workspace):
         raise _failure(rc, fn)
 
 
-_SCRATCH_KEPT = 4 << 20   # bytes kept per (device, stream)
-_scratch: dict[tuple[int, int], torch.Tensor] = {}
+_SCRATCH_KEPT = 4 << 20   # bytes kept per (device, stream, thread)
+_scratch: dict[tuple[int, int, int], torch.Tensor] = {}
 
 
 def _workspace(n: int, dev: int) -> torch.Tensor:
     """Scratch of n bytes for a call on the device's current stream.  Small ones are kept per
-    (device, stream): the calls of one stream run one after another.  Large ones, and those of a
-    graph capture (whose replays would share them with later calls), are allocated per call."""
+    (device, stream, host thread): such calls are enqueued, and run, one after another, while two
+    threads could enqueue the kernels of their calls in turn.  Large ones, and those of a graph
+    capture (whose replays would share them with later calls), are allocated per call."""
     if n > _SCRATCH_KEPT or torch.cuda.is_current_stream_capturing():
         return torch.empty(n, dtype=torch.uint8, device=dev)
-    key = (dev, torch._C._cuda_getCurrentRawStream(dev))
+    key = (dev, torch._C._cuda_getCurrentRawStream(dev), threading.get_ident())
     ws = _scratch.get(key)
     if ws is None:
         ws = _scratch[key] = torch.empty(_SCRATCH_KEPT, dtype=torch.uint8, device=dev)
@@ -168,7 +169,7 @@ def block_norm(y: torch.Tensor | None, residual: torch.Tensor | None, *, post_we
         x  = rms_norm(r') * (pre_weight + weight_offset)      (no x without pre_weight)
 
     ``y`` [rows, cols] is the block's output (None: x is the norm of ``residual``), ``residual``
-    has y's type or fp32 (None: 0), ``gate`` is [cols], [1, cols], [rows, 1], [1, 1] or [rows, cols].
+    may have another type (None: 0; fp32 if y is), ``gate`` is [cols], [1, cols], [rows, 1], [1, 1] or [rows, cols].
     ``x_dtype`` is the type of x (y's by default); ``torch.float8_e4m3fn`` quantises x per row and
     128 columns and returns ``x_scale`` [ceil(cols / 128), rows]: the ``hidden_states`` and
     ``hidden_states_scale`` of :func:`moe_swarm_b200.run`.  ``residual_out`` (may be ``residual``)
@@ -181,7 +182,7 @@ def block_norm(y: torch.Tensor | None, residual: torch.Tensor | None, *, post_we
     if y is not None:
         y_ld = _rows(y, "y")
         if residual is not None:
-            r_ld = _rows(residual, "residual", shape, (y.dtype, torch.float32), dev)
+            r_ld = _rows(residual, "residual", shape, _FP32 if y.dtype == torch.float32 else _FLOATS, dev)
     else:
         r_ld = _rows(residual, "residual")
     rows, cols = shape
@@ -230,7 +231,7 @@ def block_norm_backward(dx: torch.Tensor | None, dresidual: torch.Tensor | None,
     shape, dev, r_dtype = residual.shape, residual.get_device(), residual.dtype
     rows, cols = shape
     y_dtype = (residual if y is None and dx is None else dx if y is None else y).dtype
-    _check(r_dtype is y_dtype or r_dtype is torch.float32, "residual must have y's type or fp32")
+    _check(r_dtype is torch.float32 or y_dtype is not torch.float32, "with a y of fp32 the residual must be fp32")
     _check(dx is not None or dresidual is not None, "dx or dresidual is required")
     _check(dx is None or pre_weight is not None, "dx needs pre_weight")
     _check(y is not None or (post_weight is None and gate is None), "post_weight and gate need y")

@@ -28,12 +28,13 @@ def make(T, H, y_dtype, r_dtype, post, gate, seed=0, pad=0, wdt=BF):
         gate=None if shape is None else torch.rand(shape, generator=g, device="cuda").to(y_dtype))
 
 
+# (few rows: one CTA or warp each; many: the ring, below)
 SHAPES = [(1, 1), (1, 7168), (3, 7), (5, 8), (9, 129), (17, 512), (2, 513), (33, 1000), (7, 4096), (3, 5001),
           (2, 8192), (2, 8193), (1, 16384), (300, 64)]
 
 
 @pytest.mark.parametrize("T,H", SHAPES)
-@pytest.mark.parametrize("y_dtype,r_dtype", [(BF, BF), (BF, F32), (FP, FP), (FP, F32), (F32, F32)])
+@pytest.mark.parametrize("y_dtype,r_dtype", [(BF, BF), (BF, F32), (FP, FP), (FP, F32), (F32, F32), (FP, BF), (BF, FP)])
 @pytest.mark.parametrize("post,gate", [(False, None), (True, "token"), (True, "channel"), (False, "full")])
 def test_forward(T, H, y_dtype, r_dtype, post, gate):
     a = make(T, H, y_dtype, r_dtype, post, gate)
@@ -150,7 +151,7 @@ def test_rows_do_not_touch_each_other():
 
 @pytest.mark.parametrize("T,H", [(1, 1), (1, 7168), (2, 513), (5, 129), (64, 640), (300, 96), (333, 1001), (700, 2048),
                                  (3, 8200), (2, 16384)])
-@pytest.mark.parametrize("y_dtype,r_dtype", [(BF, BF), (BF, F32), (FP, F32), (F32, F32)])
+@pytest.mark.parametrize("y_dtype,r_dtype", [(BF, BF), (BF, F32), (FP, F32), (F32, F32), (FP, BF), (BF, FP)])
 @pytest.mark.parametrize("post,gate", [(False, None), (True, "token"), (True, "channel"), (True, "full"),
                                        (False, "one"), (False, "vector")])
 def test_backward(T, H, y_dtype, r_dtype, post, gate):
@@ -184,6 +185,42 @@ def test_backward(T, H, y_dtype, r_dtype, post, gate):
     summed = gate != "full" or T == 1 or H == 1
     assert o.gate.dtype == (F32 if summed else y_dtype)
     R.close(o.gate.reshape(dg.shape), dg, mag, steps=steps)
+
+
+@pytest.mark.parametrize("T,H", [(1500, 512), (800, 1536), (700, 2880), (650, 7168), (620, 4104), (3000, 96), (600, 8192)])
+@pytest.mark.parametrize("y_dtype,r_dtype", [(BF, BF), (FP, F32), (F32, F32)])
+@pytest.mark.parametrize("post,gate", [(False, None), (True, "token"), (True, "channel"), (True, "full"), (False, "one"),
+                                       (False, "full"), (False, "token")])
+def test_many_rows(T, H, y_dtype, r_dtype, post, gate):
+    """Sizes at which rows stream through shared memory, in every combination of their parts."""
+    a = make(T, H, y_dtype, r_dtype, post, gate, seed=T)
+    kw = dict(scale=0.75, eps=1e-5, off=0.5)
+    o = M.block_norm(**a, scale=0.75, eps=1e-5, weight_offset=0.5)
+    r, x, rm, xm = R.block_norm(**a, **kw)
+    R.close(o.residual, r, rm)
+    R.close(o.x, x, xm)
+    g = gen(5)
+    dx = torch.randn(T, H, generator=g, device="cuda").to(y_dtype)
+    dr = torch.randn(T, H, generator=g, device="cuda").to(r_dtype)
+    w = dict(post_weight=a["post_weight"], gate=a["gate"], scale=0.5, pre_weight=a["pre_weight"])
+    for d in (dr, None):
+        b = M.block_norm_backward(dx, d, a["residual"], a["y"], weight_offset=0.5, **w)
+        ref = R.block_norm_backward(dx, d, a["residual"], a["y"], off=0.5, **w)
+        R.close(b.residual, *ref["residual"])
+        R.close(b.y, *ref["y"], steps=3 * R.STEPS)
+        steps = 3 * R.STEPS + T // 148 + 64
+        R.close(b.pre_weight, *ref["pre_weight"], steps=steps)
+        if post:
+            R.close(b.post_weight, *ref["post_weight"], steps=steps)
+        if gate is not None:
+            dg, mag = ref["gate"]
+            if gate == "channel":
+                dg, mag = dg.sum(0, keepdim=True), mag.sum(0, keepdim=True)
+            elif gate == "token":
+                dg, mag = dg.sum(1, keepdim=True), mag.sum(1, keepdim=True)
+            elif gate == "one":
+                dg, mag = dg.sum().view(1, 1), mag.sum().view(1, 1)
+            R.close(b.gate, dg, mag, steps=steps)
 
 
 def test_backward_partial_forms():
@@ -272,7 +309,7 @@ def test_refusals():
         lambda: M.block_norm(None, None),
         lambda: M.block_norm(None, y),                                    # nothing to compute
         lambda: M.block_norm(y, y[:, :16]),
-        lambda: M.block_norm(y, y.half()),
+        lambda: M.block_norm(y.float(), y),                               # a 16-bit residual of a 32-bit y
         lambda: M.block_norm(y.t(), y.t()),                               # rows not contiguous
         lambda: M.block_norm(y, y, pre_weight=w[:16]),
         lambda: M.block_norm(y, y, pre_weight=w.double()),
@@ -286,7 +323,8 @@ def test_refusals():
         lambda: M.block_norm_backward(None, None, y, y),
         lambda: M.block_norm_backward(y, None, y, y),                     # dx without its weight
         lambda: M.block_norm_backward(None, y, y, None, gate=w),
-        lambda: M.block_norm_backward(None, y.half(), y, y),
+        lambda: M.block_norm_backward(None, y.half(), y, y),              # dresidual of another type
+        lambda: M.block_norm_backward(None, y, y, y.float()),
     ]
     for f in bad:
         with pytest.raises(M.MoEArgumentError):

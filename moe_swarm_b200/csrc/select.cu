@@ -201,9 +201,10 @@ __device__ __forceinline__ float scores(const float* x, float lowest, float* s) 
 
 // Two sides of a decision are told apart by the 32-bit scores if they differ by more than this
 // share of the sizes involved.  An expert's score is off by 2^-19 of the row's size and its key by
-// 2^-19 of itself (the lane in the low bits), a group's by 2^-19 of the size for either of its two;
-// their sums round by 2^-23.  For both sides of a decision that is less than 2^-16.
-constexpr float kMargin = 1.52587890625e-05f;
+// 2^-19 of itself (the lane in the low bits); a group's score is the sum of two such keys, and its
+// own key off by 2^-19 once more; sums round by 2^-23.  For both sides of a decision that is less
+// than 2^-15.
+constexpr float kMargin = 3.0517578125e-05f;
 
 // Whether `in` (the weakest taken) is above `out` (the strongest left) for certain.  -inf for
 // either: nothing was taken or left, no decision.
@@ -213,7 +214,7 @@ __device__ __forceinline__ bool apart(float in, float out, float size) {
 
 // Keys of the fast choice: sel (below kHuge in size) with the lane in its low 5 bits, so that no two
 // lanes have equal ones; at most kNone: not to be chosen.
-constexpr float kNone = -3.39e38f, kHuge = 1e30f;
+constexpr float kNone = -3.39e38f, kFloor = -3.38e38f, kHuge = 1e30f;
 __device__ __forceinline__ float lane_key(float sel, int lane) {
   return __uint_as_float((__float_as_uint(fmaxf(sel, -3.4e38f)) & ~31u) | lane);
 }
@@ -236,18 +237,27 @@ __device__ __forceinline__ float group_score(const SelectArgs& a, float m1, floa
 }
 
 // Whether group g (its score in each of its lanes, lane h * lanes first) is among the topk_group
-// best; *sure: no decision within the margin.
-__device__ __forceinline__ bool keep_group(const SelectArgs& a, float score, int g, int lanes, float size, bool* sure) {
+// best, equal ones from the first up.
+__device__ __forceinline__ bool keep_group(const SelectArgs& a, float score, int g, int lanes) {
   int rank = 0;
   for (int h = 0; h < a.n_group; ++h) {
     const float o = __shfl_sync(0xffffffffu, score, h * lanes);
     rank += (o > score || (o == score && h < g)) ? 1 : 0;
   }
-  const bool kept = g < a.n_group && rank < a.topk_group;
-  const float in = redux_min(kept && score != -INFINITY ? score : INFINITY);
-  const float out = redux_max(g < a.n_group && !kept ? score : -INFINITY);
-  *sure = in == INFINITY || apart(in, out, size);
-  return kept;
+  return g < a.n_group && rank < a.topk_group;
+}
+// The same by 32-bit scores: rounds of the highest score left, the group in its low 5 bits; *sure:
+// the last one kept is apart from the best one dropped.
+__device__ __forceinline__ bool keep_group_fast(const SelectArgs& a, float score, int g, float size, bool* sure) {
+  const float key = g < a.n_group ? lane_key(score, g) : -3.4e38f;
+  float left = key, last = 0.f;
+#pragma unroll 4
+  for (int r = 0; r < a.topk_group; ++r) {
+    last = redux_max(left);   // (kNone or below where nothing is left)
+    left = left == last ? -3.4e38f : left;
+  }
+  *sure = apart(or_none(last), or_none(redux_max(left)), size);
+  return key >= fmaxf(last, kFloor);
 }
 
 // Whether a group is a power of two of neighbouring lanes (*lanes); otherwise groups are scored
@@ -258,20 +268,20 @@ __device__ __forceinline__ bool groups_by_lane(const SelectArgs& a, int* lanes) 
   *lanes = gs / V;
   return gs % V == 0 && (*lanes & (*lanes - 1)) == 0;
 }
-// A lane's part of its group, of which m1 >= m2 are its two highest, is it kept?
-__device__ __forceinline__ bool keep_by_lane(const SelectArgs& a, float m1, float m2, int lane, int lanes, float size,
-                                             bool* sure) {
+// The score of a lane's group, m1 >= m2 being the two highest of the lane's own part of it.
+__device__ __forceinline__ float score_by_lane(const SelectArgs& a, float m1, float m2, int lanes) {
   for (int d = 1; d < lanes; d <<= 1) {
     const float o1 = __shfl_xor_sync(0xffffffffu, m1, d), o2 = __shfl_xor_sync(0xffffffffu, m2, d);
     m2 = fmaxf(fminf(m1, o1), fmaxf(m2, o2));
     m1 = fmaxf(m1, o1);
   }
-  return keep_group(a, group_score(a, m1, m2), lane / lanes, lanes, size, sure);
+  return group_score(a, m1, m2);
 }
 
 // Drops what is not in a kept group from sel, through shared memory: groups of any size.
 template <int V>
-__device__ __forceinline__ void drop_groups(const SelectArgs& a, float* sel, float* s_sel, int lane, float size, bool* sure) {
+__device__ __forceinline__ void drop_groups(const SelectArgs& a, float* sel, float* s_sel, int lane, bool fast, float size,
+                                            bool* sure) {
   const int first = lane * V, gs = a.E / a.n_group;
 #pragma unroll
   for (int i = 0; i < V; ++i)
@@ -279,7 +289,9 @@ __device__ __forceinline__ void drop_groups(const SelectArgs& a, float* sel, flo
   __syncwarp();
   float m1, m2;
   scan_group(s_sel, lane, a.n_group, gs, &m1, &m2);
-  const uint32_t kept = __ballot_sync(0xffffffffu, keep_group(a, group_score(a, m1, m2), lane, 1, size, sure));
+  const float score = group_score(a, m1, m2);
+  const uint32_t kept =
+      __ballot_sync(0xffffffffu, fast ? keep_group_fast(a, score, lane, size, sure) : keep_group(a, score, lane, 1));
 #pragma unroll
   for (int i = 0; i < V; ++i)
     if (first + i < a.E && !((kept >> ((first + i) / gs)) & 1u)) sel[i] = -INFINITY;
@@ -289,7 +301,7 @@ __device__ __forceinline__ void drop_groups(const SelectArgs& a, float* sel, flo
 // The choice by the defined scores: bit i of the result says that this lane's expert i is chosen.
 template <int V>
 __device__ __forceinline__ uint32_t choose_exact(const SelectArgs& a, float* sel, float* s_sel, int lane) {
-  bool sure, kept = true;
+  bool kept = true;
   int lanes;
   if (a.n_group > 1) {
     if (groups_by_lane<V>(a, &lanes)) {
@@ -299,9 +311,9 @@ __device__ __forceinline__ uint32_t choose_exact(const SelectArgs& a, float* sel
         m2 = fmaxf(m2, fminf(m1, sel[i]));
         m1 = fmaxf(m1, sel[i]);
       }
-      kept = keep_by_lane(a, m1, m2, lane, lanes, 1.f, &sure);
+      kept = keep_group(a, score_by_lane(a, m1, m2, lanes), lane / lanes, lanes);
     } else {
-      drop_groups<V>(a, sel, s_sel, lane, 1.f, &sure);
+      drop_groups<V>(a, sel, s_sel, lane, false, 0.f, nullptr);
     }
   }
   uint32_t key[V], taken = 0;   // key 0: not to be chosen
@@ -328,30 +340,42 @@ __device__ __forceinline__ uint32_t choose_exact(const SelectArgs& a, float* sel
   return taken;
 }
 
-// The choice by 32-bit scores; *sure tells whether they decide it.  Each lane sorts its keys; a round
-// is then one maximum over the warp's first keys and a shift of the list that held it.  What is
-// chosen is what reaches the last round's maximum.
+// K rounds of the highest key left in the warp, each a maximum over the lanes' first keys and a
+// shift of the list that held it; returns the last one's (kNone or below where there are fewer).
+// Up to eight rounds are unrolled, so that a list is shifted only as far as later rounds may reach.
+template <int V>
+__device__ __forceinline__ float last_of_rounds(float (&list)[V + 1], int K) {
+  float last = 0.f;
+  if (K <= 8) {
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      if (r >= K) break;
+      last = redux_max(list[0]);
+      const bool mine = list[0] == last;
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (i <= 7 - r) list[i] = mine ? list[i + 1] : list[i];
+    }
+  } else {
+    for (int r = 0; r < K; ++r) {
+      last = redux_max(list[0]);
+      const bool mine = list[0] == last;
+#pragma unroll
+      for (int i = 0; i < V; ++i) list[i] = mine ? list[i + 1] : list[i];
+    }
+  }
+  return last;
+}
+
+// The choice by 32-bit scores; *sure tells whether they decide it.  Each lane sorts its keys; what
+// is chosen is what reaches the last round's maximum.
 template <int V>
 __device__ __forceinline__ uint32_t choose_fast(const SelectArgs& a, float* sel, float* s_sel, int lane, float size,
                                                 bool* sure) {
   *sure = true;
-  if (a.n_group > 1) {
-    int lanes;
-    if (groups_by_lane<V>(a, &lanes)) {
-      float m1 = -INFINITY, m2 = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        m2 = fmaxf(m2, fminf(m1, sel[i]));
-        m1 = fmaxf(m1, sel[i]);
-      }
-      if (!keep_by_lane(a, m1, m2, lane, lanes, size, sure)) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) sel[i] = -INFINITY;
-      }
-    } else {
-      drop_groups<V>(a, sel, s_sel, lane, size, sure);
-    }
-  }
+  int lanes = 0;
+  const bool by_lane = a.n_group > 1 && groups_by_lane<V>(a, &lanes);
+  if (a.n_group > 1 && !by_lane) drop_groups<V>(a, sel, s_sel, lane, true, size, sure);
   float key[V], list[V + 1];
 #pragma unroll
   for (int i = 0; i < V; ++i) key[i] = lane_key(sel[i], lane);
@@ -364,20 +388,20 @@ __device__ __forceinline__ uint32_t choose_fast(const SelectArgs& a, float* sel,
     for (int i = 0; i < V; ++i) list[i] = sorted[i];
     list[V] = -3.4e38f;
   }
-  float last = INFINITY;
-  for (int r = 0; r < a.K; ++r) {
-    const float m = redux_max(list[0]);
-    if (m <= kNone) break;
-    last = m;
-    const bool mine = list[0] == m;
+  bool kept = true;
+  if (by_lane) {
+    const float score = score_by_lane(a, or_none(list[0]), V > 1 ? or_none(list[V > 1 ? 1 : 0]) : -INFINITY, lanes);
+    kept = keep_group_fast(a, score, lane / lanes, size, sure);
 #pragma unroll
-    for (int i = 0; i < V; ++i) list[i] = mine ? list[i + 1] : list[i];
+    for (int i = 0; i < V; ++i) list[i] = kept ? list[i] : -3.4e38f;
   }
+  const float last = last_of_rounds<V>(list, a.K);
   // (equal keys of one lane on both sides of the end are not apart)
-  *sure = *sure && (last == INFINITY || apart(last, or_none(redux_max(list[0])), size));
+  *sure = *sure && apart(or_none(last), or_none(redux_max(list[0])), size);
+  const float least = kept ? fmaxf(last, kFloor) : INFINITY;
   uint32_t taken = 0;
 #pragma unroll
-  for (int i = 0; i < V; ++i) taken |= key[i] >= last ? 1u << i : 0u;
+  for (int i = 0; i < V; ++i) taken |= key[i] >= least ? 1u << i : 0u;
   return taken;
 }
 
@@ -405,9 +429,12 @@ __global__ void __launch_bounds__(kSelWarps * 32) select_kernel(SelectArgs a) {
   }
   // biases so large that sums of two overflow: every choice by the defined scores
   wild = __any_sync(0xffffffffu, wild);
-  for (int t = blockIdx.x * kSelWarps + warp; t < a.T; t += gridDim.x * kSelWarps) {
+  const int step = gridDim.x * kSelWarps;
+  for (int t = blockIdx.x * kSelWarps + warp; t < a.T; t += step) {
     float x[V], s[V], sel[V];
     load_logits<V>(a.logits, a.type, t * a.ld, first, a.E, a.vec, x);
+    if (t < a.T - step && first < a.E)   // the next token's, toward L2
+      prefetch_l2(static_cast<const uint8_t*>(a.logits) + ((t + step) * a.ld + first) * (a.type == MOE_B200_FP32 ? 4 : 2));
     const float size = scores<V, SOFTMAX, false>(x, lowest, s);
     float nan = 0.f;
 #pragma unroll
@@ -488,13 +515,25 @@ __global__ void __launch_bounds__(kSelWarps * 32) select_bwd_kernel(SelectBwdArg
   const float lowest = lowest_of(a.type);
   const int first = lane * V;
   float* row = s_row[warp];
-  for (int t = blockIdx.x * kSelWarps + warp; t < a.T; t += gridDim.x * kSelWarps) {
-    float x[V], s[V];
-    load_logits<V>(a.logits, a.type, t * a.ld, first, a.E, a.vec, x);
+  // a token's logits, ids and gradients are loaded while the one before it is computed
+  float next_x[V], next_d = 0.f;
+  int next_id = -1;
+  auto load = [&](int t) {
+    load_logits<V>(a.logits, a.type, t * a.ld, first, a.E, a.vec, next_x);
     const int64_t at = static_cast<int64_t>(t) * a.K + lane;
-    const int id = lane < a.K ? a.idx[at] : -1;
+    next_id = lane < a.K ? a.idx[at] : -1;
+    next_d = lane < a.K ? a.dw[at] : 0.f;
+  };
+  int t = blockIdx.x * kSelWarps + warp;
+  if (t < a.T) load(t);
+  for (const int step = gridDim.x * kSelWarps; t < a.T; t += step) {
+    float x[V], s[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = next_x[i];
+    const int id = next_id;
     const bool have = id >= 0 && id < a.E;
-    float d = have ? a.dw[at] * a.scale : 0.f;
+    float d = have ? next_d * a.scale : 0.f;
+    if (t < a.T - step) load(t + step);
     if constexpr (SOFTMAX) {
       float m = -INFINITY;
 #pragma unroll

@@ -95,8 +95,8 @@ def _matrix(t, name: str, shape, dtype, dev):
         raise MoEArgumentError(f"{name} must be a contiguous {dtype} {list(shape)} tensor on the device")
 
 
-def _ptr(t):
-    return None if t is None else t.data_ptr()
+def _ptr(t) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def _type(t) -> int:
@@ -110,7 +110,7 @@ def _call(fn: str, dev: int, args, *workspace):
     """Calls moe_b200_<fn> on the device's current stream, with that device current."""
     f = _functions.get(fn)
     if f is None:
-        f = _functions[fn] = getattr(_native.lib(), "moe_b200_" + fn)
+        f = _functions[fn] = _native.packed_entry(fn, bool(workspace))
     if torch._C._cuda_getDevice() == dev:
         rc = f(args, *workspace, torch._C._cuda_getCurrentRawStream(dev))
     else:
@@ -208,7 +208,7 @@ def block_norm(y: torch.Tensor | None, residual: torch.Tensor | None, *, post_we
             x, x_ld = out, _result(out, "out", shape, (x_dtype,), dev)
         if x_dtype == torch.float8_e4m3fn:
             x_scale = torch.empty(((cols + 127) // 128, rows), dtype=torch.float32, device=first.device)
-    _call("block_norm", dev, _native.NormArgs(
+    _call("block_norm", dev, _native.NormArgs.pack(
         _ptr(y), _ptr(residual), _ptr(post_weight), _ptr(pre_weight), _ptr(gate), _ptr(residual_out), _ptr(x),
         _ptr(x_scale), y_ld, r_ld, ro_ld, x_ld, gate_ld, rows, cols, _TYPES[first.dtype], _TYPES[stream.dtype],
         _type(post_weight), _type(pre_weight), _type(gate), _type(x), gate_cols, scale, eps, weight_offset))
@@ -256,7 +256,7 @@ def block_norm_backward(dx: torch.Tensor | None, dresidual: torch.Tensor | None,
     n = _native.lib().moe_b200_block_norm_backward_workspace_size(rows, cols)
     _check(n > 0, "unsupported sizes")
     ws = _workspace(n, dev)
-    _call("block_norm_backward", dev, _native.NormBackwardArgs(
+    _call("block_norm_backward", dev, _native.NormBackwardArgs.pack(
         _ptr(dx), _ptr(dresidual), _ptr(residual), _ptr(y), _ptr(post_weight), _ptr(pre_weight), _ptr(gate),
         _ptr(dres), _ptr(dy), _ptr(dpre), _ptr(dpost), _ptr(dgate), dx_ld, dr_ld, r_ld, y_ld, gate_ld, cols, cols,
         cols, rows, cols, _TYPES[y_dtype], _TYPES[r_dtype], _type(post_weight), _type(pre_weight), _type(gate),
@@ -288,12 +288,13 @@ def select_experts(logits: torch.Tensor, top_k: int, *, score: str = "sigmoid", 
     _check(score in _SCORES, "score must be 'sigmoid' or 'softmax'")
     _check(group_score in _GROUP_SCORES, "group_score must be 'top2' or 'max'")
     _check(1 <= top_k <= E, "top_k must be in [1, number of experts]")
+    _check(1 <= topk_group <= n_group <= E, "topk_group must be in [1, n_group], n_group in [1, number of experts]")
     if bias is not None:
         _vector(bias, "bias", E, _FLOATS, dev)
     idx = torch.empty((T, top_k), dtype=torch.int32, device=device)
     w = torch.empty_like(idx, dtype=torch.float32)
     n = torch.empty(E, dtype=torch.int32, device=device) if counts else None
-    _call("select_experts", dev, _native.SelectArgs(
+    _call("select_experts", dev, _native.SelectArgs.pack(
         logits.data_ptr(), _ptr(bias), idx.data_ptr(), w.data_ptr(), _ptr(n), ld, T, E, top_k, _TYPES[logits.dtype],
         _type(bias), _SCORES[score], n_group, topk_group, _GROUP_SCORES[group_score], bool(renormalize), scale))
     return Selection(idx, w, n)
@@ -311,7 +312,7 @@ def select_experts_backward(dw: torch.Tensor, logits: torch.Tensor, idx: torch.T
     _matrix(idx, "idx", (T, idx.shape[1]), torch.int32, dev)
     _matrix(dw, "dw", idx.shape, torch.float32, dev)
     out = torch.empty_like(logits)
-    _call("select_experts_backward", dev, _native.SelectBackwardArgs(
+    _call("select_experts_backward", dev, _native.SelectBackwardArgs.pack(
         logits.data_ptr(), idx.data_ptr(), dw.data_ptr(), out.data_ptr(), ld, E, T, E, idx.shape[1],
         _TYPES[logits.dtype], _SCORES[score], bool(renormalize), scale))
     return out
@@ -329,7 +330,7 @@ def quantize_int8(x: torch.Tensor, *, swiglu: bool = False):
         cols //= 2
     q = torch.empty((rows, cols), dtype=torch.int8, device=device)
     scale = torch.empty(rows, dtype=torch.float32, device=device)
-    _call("quantize_int8", dev, _native.QuantizeArgs(x.data_ptr(), q.data_ptr(), scale.data_ptr(), ld, cols, rows, cols,
+    _call("quantize_int8", dev, _native.QuantizeArgs.pack(x.data_ptr(), q.data_ptr(), scale.data_ptr(), ld, cols, rows, cols,
                                                      _TYPES[x.dtype], bool(swiglu)))
     return q, scale
 
@@ -371,7 +372,7 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     n = _native.lib().moe_b200_int8_linear_workspace_size(T, N, K, x_type)
     _check(n > 0, "unsupported sizes")
     ws = _workspace(n, dev)
-    _call("int8_linear", dev, _native.LinearArgs(
+    _call("int8_linear", dev, _native.LinearArgs.pack(
         x.data_ptr(), _ptr(x_scale), weight.data_ptr(), weight_scale.data_ptr(), _ptr(bias), out.data_ptr(), x_ld, w_ld,
         out_ld, T, N, K, x_type, _TYPES[out.dtype], _type(bias), bool(swiglu)), ws.data_ptr(), ws.numel())
     return out

@@ -242,8 +242,9 @@ MOE_B200_API int moe_b200_timer_read(moe_b200_timer* timer, float* stage_ms, int
  * ---------------------------------------------------------------------------
  * Operators around the layer, for a transformer block that holds it.  They
  * take row-major tensors whose rows may be further apart than their length
- * (strides in elements; elements of a row are adjacent), enqueue on `stream`
- * without a host synchronisation, and return the status codes above.
+ * (strides in elements; elements of a row are adjacent; the stride of a single
+ * row is not read), enqueue on `stream` without a host synchronisation, and
+ * return the status codes above.  A call has at most 2^30 rows or tokens.
  */
 
 /* Element types. */

@@ -375,7 +375,8 @@ cudaError_t gemv_launch(const GemvArgs& g, int x_type, int sms, cudaStream_t st)
 }
 
 int quant_check(const void* x, int type, int rows, int cols, const char** why) {
-  if (rows < 0 || cols < 1 || cols > kQuantMaxCols) *why = "int8 quantisation: rows must be >= 0 and cols in [1, 32768]";
+  if (rows < 0 || rows > kOpMaxRows || cols < 1 || cols > kQuantMaxCols)
+    *why = "int8 quantisation: rows must be in [0, 2^30] and cols in [1, 32768]";
   else if (!is_float_type(type)) *why = "int8 quantisation: x is bf16, fp16 or fp32";
   else if (rows > 0 && !x) *why = "null tensor pointer";
   else return 0;
@@ -415,7 +416,7 @@ MOE_B200_API int moe_b200_quantize_int8(const moe_b200_quantize_args* a, void* s
 MOE_B200_API size_t moe_b200_int8_linear_workspace_size(int32_t num_tokens, int32_t out_features, int32_t in_features,
                                                         int32_t x_type) {
   using namespace moe;
-  if (num_tokens < 0 || out_features < 1 || in_features < 1 || in_features > kInt8MaxK) return 0;
+  if (num_tokens < 0 || num_tokens > kOpMaxRows || out_features < 1 || in_features < 1 || in_features > kInt8MaxK) return 0;
   const size_t T = num_tokens;
   return 256 + (x_type == MOE_B200_INT8 ? 0 : align256(T * in_features) + align256(T * sizeof(float)));
 }
@@ -424,9 +425,9 @@ MOE_B200_API int moe_b200_int8_linear(const moe_b200_linear_args* a, void* works
                                       void* stream) {
   using namespace moe;
   if (!a) return report_error(MOE_B200_ERR_ARG, "null args");
-  if (a->num_tokens < 0 || a->out_features < 1 || a->in_features < 16 || a->in_features > kInt8MaxK ||
-      a->in_features % 16)
-    return report_error(MOE_B200_ERR_ARG, "int8_linear: num_tokens must be >= 0, out_features >= 1 and in_features a multiple of 16 up to 131056");
+  if (a->num_tokens < 0 || a->num_tokens > kOpMaxRows || a->out_features < 1 || a->out_features > kOpMaxRows ||
+      a->in_features < 16 || a->in_features > kInt8MaxK || a->in_features % 16)
+    return report_error(MOE_B200_ERR_ARG, "int8_linear: num_tokens must be in [0, 2^30], out_features in [1, 2^30] and in_features a multiple of 16 up to 131056");
   const bool quantise = a->x_type != MOE_B200_INT8;
   const char* why = nullptr;
   if (quantise && quant_check(a->x, a->x_type, a->num_tokens, a->in_features, &why))

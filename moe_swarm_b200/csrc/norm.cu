@@ -235,8 +235,8 @@ extern "C" {
 MOE_B200_API int moe_b200_block_norm(const moe_b200_norm_args* a, void* stream) {
   using namespace moe;
   if (!a) return report_error(MOE_B200_ERR_ARG, "null args");
-  if (a->rows < 0 || a->cols < 1 || a->cols > kNormMaxCols)
-    return report_error(MOE_B200_ERR_ARG, "block_norm: rows must be >= 0 and cols in [1, 16384]");
+  if (a->rows < 0 || a->rows > kOpMaxRows || a->cols < 1 || a->cols > kNormMaxCols)
+    return report_error(MOE_B200_ERR_ARG, "block_norm: rows must be in [0, 2^30] and cols in [1, 16384]");
   if (!type_pair_ok(a->y_type, a->residual_type))
     return report_error(MOE_B200_ERR_ARG, "block_norm: with a y of fp32 the residual is fp32 too (types bf16, fp16, fp32)");
   if (a->rows == 0) return MOE_B200_OK;

@@ -397,7 +397,7 @@ extern "C" {
 
 MOE_B200_API size_t moe_b200_block_norm_backward_workspace_size(int32_t rows, int32_t cols) {
   using namespace moe;
-  if (rows < 0 || cols < 1 || cols > kNormMaxCols) return 0;
+  if (rows < 0 || rows > kOpMaxRows || cols < 1 || cols > kNormMaxCols) return 0;
   const NormBwdShape shape = bwd_shape(rows, cols);
   const int parts = shape.direct_parts > shape.ring_parts ? shape.direct_parts : shape.ring_parts;
   return static_cast<size_t>(align256(static_cast<int64_t>(2) * parts * cols * 4) + align256(static_cast<int64_t>(rows) * 4) +
@@ -408,8 +408,8 @@ MOE_B200_API int moe_b200_block_norm_backward(const moe_b200_norm_backward_args*
                                               size_t workspace_bytes, void* stream) {
   using namespace moe;
   if (!a) return report_error(MOE_B200_ERR_ARG, "null args");
-  if (a->rows < 0 || a->cols < 1 || a->cols > kNormMaxCols)
-    return report_error(MOE_B200_ERR_ARG, "block_norm_backward: rows must be >= 0 and cols in [1, 16384]");
+  if (a->rows < 0 || a->rows > kOpMaxRows || a->cols < 1 || a->cols > kNormMaxCols)
+    return report_error(MOE_B200_ERR_ARG, "block_norm_backward: rows must be in [0, 2^30] and cols in [1, 16384]");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   // what the gate varies over: columns only, rows only, both, neither
   const bool g_rows = a->gate_row_stride != 0, g_cols = a->gate_per_column;

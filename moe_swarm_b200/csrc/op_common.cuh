@@ -40,6 +40,9 @@ class SmemOnce {
   std::atomic<uint64_t> done_{0};
 };
 
+// Most rows (tokens, outputs) of a call: row counters then stay clear of 32 bits.
+constexpr int kOpMaxRows = 1 << 30;
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline int type_bytes(int t) { return t == MOE_B200_FP32 ? 4 : t == MOE_B200_E4M3 ? 1 : 2; }
 inline bool is_float_type(int t) { return t == MOE_B200_BF16 || t == MOE_B200_FP16 || t == MOE_B200_FP32; }

@@ -621,8 +621,8 @@ extern "C" {
 MOE_B200_API int moe_b200_select_experts(const moe_b200_select_args* a, void* stream) {
   using namespace moe;
   if (!a) return report_error(MOE_B200_ERR_ARG, "null args");
-  if (a->num_tokens < 0 || a->num_experts < 1 || a->num_experts > kSelMaxE)
-    return report_error(MOE_B200_ERR_ARG, "select_experts: num_tokens must be >= 0 and num_experts in [1, 512]");
+  if (a->num_tokens < 0 || a->num_tokens > kOpMaxRows || a->num_experts < 1 || a->num_experts > kSelMaxE)
+    return report_error(MOE_B200_ERR_ARG, "select_experts: num_tokens must be in [0, 2^30] and num_experts in [1, 512]");
   if (a->n_group < 1 || a->n_group > 32 || a->num_experts % a->n_group)
     return report_error(MOE_B200_ERR_ARG, "select_experts: n_group must be in [1, 32] and divide num_experts");
   const int gs = a->num_experts / a->n_group;
@@ -686,8 +686,8 @@ MOE_B200_API int moe_b200_select_experts(const moe_b200_select_args* a, void* st
 MOE_B200_API int moe_b200_select_experts_backward(const moe_b200_select_backward_args* a, void* stream) {
   using namespace moe;
   if (!a) return report_error(MOE_B200_ERR_ARG, "null args");
-  if (a->num_tokens < 0 || a->num_experts < 1 || a->num_experts > kSelMaxE)
-    return report_error(MOE_B200_ERR_ARG, "select_experts_backward: num_tokens must be >= 0 and num_experts in [1, 512]");
+  if (a->num_tokens < 0 || a->num_tokens > kOpMaxRows || a->num_experts < 1 || a->num_experts > kSelMaxE)
+    return report_error(MOE_B200_ERR_ARG, "select_experts_backward: num_tokens must be in [0, 2^30] and num_experts in [1, 512]");
   if (a->top_k < 1 || a->top_k > kSelMaxK || a->top_k > a->num_experts)
     return report_error(MOE_B200_ERR_ARG, "select_experts_backward: top_k must be in [1, 32] and at most num_experts");
   if (a->score != MOE_B200_SCORE_SIGMOID && a->score != MOE_B200_SCORE_SOFTMAX)

@@ -207,7 +207,7 @@ def block_norm(y: torch.Tensor | None, residual: torch.Tensor | None, *, post_we
         else:
             x, x_ld = out, _result(out, "out", shape, (x_dtype,), dev)
         if x_dtype == torch.float8_e4m3fn:
-            x_scale = torch.empty(((cols + 127) // 128, rows), dtype=torch.float32, device=first.device)
+            x_scale = first.new_empty(((cols + 127) // 128, rows), dtype=torch.float32)
     _call("block_norm", dev, _native.NormArgs.pack(
         _ptr(y), _ptr(residual), _ptr(post_weight), _ptr(pre_weight), _ptr(gate), _ptr(residual_out), _ptr(x),
         _ptr(x_scale), y_ld, r_ld, ro_ld, x_ld, gate_ld, rows, cols, _TYPES[first.dtype], _TYPES[stream.dtype],
@@ -284,16 +284,16 @@ def select_experts(logits: torch.Tensor, top_k: int, *, score: str = "sigmoid", 
     """
     ld = _rows(logits, "logits")
     T, E = logits.shape
-    dev, device = logits.get_device(), logits.device
+    dev = logits.get_device()
     _check(score in _SCORES, "score must be 'sigmoid' or 'softmax'")
     _check(group_score in _GROUP_SCORES, "group_score must be 'top2' or 'max'")
     _check(1 <= top_k <= E, "top_k must be in [1, number of experts]")
     _check(1 <= topk_group <= n_group <= E, "topk_group must be in [1, n_group], n_group in [1, number of experts]")
     if bias is not None:
         _vector(bias, "bias", E, _FLOATS, dev)
-    idx = torch.empty((T, top_k), dtype=torch.int32, device=device)
-    w = torch.empty_like(idx, dtype=torch.float32)
-    n = torch.empty(E, dtype=torch.int32, device=device) if counts else None
+    idx = logits.new_empty((T, top_k), dtype=torch.int32)
+    w = logits.new_empty((T, top_k)) if logits.dtype == torch.float32 else torch.empty_like(idx, dtype=torch.float32)
+    n = idx.new_empty(E) if counts else None
     _call("select_experts", dev, _native.SelectArgs.pack(
         logits.data_ptr(), _ptr(bias), idx.data_ptr(), w.data_ptr(), _ptr(n), ld, T, E, top_k, _TYPES[logits.dtype],
         _type(bias), _SCORES[score], n_group, topk_group, _GROUP_SCORES[group_score], bool(renormalize), scale))
@@ -323,13 +323,13 @@ def quantize_int8(x: torch.Tensor, *, swiglu: bool = False):
     scale = max(amax / 127, 2**-126).  With ``swiglu``, of silu(x[:, cols:]) * x[:, :cols] (the
     expert layer's order of the two halves).  For weights [out, in] the rows are the channels."""
     ld = _rows(x, "x")
-    dev, device = x.get_device(), x.device
+    dev = x.get_device()
     rows, cols = x.shape
     if swiglu:
         _check(cols % 2 == 0, "swiglu needs an even number of columns")
         cols //= 2
-    q = torch.empty((rows, cols), dtype=torch.int8, device=device)
-    scale = torch.empty(rows, dtype=torch.float32, device=device)
+    q = x.new_empty((rows, cols), dtype=torch.int8)
+    scale = x.new_empty(rows, dtype=torch.float32)
     _call("quantize_int8", dev, _native.QuantizeArgs.pack(x.data_ptr(), q.data_ptr(), scale.data_ptr(), ld, cols, rows, cols,
                                                      _TYPES[x.dtype], bool(swiglu)))
     return q, scale
@@ -364,7 +364,7 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
         if out_dtype is None:
             out_dtype = torch.bfloat16 if x_type == _native.INT8 else x.dtype
         _check(out_dtype in _FLOATS, "unsupported out_dtype")
-        out, out_ld = torch.empty((T, N), dtype=out_dtype, device=x.device), N
+        out, out_ld = x.new_empty((T, N)) if out_dtype == x.dtype else x.new_empty((T, N), dtype=out_dtype), N
     else:
         out_ld = _result(out, "out", (T, N), _FLOATS if out_dtype is None else (out_dtype,), dev)
     if T == 0 or N == 0:

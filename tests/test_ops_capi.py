@@ -24,7 +24,7 @@ def refused(rc, code=N.ERR_ARG):
 
 
 @pytest.mark.parametrize("kw", [
-    dict(rows=-1), dict(cols=0), dict(cols=16385), dict(y=None, residual=None), dict(residual_out=None), dict(x=None),
+    dict(rows=-1), dict(rows=(1 << 30) + 1), dict(cols=0), dict(cols=16385), dict(y=None, residual=None), dict(residual_out=None), dict(x=None),
     dict(x_type=7), dict(x_type=N.E4M3), dict(residual_type=N.E4M3), dict(y_type=N.E4M3), dict(y_type=N.FP32),
     dict(pre_weight_type=N.E4M3), dict(gate=PTR, gate_type=N.INT8), dict(y=None, gate=PTR), dict(y=None, pre_weight=None)])
 def test_block_norm_refusals(kw):
@@ -49,7 +49,7 @@ def back_args(**kw):
 
 
 @pytest.mark.parametrize("kw", [
-    dict(rows=-1), dict(cols=0), dict(cols=16385), dict(dx=None, dresidual=None), dict(pre_weight=None),
+    dict(rows=-1), dict(rows=(1 << 30) + 1), dict(cols=0), dict(cols=16385), dict(dx=None, dresidual=None), dict(pre_weight=None),
     dict(dpre_weight=None), dict(residual=None), dict(post_weight=PTR), dict(gate=PTR), dict(y=None, post_weight=PTR),
     dict(y=None), dict(y_type=N.FP32), dict(residual_type=N.INT8)])
 def test_block_norm_backward_refusals(kw):
@@ -83,7 +83,7 @@ def test_empty_calls_need_no_device():
 
 
 @pytest.mark.parametrize("kw", [
-    dict(num_tokens=-1), dict(num_experts=0), dict(num_experts=513), dict(top_k=0), dict(top_k=33), dict(n_group=0),
+    dict(num_tokens=-1), dict(num_tokens=(1 << 30) + 1), dict(num_experts=0), dict(num_experts=513), dict(top_k=0), dict(top_k=33), dict(n_group=0),
     dict(n_group=33), dict(n_group=5), dict(topk_group=0), dict(topk_group=9), dict(top_k=20, topk_group=1),
     dict(group_score=2), dict(n_group=32, topk_group=32, num_experts=32), dict(score=2), dict(logits_type=N.E4M3),
     dict(bias_type=N.INT8), dict(logits=None), dict(idx=None), dict(weight=None)])
@@ -96,7 +96,7 @@ def test_select_refusals(kw):
 
 
 @pytest.mark.parametrize("kw", [
-    dict(num_tokens=-1), dict(num_experts=0), dict(num_experts=513), dict(top_k=0), dict(top_k=33), dict(top_k=9),
+    dict(num_tokens=-1), dict(num_tokens=(1 << 30) + 1), dict(num_experts=0), dict(num_experts=513), dict(top_k=0), dict(top_k=33), dict(top_k=9),
     dict(score=5), dict(logits_type=N.INT8), dict(logits=None), dict(idx=None), dict(dweight=None), dict(dlogits=None)])
 def test_select_backward_refusals(kw):
     a = N.SelectBackwardArgs(logits=PTR, idx=PTR, dweight=PTR, dlogits=PTR, logits_stride=8, dlogits_stride=8, num_tokens=4,
@@ -107,7 +107,7 @@ def test_select_backward_refusals(kw):
 
 
 @pytest.mark.parametrize("kw", [
-    dict(num_tokens=-1), dict(out_features=0), dict(in_features=8), dict(in_features=40), dict(in_features=131072),
+    dict(num_tokens=-1), dict(num_tokens=(1 << 30) + 1), dict(out_features=(1 << 30) + 1), dict(out_features=0), dict(in_features=8), dict(in_features=40), dict(in_features=131072),
     dict(in_features=65536), dict(x_type=N.E4M3), dict(x_type=N.INT8, swiglu=1), dict(x_type=N.INT8), dict(y_type=N.INT8),
     dict(bias=PTR, bias_type=N.E4M3), dict(x=None), dict(weight=None), dict(weight_scale=None), dict(y=None),
     dict(weight=PTR + 8), dict(weight_stride=72), dict(weight_stride=48),

@@ -90,8 +90,10 @@ __device__ __forceinline__ void store_x(const NormArgs& a, int row, int cols, Ro
   }
 }
 
-// One row per group of warps.  blockDim = (32 * warps, rows per CTA).  Rows beyond the last run
-// with no elements.
+// One row per group of warps.  blockDim = (32 * warps, rows per CTA), or less than a warp per row
+// (kPacked).  Rows beyond the last run with no elements.  Bound by latency where rows are few (one row
+// of 7168: 2.6 us), by HBM where many: 592 rows 6.4 us, 16384 x 512 11.6 us (5.8 TB/s), 901 x 5001
+// with both norms 15.5 us (3.5 TB/s: odd rows are read and written two bytes at a time).
 template <class YT, class RT, int LAY, int MAXT>
 __global__ void __launch_bounds__(MAXT, 1024 / MAXT) norm_fwd_kernel(NormArgs a) {
   __shared__ float buf[2][8 * 32];
@@ -113,8 +115,9 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) norm_fwd_kernel(NormArgs a)
     float k = a.scale;
     if (a.post_w) {
       load_weight<LAY>(a.post_w, a.post_type, a.off, cols, w);
-      float ss[1] = {dot16(y, y)};
-      row_sum(ss, a.warps, buf[0]);
+      float ss[1] = {dot16<LAY>(y, y)};
+      if constexpr (LAY == kPacked) packed_sum(ss);
+      else row_sum(ss, a.warps, buf[0]);
       k *= rsqrtf(ss[0] / a.cols + a.eps);
 #pragma unroll
       for (int i = 0; i < 8; ++i) y.v[i] = mul2(y.v[i], w.v[i]);
@@ -133,14 +136,17 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) norm_fwd_kernel(NormArgs a)
   if (!a.pre_w) return;
   load_weight<LAY>(a.pre_w, a.pre_type, a.off, cols, w);
   float ss[1] = {squares_existing<LAY>(r, cols)};
-  row_sum(ss, a.warps, buf[1]);
+  if constexpr (LAY == kPacked) packed_sum(ss);
+  else row_sum(ss, a.warps, buf[1]);
   store_x<LAY>(a, row, cols, r, w, rsqrtf(ss[0] / a.cols + a.eps));
 }
 
 // Many rows: persistent CTAs, whose next rows (y, residual, gate per element) are on their way
 // to shared memory as bulk copies while a row is computed, so that the row's barriers and latencies
 // leave the memory busy.  Weights and a gate per column come from L1.  A stage is refilled after
-// the row's last barrier, when every thread holds its part.
+// the row's last barrier, when every thread holds its part.  1024 threads of an SM, whose rows in flight
+// are about 200 KB; 4096 x 7168 from bf16 to e4m3 35.3 us (5.8 TB/s, HBM), to bf16 40.6, with both
+// norms and a gate per element 54 (5.4 TB/s).
 template <class YT, class RT, bool POST, int LAY>
 __global__ void __launch_bounds__(512, 2) norm_ring_kernel(NormArgs a, RingPlan g) {
   extern __shared__ __align__(128) uint8_t ring[];
@@ -182,7 +188,7 @@ __global__ void __launch_bounds__(512, 2) norm_ring_kernel(NormArgs a, RingPlan 
     float k = a.scale;
     if (POST) {
       load_weight<LAY>(a.post_w, a.post_type, a.off, cols, w);
-      float ss[1] = {dot16(y, y)};
+      float ss[1] = {dot16<LAY>(y, y)};
       row_sum(ss, a.warps, buf[0]);
       k *= rsqrtf(ss[0] * inv_cols + a.eps);
 #pragma unroll
@@ -292,7 +298,11 @@ MOE_B200_API int moe_b200_block_norm(const moe_b200_norm_args* a, void* stream) 
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaSuccess;
   // The ring: aligned rows of two warps or more, at least four per SM, and two or more of them in
-  // a CTA's share of shared memory.
+  // a CTA's share of shared memory.  7168 columns, bf16 in, e4m3 out, ring against direct: 592 rows
+  // 5.7 us against 6.4, 4096 rows 35.3 (5.8 TB/s) against 51.9; at 148 and 296 rows the ring is 0.1
+  // to 0.2 us behind.  Not for a 32-bit residual with nothing but the sum and its norm to compute, whose
+  // wide loads keep the memory busy without it: 4096 x 7168 63.9 against 56.4 (6.2 TB/s), 8192 x
+  // 4096 72.6 against 61.0; with a gate per token 58.8 against 63.6, with post_weight 66 against 78.
   RingPlan g{};
   ring_add(&g, a->y, n.y_ld, a->cols, a->y_type);
   ring_add(&g, a->residual, n.r_ld, a->cols, a->residual_type);
@@ -300,7 +310,8 @@ MOE_B200_API int moe_b200_block_norm(const moe_b200_norm_args* a, void* stream) 
   const int ctas = n.warps >= 2 && n.warps <= 16 ? 32 / n.warps : 0;   // 1024 threads of an SM
   g.stages = ctas ? kRingSmem / ctas / g.stage_bytes : 0;
   if (g.stages > kRingMaxStages) g.stages = kRingMaxStages;
-  if (vec && a->y && a->rows >= 4 * sms && g.stages >= 2) {
+  const bool sum_alone = a->residual_type == MOE_B200_FP32 && !a->post_weight && !a->gate;
+  if (vec && a->y && a->rows >= 4 * sms && g.stages >= 2 && !sum_alone) {
     const dim3 grid(a->rows < ctas * sms ? a->rows : ctas * sms), block(n.warps * 32);
     const size_t smem = static_cast<size_t>(g.stages) * g.stage_bytes;
     dispatch_types(a->y_type, a->residual_type, [&](auto yt, auto rt) {
@@ -317,14 +328,20 @@ MOE_B200_API int moe_b200_block_norm(const moe_b200_norm_args* a, void* stream) 
     });
     return e == cudaSuccess ? MOE_B200_OK : report_cuda(e, "block_norm launch");
   }
-  const dim3 block(n.warps * 32, rpc), grid((a->rows + rpc - 1) / rpc);
+  // Rows of up to 256 columns: several to a warp (65536 x 128: 11.7 us, 5.7 TB/s, against 31.5 with
+  // one).  An e4m3 block's maximum wants a half warp.
+  const bool packed = vec && a->cols <= 256 && !(a->pre_weight && a->x_type == MOE_B200_E4M3);
+  const int lanes = packed ? packed_lanes(a->cols) : n.warps * 32;
+  if (packed) rpc = 256 / lanes;
+  const dim3 block(lanes, rpc), grid((a->rows + rpc - 1) / rpc);
   dispatch_types(a->y_type, a->residual_type, [&](auto yt, auto rt) {
     using YT = decltype(yt);
     using RT = decltype(rt);
     // rows of up to 8192 columns take at most 512 threads, which may then use twice the registers
     auto sized = [&](auto t) {
       constexpr int MAXT = decltype(t)::value;
-      return vec                             ? norm_fwd_kernel<YT, RT, kVec, MAXT>
+      return packed                          ? norm_fwd_kernel<YT, RT, kPacked, 512>
+             : vec                           ? norm_fwd_kernel<YT, RT, kVec, MAXT>
              : a->cols >= 384 * n.warps ? norm_fwd_kernel<YT, RT, kTail, MAXT>
                                         : norm_fwd_kernel<YT, RT, kScattered, MAXT>;
     };

@@ -71,14 +71,15 @@ __device__ __forceinline__ void bwd_row(const NormBwdArgs& a, int row, int cols,
     load(5, G);
 #pragma unroll
     for (int i = 0; i < 8; ++i) G.v[i] = mul2(G.v[i], dx.v[i]);
-    s[0] = dot16(r, r);
-    s[1] = dot16(G, r);
+    s[0] = dot16<LAY>(r, r);
+    s[1] = dot16<LAY>(G, r);
   }
   if (has_y) {
     load(2, y);
-    if (post) s[2] = dot16(y, y);
+    if (post) s[2] = dot16<LAY>(y, y);
   }
-  if (LAY == kFull || a.warps <= 16) row_sum3(s, a.warps, buf0);
+  if constexpr (LAY == kPacked) packed_sum(s);
+  else if (LAY == kFull || a.warps <= 16) row_sum3(s, a.warps, buf0);
   else row_sum(s, a.warps, buf0);
   const float rstd = rsqrtf(s[0] * inv_cols + a.eps);
   {
@@ -132,10 +133,11 @@ __device__ __forceinline__ void bwd_row(const NormBwdArgs& a, int row, int cols,
   }
   float k = 0.f;
   if (post || gate == 1) {
-    float t[1] = {dot16(G, y)};   // sum of b G y
-    row_sum(t, a.warps, buf1);
+    float t[1] = {dot16<LAY>(G, y)};   // sum of b G y
+    if constexpr (LAY == kPacked) packed_sum(t);
+    else row_sum(t, a.warps, buf1);
     done();
-    if (gate == 1 && threadIdx.x == 0) static_cast<float*>(a.dgate)[row] = a.scale * ystd * t[0];
+    if (gate == 1 && threadIdx.x == 0 && (LAY != kPacked || cols > 0)) static_cast<float*>(a.dgate)[row] = a.scale * ystd * t[0];
     if (post) k = -t[0] * inv_cols * ystd * ystd;
   } else {
     done();
@@ -172,18 +174,25 @@ __device__ __forceinline__ void bwd_store_sums(const NormBwdArgs& a, const NormB
 }
 
 // Any alignment, any set of tensors: rows straight from global memory, one per CTA at a time.
+// kPacked: blockDim.y of them; those beyond the last run with no elements (65536 x 128: 40 us, 2.5
+// TB/s, against 98 with a warp per row).  kThin: rows on odd boundaries, whose 2-byte loads, stores and
+// checks make many instructions; eight elements a thread let twice the warps share them (4096 x 5001
+// with a 32-bit residual: 206 us against 304 with sixteen; 5000 x 700 35 against 49).  What bounds it is still
+// that chain of instructions, not memory: bulk copies of the rows ahead (their ends by plain
+// loads) left 901 x 5001 at 55 us against 53, prefetching them to L2 at 52.
 template <class YT, class RT, int LAY>
-__device__ __forceinline__ void bwd_direct(const NormBwdArgs& a, float (*buf)[3 * 32]) {
+__device__ __forceinline__ void bwd_direct(const NormBwdArgs& a, float (*buf)[3 * 32], float* shared) {
   NormBwdSums sum;
 #pragma unroll
   for (int i = 0; i < 8; ++i) sum.pre.v[i] = sum.post.v[i] = dup2(0.f);
-  const int cols = a.cols;
   // a row without a second sum alternates the first one's buffer by itself
   const bool two = a.y && (a.post_w || a.gate_grad == kGateRow);
   int first = 0;
-  for (int row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const float g_row = a.gate_grad == kGateRow ? load1_dyn(a.gate, a.gate_type, row * a.g_ld) : 0.f;
-    bwd_row<YT, RT, LAY, -1, -1>(a, row, cols, 1.f / cols, buf[first], buf[1], sum, g_row, [&](int which, Row16& v) {
+  const int many = LAY == kPacked ? blockDim.y : 1;
+  for (int row0 = blockIdx.x * many; row0 < a.rows; row0 += gridDim.x * many) {
+    const int row = LAY == kPacked ? row0 + threadIdx.y : row0, cols = row < a.rows ? a.cols : 0;
+    const float g_row = a.gate_grad == kGateRow && cols ? load1_dyn(a.gate, a.gate_type, row * a.g_ld) : 0.f;
+    bwd_row<YT, RT, LAY, -1, -1>(a, row, cols, 1.f / a.cols, buf[first], buf[1], sum, g_row, [&](int which, Row16& v) {
       if (which == 0) load_row<YT, LAY>(static_cast<const YT*>(a.dx) + row * a.dx_ld, cols, v);
       else if (which == 1) load_row<RT, LAY>(static_cast<const RT*>(a.r) + row * a.r_ld, cols, v);
       else if (which == 2) load_row<YT, LAY>(static_cast<const YT*>(a.y) + row * a.y_ld, cols, v);
@@ -194,22 +203,25 @@ __device__ __forceinline__ void bwd_direct(const NormBwdArgs& a, float (*buf)[3 
     }, [] {});
     if (!two) first ^= 1;
   }
-  bwd_store_sums<LAY>(a, sum, nullptr);
+  bwd_store_sums<LAY>(a, sum, shared);
 }
 
 template <class YT, class RT, int LAY, int MAXT>
 __global__ void __launch_bounds__(MAXT, 1) norm_bwd_kernel(NormBwdArgs a) {
+  extern __shared__ __align__(16) float packed_sums[];
   __shared__ float buf[2][3 * 32];
   pdl_wait();
   pdl_launch_dependents();
-  bwd_direct<YT, RT, LAY>(a, buf);
+  bwd_direct<YT, RT, LAY>(a, buf, packed_sums);
 }
 
 // Aligned rows with all of dx, r', y: the next rows (dx, r', y, dr, gate per element) are on their
 // way to shared memory as bulk copies while a row is computed.  The factors per column are put
 // into shared memory once, 32-bit, as each thread reads them, beside a 16-bit residual; a 32-bit one
 // leaves its ring too little room, and they are read in place.  Rows of one warp go eight to a CTA,
-// each warp with a ring of its own and no CTA barrier until the sums are written.
+// each warp with a ring of its own and no CTA barrier until the sums are written.  4096 x 7168 with
+// both norms and a gate per column: 66.5 us with its column sums (5.3 TB/s) against 176 straight from
+// memory; 64 rows 9.0 against 10.1, so there is no lower limit of rows.
 template <class YT, class RT, int LAY, int POST, int GATE>
 __global__ void __launch_bounds__(512, 1) norm_bwd_ring_kernel(NormBwdArgs a, RingPlan g) {
   extern __shared__ __align__(128) uint8_t ring[];
@@ -284,7 +296,7 @@ __global__ void __launch_bounds__(512, 1) norm_bwd_ring_kernel(NormBwdArgs a, Ri
             return;
           }
           // the ring's order: dx, r', y, dr (if any), gate (if per element)
-          const uint8_t* p = src + (which == 4 ? (a.dr ? g.t[4].at : g.t[3].at) : g.t[which].at);
+          const uint8_t* p = src + g.t[which == 4 && !a.dr ? 3 : which].at;
           if (which == 0 || which == 2) load_row<YT, LAY>(reinterpret_cast<const YT*>(p), cols, v);
           else if (which != 4) load_row<RT, LAY>(reinterpret_cast<const RT*>(p), cols, v);
           else load_row_dyn<LAY>(p, a.gate_type, 0, cols, v);
@@ -311,9 +323,10 @@ __global__ void __launch_bounds__(512, 1) norm_bwd_ring_kernel(NormBwdArgs a, Ri
   bwd_store_sums<LAY>(a, sum, reinterpret_cast<float*>(ring + factor_bytes));
 }
 
-// Adds up the parts of a column, 32 columns per CTA, eight warps over the parts, their sums in
-// warp order.  blockIdx.y selects the sum: that of dx r^ is dpre_weight; that of G y^ gives
-// dpost_weight and the gradient of a gate per column.
+// Adds up the parts of a column, 32 columns per CTA: eight parts per warp in flight together, the
+// warps' sums in their order.  blockIdx.y selects the sum: that of dx r^ is dpre_weight; that of G y^
+// gives dpost_weight and the gradient of a gate per column.  Bound by the loads' latency: 148 parts
+// of 7168 columns about 4 us behind the rows; 1184 parts of 700 took 22 us with eight warps and one load at a time.
 struct NormSumArgs {
   const float* partial;
   float *pre, *post, *gate;
@@ -321,20 +334,26 @@ struct NormSumArgs {
   int parts, cols, pre_slot, post_type, chan_type;
   float scale, off;
 };
-__global__ void __launch_bounds__(256) norm_sum_kernel(NormSumArgs a) {
-  __shared__ float buf[8][32];
+__global__ void __launch_bounds__(1024) norm_sum_kernel(NormSumArgs a) {
+  __shared__ float buf[32][32];
   pdl_wait();
   pdl_launch_dependents();
-  const int c = blockIdx.x * 32 + threadIdx.x;
+  const int c = blockIdx.x * 32 + threadIdx.x, warps = blockDim.y;
   const float* p = a.partial + static_cast<int64_t>(blockIdx.y) * a.parts * a.cols + c;
   float s = 0.f;
   if (c < a.cols)
-    for (int i = threadIdx.y; i < a.parts; i += 8) s += p[static_cast<int64_t>(i) * a.cols];
+    for (int i = threadIdx.y; i < a.parts; i += 8 * warps) {
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        v[j] = i + j * warps < a.parts ? p[static_cast<int64_t>(i + j * warps) * a.cols] : 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s += v[j];
+    }
   buf[threadIdx.y][threadIdx.x] = s;
   __syncthreads();
   if (threadIdx.y != 0 || c >= a.cols) return;
-#pragma unroll
-  for (int w = 1; w < 8; ++w) s += buf[w][threadIdx.x];
+  for (int w = 1; w < warps; ++w) s += buf[w][threadIdx.x];
   if (static_cast<int>(blockIdx.y) == a.pre_slot) {
     a.pre[c] = s;
     return;
@@ -361,6 +380,8 @@ namespace {
 // goes by them): 148 SMs, each with 512 threads' worth of registers.
 struct NormBwdShape {
   int warps, direct_parts, ring_ctas, ring_rows, ring_parts;   // ring_rows: rows side by side in a CTA
+  int lanes, packed_rows, packed_parts;
+  int thin_warps, thin_parts;   // 0: too long
 };
 NormBwdShape bwd_shape(int rows, int cols) {
   NormBwdShape s{};
@@ -379,6 +400,17 @@ NormBwdShape bwd_shape(int rows, int cols) {
     }
     const int need = (rows + s.ring_rows - 1) / s.ring_rows;
     s.ring_parts = need < 148 * s.ring_ctas ? need : 148 * s.ring_ctas;
+  }
+  s.lanes = packed_lanes(cols);
+  const int of_warp = s.lanes < 32 ? 32 / s.lanes : 1;   // whole warps, few rows spread over the SMs
+  const int even = ((rows + 147) / 148 + of_warp - 1) / of_warp * of_warp;
+  s.packed_rows = even < 16 * of_warp ? even : 16 * of_warp;
+  const int need = (rows + s.packed_rows - 1) / s.packed_rows;
+  s.packed_parts = need < 148 ? need : 148;
+  if (cols <= 32 * 256) {   // 1024 threads of an SM, eight elements each
+    s.thin_warps = (cols + 255) / 256;
+    const int ctas = 148 * (32 / s.thin_warps);
+    s.thin_parts = rows < ctas ? rows : ctas;
   }
   return s;
 }
@@ -399,7 +431,9 @@ MOE_B200_API size_t moe_b200_block_norm_backward_workspace_size(int32_t rows, in
   using namespace moe;
   if (rows < 0 || rows > kOpMaxRows || cols < 1 || cols > kNormMaxCols) return 0;
   const NormBwdShape shape = bwd_shape(rows, cols);
-  const int parts = shape.direct_parts > shape.ring_parts ? shape.direct_parts : shape.ring_parts;
+  int parts = shape.direct_parts > shape.ring_parts ? shape.direct_parts : shape.ring_parts;
+  if (parts < shape.packed_parts) parts = shape.packed_parts;
+  if (parts < shape.thin_parts) parts = shape.thin_parts;
   return static_cast<size_t>(align256(static_cast<int64_t>(2) * parts * cols * 4) + align256(static_cast<int64_t>(rows) * 4) +
                              256);
 }
@@ -500,8 +534,11 @@ MOE_B200_API int moe_b200_block_norm_backward(const moe_b200_norm_backward_args*
   const int factors = shared_factors(a->residual_type) ? kFactorBytes * n.warps * 32 : 0;
   g.stages = shape.ring_ctas ? (kRingSmem / shape.ring_ctas - factors) / shape.ring_rows / g.stage_bytes : 0;
   if (g.stages > kRingMaxStages) g.stages = kRingMaxStages;
-  const bool ring = vec && a->dx && a->y && g.stages >= 1;
-  n.parts = ring ? shape.ring_parts : shape.direct_parts;
+  // rows of up to 256 columns: several to a warp; odd ones: kThin; the ring takes what has both of dx and y
+  const bool packed = vec && a->cols <= 256;
+  const bool ring = vec && !packed && a->dx && a->y && g.stages >= 1;
+  const bool thin = !vec && shape.thin_warps > 0;
+  n.parts = packed ? shape.packed_parts : thin ? shape.thin_parts : ring ? shape.ring_parts : shape.direct_parts;
   // the row sums of a gate that is one number go through the workspace
   float* row_dots = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) +
                                              align256(static_cast<int64_t>(2) * n.parts * a->cols * 4));
@@ -520,21 +557,20 @@ MOE_B200_API int moe_b200_block_norm_backward(const moe_b200_norm_backward_args*
         return a->post_weight ? of_gate(lay, std::integral_constant<int, 1>{}) : of_gate(lay, std::integral_constant<int, 0>{});
       };
       auto kernel = a->cols == n.warps * 32 * kNormPerThread ? of_post(std::integral_constant<int, kFull>{})
-                    : a->cols >= 256                         ? of_post(std::integral_constant<int, kHalf>{})
-                                                             : norm_bwd_ring_kernel<YT, RT, kVec, -1, -1>;
+                                                             : of_post(std::integral_constant<int, kHalf>{});
       e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem);
       if (e == cudaSuccess)
         e = launch_pdl(kernel, dim3(n.parts), dim3(n.warps * 32, shape.ring_rows),
                        factors + static_cast<size_t>(g.stages) * g.stage_bytes * shape.ring_rows, st, n, g);
     } else {
-      auto sized = [&](auto t) {
-        constexpr int MAXT = decltype(t)::value;
-        return vec                             ? norm_bwd_kernel<YT, RT, kVec, MAXT>
-               : a->cols >= 384 * n.warps ? norm_bwd_kernel<YT, RT, kTail, MAXT>
-                                          : norm_bwd_kernel<YT, RT, kScattered, MAXT>;
-      };
-      auto kernel = n.warps <= 16 ? sized(std::integral_constant<int, 512>{}) : sized(std::integral_constant<int, 1024>{});
-      e = launch_pdl(kernel, dim3(n.parts), dim3(n.warps * 32), 0, st, n);
+      if (thin) n.warps = shape.thin_warps;
+      auto kernel = packed          ? norm_bwd_kernel<YT, RT, kPacked, 512>
+                    : thin          ? norm_bwd_kernel<YT, RT, kThin, 1024>
+                    : !vec          ? norm_bwd_kernel<YT, RT, kTail, 1024>
+                    : n.warps <= 16 ? norm_bwd_kernel<YT, RT, kVec, 512>
+                                    : norm_bwd_kernel<YT, RT, kVec, 1024>;
+      const dim3 block(packed ? shape.lanes : n.warps * 32, packed ? shape.packed_rows : 1);
+      e = launch_pdl(kernel, dim3(n.parts), block, packed ? sizeof(float) * shape.packed_rows * a->cols : 0, st, n);
     }
   });
   if (e != cudaSuccess) return report_cuda(e, "block_norm_backward launch");
@@ -549,7 +585,8 @@ MOE_B200_API int moe_b200_block_norm_backward(const moe_b200_norm_backward_args*
     s.chan_type = a->gate_type;
     s.scale = a->scale;
     s.off = a->weight_offset;
-    e = launch_pdl(norm_sum_kernel, dim3((a->cols + 31) / 32, sums), dim3(32, 8), 0, st, s);
+    const int sum_warps = n.parts < 8 * 32 ? (n.parts + 7) / 8 : 32;   // eight parts each, then rounds
+    e = launch_pdl(norm_sum_kernel, dim3((a->cols + 31) / 32, sums), dim3(32, sum_warps), 0, st, s);
     if (e != cudaSuccess) return report_cuda(e, "block_norm_backward sum launch");
   }
   if (n.gate_grad == kGateRow && !g_rows) {

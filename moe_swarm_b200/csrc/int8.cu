@@ -91,7 +91,8 @@ __device__ __forceinline__ void store_codes(int8_t* row, int cols, const Row16& 
 }
 
 // One row in the registers of a group of warps, N times 16 elements per thread (N = 2: the second
-// 16 are those of the row's second half of threads x 16 columns).
+// 16 are those of the row's second half of threads x 16 columns).  Few rows: bound by latency (80 x 2048
+// with the activation 2.0 us).
 template <class XT, int LAY, int N>
 __global__ void __launch_bounds__(N == 1 ? 512 : 1024, 1) quant_kernel(QuantArgs a) {
   __shared__ float buf[8 * 32];
@@ -125,6 +126,7 @@ __global__ void __launch_bounds__(N == 1 ? 512 : 1024, 1) quant_kernel(QuantArgs
 }
 
 // Many aligned rows: persistent CTAs with their next rows on the way to shared memory, as the norm's.
+// Bound by HBM: 8192 x 7168 from bf16 30.8 us (5.7 TB/s); with the activation, 8192 x 2048, 16.6 us (5.1).
 template <class XT, int LAY>
 __global__ void __launch_bounds__(512, 2) quant_ring_kernel(QuantArgs a, RingPlan g) {
   extern __shared__ __align__(128) uint8_t ring[];
@@ -328,7 +330,8 @@ cudaError_t quant_launch(const QuantArgs& q0, int sms, cudaStream_t st) {
   cudaError_t e = cudaSuccess;
   auto go = [&](auto t) {
     using XT = decltype(t);
-    // the ring: aligned rows of two warps or more, at least four per SM
+    // The ring: aligned rows of two warps or more, at least four per SM (7168 columns, ring against
+    // direct: 148 rows 1.9 us against 1.8, 592 rows 3.2 against 3.3, 8192 rows 30.8 against 51.5).
     RingPlan g{};
     ring_add(&g, q.x, q.x_ld, q.cols, q.type);
     if (q.swiglu) ring_add(&g, static_cast<const XT*>(q.x) + q.cols, q.x_ld, q.cols, q.type);

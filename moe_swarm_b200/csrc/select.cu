@@ -21,6 +21,11 @@
 // last expert chosen against the best one left) is further apart than that allows for; otherwise,
 // which for continuous logits is one token in some hundreds, the scores
 // are computed as defined and the choice is made again from those.
+//
+// Bound by the warps' instructions, about 850 per token of 256 experts in 8 groups (scores, a sort of
+// eight keys per lane, rounds of maxima), not by HBM: 16384 tokens 20.7 us with counts (18.1 without
+// groups, 17.3 softmax) where the logits alone would take 2.7; 512 experts 46 us, 64 experts 11.  Few
+// tokens are bound by the one token's chain of operations: 16 tokens 4.6 us.
 #include <type_traits>
 
 #include "exp64.cuh"
@@ -505,7 +510,8 @@ __global__ void __launch_bounds__(kSelMaxE) select_zero_kernel(int* counts, int 
 //   renormalised, S = sum of the chosen s + 1e-20:  ds_k = scale * (dw_k - sum_j dw_j s_j / S) / S
 //   softmax: dx_e = s_e (ds_e - sum_j ds_j s_j);  sigmoid: dx_e = ds_e s_e (1 - s_e)
 // The scores go to shared memory, where a lane per chosen expert finds its own; those lanes work out
-// the sums and put their own results among what every lane stores.
+// the sums and put their own results among what every lane stores.  16384 x 256 softmax 10.3 us (3.4
+// TB/s: about half by memory, half by the exponentials and sums), sigmoid 9.6, 512 experts 33.
 template <int V, bool SOFTMAX>
 __global__ void __launch_bounds__(kSelWarps * 32) select_bwd_kernel(SelectBwdArgs a) {
   __shared__ __align__(16) float s_row[kSelWarps][32 * V];
@@ -608,6 +614,8 @@ void dispatch_select(int E, F&& f) {
   else f(std::integral_constant<int, 16>{});
 }
 
+// Eight CTAs of eight warps are all the warps of an SM; with four the backward of 16384 x 256 takes
+// 15.7 us instead of 10.3, the forward 21.1 instead of 20.7.
 int select_grid(int T, int sms) {
   const int need = (T + kSelWarps - 1) / kSelWarps;
   return need < 8 * sms ? need : 8 * sms;
@@ -645,7 +653,9 @@ MOE_B200_API int moe_b200_select_experts(const moe_b200_select_args* a, void* st
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaSuccess;
   // Counts: up to 64 tokens are one cluster's, which adds up its CTAs' histograms; beyond that
-  // the CTAs add theirs to counts zeroed first.
+  // the CTAs add theirs to counts zeroed first.  On the device the two are alike (1 token 3.7 us
+  // against 4.2, 16 tokens 4.6 against 4.4, 64 tokens 4.6 against 5.3), but the cluster is one launch,
+  // 2.5 us of the caller's time less.
   const int ctas = select_grid(a->num_tokens, sms);
   const bool cluster = a->counts && a->num_tokens > 0 && ctas <= 8;
   if (a->counts && !cluster) {

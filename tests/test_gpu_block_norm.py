@@ -223,6 +223,14 @@ def test_many_rows(T, H, y_dtype, r_dtype, post, gate):
             R.close(b.gate, dg, mag, steps=steps)
 
 
+@pytest.mark.parametrize("T,H", [(2500, 8), (257, 16), (9, 24), (1000, 200), (1301, 128), (130, 256), (5, 250), (700, 257)])
+@pytest.mark.parametrize("y_dtype,r_dtype", [(BF, BF), (FP, F32)])
+@pytest.mark.parametrize("post,gate", [(False, None), (True, "token"), (True, "channel"), (True, "full"), (False, "one")])
+def test_short_rows(T, H, y_dtype, r_dtype, post, gate):
+    """Several rows to a warp, whose last ones do not fill theirs."""
+    test_many_rows(T, H, y_dtype, r_dtype, post, gate)
+
+
 def test_backward_partial_forms():
     a = make(50, 520, BF, BF, True, "token", seed=6)
     g = gen(7)

@@ -369,6 +369,7 @@ MOE_B200_API int moe_b200_select_experts_backward(const moe_b200_select_backward
 
 /* 8-bit codes and scales of the rows of x (cols <= 32768): scale = max(amax / 127, 2^-126),
  * q = rint(v / scale), v = x or, with swiglu, silu(x[:, cols:]) * x[:, :cols] of x [rows, 2 cols].
+ * Without swiglu the codes are those of 64-bit arithmetic with the scale amax * (1 / 127).
  * A row with a NaN or an infinity gets a NaN scale and zero codes. */
 typedef struct moe_b200_quantize_args {
   const void* x;

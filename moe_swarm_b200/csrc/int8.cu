@@ -3,7 +3,8 @@
 //   q[t][k] = rint(v[t][k] / sx[t]) in [-127, 127],  sx[t] = max(max_k |v[t][k]| / 127, 2^-126)
 //   y[t][n] = sx[t] * sw[n] * sum_k q[t][k] * w[n][k]  (+ bias[n])
 //
-// v is x, or silu(x2) * x1 of x = [x1 | x2] (the expert layer's order).  Sums of products are
+// v is x, or silu(x2) * x1 of x = [x1 | x2] (the expert layer's order).  The codes of x are those of
+// 64-bit arithmetic with max |x| * (1 / 127) for a scale; sx is that in 32 bits.  Sums of products are
 // exact 32-bit integers (|sum| <= K * 2^14, so K <= 131056 cannot overflow).  A row holding a NaN
 // or an infinity gets a NaN scale, so its outputs are NaN.
 #include <type_traits>
@@ -15,6 +16,8 @@ namespace moe {
 
 constexpr int kQuantMaxCols = 2 * kNormMaxCols;
 constexpr int kInt8MaxK = 131056;
+
+constexpr float kQuantMinScale = 1.17549435082228751e-38f;   // 2^-126
 
 struct QuantArgs {
   const void* x;
@@ -38,26 +41,26 @@ __device__ __forceinline__ float row_amax(const Row16& v) {
   for (int j = 1; j < 16; ++j) m = max_nan(m, fabsf(v[j]));
   return m;
 }
+// Magnitudes are ordered as their bits are, NaN above all.
+__device__ __forceinline__ float warp_amax(float m) {
+  return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
+}
 // Maximum over a row's warps (blockDim = (32 * warps, rows)); `buf` [rows][32] is free again after
 // the next CTA barrier.
 __device__ __forceinline__ float row_max(float m, int warps, float* buf) {
-#pragma unroll
-  for (int d = 16; d >= 1; d >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
+  m = warp_amax(m);
   if (warps == 1) return m;
   const int lane = threadIdx.x & 31;
   float* b = buf + threadIdx.y * 32;
   if (lane == 0) b[threadIdx.x >> 5] = m;
   __syncthreads();
-  m = lane < warps ? b[lane] : 0.f;
-#pragma unroll
-  for (int d = 16; d >= 1; d >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
-  return m;
+  return warp_amax(lane < warps ? b[lane] : 0.f);
 }
 
 // A row's scale and its reciprocal; a row with a NaN or an infinity: NaN, and 0 for zero codes.
 __device__ __forceinline__ float quant_scale(float m, float* inv) {
   const bool finite = m <= 3.4028234663852886e38f;
-  const float sc = finite ? fmaxf(m / 127.f, 1.17549435082228751e-38f) : __uint_as_float(0x7fc00000u);
+  const float sc = finite ? fmaxf(m / 127.f, kQuantMinScale) : __uint_as_float(0x7fc00000u);
   *inv = finite ? 1.f / sc : 0.f;
   return sc;
 }
@@ -73,12 +76,104 @@ __device__ __forceinline__ uint32_t codes4(float2 a, float2 b, float2 inv) {
   const uint32_t hi = __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0040);
   return __byte_perm(lo, hi, 0x5410);
 }
-template <int LAY>
-__device__ __forceinline__ void store_codes(int8_t* row, int cols, const Row16& v, float inv) {
-  uint32_t c[4];
-  const float2 k = dup2(inv);
+
+// Of given 16-bit values, one in some hundreds lies on a tie of v / s (one half of the row's largest
+// always does), where 32-bit arithmetic would take either side; a whole code is much beside the
+// result's other errors.  With integer mantissas a of v and b of m, v / s = 127 a 2^z / b is either a tie or
+// away from one by 1 / (254 * 2047) > 2^-19 of itself.  So the codes of inv (1 - 2^-21) and inv (1 + 2^-21)
+// differ where there is a tie and nowhere else, and are the two sides of it.
+//
+// Which side: s = m * fl(1 / 127) in 64 bits is m / 127 (1 + e) with |e| of about 2^-53.  The quotient,
+// t (1 - e) of a tie t = k + 1/2, is rounded back to t, and then to even, if t |e| is at most half the
+// spacing of 64-bit numbers at t, that is if mantissa(t) |e| 2^53 <= 1; otherwise it goes the way of -e.
+// With d = 127 s - m (exact) and |e| = |d| / m that is the same for a whole row where 2^54 |d| <= m or
+// 2^53 |d| > m.
+//
+// (d is a multiple of the last place of s, of which there are 64 at most: seven bits, and mantissa(t) has
+// eight, so their product is exact in 32 bits.)
+enum : int { kTieEven, kTieDown, kTieUp, kTieMixed };
+struct TieRule {
+  float d53, m;   // 2^53 |d| and m, both by 2^-4
+  int mode;
+  bool down;
+};
+__device__ __forceinline__ double scale64(float m) { return fmax(m * (1.0 / 127.0), static_cast<double>(kQuantMinScale)); }
+__device__ __forceinline__ TieRule tie_rule(float m) {
+  TieRule r;
+  const double s = m * (1.0 / 127.0);
+  const float d = m < 127.f * kQuantMinScale ? 0.f   // the scale is a power of two
+                                             : static_cast<float>(fma(s, 127.0, -static_cast<double>(m)) * 0x1p49);
+  r.m = m * 0x1p-4f;
+  r.down = d > 0.f;
+  r.d53 = fabsf(d);
+  r.mode = 2.f * r.d53 <= r.m ? kTieEven : r.d53 <= r.m ? kTieMixed : r.down ? kTieDown : kTieUp;
+  return r;
+}
+// lo, hi: four codes on the sides of their ties towards 0 and away from it.
+__device__ __forceinline__ uint32_t even4(uint32_t lo, uint32_t hi) {
+  const uint32_t odd = (hi & 0x01010101u) * 255u;
+  return (lo & odd) | (hi & ~odd);
+}
+__device__ __forceinline__ uint32_t mixed4(const TieRule& r, uint32_t lo, uint32_t hi) {
+  uint32_t c = even4(lo, hi);
+  for (uint32_t diff = lo ^ hi; diff != 0;) {
+    const int shift = (__ffs(diff) - 1) & 24;
+    const uint32_t byte = 255u << shift;
+    diff &= ~byte;
+    const float t = fabsf(static_cast<float>(static_cast<int8_t>(lo >> shift))) + 0.5f;
+    // 1 to 2; below t = 1/2 numbers are twice as dense
+    const float mantissa = t == 0.5f && r.down ? 2.f : __uint_as_float((__float_as_uint(t) & 0x7fffffu) | 0x3f800000u);
+    const float part = mantissa * r.d53;
+    if (part > r.m || (part == r.m && !r.down)) c = (c & ~byte) | ((r.down ? lo : hi) & byte);
+  }
+  return c;
+}
+// 32-bit values may be near a tie without being on it: where the two codes differ, 64 bits decide.
+__device__ __forceinline__ uint32_t near4(double s, uint32_t lo, uint32_t hi, float2 a, float2 b) {
+  const float v[4] = {a.x, a.y, b.x, b.y};
+  uint32_t c = lo;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) c[i] = inv != 0.f ? codes4(v.v[2 * i], v.v[2 * i + 1], k) : 0u;
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t byte = 255u << (8 * j);
+    if (((lo ^ hi) & byte) == 0) continue;
+    const int q = static_cast<int>(fmin(fmax(rint(v[j] / s), -127.0), 127.0));
+    c = (c & ~byte) | ((static_cast<uint32_t>(q) << (8 * j)) & byte);
+  }
+  return c;
+}
+// The codes of 4 N given values, as 64-bit arithmetic has them; v: pairs.
+template <class XT, int N>
+__device__ __forceinline__ void given_codes(const float2* v, float m, float inv, uint32_t (&c)[N]) {
+  const float2 down = dup2(inv * (1.f - 0x1p-21f)), up = dup2(inv * (1.f + 0x1p-21f));
+  uint32_t hi[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    c[i] = codes4(v[2 * i], v[2 * i + 1], down);
+    hi[i] = codes4(v[2 * i], v[2 * i + 1], up);
+  }
+  if constexpr (sizeof(XT) == 4) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (c[i] != hi[i]) c[i] = near4(scale64(m), c[i], hi[i], v[2 * i], v[2 * i + 1]);
+  } else {
+    const TieRule r = tie_rule(m);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (r.mode == kTieMixed && c[i] != hi[i]) c[i] = mixed4(r, c[i], hi[i]);
+      else if (r.mode != kTieDown) c[i] = r.mode == kTieUp ? hi[i] : even4(c[i], hi[i]);
+    }
+  }
+}
+
+template <class XT, int LAY>
+__device__ __forceinline__ void store_codes(int8_t* row, int cols, const Row16& v, float m, float inv, bool given) {
+  uint32_t c[4] = {0, 0, 0, 0};
+  if (inv != 0.f && given) {
+    given_codes<XT>(v.v, m, inv, c);
+  } else if (inv != 0.f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] = codes4(v.v[2 * i], v.v[2 * i + 1], dup2(inv));
+  }
   if constexpr (is_vec(LAY)) {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -92,7 +187,7 @@ __device__ __forceinline__ void store_codes(int8_t* row, int cols, const Row16& 
 
 // One row in the registers of a group of warps, N times 16 elements per thread (N = 2: the second
 // 16 are those of the row's second half of threads x 16 columns).  Few rows: bound by latency (80 x 2048
-// with the activation 2.0 us).
+// with the activation 1.9 us).
 template <class XT, int LAY, int N>
 __global__ void __launch_bounds__(N == 1 ? 512 : 1024, 1) quant_kernel(QuantArgs a) {
   __shared__ float buf[8 * 32];
@@ -121,12 +216,14 @@ __global__ void __launch_bounds__(N == 1 ? 512 : 1024, 1) quant_kernel(QuantArgs
 #pragma unroll
   for (int n = 0; n < N; ++n) {
     const int at = n * 16 * blockDim.x;
-    if (at < a.cols) store_codes<LAY>(a.q + row * a.q_ld + at, a.cols - at, v[n], inv);
+    if (at < a.cols) store_codes<XT, LAY>(a.q + row * a.q_ld + at, a.cols - at, v[n], m, inv, !a.swiglu);
   }
 }
 
 // Many aligned rows: persistent CTAs with their next rows on the way to shared memory, as the norm's.
-// Bound by HBM: 8192 x 7168 from bf16 30.8 us (5.7 TB/s); with the activation, 8192 x 2048, 16.6 us (5.1).
+// 8192 x 7168 from bf16 39.7 us (4.4 TB/s): 280 instructions per warp and row, a third of them for the
+// ties (without which 30.8, but for 16-bit values on the tie of their scale the codes are then chance);
+// with the activation, 8192 x 2048, 15.8 us (5.3 TB/s), bound by HBM.
 template <class XT, int LAY>
 __global__ void __launch_bounds__(512, 2) quant_ring_kernel(QuantArgs a, RingPlan g) {
   extern __shared__ __align__(128) uint8_t ring[];
@@ -173,7 +270,7 @@ __global__ void __launch_bounds__(512, 2) quant_ring_kernel(QuantArgs a, RingPla
     float inv;
     const float sc = quant_scale(m, &inv);
     if (threadIdx.x == 0) a.scale[row] = sc;
-    store_codes<LAY>(a.q + row * a.q_ld, cols, v, inv);
+    store_codes<XT, LAY>(a.q + row * a.q_ld, cols, v, m, inv, !a.swiglu);
   }
   if (!ok && threadIdx.x == 0)   // given up: the loads in flight land first
     for (int i = 0; i < g.stages; ++i) {
@@ -187,7 +284,7 @@ __global__ void __launch_bounds__(512, 2) quant_ring_kernel(QuantArgs a, RingPla
 // The whole layer in one launch: every CTA quantises the tokens for itself into shared memory (they
 // come from L2; 14 KB each at 7168), then each warp takes whole weight rows, 4 KB of them in
 // flight, and adds up four products per instruction (dp4a).  The weights cross HBM once; the warps
-// per SM are chosen so that the rows come out even.  One token 7168 -> 4096 from bf16: 5.1 us, 5.7
+// per SM are chosen so that the rows come out even.  One token 7168 -> 4096 from bf16: 5.6 us, 5.2
 // TB/s (the streaming kernel and its quantisation: 9.2).  From three tokens on the products take
 // longer than the weights: 11 us against 9.2.
 constexpr int kGemvMaxT = 2;
@@ -253,16 +350,13 @@ __global__ void __launch_bounds__(1024, 1) int8_gemv_kernel(GemvArgs a) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) m = max_nan(m, fabsf(v[j]));
         }
-#pragma unroll
-      for (int d = 16; d >= 1; d >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
+      m = warp_amax(m);
       if (lane == 0) s_max[t][warp] = m;
     }
     __syncthreads();
 #pragma unroll
     for (int t = 0; t < TT; ++t) {
-      float m = lane < warps ? s_max[t][lane] : 0.f;
-#pragma unroll
-      for (int d = 16; d >= 1; d >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
+      const float m = warp_amax(lane < warps ? s_max[t][lane] : 0.f);
       float inv;
       const float sc = quant_scale(m, &inv);
       if (threadIdx.x == 0) s_scale[t] = sc;
@@ -272,9 +366,16 @@ __global__ void __launch_bounds__(1024, 1) int8_gemv_kernel(GemvArgs a) {
         if (t < a.T && inv != 0.f) {
           float v[8];
           gemv_load8(a, x + t * a.x_ld, e, v);
-          const float2 k = dup2(inv);
-          c.x = codes4(make_float2(v[0], v[1]), make_float2(v[2], v[3]), k);
-          c.y = codes4(make_float2(v[4], v[5]), make_float2(v[6], v[7]), k);
+          const float2 p[4] = {make_float2(v[0], v[1]), make_float2(v[2], v[3]), make_float2(v[4], v[5]),
+                               make_float2(v[6], v[7])};
+          uint32_t q[2];
+          if (a.swiglu) {
+            q[0] = codes4(p[0], p[1], dup2(inv));
+            q[1] = codes4(p[2], p[3], dup2(inv));
+          } else {
+            given_codes<XT>(p, m, inv, q);
+          }
+          c = make_uint2(q[0], q[1]);
         }
         dst[e / 8] = c;
       }
@@ -331,7 +432,7 @@ cudaError_t quant_launch(const QuantArgs& q0, int sms, cudaStream_t st) {
   auto go = [&](auto t) {
     using XT = decltype(t);
     // The ring: aligned rows of two warps or more, at least four per SM (7168 columns, ring against
-    // direct: 148 rows 1.9 us against 1.8, 592 rows 3.2 against 3.3, 8192 rows 30.8 against 51.5).
+    // direct: 148 rows 1.9 us against 1.8, 592 rows 3.2 against 3.3, 8192 rows 30.8 against 51.5, before the rule for ties).
     RingPlan g{};
     ring_add(&g, q.x, q.x_ld, q.cols, q.type);
     if (q.swiglu) ring_add(&g, static_cast<const XT*>(q.x) + q.cols, q.x_ld, q.cols, q.type);

@@ -321,7 +321,8 @@ def select_experts_backward(dw: torch.Tensor, logits: torch.Tensor, idx: torch.T
 def quantize_int8(x: torch.Tensor, *, swiglu: bool = False):
     """8-bit codes and scales of the rows of ``x``: (int8 [rows, cols], float32 [rows]) with
     scale = max(amax / 127, 2**-126).  With ``swiglu``, of silu(x[:, cols:]) * x[:, :cols] (the
-    expert layer's order of the two halves).  For weights [out, in] the rows are the channels."""
+    expert layer's order of the two halves).  For weights [out, in] the rows are the channels.
+    Without ``swiglu`` the codes are those of 64-bit arithmetic with amax * (1 / 127) for a scale."""
     ld = _rows(x, "x")
     dev = x.get_device()
     rows, cols = x.shape

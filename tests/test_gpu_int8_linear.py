@@ -191,3 +191,47 @@ def test_refusals():
     for f in bad:
         with pytest.raises(M.MoEArgumentError):
             f()
+
+
+def exact_codes(x):
+    """Codes and scales in 64 bits."""
+    v = x.double()
+    scale = torch.clamp(v.abs().amax(dim=1) * (1.0 / 127.0), min=2.0 ** -126)
+    return torch.round(v / scale[:, None]), scale
+
+
+@pytest.mark.parametrize("dtype", [BF, FP, F32])
+@pytest.mark.parametrize("T,K", [(3000, 2048), (700, 7168), (40, 20000), (900, 1001), (5000, 40), (30, 8192)])
+def test_codes_are_those_of_64_bits(T, K, dtype):
+    """Millions of codes, thousands of ties among them, without one on the other side."""
+    g = torch.Generator(device="cuda").manual_seed(T + K)
+    x = (torch.randn(T, K, generator=g, device="cuda") * 3).to(dtype)
+    q, s = M.quantize_int8(x)
+    ref, scale = exact_codes(x)
+    assert torch.equal(q.double(), ref)
+    assert ((s.double() - scale).abs() <= 2.0 ** -23 * scale).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("size", [6e37, 1e-36, 3e-39])
+def test_codes_of_large_and_small_values(dtype, size):
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = (torch.randn(500, 1024, generator=g, device="cuda").clamp(-4, 4) * size).to(dtype)
+    q, s = M.quantize_int8(x)
+    ref, scale = exact_codes(x)
+    assert torch.equal(q.double(), ref)
+    assert ((s.double() - scale).abs() <= 2.0 ** -23 * scale).all()
+
+
+@pytest.mark.parametrize("T", [1, 2])
+@pytest.mark.parametrize("dtype", [BF, FP, F32])
+def test_few_tokens_codes_are_those_of_64_bits(T, dtype):
+    """One or two tokens are quantised inside the product: an identity for weights returns their codes."""
+    K = 2048
+    w, one = torch.eye(K, dtype=torch.int8, device="cuda"), torch.ones(K, device="cuda")
+    for seed in range(40):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        x = (torch.randn(T, K, generator=g, device="cuda") * 3).to(dtype)
+        y = M.int8_linear(x, w, one, out_dtype=F32)
+        ref, scale = exact_codes(x)
+        assert torch.equal(torch.round(y.double() / scale[:, None]), ref)

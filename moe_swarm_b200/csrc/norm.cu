@@ -342,6 +342,8 @@ MOE_B200_API int moe_b200_block_norm(const moe_b200_norm_args* a, void* stream) 
       constexpr int MAXT = decltype(t)::value;
       return packed                          ? norm_fwd_kernel<YT, RT, kPacked, 512>
              : vec                           ? norm_fwd_kernel<YT, RT, kVec, MAXT>
+             : a->cols <= 128           ? norm_fwd_kernel<YT, RT, kShort, 512>
+             : a->cols <= 256           ? norm_fwd_kernel<YT, RT, kThin, 512>
              : a->cols >= 384 * n.warps ? norm_fwd_kernel<YT, RT, kTail, MAXT>
                                         : norm_fwd_kernel<YT, RT, kScattered, MAXT>;
     };

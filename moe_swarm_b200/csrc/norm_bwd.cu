@@ -137,7 +137,7 @@ __device__ __forceinline__ void bwd_row(const NormBwdArgs& a, int row, int cols,
     if constexpr (LAY == kPacked) packed_sum(t);
     else row_sum(t, a.warps, buf1);
     done();
-    if (gate == 1 && threadIdx.x == 0 && (LAY != kPacked || cols > 0)) static_cast<float*>(a.dgate)[row] = a.scale * ystd * t[0];
+    if (gate == 1 && threadIdx.x == 0 && cols > 0) static_cast<float*>(a.dgate)[row] = a.scale * ystd * t[0];
     if (post) k = -t[0] * inv_cols * ystd * ystd;
   } else {
     done();
@@ -188,16 +188,18 @@ __device__ __forceinline__ void bwd_direct(const NormBwdArgs& a, float (*buf)[3 
   // a row without a second sum alternates the first one's buffer by itself
   const bool two = a.y && (a.post_w || a.gate_grad == kGateRow);
   int first = 0;
-  const int many = LAY == kPacked ? blockDim.y : 1;
+  constexpr bool kMany = LAY == kPacked || LAY == kShort || LAY == kThin;
+  const int many = kMany ? blockDim.y : 1;
   for (int row0 = blockIdx.x * many; row0 < a.rows; row0 += gridDim.x * many) {
-    const int row = LAY == kPacked ? row0 + threadIdx.y : row0, cols = row < a.rows ? a.cols : 0;
+    const int row = kMany ? row0 + threadIdx.y : row0, cols = row < a.rows ? a.cols : 0;
+    const int from = min(row, a.rows - 1);   // a row that exists
     const float g_row = a.gate_grad == kGateRow && cols ? load1_dyn(a.gate, a.gate_type, row * a.g_ld) : 0.f;
     bwd_row<YT, RT, LAY, -1, -1>(a, row, cols, 1.f / a.cols, buf[first], buf[1], sum, g_row, [&](int which, Row16& v) {
-      if (which == 0) load_row<YT, LAY>(static_cast<const YT*>(a.dx) + row * a.dx_ld, cols, v);
-      else if (which == 1) load_row<RT, LAY>(static_cast<const RT*>(a.r) + row * a.r_ld, cols, v);
-      else if (which == 2) load_row<YT, LAY>(static_cast<const YT*>(a.y) + row * a.y_ld, cols, v);
-      else if (which == 3) load_row<RT, LAY>(static_cast<const RT*>(a.dr) + row * a.dr_ld, cols, v);
-      else if (which == 4) load_row_dyn<LAY>(a.gate, a.gate_type, row * a.g_ld, cols, v);
+      if (which == 0) load_row<YT, LAY>(static_cast<const YT*>(a.dx) + from * a.dx_ld, cols, v);
+      else if (which == 1) load_row<RT, LAY>(static_cast<const RT*>(a.r) + from * a.r_ld, cols, v);
+      else if (which == 2) load_row<YT, LAY>(static_cast<const YT*>(a.y) + from * a.y_ld, cols, v);
+      else if (which == 3) load_row<RT, LAY>(static_cast<const RT*>(a.dr) + from * a.dr_ld, cols, v);
+      else if (which == 4) load_row_dyn<LAY>(a.gate, a.gate_type, from * a.g_ld, cols, v);
       else if (which == 5) factor_w<LAY>(a, v);
       else factor_b<LAY>(a, v);
     }, [] {});
@@ -381,7 +383,7 @@ namespace {
 struct NormBwdShape {
   int warps, direct_parts, ring_ctas, ring_rows, ring_parts;   // ring_rows: rows side by side in a CTA
   int lanes, packed_rows, packed_parts;
-  int thin_warps, thin_parts;   // 0: too long
+  int thin_warps, thin_rows, thin_parts;   // 0: too long
 };
 NormBwdShape bwd_shape(int rows, int cols) {
   NormBwdShape s{};
@@ -409,8 +411,15 @@ NormBwdShape bwd_shape(int rows, int cols) {
   s.packed_parts = need < 148 ? need : 148;
   if (cols <= 32 * 256) {   // 1024 threads of an SM, eight elements each
     s.thin_warps = (cols + 255) / 256;
-    const int ctas = 148 * (32 / s.thin_warps);
-    s.thin_parts = rows < ctas ? rows : ctas;
+    s.thin_rows = 1;
+    int ctas = 148 * (32 / s.thin_warps);
+    if (s.thin_warps == 1) {   // one warp each, side by side
+      const int each = (rows + 147) / 148;
+      s.thin_rows = each < 32 ? each : 32;
+      ctas = 148;
+    }
+    const int wanted = (rows + s.thin_rows - 1) / s.thin_rows;
+    s.thin_parts = wanted < ctas ? wanted : ctas;
   }
   return s;
 }
@@ -565,12 +574,14 @@ MOE_B200_API int moe_b200_block_norm_backward(const moe_b200_norm_backward_args*
     } else {
       if (thin) n.warps = shape.thin_warps;
       auto kernel = packed          ? norm_bwd_kernel<YT, RT, kPacked, 512>
-                    : thin          ? norm_bwd_kernel<YT, RT, kThin, 1024>
+                    : thin          ? (a->cols <= 128 ? norm_bwd_kernel<YT, RT, kShort, 1024>
+                                                      : norm_bwd_kernel<YT, RT, kThin, 1024>)
                     : !vec          ? norm_bwd_kernel<YT, RT, kTail, 1024>
                     : n.warps <= 16 ? norm_bwd_kernel<YT, RT, kVec, 512>
                                     : norm_bwd_kernel<YT, RT, kVec, 1024>;
-      const dim3 block(packed ? shape.lanes : n.warps * 32, packed ? shape.packed_rows : 1);
-      e = launch_pdl(kernel, dim3(n.parts), block, packed ? sizeof(float) * shape.packed_rows * a->cols : 0, st, n);
+      const int side = packed ? shape.packed_rows : thin ? shape.thin_rows : 1;   // rows of a CTA
+      const dim3 block(packed ? shape.lanes : n.warps * 32, side);
+      e = launch_pdl(kernel, dim3(n.parts), block, side > 1 ? sizeof(float) * side * a->cols : 0, st, n);
     }
   });
   if (e != cudaSuccess) return report_cuda(e, "block_norm_backward launch");

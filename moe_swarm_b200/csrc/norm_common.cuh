@@ -53,11 +53,12 @@ __device__ __forceinline__ float2 dup2(float a) { return make_float2(a, a); }
 // kScattered: 128-column blocks by warp, lane + 32 m within one, so that the accesses of a warp are
 // neighbours whatever the row's alignment.  kTail: the same, where only the last four elements of a
 // thread may be missing (rows of at least 384 x their warps, so all of more than 1536 columns).
-// kThin: the same with eight elements to a thread.
+// kThin, kShort: the same with eight and four elements to a thread.
 // In each of these a 128-column block belongs to a half warp (eight elements each) or to a warp (four
 // each).  kPacked: as kVec, several rows to a warp: blockDim.x, a power of two below 32, threads each.
-enum : int { kThin = -1, kScattered = 0, kTail = 1, kVec = 2, kHalf = 3, kFull = 4, kPacked = 5 };
+enum : int { kShort = -2, kThin = -1, kScattered = 0, kTail = 1, kVec = 2, kHalf = 3, kFull = 4, kPacked = 5 };
 constexpr bool is_vec(int lay) { return lay >= kVec; }
+constexpr int slots(int lay) { return lay == kShort ? 4 : lay == kThin ? 8 : 16; }
 
 // The column of this thread's element q.
 template <int LAY>
@@ -68,7 +69,7 @@ __device__ __forceinline__ int col_of(int q) {
 }
 template <int LAY>
 __device__ __forceinline__ bool exists(int q, int cols) {
-  if (LAY == kThin && q >= 8) return false;
+  if (q >= slots(LAY)) return false;
   return LAY == kFull || (LAY == kHalf && q < 8) || (LAY == kTail && q < 12) || col_of<LAY>(q) < cols;
 }
 
@@ -115,7 +116,7 @@ __device__ __forceinline__ void load_row(const T* row, int cols, Row16& r) {
 #pragma unroll
     for (int q = 0; q < 16; ++q) {
       const bool ok = exists<LAY>(q, cols);
-      if (LAY == kTail || (LAY == kThin && q >= 8)) {
+      if (LAY == kTail || q >= slots(LAY)) {
         r[q] = ok ? to_f(row[col_of<LAY>(q)]) : 0.f;
       } else {
         const float f = to_f(row[ok ? col_of<LAY>(q) : 0]);
@@ -192,7 +193,7 @@ template <int LAY>
 __device__ __forceinline__ float dot16(const Row16& a, const Row16& b) {
   float2 s = mul2(a.v[0], b.v[0]);
 #pragma unroll
-  for (int i = 1; i < (LAY == kThin ? 4 : 8); ++i) s = fma2(a.v[i], b.v[i], s);
+  for (int i = 1; i < slots(LAY) / 2; ++i) s = fma2(a.v[i], b.v[i], s);
   return s.x + s.y;
 }
 

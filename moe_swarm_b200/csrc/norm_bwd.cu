@@ -15,6 +15,7 @@
 
 namespace moe {
 
+constexpr int kBwdSide = 8;   // rows of several warps side by side in a CTA
 constexpr int kFactorBytes = 2 * kNormPerThread * 4;   // per thread of a row
 enum : int { kGateNone = 0, kGateColumn = 1, kGateRow = 2, kGateElement = 3 };
 
@@ -173,29 +174,60 @@ __device__ __forceinline__ void bwd_store_sums(const NormBwdArgs& a, const NormB
   if (a.post_slot >= 0) put(dst + a.post_slot * slot, sum.post);
 }
 
-// Any alignment, any set of tensors: rows straight from global memory, one per CTA at a time.
-// kPacked: blockDim.y of them; those beyond the last run with no elements (65536 x 128: 40 us, 2.5
-// TB/s, against 98 with a warp per row).  kThin: rows on odd boundaries, whose 2-byte loads, stores and
-// checks make many instructions; eight elements a thread let twice the warps share them (4096 x 5001
-// with a 32-bit residual: 206 us against 304 with sixteen; 5000 x 700 35 against 49).  What bounds it is still
-// that chain of instructions, not memory: bulk copies of the rows ahead (their ends by plain
-// loads) left 901 x 5001 at 55 us against 53, prefetching them to L2 at 52.
+// Any alignment, any set of tensors: rows straight from global memory, one per CTA at a time, or
+// blockDim.y side by side, of which those beyond the last run with no elements.
+// kPacked: 65536 x 128 40 us (2.5 TB/s) against 98 with a warp per row.
+// kShort, kThin: rows on odd boundaries, whose 2-byte loads, stores and checks make many instructions.  Four
+// elements a thread (eight beyond 4096 columns) let two to four times the warps share them, and the factors
+// per column are put into shared memory once: 16384 x 301 44.6 us against 65 with eight and factors
+// in place, 16384 x 99 14.8 against 41 with all sixteen, 4096 x 5001 with a 32-bit residual 193 against
+// 304.  What bounds it is still that chain of instructions, not memory: bulk copies of the rows
+// ahead (their ends by plain loads) left 901 x 5001 at 55 us against 53, prefetching them to L2 at 52.
 template <class YT, class RT, int LAY>
-__device__ __forceinline__ void bwd_direct(const NormBwdArgs& a, float (*buf)[3 * 32], float* shared) {
+__device__ __forceinline__ void bwd_direct(const NormBwdArgs& a, float (*buf)[kBwdSide * 3 * 32], float4* shared) {
+  constexpr bool kMany = LAY == kPacked || LAY == kShort || LAY == kThin, kFactors = LAY == kShort || LAY == kThin;
+  constexpr int kQuads = slots(LAY) / 4;
+  float4* sums_of_rows = shared;
+  if constexpr (kFactors) {   // w and b as this thread reads them
+    sums_of_rows += 2 * kQuads * blockDim.x;
+    if (threadIdx.y == 0) {
+      Row16 f;
+      auto put = [&](int at) {
+#pragma unroll
+        for (int i = 0; i < kQuads; ++i)
+          shared[(at + i) * blockDim.x + threadIdx.x] = make_float4(f.v[2 * i].x, f.v[2 * i].y, f.v[2 * i + 1].x, f.v[2 * i + 1].y);
+      };
+      if (a.dx) {
+        factor_w<LAY>(a, f);
+        put(0);
+      }
+      if (a.y) {
+        factor_b<LAY>(a, f);
+        put(kQuads);
+      }
+    }
+    if (blockDim.y > 1) __syncthreads();   // (a row's threads read what they wrote themselves)
+  }
   NormBwdSums sum;
 #pragma unroll
   for (int i = 0; i < 8; ++i) sum.pre.v[i] = sum.post.v[i] = dup2(0.f);
   // a row without a second sum alternates the first one's buffer by itself
   const bool two = a.y && (a.post_w || a.gate_grad == kGateRow);
   int first = 0;
-  constexpr bool kMany = LAY == kPacked || LAY == kShort || LAY == kThin;
   const int many = kMany ? blockDim.y : 1;
   for (int row0 = blockIdx.x * many; row0 < a.rows; row0 += gridDim.x * many) {
-    const int row = kMany ? row0 + threadIdx.y : row0, cols = row < a.rows ? a.cols : 0;
-    const int from = min(row, a.rows - 1);   // a row that exists
+    const int row = kMany ? row0 + threadIdx.y : row0, cols = kMany && row >= a.rows ? 0 : a.cols;
+    const int from = kMany ? min(row, a.rows - 1) : row;   // a row that exists
     const float g_row = a.gate_grad == kGateRow && cols ? load1_dyn(a.gate, a.gate_type, row * a.g_ld) : 0.f;
     bwd_row<YT, RT, LAY, -1, -1>(a, row, cols, 1.f / a.cols, buf[first], buf[1], sum, g_row, [&](int which, Row16& v) {
-      if (which == 0) load_row<YT, LAY>(static_cast<const YT*>(a.dx) + from * a.dx_ld, cols, v);
+      if (kFactors && which >= 5) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float4 f = i < kQuads ? shared[((which - 5) * kQuads + i) * blockDim.x + threadIdx.x] : make_float4(0.f, 0.f, 0.f, 0.f);
+          v.v[2 * i] = make_float2(f.x, f.y);
+          v.v[2 * i + 1] = make_float2(f.z, f.w);
+        }
+      } else if (which == 0) load_row<YT, LAY>(static_cast<const YT*>(a.dx) + from * a.dx_ld, cols, v);
       else if (which == 1) load_row<RT, LAY>(static_cast<const RT*>(a.r) + from * a.r_ld, cols, v);
       else if (which == 2) load_row<YT, LAY>(static_cast<const YT*>(a.y) + from * a.y_ld, cols, v);
       else if (which == 3) load_row<RT, LAY>(static_cast<const RT*>(a.dr) + from * a.dr_ld, cols, v);
@@ -205,16 +237,16 @@ __device__ __forceinline__ void bwd_direct(const NormBwdArgs& a, float (*buf)[3 
     }, [] {});
     if (!two) first ^= 1;
   }
-  bwd_store_sums<LAY>(a, sum, shared);
+  bwd_store_sums<LAY>(a, sum, reinterpret_cast<float*>(sums_of_rows));
 }
 
 template <class YT, class RT, int LAY, int MAXT>
 __global__ void __launch_bounds__(MAXT, 1) norm_bwd_kernel(NormBwdArgs a) {
-  extern __shared__ __align__(16) float packed_sums[];
-  __shared__ float buf[2][3 * 32];
+  extern __shared__ float4 shared[];   // factors per column, sums of rows side by side
+  __shared__ float buf[2][kBwdSide * 3 * 32];
   pdl_wait();
   pdl_launch_dependents();
-  bwd_direct<YT, RT, LAY>(a, buf, packed_sums);
+  bwd_direct<YT, RT, LAY>(a, buf, shared);
 }
 
 // Aligned rows with all of dx, r', y: the next rows (dx, r', y, dr, gate per element) are on their
@@ -409,15 +441,13 @@ NormBwdShape bwd_shape(int rows, int cols) {
   s.packed_rows = even < 16 * of_warp ? even : 16 * of_warp;
   const int need = (rows + s.packed_rows - 1) / s.packed_rows;
   s.packed_parts = need < 148 ? need : 148;
-  if (cols <= 32 * 256) {   // 1024 threads of an SM, eight elements each
-    s.thin_warps = (cols + 255) / 256;
-    s.thin_rows = 1;
-    int ctas = 148 * (32 / s.thin_warps);
-    if (s.thin_warps == 1) {   // one warp each, side by side
-      const int each = (rows + 147) / 148;
-      s.thin_rows = each < 32 ? each : 32;
-      ctas = 148;
-    }
+  if (cols <= 32 * 256) {   // 1024 threads of an SM, four or eight elements each
+    s.thin_warps = cols <= 32 * 128 ? (cols + 127) / 128 : (cols + 255) / 256;
+    // rows of one warp need no barrier, 32 of them make a CTA; 16 warps of longer ones
+    const int side = s.thin_warps == 1 ? 32 : s.thin_warps <= 8 ? 16 / s.thin_warps : 1;
+    const int per_sm = 32 / (side * s.thin_warps), each = (rows + 148 * per_sm - 1) / (148 * per_sm);
+    s.thin_rows = each < side ? each : side;
+    const int ctas = 148 * per_sm;
     const int wanted = (rows + s.thin_rows - 1) / s.thin_rows;
     s.thin_parts = wanted < ctas ? wanted : ctas;
   }
@@ -574,14 +604,18 @@ MOE_B200_API int moe_b200_block_norm_backward(const moe_b200_norm_backward_args*
     } else {
       if (thin) n.warps = shape.thin_warps;
       auto kernel = packed          ? norm_bwd_kernel<YT, RT, kPacked, 512>
-                    : thin          ? (a->cols <= 128 ? norm_bwd_kernel<YT, RT, kShort, 1024>
+                    : thin          ? (a->cols <= 32 * 128 ? norm_bwd_kernel<YT, RT, kShort, 1024>
                                                       : norm_bwd_kernel<YT, RT, kThin, 1024>)
                     : !vec          ? norm_bwd_kernel<YT, RT, kTail, 1024>
                     : n.warps <= 16 ? norm_bwd_kernel<YT, RT, kVec, 512>
                                     : norm_bwd_kernel<YT, RT, kVec, 1024>;
       const int side = packed ? shape.packed_rows : thin ? shape.thin_rows : 1;   // rows of a CTA
       const dim3 block(packed ? shape.lanes : n.warps * 32, side);
-      e = launch_pdl(kernel, dim3(n.parts), block, side > 1 ? sizeof(float) * side * a->cols : 0, st, n);
+      const int quads = !thin ? 0 : a->cols <= 32 * 128 ? 2 : 4;   // factors of a thread
+      const size_t smem = sizeof(float4) * quads * block.x + (side > 1 ? sizeof(float) * side * a->cols : 0);
+      if (smem > 48 * 1024)
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem);
+      if (e == cudaSuccess) e = launch_pdl(kernel, dim3(n.parts), block, smem, st, n);
     }
   });
   if (e != cudaSuccess) return report_cuda(e, "block_norm_backward launch");

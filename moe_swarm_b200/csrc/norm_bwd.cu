@@ -185,29 +185,27 @@ __device__ __forceinline__ void bwd_store_sums(const NormBwdArgs& a, const NormB
 // ahead (their ends by plain loads) left 901 x 5001 at 55 us against 53, prefetching them to L2 at 52.
 template <class YT, class RT, int LAY>
 __device__ __forceinline__ void bwd_direct(const NormBwdArgs& a, float (*buf)[kBwdSide * 3 * 32], float4* shared) {
-  constexpr bool kMany = LAY == kPacked || LAY == kShort || LAY == kThin, kFactors = LAY == kShort || LAY == kThin;
+  constexpr bool kMany = LAY == kPacked || LAY == kShort || LAY == kThin;
   constexpr int kQuads = slots(LAY) / 4;
-  float4* sums_of_rows = shared;
-  if constexpr (kFactors) {   // w and b as this thread reads them
-    sums_of_rows += 2 * kQuads * blockDim.x;
-    if (threadIdx.y == 0) {
-      Row16 f;
-      auto put = [&](int at) {
+  // w and b as this thread reads them, then the sums of rows side by side
+  float4* sums_of_rows = shared + 2 * kQuads * blockDim.x;
+  if (threadIdx.y == 0) {
+    Row16 f;
+    auto put = [&](int at) {
 #pragma unroll
-        for (int i = 0; i < kQuads; ++i)
-          shared[(at + i) * blockDim.x + threadIdx.x] = make_float4(f.v[2 * i].x, f.v[2 * i].y, f.v[2 * i + 1].x, f.v[2 * i + 1].y);
-      };
-      if (a.dx) {
-        factor_w<LAY>(a, f);
-        put(0);
-      }
-      if (a.y) {
-        factor_b<LAY>(a, f);
-        put(kQuads);
-      }
+      for (int i = 0; i < kQuads; ++i)
+        shared[(at + i) * blockDim.x + threadIdx.x] = make_float4(f.v[2 * i].x, f.v[2 * i].y, f.v[2 * i + 1].x, f.v[2 * i + 1].y);
+    };
+    if (a.dx) {
+      factor_w<LAY>(a, f);
+      put(0);
     }
-    if (blockDim.y > 1) __syncthreads();   // (a row's threads read what they wrote themselves)
+    if (a.y) {
+      factor_b<LAY>(a, f);
+      put(kQuads);
+    }
   }
+  if (blockDim.y > 1) __syncthreads();   // (a row's threads read what they wrote themselves)
   NormBwdSums sum;
 #pragma unroll
   for (int i = 0; i < 8; ++i) sum.pre.v[i] = sum.post.v[i] = dup2(0.f);
@@ -220,7 +218,7 @@ __device__ __forceinline__ void bwd_direct(const NormBwdArgs& a, float (*buf)[kB
     const int from = kMany ? min(row, a.rows - 1) : row;   // a row that exists
     const float g_row = a.gate_grad == kGateRow && cols ? load1_dyn(a.gate, a.gate_type, row * a.g_ld) : 0.f;
     bwd_row<YT, RT, LAY, -1, -1>(a, row, cols, 1.f / a.cols, buf[first], buf[1], sum, g_row, [&](int which, Row16& v) {
-      if (kFactors && which >= 5) {
+      if (which >= 5) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float4 f = i < kQuads ? shared[((which - 5) * kQuads + i) * blockDim.x + threadIdx.x] : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -231,9 +229,7 @@ __device__ __forceinline__ void bwd_direct(const NormBwdArgs& a, float (*buf)[kB
       else if (which == 1) load_row<RT, LAY>(static_cast<const RT*>(a.r) + from * a.r_ld, cols, v);
       else if (which == 2) load_row<YT, LAY>(static_cast<const YT*>(a.y) + from * a.y_ld, cols, v);
       else if (which == 3) load_row<RT, LAY>(static_cast<const RT*>(a.dr) + from * a.dr_ld, cols, v);
-      else if (which == 4) load_row_dyn<LAY>(a.gate, a.gate_type, from * a.g_ld, cols, v);
-      else if (which == 5) factor_w<LAY>(a, v);
-      else factor_b<LAY>(a, v);
+      else load_row_dyn<LAY>(a.gate, a.gate_type, from * a.g_ld, cols, v);
     }, [] {});
     if (!two) first ^= 1;
   }
@@ -611,7 +607,7 @@ MOE_B200_API int moe_b200_block_norm_backward(const moe_b200_norm_backward_args*
                                     : norm_bwd_kernel<YT, RT, kVec, 1024>;
       const int side = packed ? shape.packed_rows : thin ? shape.thin_rows : 1;   // rows of a CTA
       const dim3 block(packed ? shape.lanes : n.warps * 32, side);
-      const int quads = !thin ? 0 : a->cols <= 32 * 128 ? 2 : 4;   // factors of a thread
+      const int quads = !thin ? 8 : a->cols <= 32 * 128 ? 2 : 4;   // factors of a thread
       const size_t smem = sizeof(float4) * quads * block.x + (side > 1 ? sizeof(float) * side * a->cols : 0);
       if (smem > 48 * 1024)
         e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem);

@@ -17,6 +17,7 @@ namespace moe {
 
 constexpr int kBwdSide = 8;   // rows of several warps side by side in a CTA
 constexpr int kFactorBytes = 2 * kNormPerThread * 4;   // per thread of a row
+constexpr int kNoBlock = 3;
 enum : int { kGateNone = 0, kGateColumn = 1, kGateRow = 2, kGateElement = 3 };
 
 struct NormBwdArgs {
@@ -57,13 +58,13 @@ __device__ __forceinline__ void factor_b(const NormBwdArgs& a, Row16& b) {
 
 // One row.  load(which, v): which = 0 dx, 1 r', 2 y, 3 dr, 4 the gate per element, 5 w, 6 b; done()
 // is called when everything is loaded.  POST, GATE (0 none or per column, 1 per row, 2 per
-// element): -1 = known at run time only.
+// element, kNoBlock: there is no y): -1 = known at run time only.
 template <class YT, class RT, int LAY, int POST, int GATE, class Load, class Done>
 __device__ __forceinline__ void bwd_row(const NormBwdArgs& a, int row, int cols, float inv_cols, float* buf0, float* buf1,
                                         NormBwdSums& sum, float g_of_row, Load&& load, Done&& done) {
   const bool post = POST < 0 ? a.post_w != nullptr : POST == 1;
   const int gate = GATE < 0 ? (a.gate_grad == kGateElement ? 2 : a.gate_grad == kGateRow ? 1 : 0) : GATE;
-  const bool has_dx = GATE < 0 ? a.dx != nullptr : true, has_y = GATE < 0 ? a.y != nullptr : true;
+  const bool has_dx = GATE < 0 ? a.dx != nullptr : true, has_y = GATE < 0 ? a.y != nullptr : GATE != kNoBlock;
   Row16 r, dx, y, G;
   float s[3] = {0.f, 0.f, 0.f};   // sum r'^2, sum w dx r', sum y^2
   if (has_dx) {
@@ -245,7 +246,7 @@ __global__ void __launch_bounds__(MAXT, 1) norm_bwd_kernel(NormBwdArgs a) {
   bwd_direct<YT, RT, LAY>(a, buf, shared);
 }
 
-// Aligned rows with all of dx, r', y: the next rows (dx, r', y, dr, gate per element) are on their
+// Aligned rows with dx and r': the next rows (dx, r', y, dr, gate per element) are on their
 // way to shared memory as bulk copies while a row is computed.  The factors per column are put
 // into shared memory once, 32-bit, as each thread reads them, beside a 16-bit residual; a 32-bit one
 // leaves its ring too little room, and they are read in place.  Rows of one warp go eight to a CTA,
@@ -325,8 +326,8 @@ __global__ void __launch_bounds__(512, 1) norm_bwd_ring_kernel(NormBwdArgs a, Ri
             }
             return;
           }
-          // the ring's order: dx, r', y, dr (if any), gate (if per element)
-          const uint8_t* p = src + g.t[which == 4 && !a.dr ? 3 : which].at;
+          // the ring's order: dx, r', y (if any), dr (if any), gate (if per element)
+          const uint8_t* p = src + g.t[which == 4 && !a.dr ? 3 : which == 3 && GATE == kNoBlock ? 2 : which].at;
           if (which == 0 || which == 2) load_row<YT, LAY>(reinterpret_cast<const YT*>(p), cols, v);
           else if (which != 4) load_row<RT, LAY>(reinterpret_cast<const RT*>(p), cols, v);
           else load_row_dyn<LAY>(p, a.gate_type, 0, cols, v);
@@ -569,9 +570,9 @@ MOE_B200_API int moe_b200_block_norm_backward(const moe_b200_norm_backward_args*
   const int factors = shared_factors(a->residual_type) ? kFactorBytes * n.warps * 32 : 0;
   g.stages = shape.ring_ctas ? (kRingSmem / shape.ring_ctas - factors) / shape.ring_rows / g.stage_bytes : 0;
   if (g.stages > kRingMaxStages) g.stages = kRingMaxStages;
-  // rows of up to 256 columns: several to a warp; odd ones: kThin; the ring takes what has both of dx and y
+  // rows of up to 256 columns: several to a warp; odd ones: kThin; the ring takes the others that have dx
   const bool packed = vec && a->cols <= 256;
-  const bool ring = vec && !packed && a->dx && a->y && g.stages >= 1;
+  const bool ring = vec && !packed && a->dx && g.stages >= 1;
   const bool thin = !vec && shape.thin_warps > 0;
   n.parts = packed ? shape.packed_parts : thin ? shape.thin_parts : ring ? shape.ring_parts : shape.direct_parts;
   // the row sums of a gate that is one number go through the workspace
@@ -589,7 +590,8 @@ MOE_B200_API int moe_b200_block_norm_backward(const moe_b200_norm_backward_args*
                                            : norm_bwd_ring_kernel<YT, RT, L, P, 0>;
       };
       auto of_post = [&](auto lay) {
-        return a->post_weight ? of_gate(lay, std::integral_constant<int, 1>{}) : of_gate(lay, std::integral_constant<int, 0>{});
+        return !a->y            ? norm_bwd_ring_kernel<YT, RT, decltype(lay)::value, 0, kNoBlock>
+               : a->post_weight ? of_gate(lay, std::integral_constant<int, 1>{}) : of_gate(lay, std::integral_constant<int, 0>{});
       };
       auto kernel = a->cols == n.warps * 32 * kNormPerThread ? of_post(std::integral_constant<int, kFull>{})
                                                              : of_post(std::integral_constant<int, kHalf>{});

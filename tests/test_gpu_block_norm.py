@@ -231,6 +231,22 @@ def test_short_rows(T, H, y_dtype, r_dtype, post, gate):
     test_many_rows(T, H, y_dtype, r_dtype, post, gate)
 
 
+@pytest.mark.parametrize("T,H", [(1, 7168), (64, 640), (1500, 512), (700, 2880), (650, 7168), (600, 8192), (40, 12000),
+                                 (300, 96), (700, 1001)])
+@pytest.mark.parametrize("y_dtype,r_dtype", [(BF, BF), (BF, F32), (FP, BF), (F32, F32)])
+def test_backward_of_the_norm_alone(T, H, y_dtype, r_dtype):
+    a = make(T, H, y_dtype, r_dtype, False, None, seed=T + H)
+    g = gen(6)
+    dx = torch.randn(T, H, generator=g, device="cuda").to(y_dtype)
+    dr = torch.randn(T, H, generator=g, device="cuda").to(r_dtype)
+    for d in (dr, None):
+        b = M.block_norm_backward(dx, d, a["residual"], None, pre_weight=a["pre_weight"], weight_offset=0.5)
+        ref = R.block_norm_backward(dx, d, a["residual"], None, pre_weight=a["pre_weight"], off=0.5)
+        assert b.y is None and b.gate is None and b.post_weight is None
+        R.close(b.residual, *ref["residual"])
+        R.close(b.pre_weight, *ref["pre_weight"], steps=3 * R.STEPS + T // 148 + 64)
+
+
 def test_backward_partial_forms():
     a = make(50, 520, BF, BF, True, "token", seed=6)
     g = gen(7)

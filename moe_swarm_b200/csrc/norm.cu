@@ -147,7 +147,9 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) norm_fwd_kernel(NormArgs a)
 // the row's last barrier, when every thread holds its part.  1024 threads of an SM, whose rows in flight
 // are about 200 KB; 4096 x 7168 from bf16 to e4m3 35.3 us (5.8 TB/s, HBM), to bf16 40.6, with both
 // norms and a gate per element 54 (5.4 TB/s).
-template <class YT, class RT, bool POST, int LAY>
+// POST: 0, 1: without and with post_weight; kNoBlock: there is no y.
+constexpr int kNoBlock = 2;
+template <class YT, class RT, int POST, int LAY>
 __global__ void __launch_bounds__(512, 2) norm_ring_kernel(NormArgs a, RingPlan g) {
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ float buf[3][32];   // sums of y^2; of r'^2 of even and odd rows
@@ -177,34 +179,39 @@ __global__ void __launch_bounds__(512, 2) norm_ring_kernel(NormArgs a, RingPlan 
     // after a wait that ran out the CTA still goes through its rows, without their contents
     if (ok) ok = mbar_wait(&full[stage], phase, &abort, &g_op_status, kStWaitProducer);
     uint8_t* src = ring + stage * g.stage_bytes;
-    Row16 r, y, w;
-    load_row<YT, LAY>(reinterpret_cast<const YT*>(src + g.t[0].at), cols, y);
-    if (a.residual) {
-      load_row<RT, LAY>(reinterpret_cast<const RT*>(src + g.t[1].at), cols, r);
+    Row16 r, w;
+    if constexpr (POST == kNoBlock) {
+      load_row<RT, LAY>(reinterpret_cast<const RT*>(src + g.t[0].at), cols, r);
     } else {
+      Row16 y;
+      load_row<YT, LAY>(reinterpret_cast<const YT*>(src + g.t[0].at), cols, y);
+      if (a.residual) {
+        load_row<RT, LAY>(reinterpret_cast<const RT*>(src + g.t[1].at), cols, r);
+      } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) r.v[i] = dup2(0.f);
+        for (int i = 0; i < 8; ++i) r.v[i] = dup2(0.f);
+      }
+      float k = a.scale;
+      if constexpr (POST == 1) {
+        load_weight<LAY>(a.post_w, a.post_type, a.off, cols, w);
+        float ss[1] = {dot16<LAY>(y, y)};
+        row_sum(ss, a.warps, buf[0]);
+        k *= rsqrtf(ss[0] * inv_cols + a.eps);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y.v[i] = mul2(y.v[i], w.v[i]);
+      }
+      if (a.gate && !a.gate_cols) {
+        k *= g_next;   // loaded a row ahead
+        if (row + static_cast<int64_t>(step) < a.rows) g_next = load1_dyn(a.gate, a.gate_type, (row + step) * a.g_ld);
+      } else if (a.gate) {
+        load_row_dyn<LAY>(g_element ? static_cast<const void*>(src + g.t[a.residual ? 2 : 1].at) : a.gate, a.gate_type, 0, cols, w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y.v[i] = mul2(y.v[i], w.v[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) r.v[i] = fma2(dup2(k), y.v[i], r.v[i]);
+      store_row<RT, LAY>(static_cast<RT*>(a.residual_out) + row * a.ro_ld, cols, r);
     }
-    float k = a.scale;
-    if (POST) {
-      load_weight<LAY>(a.post_w, a.post_type, a.off, cols, w);
-      float ss[1] = {dot16<LAY>(y, y)};
-      row_sum(ss, a.warps, buf[0]);
-      k *= rsqrtf(ss[0] * inv_cols + a.eps);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y.v[i] = mul2(y.v[i], w.v[i]);
-    }
-    if (a.gate && !a.gate_cols) {
-      k *= g_next;   // loaded a row ahead
-      if (row + static_cast<int64_t>(step) < a.rows) g_next = load1_dyn(a.gate, a.gate_type, (row + step) * a.g_ld);
-    } else if (a.gate) {
-      load_row_dyn<LAY>(g_element ? static_cast<const void*>(src + g.t[a.residual ? 2 : 1].at) : a.gate, a.gate_type, 0, cols, w);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y.v[i] = mul2(y.v[i], w.v[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) r.v[i] = fma2(dup2(k), y.v[i], r.v[i]);
-    store_row<RT, LAY>(static_cast<RT*>(a.residual_out) + row * a.ro_ld, cols, r);
     float ss[1] = {squares_existing<LAY>(r, cols)};
     if (a.pre_w) load_weight<LAY>(a.pre_w, a.pre_type, a.off, cols, w);
     row_sum(ss, a.warps, buf[1 + parity]);
@@ -297,12 +304,16 @@ MOE_B200_API int moe_b200_block_norm(const moe_b200_norm_args* a, void* stream) 
                                                : rows_aligned(a->x, n.x_ld, a->x_type));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaSuccess;
+  // Rows of up to 256 columns: several to a warp (65536 x 128: 11.7 us, 5.7 TB/s, against 31.5 with
+  // one).  An e4m3 block's maximum wants a half warp.
+  const bool packed = vec && a->cols <= 256 && !(a->pre_weight && a->x_type == MOE_B200_E4M3);
   // The ring: aligned rows of two warps or more, at least four per SM, and two or more of them in
   // a CTA's share of shared memory.  7168 columns, bf16 in, e4m3 out, ring against direct: 592 rows
   // 5.7 us against 6.4, 4096 rows 35.3 (5.8 TB/s) against 51.9; at 148 and 296 rows the ring is 0.1
   // to 0.2 us behind.  Not for a 32-bit residual with nothing but the sum and its norm to compute, whose
   // wide loads keep the memory busy without it: 4096 x 7168 63.9 against 56.4 (6.2 TB/s), 8192 x
   // 4096 72.6 against 61.0; with a gate per token 58.8 against 63.6, with post_weight 66 against 78.
+  // The norm alone of 4096 x 7168 in 16 bits: 24.8 us against 33.7.
   RingPlan g{};
   ring_add(&g, a->y, n.y_ld, a->cols, a->y_type);
   ring_add(&g, a->residual, n.r_ld, a->cols, a->residual_type);
@@ -311,26 +322,25 @@ MOE_B200_API int moe_b200_block_norm(const moe_b200_norm_args* a, void* stream) 
   g.stages = ctas ? kRingSmem / ctas / g.stage_bytes : 0;
   if (g.stages > kRingMaxStages) g.stages = kRingMaxStages;
   const bool sum_alone = a->residual_type == MOE_B200_FP32 && !a->post_weight && !a->gate;
-  if (vec && a->y && a->rows >= 4 * sms && g.stages >= 2 && !sum_alone) {
+  if (vec && !packed && a->rows >= 4 * sms && g.stages >= 2 && !sum_alone) {
     const dim3 grid(a->rows < ctas * sms ? a->rows : ctas * sms), block(n.warps * 32);
     const size_t smem = static_cast<size_t>(g.stages) * g.stage_bytes;
     dispatch_types(a->y_type, a->residual_type, [&](auto yt, auto rt) {
       using YT = decltype(yt);
       using RT = decltype(rt);
       auto laid = [&](auto post) {
-        constexpr bool P = decltype(post)::value;
+        constexpr int P = decltype(post)::value;
         return a->cols == n.warps * 32 * kNormPerThread ? norm_ring_kernel<YT, RT, P, kFull>
                                                         : norm_ring_kernel<YT, RT, P, kHalf>;
       };
-      auto kernel = a->post_weight ? laid(std::true_type{}) : laid(std::false_type{});
+      auto kernel = !a->y            ? laid(std::integral_constant<int, kNoBlock>{})
+                    : a->post_weight ? laid(std::integral_constant<int, 1>{})
+                                     : laid(std::integral_constant<int, 0>{});
       e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem);
       if (e == cudaSuccess) e = launch_pdl(kernel, grid, block, smem, st, n, g);
     });
     return e == cudaSuccess ? MOE_B200_OK : report_cuda(e, "block_norm launch");
   }
-  // Rows of up to 256 columns: several to a warp (65536 x 128: 11.7 us, 5.7 TB/s, against 31.5 with
-  // one).  An e4m3 block's maximum wants a half warp.
-  const bool packed = vec && a->cols <= 256 && !(a->pre_weight && a->x_type == MOE_B200_E4M3);
   const int lanes = packed ? packed_lanes(a->cols) : n.warps * 32;
   if (packed) rpc = 256 / lanes;
   const dim3 block(lanes, rpc), grid((a->rows + rpc - 1) / rpc);

@@ -98,6 +98,25 @@ def test_partial_forms():
     R.close(a["residual"], ref[0], ref[2])
 
 
+@pytest.mark.parametrize("T,H", [(1500, 512), (650, 7168), (700, 2880), (600, 8192), (2000, 96), (700, 1001)])
+@pytest.mark.parametrize("dtype", [BF, FP, F32])
+def test_partial_forms_of_many_rows(T, H, dtype):
+    a = make(T, H, dtype, dtype, True, None, seed=T)
+    w = dict(pre_weight=a["pre_weight"])
+    o = M.block_norm(None, a["residual"], **w, weight_offset=1.0)
+    ref = R.block_norm(None, a["residual"], **w, off=1.0)
+    R.close(o.x, ref[1], ref[3])
+    e = M.block_norm(None, a["residual"], **w, weight_offset=1.0, x_dtype=torch.float8_e4m3fn)
+    val = e.x.double() * e.x_scale.t().double().repeat_interleave(128, dim=1)[:, :H]
+    assert ((val.cpu() - ref[1]).abs() <= ref[1].abs() * 2.0 ** -4 * 1.01 + e.x_scale.max().item() * 2.0 ** -9).all()
+    for kw in (w, dict(post_weight=a["post_weight"]), dict(post_weight=a["post_weight"], **w)):
+        o = M.block_norm(a["y"], None, scale=3.0, **kw)
+        ref = R.block_norm(a["y"], None, scale=3.0, **kw)
+        R.close(o.residual, ref[0], ref[2])
+        if "pre_weight" in kw:
+            R.close(o.x, ref[1], ref[3])
+
+
 @pytest.mark.parametrize("T,H", [(1, 7168), (5, 128), (3, 130), (4, 1000), (2, 7), (70, 512), (3, 5001)])
 @pytest.mark.parametrize("r_dtype", [BF, F32])
 def test_e4m3_blocks(T, H, r_dtype):

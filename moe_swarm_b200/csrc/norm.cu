@@ -347,15 +347,18 @@ MOE_B200_API int moe_b200_block_norm(const moe_b200_norm_args* a, void* stream) 
   dispatch_types(a->y_type, a->residual_type, [&](auto yt, auto rt) {
     using YT = decltype(yt);
     using RT = decltype(rt);
-    // rows of up to 8192 columns take at most 512 threads, which may then use twice the registers
+    // rows of up to 8192 columns take at most 512 threads, which may then use twice the registers; odd
+    // ones of up to 256 have no loads for elements that they do not hold (30000 x 99: 10.4 us against 33.8)
     auto sized = [&](auto t) {
       constexpr int MAXT = decltype(t)::value;
-      return packed                          ? norm_fwd_kernel<YT, RT, kPacked, 512>
-             : vec                           ? norm_fwd_kernel<YT, RT, kVec, MAXT>
-             : a->cols <= 128           ? norm_fwd_kernel<YT, RT, kShort, 512>
-             : a->cols <= 256           ? norm_fwd_kernel<YT, RT, kThin, 512>
-             : a->cols >= 384 * n.warps ? norm_fwd_kernel<YT, RT, kTail, MAXT>
-                                        : norm_fwd_kernel<YT, RT, kScattered, MAXT>;
+      if constexpr (MAXT == 1024) return vec ? norm_fwd_kernel<YT, RT, kVec, MAXT> : norm_fwd_kernel<YT, RT, kTail, MAXT>;
+      else
+        return packed                     ? norm_fwd_kernel<YT, RT, kPacked, MAXT>
+               : vec                      ? norm_fwd_kernel<YT, RT, kVec, MAXT>
+               : a->cols <= 128           ? norm_fwd_kernel<YT, RT, kShort, MAXT>
+               : a->cols <= 256           ? norm_fwd_kernel<YT, RT, kThin, MAXT>
+               : a->cols >= 384 * n.warps ? norm_fwd_kernel<YT, RT, kTail, MAXT>
+                                          : norm_fwd_kernel<YT, RT, kScattered, MAXT>;
     };
     auto kernel = block.x * block.y <= 512 ? sized(std::integral_constant<int, 512>{})
                                            : sized(std::integral_constant<int, 1024>{});

@@ -11,6 +11,7 @@ results.
 
 from __future__ import annotations
 
+import functools
 import threading
 from typing import NamedTuple
 
@@ -120,6 +121,11 @@ def _call(fn: str, dev: int, args, *workspace):
         raise _failure(rc, fn)
 
 
+@functools.lru_cache(maxsize=256)
+def _workspace_size(fn: str, *sizes: int) -> int:
+    return getattr(_native.lib(), f"moe_b200_{fn}_workspace_size")(*sizes)
+
+
 _SCRATCH_KEPT = 4 << 20   # bytes kept per (device, stream, thread)
 _scratch: dict[tuple[int, int, int], torch.Tensor] = {}
 
@@ -129,7 +135,7 @@ def _workspace(n: int, dev: int) -> torch.Tensor:
     (device, stream, host thread): such calls are enqueued, and run, one after another, while two
     threads could enqueue the kernels of their calls in turn.  Large ones, and those of a graph
     capture (whose replays would share them with later calls), are allocated per call."""
-    if n > _SCRATCH_KEPT or torch.cuda.is_current_stream_capturing():
+    if n > _SCRATCH_KEPT or torch._C._cuda_isCurrentStreamCapturing():
         return torch.empty(n, dtype=torch.uint8, device=dev)
     key = (dev, torch._C._cuda_getCurrentRawStream(dev), threading.get_ident())
     ws = _scratch.get(key)
@@ -148,14 +154,16 @@ def _gate_layout(gate, rows: int, cols: int, dev: int):
     """(row stride, varies along a row) of a gate [cols], [1, cols], [rows, 1], [1, 1] or [rows, cols]."""
     _check(gate.dtype in _FLOATS, "gate has an unsupported type")
     _check(gate.get_device() == dev, "all tensors must be on one device")
-    g = gate.unsqueeze(0) if gate.dim() == 1 else gate
-    _check(g.dim() == 2 and g.shape[0] in (1, rows) and g.shape[1] in (1, cols),
+    size, st = gate.shape, gate.stride()
+    if len(st) == 1:
+        size, st = (1, *size), (0, *st)
+    _check(len(st) == 2 and size[0] in (1, rows) and size[1] in (1, cols),
            "gate must be broadcastable to [rows, cols]")
-    per_column = cols > 1 and g.shape[1] == cols
-    per_row = rows > 1 and g.shape[0] == rows
-    _check(not per_column or g.stride(1) == 1, "gate must have adjacent elements in a row")
-    _check(not per_row or g.stride(0) > 0, "gate: pass a broadcast gate with its own size, not expanded")
-    return g.stride(0) if per_row else 0, int(per_column)
+    per_column = cols > 1 and size[1] == cols
+    per_row = rows > 1 and size[0] == rows
+    _check(not per_column or st[1] == 1, "gate must have adjacent elements in a row")
+    _check(not per_row or st[0] > 0, "gate: pass a broadcast gate with its own size, not expanded")
+    return st[0] if per_row else 0, int(per_column)
 
 
 def block_norm(y: torch.Tensor | None, residual: torch.Tensor | None, *, post_weight: torch.Tensor | None = None,
@@ -251,9 +259,8 @@ def block_norm_backward(dx: torch.Tensor | None, dresidual: torch.Tensor | None,
         dpost = torch.empty_like(post_weight, dtype=torch.float32)
     if gate is not None:
         gate_ld, gate_cols = _gate_layout(gate, rows, cols, dev)
-        dgate = torch.empty_like(gate, dtype=gate.dtype if gate_ld and gate_cols else torch.float32,
-                                 memory_format=torch.contiguous_format)
-    n = _native.lib().moe_b200_block_norm_backward_workspace_size(rows, cols)
+        dgate = gate.new_empty(gate.shape, dtype=gate.dtype if gate_ld and gate_cols else torch.float32)
+    n = _workspace_size("block_norm_backward", rows, cols)
     _check(n > 0, "unsupported sizes")
     ws = _workspace(n, dev)
     _call("block_norm_backward", dev, _native.NormBackwardArgs.pack(
@@ -370,7 +377,7 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
         out_ld = _result(out, "out", (T, N), _FLOATS if out_dtype is None else (out_dtype,), dev)
     if T == 0 or N == 0:
         return out
-    n = _native.lib().moe_b200_int8_linear_workspace_size(T, N, K, x_type)
+    n = _workspace_size("int8_linear", T, N, K, x_type)
     _check(n > 0, "unsupported sizes")
     ws = _workspace(n, dev)
     _call("int8_linear", dev, _native.LinearArgs.pack(

@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(N == 1 ? 512 : 1024, 1) quant_kernel(QuantArgs
 }
 
 // Many aligned rows: persistent CTAs with their next rows on the way to shared memory, as the norm's.
-// 8192 x 7168 from bf16 39.7 us (4.4 TB/s): 280 instructions per warp and row, a third of them for the
+// 8192 x 7168 from bf16 39.7 us (4.4 TB/s): 250 instructions per warp and row, a third of them for the
 // ties (without which 30.8, but for 16-bit values on the tie of their scale the codes are then chance);
 // with the activation, 8192 x 2048, 15.8 us (5.3 TB/s), bound by HBM.
 template <class XT, int LAY>

@@ -24,7 +24,7 @@
 //
 // Bound by the warps' instructions, about 850 per token of 256 experts in 8 groups (scores, a sort of
 // eight keys per lane, rounds of maxima), not by HBM: 16384 tokens 20.7 us with counts (18.1 without
-// groups, 17.3 softmax) where the logits alone would take 2.7; 512 experts 46 us, 64 experts 11.  Few
+// groups, 17.3 softmax) where the logits alone would take 2.7; 512 experts 41 us, 64 experts 11.  Few
 // tokens are bound by the one token's chain of operations: 16 tokens 4.6 us.
 #include <type_traits>
 
@@ -410,8 +410,10 @@ __device__ __forceinline__ uint32_t choose_fast(const SelectArgs& a, float* sel,
   return taken;
 }
 
+// Registers: 64 a thread for up to 256 experts (more CTAs on an SM with less gain nothing: 16384 x 256
+// 21.3 us with five, 22.0 with six), 80 for 512 (41.4 us against 47.7 with as many as it would take, two CTAs).
 template <int V, bool SOFTMAX>
-__global__ void __launch_bounds__(kSelWarps * 32) select_kernel(SelectArgs a) {
+__global__ void __launch_bounds__(kSelWarps * 32, V == 16 ? 3 : 4) select_kernel(SelectArgs a) {
   extern __shared__ __align__(16) float s_dyn[];   // [warps][32 V] values of a token, then [E] counts
   __shared__ int s_id[kSelWarps][kSelMaxK];
   pdl_wait();
@@ -614,8 +616,9 @@ void dispatch_select(int E, F&& f) {
   else f(std::integral_constant<int, 16>{});
 }
 
-// Eight CTAs of eight warps are all the warps of an SM; with four the backward of 16384 x 256 takes
-// 15.7 us instead of 10.3, the forward 21.1 instead of 20.7.
+// Eight CTAs of eight warps for every SM, which are all its warps; registers leave the forward four at a
+// time.  With four the backward of 16384 x 256 takes 15.7 us instead of 10.3, the forward 21.1 instead of
+// 20.7.
 int select_grid(int T, int sms) {
   const int need = (T + kSelWarps - 1) / kSelWarps;
   return need < 8 * sms ? need : 8 * sms;

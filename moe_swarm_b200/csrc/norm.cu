@@ -25,8 +25,8 @@ struct NormArgs {
   float scale, eps, off;
 };
 
-// x = r * rstd * w of this thread's elements, stored in the type asked for.  Whole warps call it:
-// a 128-column block's maximum is a shuffle over its half warp (eight elements each, two blocks in
+// x = r * rstd * w of this thread's elements, stored in the type asked for.  Whole warps call it
+// (kPacked, which has no e4m3, aside): a 128-column block's maximum is a shuffle over its half warp (eight elements each, two blocks in
 // a thread) or warp (four each, four blocks).
 template <int LAY>
 __device__ __forceinline__ void store_x(const NormArgs& a, int row, int cols, Row16& r, const Row16& w, float rstd) {
@@ -91,7 +91,8 @@ __device__ __forceinline__ void store_x(const NormArgs& a, int row, int cols, Ro
 }
 
 // One row per group of warps.  blockDim = (32 * warps, rows per CTA), or less than a warp per row
-// (kPacked).  Rows beyond the last run with no elements.  Bound by latency where rows are few (one row
+// (kPacked).  Rows beyond the last are the last one again, without a store: what a layout promises of
+// its elements (exists()) holds for rows that exist only.  Bound by latency where rows are few (one row
 // of 7168: 2.6 us), by HBM where many: 592 rows 6.4 us, 16384 x 512 11.6 us (5.8 TB/s), 901 x 5001
 // with both norms 15.5 us (3.5 TB/s: odd rows are read and written two bytes at a time).
 template <class YT, class RT, int LAY, int MAXT>
@@ -100,7 +101,8 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) norm_fwd_kernel(NormArgs a)
   pdl_wait();
   pdl_launch_dependents();
   const int row = blockIdx.x * blockDim.y + threadIdx.y;
-  const int cols = row < a.rows ? a.cols : 0;
+  const int cols = a.cols;
+  const bool live = row < a.rows;
   const int from = min(row, a.rows - 1);   // a row that exists
   Row16 r, w;
   if (a.residual) {
@@ -126,19 +128,19 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) norm_fwd_kernel(NormArgs a)
       load_row_dyn<LAY>(a.gate, a.gate_type, from * a.g_ld, cols, w);
 #pragma unroll
       for (int i = 0; i < 8; ++i) y.v[i] = mul2(y.v[i], w.v[i]);
-    } else if (a.gate && cols) {
-      k *= load1_dyn(a.gate, a.gate_type, row * a.g_ld);
+    } else if (a.gate) {
+      k *= load1_dyn(a.gate, a.gate_type, from * a.g_ld);
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) r.v[i] = fma2(dup2(k), y.v[i], r.v[i]);
-    if (a.residual_out) store_row<RT, LAY>(static_cast<RT*>(a.residual_out) + row * a.ro_ld, cols, r);
+    if (a.residual_out && live) store_row<RT, LAY>(static_cast<RT*>(a.residual_out) + row * a.ro_ld, cols, r);
   }
   if (!a.pre_w) return;
   load_weight<LAY>(a.pre_w, a.pre_type, a.off, cols, w);
   float ss[1] = {squares_existing<LAY>(r, cols)};
   if constexpr (LAY == kPacked) packed_sum(ss);
   else row_sum(ss, a.warps, buf[1]);
-  store_x<LAY>(a, row, cols, r, w, rsqrtf(ss[0] / a.cols + a.eps));
+  if (live) store_x<LAY>(a, row, cols, r, w, rsqrtf(ss[0] / a.cols + a.eps));   // (the same in all of a warp but kPacked's)
 }
 
 // Many rows: persistent CTAs, whose next rows (y, residual, gate per element) are on their way

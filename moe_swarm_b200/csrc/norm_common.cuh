@@ -60,6 +60,9 @@ enum : int { kShort = -2, kThin = -1, kScattered = 0, kTail = 1, kVec = 2, kHalf
 constexpr bool is_vec(int lay) { return lay >= kVec; }
 constexpr int slots(int lay) { return lay == kShort ? 4 : lay == kThin ? 8 : 16; }
 
+// (kHalf, kFull and kTail say that elements exist without a look at `cols`: they are for rows that exist,
+// of the lengths named, and not for a missing row given as one of no columns.)
+
 // The column of this thread's element q.
 template <int LAY>
 __device__ __forceinline__ int col_of(int q) {

@@ -1,0 +1,61 @@
+"""GPU: where the operators around the layer end: rows that do not fill a CTA, infinite factors, biases that
+cancel, rows that overlap, scores next to 0 and 1."""
+import pytest
+import torch
+
+import moe_swarm_b200 as M
+from tests import _ops_ref as R
+
+pytestmark = pytest.mark.gpu
+BF, FP, F32, E4M3 = torch.bfloat16, torch.float16, torch.float32, torch.float8_e4m3fn
+BEHIND = 9   # rows behind a result, more than a CTA holds of any length
+
+
+def randn(seed, *shape, std=1.0, dtype=F32):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device="cuda") * std).to(dtype)
+
+
+# rows of one to four warps on odd boundaries: by their length, their pitch or their base
+@pytest.mark.parametrize("T,H,pad,base", [(5, 500, 0, 0), (3, 1001, 0, 0), (3, 1300, 0, 0), (5, 2047, 0, 0), (1, 500, 0, 0),
+                                          (5, 512, 1, 0), (3, 1024, 3, 0), (2, 2048, 0, 1), (7, 400, 0, 3), (9, 99, 0, 0),
+                                          (3, 250, 0, 0), (5, 300, 0, 0), (3, 3001, 0, 0)])
+@pytest.mark.parametrize("y_dtype,r_dtype", [(BF, BF), (BF, F32), (F32, F32)])
+@pytest.mark.parametrize("x_dtype", [BF, F32, E4M3])
+@pytest.mark.parametrize("post", [False, True])
+def test_nothing_is_written_behind_the_last_row(T, H, pad, base, y_dtype, r_dtype, x_dtype, post):
+    def rows(seed, dtype):
+        flat = randn(seed, base + T * (H + pad), dtype=dtype)
+        return flat[base:].view(T, H + pad)[:, :H]
+
+    def buffer(dtype):
+        flat = torch.full((base + (T + BEHIND) * (H + pad),), 77, dtype=torch.uint8, device="cuda").to(dtype)
+        return flat, flat[base:].view(T + BEHIND, H + pad)[:T, :H]
+
+    y, r = rows(1, y_dtype), rows(2, r_dtype)
+    w = (1 + randn(3, H, std=0.2)).to(BF)
+    kw = dict(post_weight=w if post else None, gate=torch.rand(T, 1, device="cuda").to(BF), pre_weight=w)
+    all_r, ro = buffer(r_dtype)
+    all_x, x = buffer(x_dtype)
+    o = M.block_norm(y, r, residual_out=ro, out=x, x_dtype=x_dtype, **kw)
+    ref_r, ref_x, rm, xm = R.block_norm(y, r, **kw)
+    R.close(ro, ref_r, rm)
+    if x_dtype != E4M3:
+        R.close(x, ref_x, xm)
+    else:
+        assert torch.isfinite(o.x_scale).all()
+        s = o.x_scale.t().double().repeat_interleave(128, dim=1)[:, :H].cpu()
+        tol = (ref_x.abs() * 2.0 ** -4).maximum(s * 2.0 ** -10) * 1.001 + 2 * R.STEPS * R.U32 * (xm + ref_x.abs())
+        assert ((x.double().cpu() * s - ref_x).abs() <= tol).all()
+    for flat, view in ((all_r, ro), (all_x, x)):
+        untouched = torch.ones_like(flat, dtype=torch.bool)
+        untouched[base:].view(T + BEHIND, H + pad)[:T, :H] = False
+        assert (flat[untouched].float() == torch.tensor(77.0).to(flat.dtype).float().item()).all()
+
+
+def test_a_slice_of_a_live_stream():
+    """r' written over the first rows of a stream leaves the rows behind them."""
+    stream = randn(1, 40, 1000, dtype=BF)[:, :500]
+    before = stream.clone()
+    M.block_norm(randn(2, 5, 500, dtype=BF), stream[:5], residual_out=stream[:5])
+    assert torch.equal(stream[5:], before[5:]) and not torch.equal(stream[:5], before[:5])

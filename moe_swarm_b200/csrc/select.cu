@@ -157,12 +157,12 @@ __device__ __forceinline__ void store_logits(void* p, int type, int64_t off, int
 
 // The scores as defined (EXACT), or 32-bit ones.  Returns the largest score of the row that is
 // known without looking (sigmoid: 1; softmax: that of the largest logit): the size that errors
-// are measured by.  A 32-bit score is off by less than 2^-19 of it:
-//   sigmoid: __expf(-x) is off by |x| 2^-24 + 2^-22 of itself, which moves s by s (1 - s) times as
-//     much, at most 2^-24 and 2^-24; the sum and the quotient add 2^-22.
-//   softmax: x - m and its product with log2(e) round by |x - m| 2^-24 each, which moves a score by
-//     at most 0.74 * 2^-24 of the largest; the exponential, the quotient and its product add 6
-//     units, a sum of 16 terms in a lane and 5 over the lanes 21 of 2^-24.
+// are measured by.  A 32-bit score is off by less than 20 * 2^-23 of it, __expf(-d) being off by
+// (2 + 1.2 d) 2^-23 of itself:
+//   sigmoid: that moves s by s (1 - s) times as much, at most 2^-23; the sum and the quotient add 3.
+//   softmax: d e^-d is at most 0.37, so its own exponential moves a score by 2.5.  The row's sum moves
+//     with the exponentials of all, up to 6 (512 experts alike, each ln 511 below the first), and by 10
+//     for its roundings, 15 in a lane and 5 over the lanes.  The quotient and the product add 1.
 template <int V, bool SOFTMAX, bool EXACT>
 __device__ __forceinline__ float scores(const float* x, float lowest, float* s) {
   if constexpr (!SOFTMAX) {
@@ -205,10 +205,12 @@ __device__ __forceinline__ float scores(const float* x, float lowest, float* s) 
 }
 
 // Two sides of a decision are told apart by the 32-bit scores if they differ by more than this
-// share of the sizes involved.  An expert's score is off by 2^-19 of the row's size and its key by
-// 2^-19 of itself (the lane in the low bits); a group's score is the sum of two such keys, and its
-// own key off by 2^-19 once more; sums round by 2^-23.  For both sides of a decision that is less
-// than 2^-15.
+// share of the sizes involved, M = max(size, both sides).  In units of 2^-18: an expert's score is off by
+// 5/8 of the row's size and its key by 1 of itself (the lane in the low five bits); for two experts that
+// is at most 3.25 M.  A group's score is the sum of two such keys, and its own key is off by 1 once more:
+// 1.25 size + |m1| + |m2| + |m1 + m2| a side.  Where m1 and m2 have opposite signs, |m1| + |m2| is up to
+// |m1 + m2| + 2 B, B = the lowest bias's distance below 0 (scores are not negative), so for sums of two M
+// counts 2 B as well (group_size): 2.5 size + 4 M + 4 B <= 6.5 M.  Sums round by 2^-6 each.  The margin is 8.
 constexpr float kMargin = 3.0517578125e-05f;
 
 // Whether `in` (the weakest taken) is above `out` (the strongest left) for certain.  -inf for
@@ -376,11 +378,11 @@ __device__ __forceinline__ float last_of_rounds(float (&list)[V + 1], int K) {
 // is chosen is what reaches the last round's maximum.
 template <int V>
 __device__ __forceinline__ uint32_t choose_fast(const SelectArgs& a, float* sel, float* s_sel, int lane, float size,
-                                                bool* sure) {
+                                                float group_size, bool* sure) {
   *sure = true;
   int lanes = 0;
   const bool by_lane = a.n_group > 1 && groups_by_lane<V>(a, &lanes);
-  if (a.n_group > 1 && !by_lane) drop_groups<V>(a, sel, s_sel, lane, true, size, sure);
+  if (a.n_group > 1 && !by_lane) drop_groups<V>(a, sel, s_sel, lane, true, group_size, sure);
   float key[V], list[V + 1];
 #pragma unroll
   for (int i = 0; i < V; ++i) key[i] = lane_key(sel[i], lane);
@@ -396,7 +398,7 @@ __device__ __forceinline__ uint32_t choose_fast(const SelectArgs& a, float* sel,
   bool kept = true;
   if (by_lane) {
     const float score = score_by_lane(a, or_none(list[0]), V > 1 ? or_none(list[V > 1 ? 1 : 0]) : -INFINITY, lanes);
-    kept = keep_group_fast(a, score, lane / lanes, size, sure);
+    kept = keep_group_fast(a, score, lane / lanes, group_size, sure);
 #pragma unroll
     for (int i = 0; i < V; ++i) list[i] = kept ? list[i] : -3.4e38f;
   }
@@ -427,15 +429,17 @@ __global__ void __launch_bounds__(kSelWarps * 32, V == 16 ? 3 : 4) select_kernel
   }
   const float lowest = lowest_of(a.type);
   const int first = lane * V;
-  float bias[V];
+  float bias[V], below = 0.f;
   bool wild = false;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     bias[i] = a.bias && first + i < a.E ? load1_dyn(a.bias, a.bias_type, first + i) : 0.f;
     wild |= fabsf(bias[i]) >= kHuge && bias[i] != -INFINITY;
+    below = bias[i] == -INFINITY ? below : fminf(below, bias[i]);
   }
   // biases so large that sums of two overflow: every choice by the defined scores
   wild = __any_sync(0xffffffffu, wild);
+  const float cancel = a.n_group > 1 && a.top2 ? -2.f * redux_min(below) : 0.f;   // 2 B of the margin
   const int step = gridDim.x * kSelWarps;
   for (int t = blockIdx.x * kSelWarps + warp; t < a.T; t += step) {
     float x[V], s[V], sel[V];
@@ -452,7 +456,7 @@ __global__ void __launch_bounds__(kSelWarps * 32, V == 16 ? 3 : 4) select_kernel
     const bool bad = __any_sync(0xffffffffu, nan != nan);
     uint32_t taken = 0;
     bool sure = bad || !wild;
-    if (!bad && sure) taken = choose_fast<V>(a, sel, s_row, lane, size, &sure);
+    if (!bad && sure) taken = choose_fast<V>(a, sel, s_row, lane, size, size + cancel, &sure);
     if (!sure) {
       scores<V, SOFTMAX, true>(x, lowest, s);
 #pragma unroll

@@ -59,3 +59,36 @@ def test_a_slice_of_a_live_stream():
     before = stream.clone()
     M.block_norm(randn(2, 5, 500, dtype=BF), stream[:5], residual_out=stream[:5])
     assert torch.equal(stream[5:], before[5:]) and not torch.equal(stream[:5], before[:5])
+
+
+def choice(x, K, score, bias, G, TG, group_score="top2"):
+    """ids of select_experts by the definition, many rows at a time: 32-bit scores whose exponential (softmax:
+    quotient) is rounded once, their 32-bit sums, stable sorts."""
+    x = x.double()
+    T, E = x.shape
+    s = 1.0 / (1.0 + torch.exp(-x).float()) if score == "sigmoid" else torch.softmax(x, dim=1).float()
+    sel = s if bias is None else s + bias
+    if G > 1:
+        per = sel.view(T, G, -1)
+        first = per.sort(dim=2, descending=True).values
+        gs = first[..., 0] + first[..., 1] if group_score == "top2" else first[..., 0]
+        rank = gs.argsort(dim=1, descending=True, stable=True).argsort(dim=1)
+        sel = per.masked_fill((rank >= TG).unsqueeze(2), float("-inf")).reshape(T, E)
+    return sel.sort(dim=1, descending=True, stable=True).indices[:, :K].sort(dim=1).values.int()
+
+
+# groups of lanes, of lanes and registers, and of a length that is scored through shared memory
+@pytest.mark.parametrize("E,G,TG", [(64, 8, 3), (256, 8, 4), (60, 4, 2), (512, 16, 5)])
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("size", [0.3, 16.0, 64.0, 1e3, 1e4])
+def test_groups_whose_biases_cancel(E, G, TG, score, size):
+    """A favoured expert beside disfavoured ones: a group's score is the small sum of two large values."""
+    T = 1 << 17
+    x = randn(E + int(size), T, E)
+    favoured = torch.full((E,), -size, device="cuda")
+    favoured[::E // G] = size
+    spread = randn(5, E, std=size)
+    for bias in (favoured, spread):
+        for group_score in ("top2", "max"):
+            o = M.select_experts(x, 6, score=score, bias=bias, n_group=G, topk_group=TG, group_score=group_score)
+            assert torch.equal(o.idx, choice(x, 6, score, bias, G, TG, group_score))

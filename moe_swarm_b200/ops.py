@@ -73,6 +73,12 @@ def _rows(t, name: str, shape=None, dtypes=_FLOATS, dev=None):
     return st[0]
 
 
+def _like(t, dtype=None):
+    """A new tensor of t's shape without gaps.  (empty_like would order the strides of rows that overlap,
+    such as a sliding window's, as it finds them: by columns.)"""
+    return torch.empty_like(t, dtype=dtype) if t.is_contiguous() else t.new_empty(t.shape, dtype=dtype)
+
+
 def _result(t, name: str, shape, dtypes, dev):
     """Checks a tensor that receives a result: rows may not overlap.  Returns its row pitch."""
     ld = _rows(t, name, shape, dtypes, dev)
@@ -201,7 +207,7 @@ def block_norm(y: torch.Tensor | None, residual: torch.Tensor | None, *, post_we
     if y is None:
         _check(residual_out is None, "residual_out is the residual itself without y")
     elif residual_out is None:
-        residual_out, ro_ld = torch.empty_like(stream), cols
+        residual_out, ro_ld = _like(stream), cols
     else:
         ro_ld = _result(residual_out, "residual_out", shape, (stream.dtype,), dev)
     x = x_scale = None
@@ -211,7 +217,7 @@ def block_norm(y: torch.Tensor | None, residual: torch.Tensor | None, *, post_we
             x_dtype = first.dtype if out is None else out.dtype
         _check(x_dtype in _TYPES and x_dtype != torch.int8, "unsupported x_dtype")
         if out is None:
-            x, x_ld = torch.empty_like(first, dtype=x_dtype), cols
+            x, x_ld = _like(first, x_dtype), cols
         else:
             x, x_ld = out, _result(out, "out", shape, (x_dtype,), dev)
         if x_dtype == torch.float8_e4m3fn:
@@ -248,9 +254,9 @@ def block_norm_backward(dx: torch.Tensor | None, dresidual: torch.Tensor | None,
     dr_ld = 0 if dresidual is None else _rows(dresidual, "dresidual", shape, (r_dtype,), dev)
     dy = dpre = dpost = dgate = None
     gate_ld = gate_cols = 0
-    dres = torch.empty_like(residual)
+    dres = _like(residual)
     if y is not None:
-        dy = torch.empty_like(y)
+        dy = _like(y)
     if dx is not None:
         _vector(pre_weight, "pre_weight", cols, _FLOATS, dev)
         dpre = torch.empty_like(pre_weight, dtype=torch.float32)
@@ -318,7 +324,7 @@ def select_experts_backward(dw: torch.Tensor, logits: torch.Tensor, idx: torch.T
     _check(idx.dim() == 2, "idx must be [T, top_k]")
     _matrix(idx, "idx", (T, idx.shape[1]), torch.int32, dev)
     _matrix(dw, "dw", idx.shape, torch.float32, dev)
-    out = torch.empty_like(logits)
+    out = _like(logits)
     _call("select_experts_backward", dev, _native.SelectBackwardArgs.pack(
         logits.data_ptr(), idx.data_ptr(), dw.data_ptr(), out.data_ptr(), ld, E, T, E, idx.shape[1],
         _TYPES[logits.dtype], _SCORES[score], bool(renormalize), scale))

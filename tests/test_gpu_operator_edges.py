@@ -92,3 +92,39 @@ def test_groups_whose_biases_cancel(E, G, TG, score, size):
         for group_score in ("top2", "max"):
             o = M.select_experts(x, 6, score=score, bias=bias, n_group=G, topk_group=TG, group_score=group_score)
             assert torch.equal(o.idx, choice(x, 6, score, bias, G, TG, group_score))
+
+
+def overlapping(seed, T, H, step, dtype=F32):
+    """[T, H] whose rows begin `step` elements apart, step < H (0: one row, seen T times)."""
+    return randn(seed, (T - 1) * step + H, dtype=dtype).as_strided((T, H), (step, 1))
+
+
+@pytest.mark.parametrize("T,H,step", [(3, 8, 1), (3, 8, 0), (5, 512, 8), (700, 1024, 8), (6, 300, 7), (900, 96, 2)])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_rows_that_overlap(T, H, step, dtype):
+    y, r, dx, dr = (overlapping(i, T, H, step, dtype) for i in range(4))
+    w = (1 + randn(9, H, std=0.2)).to(dtype)
+    o = M.block_norm(y, r, pre_weight=w)
+    ref = R.block_norm(y, r, pre_weight=w)
+    R.close(o.residual, ref[0], ref[2])
+    R.close(o.x, ref[1], ref[3])
+    b = M.block_norm_backward(dx, dr, r, y, pre_weight=w, post_weight=w)
+    ref = R.block_norm_backward(dx, dr, r, y, pre_weight=w, post_weight=w)
+    R.close(b.residual, *ref["residual"])
+    R.close(b.y, *ref["y"], steps=3 * R.STEPS)
+    for t in (o.residual, o.x, b.residual, b.y):
+        assert t.is_contiguous()
+    if H > 512:
+        return
+    logits = overlapping(5, T, H, step, dtype)
+    s = M.select_experts(logits, 4)
+    assert torch.equal(s.idx, M.select_experts(logits.contiguous(), 4).idx)
+    dw = randn(6, T, 4)
+    d = M.select_experts_backward(dw, logits, s.idx)
+    assert d.is_contiguous() and torch.equal(d, M.select_experts_backward(dw, logits.contiguous(), s.idx))
+
+
+def test_results_may_not_overlap():
+    y = randn(1, 3, 8)
+    with pytest.raises(M.MoEArgumentError):
+        M.block_norm(y, y, residual_out=overlapping(2, 3, 8, 1))

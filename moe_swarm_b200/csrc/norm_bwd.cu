@@ -57,7 +57,8 @@ __device__ __forceinline__ void factor_b(const NormBwdArgs& a, Row16& b) {
 }
 
 // One row.  load(which, v): which = 0 dx, 1 r', 2 y, 3 dr, 4 the gate per element, 5 w, 6 b; done()
-// is called when everything is loaded.  POST, GATE (0 none or per column, 1 per row, 2 per
+// is called when everything is loaded.  A row with no columns (one that is missing) adds nothing to the
+// column sums: its 1 / sqrt(0 + eps) may be infinite.  POST, GATE (0 none or per column, 1 per row, 2 per
 // element, kNoBlock: there is no y): -1 = known at run time only.
 template <class YT, class RT, int LAY, int POST, int GATE, class Load, class Done>
 __device__ __forceinline__ void bwd_row(const NormBwdArgs& a, int row, int cols, float inv_cols, float* buf0, float* buf1,
@@ -65,6 +66,7 @@ __device__ __forceinline__ void bwd_row(const NormBwdArgs& a, int row, int cols,
   const bool post = POST < 0 ? a.post_w != nullptr : POST == 1;
   const int gate = GATE < 0 ? (a.gate_grad == kGateElement ? 2 : a.gate_grad == kGateRow ? 1 : 0) : GATE;
   const bool has_dx = GATE < 0 ? a.dx != nullptr : true, has_y = GATE < 0 ? a.y != nullptr : GATE != kNoBlock;
+  const bool live = LAY == kPacked || LAY == kShort || LAY == kThin ? cols > 0 : true;
   Row16 r, dx, y, G;
   float s[3] = {0.f, 0.f, 0.f};   // sum r'^2, sum w dx r', sum y^2
   if (has_dx) {
@@ -96,7 +98,7 @@ __device__ __forceinline__ void bwd_row(const NormBwdArgs& a, int row, int cols,
       const float k = -s[1] * inv_cols * rstd * rstd;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        sum.pre.v[i] = fma2(mul2(dx.v[i], r.v[i]), dup2(rstd), sum.pre.v[i]);
+        if (live) sum.pre.v[i] = fma2(mul2(dx.v[i], r.v[i]), dup2(rstd), sum.pre.v[i]);
         G.v[i] = fma2(dup2(rstd), fma2(r.v[i], dup2(k), G.v[i]), d.v[i]);
       }
     } else {
@@ -120,14 +122,15 @@ __device__ __forceinline__ void bwd_row(const NormBwdArgs& a, int row, int cols,
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float2 gy = mul2(G.v[i], y.v[i]);
-      sum.post.v[i] = fma2(mul2(gy, ge.v[i]), dup2(q), sum.post.v[i]);
+      if (live) sum.post.v[i] = fma2(mul2(gy, ge.v[i]), dup2(q), sum.post.v[i]);
       dg.v[i] = mul2(has_b ? mul2(gy, b.v[i]) : gy, dup2(a.scale * ystd));
       G.v[i] = mul2(G.v[i], ge.v[i]);
     }
     store_row_dyn<LAY>(a.dgate, a.gate_type, row * a.dg_ld, cols, dg);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum.post.v[i] = fma2(mul2(G.v[i], y.v[i]), dup2(q), sum.post.v[i]);
+    for (int i = 0; i < 8; ++i)
+      if (live) sum.post.v[i] = fma2(mul2(G.v[i], y.v[i]), dup2(q), sum.post.v[i]);
   }
   if (has_b) {
 #pragma unroll

@@ -128,3 +128,20 @@ def test_results_may_not_overlap():
     y = randn(1, 3, 8)
     with pytest.raises(M.MoEArgumentError):
         M.block_norm(y, y, residual_out=overlapping(2, 3, 8, 1))
+
+
+@pytest.mark.parametrize("T,H", [(301, 128), (2500, 8), (333, 301), (333, 1001), (149, 99), (1301, 256), (700, 5001)])
+@pytest.mark.parametrize("gate", [None, "channel", "token", "full"])
+def test_gradients_without_an_epsilon(T, H, gate):
+    """Rows that a CTA has room for but the batch has not leave the sums over rows alone, also at eps = 0."""
+    y, r, dx, dr = (randn(i, T, H, dtype=BF) for i in range(4))
+    w, wp = ((1 + randn(i, H, std=0.2)).to(BF) for i in (8, 9))
+    shape = {None: None, "channel": (1, H), "token": (T, 1), "full": (T, H)}[gate]
+    kw = dict(pre_weight=w, post_weight=wp, gate=None if shape is None else randn(7, *shape, dtype=BF), eps=0.0)
+    b = M.block_norm_backward(dx, dr, r, y, **kw)
+    ref = R.block_norm_backward(dx, dr, r, y, **kw)
+    steps = 3 * R.STEPS + T // 148 + 64
+    R.close(b.pre_weight, *ref["pre_weight"], steps=steps)
+    R.close(b.post_weight, *ref["post_weight"], steps=steps)
+    if gate == "channel":
+        R.close(b.gate, *(t.sum(0, keepdim=True) for t in ref["gate"]), steps=steps)

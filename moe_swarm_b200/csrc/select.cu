@@ -573,12 +573,14 @@ __global__ void __launch_bounds__(kSelWarps * 32) select_bwd_kernel(SelectBwdArg
     const bool bad = __any_sync(0xffffffffu, all != all);   // a NaN logit, or an infinite one of a softmax
     __syncwarp();
     float sk = have ? row[id] : 0.f;
-    // sigmoid: from the logit that was put there (one that is switched off was not chosen)
-    float one_minus = 0.f;
+    // sigmoid: from the logit that was put there (one that is switched off was not chosen).  With h =
+    // exp(-|x| / 2) and r = 1 / (1 + h h), s (1 - s) = (h r)^2: nothing cancels where s is near 1, and nothing
+    // overflows or loses its bits where it is next to 0.
+    float root = 0.f;
     if constexpr (!SOFTMAX) {
-      const float e = expf(-sk);
-      sk = have ? 1.f / (1.f + e) : 0.f;
-      one_minus = sk < 1.f ? 1.f - sk : 0.f;
+      const float h = expf(-0.5f * fabsf(sk)), r = 1.f / fmaf(h, h, 1.f);
+      root = h * r;
+      sk = have ? (sk < 0.f ? h * root : r) : 0.f;
     }
     float dot = d * sk;
     if (a.renorm) {
@@ -592,7 +594,7 @@ __global__ void __launch_bounds__(kSelWarps * 32) select_bwd_kernel(SelectBwdArg
       dot = warp_sum(dot);
       mine = sk * (d - dot);
     } else {
-      mine = d * sk * one_minus;
+      mine = d * root * root;
     }
     __syncwarp();
 #pragma unroll

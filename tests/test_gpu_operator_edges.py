@@ -145,3 +145,26 @@ def test_gradients_without_an_epsilon(T, H, gate):
     R.close(b.post_weight, *ref["post_weight"], steps=steps)
     if gate == "channel":
         R.close(b.gate, *(t.sum(0, keepdim=True) for t in ref["gate"]), steps=steps)
+
+
+@pytest.mark.parametrize("renorm", [False, True])
+def test_sigmoid_gradient_next_to_0_and_1(renorm):
+    """s (1 - s) keeps its bits where s rounds to 1, and where exp(-x) overflows."""
+    T, E, K = 40, 16, 4
+    x = torch.linspace(-25, 25, T, device="cuda")[:, None] + 0.1 * randn(1, T, E)
+    x[0], x[1] = -100.0, 100.0
+    idx = torch.arange(K, dtype=torch.int32, device="cuda").expand(T, K).contiguous()
+    dw = randn(2, T, K)
+    got = M.select_experts_backward(dw, x, idx, renormalize=renorm, scale=2.5)
+    p = torch.sigmoid(x[:, :K].double())
+    slope = p * torch.sigmoid(-x[:, :K].double())
+    d = 2.5 * dw.double()
+    mag = d.abs()
+    if renorm:
+        S = p.sum(1, keepdim=True) + 1e-20
+        d, mag = (d - (d * p).sum(1, keepdim=True) / S) / S, (mag + (mag * p).sum(1, keepdim=True) / S) / S
+    # exponential (2), sum, quotient, product, slope; renormalised, two sums of 5 and two quotients besides;
+    # below 2^-126 numbers have an absolute spacing
+    err = (got[:, :K].double() - d * slope).abs()
+    assert (err <= 32 * R.U32 * mag * slope + 2.0 ** -148).all()
+    assert (got[:, K:] == 0).all() and (got[5:30, 0] != 0).all()

@@ -329,9 +329,10 @@ MOE_B200_API int moe_b200_block_norm_backward(const moe_b200_norm_backward_args*
  *   counts [num_experts] (or null): tokens that chose each expert
  * s is a 32-bit value with its exponential rounded once, as in the layer's routing; with
  * sigmoid, 256 experts, 8 groups of which 4 stay, top_k 8 and renormalize, idx is
- * moe_b200_route's and weight equals its weights up to the rounding of their sum.  A logit of -inf or of its type's lowest value switches its expert off; where
- * no expert is left a slot holds id -1 and weight 0 (moe_b200_forward_routed skips it).  A row
- * with a NaN score has ids -1 and NaN weights.
+ * moe_b200_route's and weight equals its weights up to the rounding of their sum.  Weights of a
+ * softmax have their exponentials in 64 bits.  A logit of -inf or of its type's lowest value
+ * switches its expert off; where no expert is left a slot holds id -1 and weight 0
+ * (moe_b200_forward_routed skips it).  A row with a NaN score has ids -1 and NaN weights.
  */
 #define MOE_B200_SCORE_SIGMOID 0
 #define MOE_B200_SCORE_SOFTMAX 1

@@ -24,7 +24,7 @@
 //
 // Bound by the warps' instructions, about 850 per token of 256 experts in 8 groups (scores, a sort of
 // eight keys per lane, rounds of maxima), not by HBM: 16384 tokens 20.7 us with counts (18.1 without
-// groups, 17.3 softmax) where the logits alone would take 2.7; 512 experts 41 us, 64 experts 11.  Few
+// groups, 19.0 softmax) where the logits alone would take 2.7; 512 experts 41 us, 64 experts 11.  Few
 // tokens are bound by the one token's chain of operations: 16 tokens 4.6 us.
 #include <type_traits>
 
@@ -155,6 +155,9 @@ __device__ __forceinline__ void store_logits(void* p, int type, int64_t off, int
   }
 }
 
+// exp(d) for d <= 0, in double (a score's numerator).
+__device__ __forceinline__ double exp_below(double d) { return d != d ? d : d < -700.0 ? 0.0 : exp_series(d); }
+
 // The scores as defined (EXACT), or 32-bit ones.  Returns the largest score of the row that is
 // known without looking (sigmoid: 1; softmax: that of the largest logit): the size that errors
 // are measured by.  A 32-bit score is off by less than 20 * 2^-23 of it, __expf(-d) being off by
@@ -163,8 +166,9 @@ __device__ __forceinline__ void store_logits(void* p, int type, int64_t off, int
 //   softmax: d e^-d is at most 0.37, so its own exponential moves a score by 2.5.  The row's sum moves
 //     with the exponentials of all, up to 6 (512 experts alike, each ln 511 below the first), and by 10
 //     for its roundings, 15 in a lane and 5 over the lanes.  The quotient and the product add 1.
+// *top: softmax: the row's largest logit.
 template <int V, bool SOFTMAX, bool EXACT>
-__device__ __forceinline__ float scores(const float* x, float lowest, float* s) {
+__device__ __forceinline__ float scores(const float* x, float lowest, float* s, float* top) {
   if constexpr (!SOFTMAX) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -177,12 +181,13 @@ __device__ __forceinline__ float scores(const float* x, float lowest, float* s) 
 #pragma unroll
     for (int i = 0; i < V; ++i) m = fmaxf(m, x[i]);   // (switched off ones do no harm)
     m = redux_max(m);
+    *top = m;
     if constexpr (EXACT) {
       double ex[V], sum = 0.0;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const double d = static_cast<double>(x[i]) - static_cast<double>(m);
-        ex[i] = x[i] <= lowest ? 0.0 : d != d ? d : d < -700.0 ? 0.0 : exp_series(d);
+        ex[i] = x[i] <= lowest ? 0.0 : exp_below(d);
         sum += ex[i];
       }
       const double inv = 1.0 / warp_sum_d(sum);
@@ -202,6 +207,36 @@ __device__ __forceinline__ float scores(const float* x, float lowest, float* s) 
       return inv;
     }
   }
+}
+
+// exp(d) in double for -700 < d <= 0, within 2^-32 of itself: the series of exp_series to degree 8 (.3466^9 /
+// 9! = 2^-32.2), ln 2 in one part, k by adding 1.5 * 2^52 in place of conversions, which run at a quarter of
+// the rate.
+__device__ __forceinline__ double exp_to_33_bits(double d) {
+  const double shifted = fma(d, 1.4426950408889634074, 0x1.8p52);
+  const double r = fma(shifted - 0x1.8p52, -6.93147180559945309417e-01, d);
+  double p = 1.0 / 40320.0;
+  p = fma(p, r, 1.0 / 5040.0);
+  p = fma(p, r, 1.0 / 720.0);
+  p = fma(p, r, 1.0 / 120.0);
+  p = fma(p, r, 1.0 / 24.0);
+  p = fma(p, r, 1.0 / 6.0);
+  p = fma(p, r, 0.5);
+  p = fma(p, r, 1.0);
+  p = fma(p, r, 1.0);
+  return __hiloint2double(__double2hiint(p) + (__double2loint(shifted) << 20), __double2loint(p));
+}
+
+// The sum of the row's exp(x - top) within 2^-32 of itself (if an expert is on), in all lanes.
+template <int V>
+__device__ __forceinline__ double softmax_sum(const float* x, float top) {
+  double sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {   // (e^-60 is next to nothing beside the largest's 1)
+    const double e = exp_to_33_bits(static_cast<double>(x[i]) - static_cast<double>(top));
+    sum += x[i] - top > -60.f ? e : 0.0;
+  }
+  return warp_sum_d(sum);
 }
 
 // Two sides of a decision are told apart by the 32-bit scores if they differ by more than this
@@ -412,6 +447,14 @@ __device__ __forceinline__ uint32_t choose_fast(const SelectArgs& a, float* sel,
   return taken;
 }
 
+// The chosen experts' weights are computed by the lanes that store them, one expert each.  A sigmoid is the
+// score as defined.  A softmax's exponentials are taken in double and rounded once; renormalised, the row's
+// sum stands beside the chosen ones' only in the 1e-20, which counts for less than 2^-28 where the best of
+// them is within e^-20 of the row's first: a share of e^-20 / 512 of the sum at least.  (Weights of the 32-bit
+// scores were off by |x - m| units, on average 5.8e-8.)  16384 x 256 softmax 19.0 us renormalised; 22.6 not,
+// for which every exponential is taken in double for the row's sum.
+constexpr float kNoneBeside = 20.f;
+
 // Registers: 64 a thread for up to 256 experts (more CTAs on an SM with less gain nothing: 16384 x 256
 // 21.3 us with five, 22.0 with six), 80 for 512 (41.4 us against 47.7 with as many as it would take, two CTAs).
 template <int V, bool SOFTMAX>
@@ -446,7 +489,8 @@ __global__ void __launch_bounds__(kSelWarps * 32, V == 16 ? 3 : 4) select_kernel
     load_logits<V>(a.logits, a.type, t * a.ld, first, a.E, a.vec, x);
     if (t < a.T - step && first < a.E)   // the next token's, toward L2
       prefetch_l2(static_cast<const uint8_t*>(a.logits) + ((t + step) * a.ld + first) * (a.type == MOE_B200_FP32 ? 4 : 2));
-    const float size = scores<V, SOFTMAX, false>(x, lowest, s);
+    float top = 0.f;
+    const float size = scores<V, SOFTMAX, false>(x, lowest, s, &top);
     float nan = 0.f;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -458,14 +502,14 @@ __global__ void __launch_bounds__(kSelWarps * 32, V == 16 ? 3 : 4) select_kernel
     bool sure = bad || !wild;
     if (!bad && sure) taken = choose_fast<V>(a, sel, s_row, lane, size, size + cancel, &sure);
     if (!sure) {
-      scores<V, SOFTMAX, true>(x, lowest, s);
+      scores<V, SOFTMAX, true>(x, lowest, s, &top);
 #pragma unroll
       for (int i = 0; i < V; ++i) sel[i] = x[i] <= lowest ? -INFINITY : s[i] + bias[i];
       taken = choose_exact<V>(a, sel, s_row, lane);
     }
     // the chosen, by ascending id, to one lane each: those compute and store the weights
 #pragma unroll
-    for (int i = 0; i < V; ++i) s_row[first + i] = SOFTMAX ? s[i] : x[i];
+    for (int i = 0; i < V; ++i) s_row[first + i] = x[i];
     const int mine = __popc(taken);
     int pos = mine;
 #pragma unroll
@@ -478,14 +522,29 @@ __global__ void __launch_bounds__(kSelWarps * 32, V == 16 ? 3 : 4) select_kernel
     __syncwarp();
     const bool have = lane < total;
     const int id = have ? s_id[warp][lane] : -1;
-    float w = have ? s_row[id] : 0.f;
+    const float logit = have ? s_row[id] : -INFINITY;
     __syncwarp();
-    if constexpr (!SOFTMAX) w = have ? __frcp_rn(1.0f + exp_to_f32(-static_cast<double>(w))) : 0.f;   // as defined
-    const float denom = warp_sum(w) + 1e-20f;
+    float w = 0.f;
+    if constexpr (!SOFTMAX) {
+      w = have ? __frcp_rn(1.0f + exp_to_f32(-static_cast<double>(logit))) : 0.f;
+      const float denom = warp_sum(w) + 1e-20f;
+      w = a.renorm ? w / denom : w;
+    } else if (total > 0) {
+      const float best = redux_max(logit);
+      if (a.renorm && top - best <= kNoneBeside) {
+        w = logit - best > -110.f ? static_cast<float>(exp_to_33_bits(static_cast<double>(logit) - static_cast<double>(best))) : 0.f;
+        w /= warp_sum(w);
+      } else {
+        const double e = logit - top > -690.f ? exp_to_33_bits(static_cast<double>(logit) - static_cast<double>(top)) : 0.0;
+        double sum = softmax_sum<V>(x, top);
+        if (a.renorm) sum = warp_sum_d(e) + 1e-20 * sum;
+        w = static_cast<float>(e / sum);
+      }
+    }
     if (lane < a.K) {
       const int64_t o = static_cast<int64_t>(t) * a.K + lane;
       a.idx[o] = id;
-      a.w[o] = bad ? __uint_as_float(0x7fc00000u) : (a.renorm ? w / denom : w) * a.scale;
+      a.w[o] = bad ? __uint_as_float(0x7fc00000u) : w * a.scale;
     }
     if (a.counts && have) atomicAdd(s_cnt + id, 1);
   }

@@ -168,3 +168,24 @@ def test_sigmoid_gradient_next_to_0_and_1(renorm):
     err = (got[:, :K].double() - d * slope).abs()
     assert (err <= 32 * R.U32 * mag * slope + 2.0 ** -148).all()
     assert (got[:, K:] == 0).all() and (got[5:30, 0] != 0).all()
+
+
+@pytest.mark.parametrize("E,K", [(60, 4), (256, 8), (512, 10), (33, 1)])
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("renorm", [False, True])
+@pytest.mark.parametrize("spread", [1.0, 9.0])
+def test_weights_are_rounded_scores(E, K, score, renorm, spread):
+    """Weights within the roundings of their definition, also of experts that a bias chose far below the
+    largest logit: score 3 units (exponential, sum, quotient; a softmax's quotient alone 1), their sum one more
+    each of five times and 1e-20, quotient, scale."""
+    T = 20000
+    x = randn(E, T, E, std=spread).clamp(-8 * spread, 8 * spread).to(BF).float()
+    if spread > 1:
+        x[:, ::5] -= 20.0
+    bias = None if spread == 1 else torch.zeros(E, device="cuda").index_fill(0, torch.arange(0, E, 5, device="cuda"), 2.0)
+    o = M.select_experts(x, K, score=score, bias=bias, renormalize=renorm, scale=2.5)
+    assert torch.equal(o.idx, choice(x, K, score, bias, 1, 1))
+    s = (torch.sigmoid(x.double()) if score == "sigmoid" else torch.softmax(x.double(), dim=1)).gather(1, o.idx.long())
+    w = 2.5 * (s / (s.sum(1, keepdim=True) + 1e-20) if renorm else s)
+    units = (3 if score == "sigmoid" else 1) * (2 if renorm else 1) + (7 if renorm else 0) + 1
+    assert ((o.w.double() - w).abs() <= units * R.U32 * w + 2.0 ** -148).all()

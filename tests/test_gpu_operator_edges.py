@@ -189,3 +189,31 @@ def test_weights_are_rounded_scores(E, K, score, renorm, spread):
     w = 2.5 * (s / (s.sum(1, keepdim=True) + 1e-20) if renorm else s)
     units = (3 if score == "sigmoid" else 1) * (2 if renorm else 1) + (7 if renorm else 0) + 1
     assert ((o.w.double() - w).abs() <= units * R.U32 * w + 2.0 ** -148).all()
+
+
+@pytest.mark.parametrize("T,H", [(700, 7168), (3, 7168), (900, 512), (301, 1001), (40, 300), (5, 5001), (9, 12000)])
+@pytest.mark.parametrize("r_dtype", [BF, F32])
+def test_e4m3_codes_are_those_of_the_quotients(T, H, r_dtype):
+    """Scales and codes equal the 32-bit quotients of the same norm in fp32, to the last bit."""
+    y, r, w = randn(1, T, H, dtype=BF), randn(2, T, H, std=1.5, dtype=r_dtype), (1 + randn(3, H, std=0.2)).to(BF)
+    kw = dict(pre_weight=w, post_weight=w)
+    x = M.block_norm(y, r, x_dtype=F32, **kw).x.cpu()
+    o = M.block_norm(y, r, x_dtype=E4M3, **kw)
+    nb = -(-H // 128)
+    blocks = torch.nn.functional.pad(x, (0, nb * 128 - H)).view(T, nb, 128)
+    scale = blocks.abs().amax(dim=2).clamp(min=1e-12) / torch.tensor(448.0)
+    assert torch.equal(o.x_scale.cpu(), scale.t())
+    codes = (blocks / scale[:, :, None]).view(T, nb * 128)[:, :H].to(E4M3)
+    assert torch.equal(o.x.cpu().view(torch.uint8), codes.view(torch.uint8))
+
+
+def test_e4m3_blocks_with_infinities():
+    """A block whose norm has an infinity (an infinite weight) has its finite elements 0 and the infinity NaN."""
+    r, w = randn(2, 5, 600), torch.ones(600, device="cuda")
+    w[300] = float("inf")
+    for cols in (600, 599):
+        o = M.block_norm(None, r[:, :cols], pre_weight=w[:cols], x_dtype=E4M3)
+        v = o.x.float()
+        assert torch.isinf(o.x_scale[2]).all() and torch.isfinite(o.x_scale[[0, 1, 3, 4]]).all()
+        assert torch.isnan(v[:, 300]).all() and (v[:, 256:300] == 0).all() and (v[:, 301:384] == 0).all()
+        assert torch.isfinite(v[:, :256]).all() and torch.isfinite(v[:, 384:]).all()

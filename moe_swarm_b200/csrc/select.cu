@@ -575,8 +575,8 @@ __global__ void __launch_bounds__(kSelMaxE) select_zero_kernel(int* counts, int 
 //   renormalised, S = sum of the chosen s + 1e-20:  ds_k = scale * (dw_k - sum_j dw_j s_j / S) / S
 //   softmax: dx_e = s_e (ds_e - sum_j ds_j s_j);  sigmoid: dx_e = ds_e s_e (1 - s_e)
 // The scores go to shared memory, where a lane per chosen expert finds its own; those lanes work out
-// the sums and put their own results among what every lane stores.  16384 x 256 softmax 10.3 us (3.4
-// TB/s: about half by memory, half by the exponentials and sums), sigmoid 9.6, 512 experts 33.
+// the sums and put their own results among what every lane stores.  16384 x 256 softmax 10.4 us (3.3
+// TB/s: about half by memory, half by the exponentials and sums), sigmoid 9.6, 512 experts 33.5 and 32.3.
 template <int V, bool SOFTMAX>
 __global__ void __launch_bounds__(kSelWarps * 32) select_bwd_kernel(SelectBwdArgs a) {
   __shared__ __align__(16) float s_row[kSelWarps][32 * V];
@@ -613,7 +613,7 @@ __global__ void __launch_bounds__(kSelWarps * 32) select_bwd_kernel(SelectBwdArg
       float sum = 0.f;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        s[i] = x[i] <= lowest ? 0.f : __expf(x[i] - m);
+        s[i] = x[i] <= lowest ? 0.f : expf(x[i] - m);
         sum += s[i];
       }
       const float inv = 1.f / max_nan(warp_sum(sum), 1e-30f);
@@ -682,7 +682,7 @@ void dispatch_select(int E, F&& f) {
 }
 
 // Eight CTAs of eight warps for every SM, which are all its warps; registers leave the forward four at a
-// time.  With four the backward of 16384 x 256 takes 15.7 us instead of 10.3, the forward 21.1 instead of
+// time.  With four the backward of 16384 x 256 takes 15.7 us instead of 10.4, the forward 21.1 instead of
 // 20.7.
 int select_grid(int T, int sms) {
   const int need = (T + kSelWarps - 1) / kSelWarps;

@@ -217,3 +217,29 @@ def test_e4m3_blocks_with_infinities():
         assert torch.isinf(o.x_scale[2]).all() and torch.isfinite(o.x_scale[[0, 1, 3, 4]]).all()
         assert torch.isnan(v[:, 300]).all() and (v[:, 256:300] == 0).all() and (v[:, 301:384] == 0).all()
         assert torch.isfinite(v[:, :256]).all() and torch.isfinite(v[:, 384:]).all()
+
+
+@pytest.mark.parametrize("renorm", [False, True])
+def test_softmax_gradient_far_below_the_first(renorm):
+    """Gradients of logits up to 85 below the row's largest keep the bits of their scores.  (Differences of
+    16-bit values are exact.)  Units: score 12 (exponential 2, sum 8, quotient, product), their products' sum 7 more,
+    slope 14 more; renormalised, the sum of the chosen, two quotients and the sum once more."""
+    T, E, K = 500, 64, 5
+    x = (randn(1, T, E) * 20).clamp(-40, 40).to(BF).float()
+    x[:, 0] = 45.0
+    idx = torch.tensor([0, 7, 20, 33, 60], dtype=torch.int32, device="cuda").expand(T, K).contiguous()
+    if renorm:
+        idx = (idx + 1) % E
+        idx = idx.sort(dim=1).values.contiguous()
+    dw = randn(2, T, K)
+    got = M.select_experts_backward(dw, x, idx, score="softmax", renormalize=renorm, scale=2.5).double()
+    x64 = x.double().requires_grad_()
+    (R.select_weights(x64, idx, "softmax", renorm, 2.5) * dw.double()).sum().backward()
+    p = torch.softmax(x.double(), dim=1)
+    s, d = p.gather(1, idx.long()), 2.5 * dw.double().abs()
+    if renorm:
+        S = s.sum(1, keepdim=True) + 1e-20
+        d = (d + (d * s).sum(1, keepdim=True) / S) / S
+    own = torch.zeros_like(p).scatter_(1, idx.long(), d)
+    mag = p * (own + (d * s).sum(1, keepdim=True))
+    assert ((got - x64.grad).abs() <= (110 if renorm else 33) * R.U32 * mag + 2.0 ** -140).all()

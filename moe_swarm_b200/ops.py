@@ -6,7 +6,9 @@ stream without a host synchronisation, and compute in the hand-written CUDA of
 ``libmoe_b200.so``; there is no CPU or PyTorch path.  Tensors are ``[rows, cols]`` with adjacent
 elements in a row; rows may be further apart than their length (slices of wider tensors).
 The backward functions are explicit: they take what the forward took and the gradients of its
-results.
+results.  Nothing here records a graph, so a tensor that requires a gradient is refused while gradients are
+enabled (call under ``torch.no_grad()``, or inside a ``torch.autograd.Function``); the backward functions
+refuse incoming gradients that do.
 """
 
 from __future__ import annotations
@@ -77,6 +79,14 @@ def _like(t, dtype=None):
     """A new tensor of t's shape without gaps.  (empty_like would order the strides of rows that overlap,
     such as a sliding window's, as it finds them: by columns.)"""
     return torch.empty_like(t, dtype=dtype) if t.is_contiguous() else t.new_empty(t.shape, dtype=dtype)
+
+
+def _no_graph(what: str, *tensors):
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise MoEArgumentError(f"{what} records no graph, and a tensor of the call requires a gradient: call it "
+                                       "under torch.no_grad() and its backward function explicitly")
 
 
 def _result(t, name: str, shape, dtypes, dev):
@@ -189,6 +199,7 @@ def block_norm(y: torch.Tensor | None, residual: torch.Tensor | None, *, post_we
     ``hidden_states_scale`` of :func:`moe_swarm_b200.run`.  ``residual_out`` (may be ``residual``)
     and ``out`` receive r' and x instead of new tensors.
     """
+    _no_graph("block_norm", y, residual, post_weight, gate, pre_weight, residual_out, out)
     first = residual if y is None else y
     _check(first is not None, "y or residual is required")
     shape, dev = first.shape, first.get_device()
@@ -241,6 +252,7 @@ def block_norm_backward(dx: torch.Tensor | None, dresidual: torch.Tensor | None,
     Weight gradients are fp32.  The gate's gradient has the gate's shape, summed over what it is
     broadcast over: fp32 where it is summed, the gate's type for a [rows, cols] gate.
     """
+    _no_graph("block_norm_backward", dx, dresidual)
     r_ld = _rows(residual, "residual")
     shape, dev, r_dtype = residual.shape, residual.get_device(), residual.dtype
     rows, cols = shape
@@ -295,6 +307,7 @@ def select_experts(logits: torch.Tensor, top_k: int, *, score: str = "sigmoid", 
     weight 0.  A row with a NaN score has ids -1 and NaN weights.  ``counts`` also returns how many
     tokens chose each expert.  idx and w are what :func:`moe_swarm_b200.run_routed` takes.
     """
+    _no_graph("select_experts", logits, bias)
     ld = _rows(logits, "logits")
     T, E = logits.shape
     dev = logits.get_device()
@@ -317,6 +330,7 @@ def select_experts_backward(dw: torch.Tensor, logits: torch.Tensor, idx: torch.T
                             renormalize: bool = True, scale: float = 1.0) -> torch.Tensor:
     """The gradient of :func:`select_experts`' weights with respect to the logits, from ``dw``
     (float32 [T, top_k]) and the ids it chose.  The choice itself has no gradient."""
+    _no_graph("select_experts_backward", dw)
     ld = _rows(logits, "logits")
     T, E = logits.shape
     dev = logits.get_device()
@@ -336,6 +350,7 @@ def quantize_int8(x: torch.Tensor, *, swiglu: bool = False):
     scale = max(amax / 127, 2**-126).  With ``swiglu``, of silu(x[:, cols:]) * x[:, :cols] (the
     expert layer's order of the two halves).  For weights [out, in] the rows are the channels.
     Without ``swiglu`` the codes are those of 64-bit arithmetic with amax * (1 / 127) for a scale."""
+    _no_graph("quantize_int8", x)
     ld = _rows(x, "x")
     dev = x.get_device()
     rows, cols = x.shape
@@ -360,6 +375,7 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     multiple of 16 and rows of int8 tensors start on 16-byte boundaries.  ``out_dtype``: bf16 by
     default (x's type if that is fp16 or fp32).
     """
+    _no_graph("int8_linear", x, weight_scale, x_scale, bias, out)
     x_ld = _rows(x, "x", None, _LINEAR_IN)
     dev = x.get_device()
     w_ld = _rows(weight, "weight", None, _INT8, dev)

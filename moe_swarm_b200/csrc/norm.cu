@@ -336,11 +336,16 @@ MOE_B200_API int moe_b200_block_norm(const moe_b200_norm_args* a, void* stream) 
   const bool packed = vec && a->cols <= 256 && !(a->pre_weight && a->x_type == MOE_B200_E4M3);
   // The ring: aligned rows of two warps or more, at least four per SM, and two or more of them in
   // a CTA's share of shared memory.  7168 columns, bf16 in, e4m3 out, ring against direct: 592 rows
-  // 5.7 us against 6.4, 4096 rows 35.3 (5.8 TB/s) against 51.9; at 148 and 296 rows the ring is 0.1
-  // to 0.2 us behind.  Not for a 32-bit residual with nothing but the sum and its norm to compute, whose
-  // wide loads keep the memory busy without it: 4096 x 7168 63.9 against 56.4 (6.2 TB/s), 8192 x
-  // 4096 72.6 against 61.0; with a gate per token 58.8 against 63.6, with post_weight 66 against 78.
-  // The norm alone of 4096 x 7168 in 16 bits: 24.8 us against 33.7.
+  // 6.0 us against 6.4, 4096 rows 36.4 (5.7 TB/s) against 51.9; at 148 and 296 rows the ring is 0.1
+  // to 0.2 us behind.  The norm alone of 4096 x 7168 in 16 bits: 24.8 us against 33.7.
+  // A 32-bit residual with nothing but the sum and its norm to compute has wide loads that keep the memory
+  // busy without a ring.  In us, ring against direct:
+  //   sum without a norm: direct (4096 x 7168 49.9 against 43.6; 1184 rows 13.2 against 13.4)
+  //   norm without a sum: the ring from 13 warps on (4096 x 7168 30.0 against 33.4, 4096 x 2048 10.4 against 9.2)
+  //   both, up to 8 warps: the ring while no CTA has two rows (1184 x 2048 4.9 against 5.3, 2368 x 2048 10.3
+  //     against 10.0, 8192 x 2048 35.4 against 31.8)
+  //   both, longer rows: the ring below 2^24 elements (1184 x 7168 16.5 against 18.3, 4096 x 7168 63.2 against
+  //     55.7), and with 13 warps beyond that for an x of another width than 16 bits (to e4m3 54.6 against 57.1)
   RingPlan g{};
   ring_add(&g, a->y, n.y_ld, a->cols, a->y_type);
   ring_add(&g, a->residual, n.r_ld, a->cols, a->residual_type);
@@ -348,8 +353,16 @@ MOE_B200_API int moe_b200_block_norm(const moe_b200_norm_args* a, void* stream) 
   const int ctas = n.warps >= 2 && n.warps <= 16 ? 32 / n.warps : 0;   // 1024 threads of an SM
   g.stages = ctas ? kRingSmem / ctas / g.stage_bytes : 0;
   if (g.stages > kRingMaxStages) g.stages = kRingMaxStages;
-  const bool sum_alone = a->residual_type == MOE_B200_FP32 && !a->post_weight && !a->gate;
-  if (vec && !packed && a->rows >= 4 * sms && g.stages >= 2 && !sum_alone) {
+  bool direct = false;
+  if (a->residual_type == MOE_B200_FP32 && !a->post_weight && !a->gate) {
+    const bool large = static_cast<int64_t>(a->rows) * a->cols >= 1 << 24, wide = n.warps > 12;
+    const bool x16 = a->x_type == MOE_B200_BF16 || a->x_type == MOE_B200_FP16;
+    direct = !a->pre_weight    ? true
+             : !a->y           ? !wide
+             : n.warps <= 8    ? a->rows > ctas * sms
+                               : large && (x16 || !wide);
+  }
+  if (vec && !packed && a->rows >= 4 * sms && g.stages >= 2 && !direct) {
     const dim3 grid(a->rows < ctas * sms ? a->rows : ctas * sms), block(n.warps * 32);
     const size_t smem = static_cast<size_t>(g.stages) * g.stage_bytes;
     dispatch_types(a->y_type, a->residual_type, [&](auto yt, auto rt) {

@@ -243,3 +243,21 @@ def test_softmax_gradient_far_below_the_first(renorm):
     own = torch.zeros_like(p).scatter_(1, idx.long(), d)
     mag = p * (own + (d * s).sum(1, keepdim=True))
     assert ((got - x64.grad).abs() <= (110 if renorm else 33) * R.U32 * mag + 2.0 ** -140).all()
+
+
+@pytest.mark.parametrize("T,H", [(600, 1024), (3000, 1024), (700, 7168), (2400, 7168), (600, 8192), (2100, 8192)])
+@pytest.mark.parametrize("x_dtype", [None, BF, F32, E4M3])
+@pytest.mark.parametrize("block", [False, True])
+def test_a_32_bit_stream_on_both_sides_of_the_ring(T, H, x_dtype, block):
+    y, r, w = randn(1, T, H, dtype=BF), randn(2, T, H), (1 + randn(3, H, std=0.2)).to(BF)
+    if not block and x_dtype is None:
+        return
+    o = M.block_norm(y if block else None, r, pre_weight=None if x_dtype is None else w, x_dtype=x_dtype)
+    ref_r, ref_x, rm, xm = R.block_norm(y if block else None, r, pre_weight=w)
+    R.close(o.residual, ref_r, rm)
+    if x_dtype == E4M3:
+        s = o.x_scale.t().double().repeat_interleave(128, dim=1)[:, :H].cpu()
+        tol = (ref_x.abs() * 2.0 ** -4).maximum(s * 2.0 ** -10) * 1.001 + 2 * R.STEPS * R.U32 * (xm + ref_x.abs())
+        assert ((o.x.double().cpu() * s - ref_x).abs() <= tol).all()
+    elif x_dtype is not None:
+        R.close(o.x, ref_x, xm)

@@ -304,8 +304,8 @@ struct GemvArgs {
 template <class XT>
 __device__ __forceinline__ void gemv_load8(const GemvArgs& a, const XT* row, int e, float* v) {
   auto load = [&](const XT* p, float* out) {
-    if (a.vec) load8<XT, true>(p, 8, out);
-    else load8<XT, false>(p, 8, out);
+    if (a.vec) load8<XT, true>(p, out);
+    else load8<XT, false>(p, out);
   };
   load(row + e, v);
   if (!a.swiglu) return;
@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(1024, 1) int8_gemv_kernel(GemvArgs a) {
     if (lane < a.T) {
       const float b = a.bias ? load1_dyn(a.bias, a.bias_type, n) : 0.f;
       const float v = fmaf(static_cast<float>(mine), s_scale[lane] * a.sw[n], b);
-      store8_dyn<false>(a.y, a.y_type, lane * a.y_ld + n, 1, &v);
+      store1_dyn(a.y, a.y_type, lane * a.y_ld + n, v);
     }
   }
 }

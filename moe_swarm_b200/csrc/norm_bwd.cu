@@ -26,7 +26,7 @@ struct NormBwdArgs {
   float* partial;                   // [slots][parts][cols]: sums of dx r^ and of G y^
   int64_t dx_ld, dr_ld, r_ld, y_ld, g_ld, dres_ld, dy_ld, dg_ld;
   int rows, cols, warps, parts;
-  int post_type, pre_type, gate_type, gate_cols;
+  int post_type, pre_type, gate_type;
   int gate_grad, pre_slot, post_slot;
   float scale, eps, off;
 };
@@ -535,7 +535,6 @@ MOE_B200_API int moe_b200_block_norm_backward(const moe_b200_norm_backward_args*
   n.post_type = a->post_weight_type;
   n.pre_type = a->pre_weight_type;
   n.gate_type = a->gate_type;
-  n.gate_cols = a->gate_per_column;
   n.scale = a->scale;
   n.eps = a->eps;
   n.off = a->weight_offset;

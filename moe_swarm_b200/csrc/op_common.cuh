@@ -101,62 +101,31 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, fp16) {
 // Plain loads, not the read-only path: a tensor may be written by the kernel that this one waits
 // for (pdl_wait), and a read-only load may be moved above that wait.
 //
-// Eight consecutive elements from p.  VEC: p is 16-byte aligned and all eight exist; otherwise
-// the first n exist (n <= 0: none) and the rest read as 0.
+// Eight consecutive elements from p.  VEC: p is 16-byte aligned.
 template <class T, bool VEC>
-__device__ __forceinline__ void load8(const T* p, int n, float* v) {
-  if constexpr (VEC) {
-    if (n <= 0) {
+__device__ __forceinline__ void load8(const T* p, float* v) {
+  if constexpr (!VEC) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = 0.f;
-    } else if constexpr (sizeof(T) == 4) {
-      const float4 a = reinterpret_cast<const float4*>(p)[0];
-      const float4 b = reinterpret_cast<const float4*>(p)[1];
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-      const uint4 u = *reinterpret_cast<const uint4*>(p);
-      unpack2(u.x, v, T{});
-      unpack2(u.y, v + 2, T{});
-      unpack2(u.z, v + 4, T{});
-      unpack2(u.w, v + 6, T{});
-    }
+    for (int j = 0; j < 8; ++j) v[j] = to_f(p[j]);
+  } else if constexpr (sizeof(T) == 4) {
+    const float4 a = reinterpret_cast<const float4*>(p)[0];
+    const float4 b = reinterpret_cast<const float4*>(p)[1];
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
   } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = j < n ? to_f(p[j]) : 0.f;
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    unpack2(u.x, v, T{});
+    unpack2(u.y, v + 2, T{});
+    unpack2(u.z, v + 4, T{});
+    unpack2(u.w, v + 6, T{});
   }
 }
 
-template <class T, bool VEC>
-__device__ __forceinline__ void store8(T* p, int n, const float* v) {
-  if constexpr (VEC) {
-    if (n <= 0) return;
-    if constexpr (sizeof(T) == 4) {
-      reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-      reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-      *reinterpret_cast<uint4*>(p) = make_uint4(pack2(v[0], v[1], T{}), pack2(v[2], v[3], T{}),
-                                                pack2(v[4], v[5], T{}), pack2(v[6], v[7], T{}));
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j < n) p[j] = from_f<T>(v[j]);
-  }
-}
-
-// The same with the element type known at run time (uniform over the grid): element `off` of p.
-template <bool VEC>
-__device__ __forceinline__ void load8_dyn(const void* p, int type, int64_t off, int n, float* v) {
-  if (type == MOE_B200_BF16) load8<bf16, VEC>(static_cast<const bf16*>(p) + off, n, v);
-  else if (type == MOE_B200_FP16) load8<fp16, VEC>(static_cast<const fp16*>(p) + off, n, v);
-  else load8<float, VEC>(static_cast<const float*>(p) + off, n, v);
-}
-template <bool VEC>
-__device__ __forceinline__ void store8_dyn(void* p, int type, int64_t off, int n, const float* v) {
-  if (type == MOE_B200_BF16) store8<bf16, VEC>(static_cast<bf16*>(p) + off, n, v);
-  else if (type == MOE_B200_FP16) store8<fp16, VEC>(static_cast<fp16*>(p) + off, n, v);
-  else store8<float, VEC>(static_cast<float*>(p) + off, n, v);
+// Element `off` of p, the element type known at run time (uniform over the grid).
+__device__ __forceinline__ void store1_dyn(void* p, int type, int64_t off, float v) {
+  if (type == MOE_B200_BF16) static_cast<bf16*>(p)[off] = from_f<bf16>(v);
+  else if (type == MOE_B200_FP16) static_cast<fp16*>(p)[off] = from_f<fp16>(v);
+  else static_cast<float*>(p)[off] = v;
 }
 __device__ __forceinline__ float load1_dyn(const void* p, int type, int64_t off) {
   if (type == MOE_B200_BF16) return to_f(static_cast<const bf16*>(p)[off]);

@@ -151,7 +151,7 @@ __device__ __forceinline__ void store_logits(void* p, int type, int64_t off, int
   } else {
 #pragma unroll
     for (int i = 0; i < V; ++i)
-      if (first + i < E) store8_dyn<false>(p, type, off + first + i, 1, x + i);
+      if (first + i < E) store1_dyn(p, type, off + first + i, x[i]);
   }
 }
 

@@ -7,7 +7,8 @@
     residual, x = block_norm(routed + shared, residual)          gate, sum and the next block's norm
 
 ``python examples/moe_block.py [--tokens T] [--experts E]`` builds a block with random weights, runs
-it, trains its router and norms for a step on a frozen body, and prints what it took.
+it, computes the gradients of its router and of the norms at its end for random gradients of its results, moves
+the selection's bias once, and prints what it took.
 """
 
 from __future__ import annotations

@@ -621,7 +621,7 @@ __global__ void __launch_bounds__(kSelWarps * 32) select_bwd_kernel(SelectBwdArg
       for (int i = 0; i < V; ++i) s[i] *= inv;
     } else {
 #pragma unroll
-      for (int i = 0; i < V; ++i) s[i] = x[i] <= lowest ? 0.f : x[i];
+      for (int i = 0; i < V; ++i) s[i] = x[i];
     }
     float all = 0.f;
 #pragma unroll
@@ -632,7 +632,7 @@ __global__ void __launch_bounds__(kSelWarps * 32) select_bwd_kernel(SelectBwdArg
     const bool bad = __any_sync(0xffffffffu, all != all);   // a NaN logit, or an infinite one of a softmax
     __syncwarp();
     float sk = have ? row[id] : 0.f;
-    // sigmoid: from the logit that was put there (one that is switched off was not chosen).  With h =
+    // sigmoid: from the logit that was put there (one that is switched off gives 0).  With h =
     // exp(-|x| / 2) and r = 1 / (1 + h h), s (1 - s) = (h r)^2: nothing cancels where s is near 1, and nothing
     // overflows or loses its bits where it is next to 0.
     float root = 0.f;

@@ -261,3 +261,20 @@ def test_a_32_bit_stream_on_both_sides_of_the_ring(T, H, x_dtype, block):
         assert ((o.x.double().cpu() * s - ref_x).abs() <= tol).all()
     elif x_dtype is not None:
         R.close(o.x, ref_x, xm)
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("renorm", [False, True])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_gradient_of_an_expert_that_is_off(score, renorm, dtype):
+    """Ids of experts that are switched off by now have score 0: no gradient, and no part in the others'."""
+    T, E = 6, 40
+    x = randn(3, T, E, dtype=dtype)
+    x[:3, 5], x[3:, 5] = float("-inf"), torch.finfo(dtype).min
+    idx = torch.tensor([2, 5, 9], dtype=torch.int32, device="cuda").expand(T, 3).contiguous()
+    dw = randn(4, T, 3)
+    got = M.select_experts_backward(dw, x, idx, score=score, renormalize=renorm)
+    without = idx.clone()
+    without[:, 1] = -1
+    assert (got[:, 5] == 0).all()
+    assert torch.equal(got, M.select_experts_backward(dw, x, without, score=score, renormalize=renorm))

@@ -150,8 +150,9 @@ def _workspace(n: int, dev: int) -> torch.Tensor:
     """Scratch of n bytes for a call on the device's current stream.  Small ones are kept per
     (device, stream, host thread): such calls are enqueued, and run, one after another, while two
     threads could enqueue the kernels of their calls in turn.  Large ones, and those of a graph
-    capture (whose replays would share them with later calls), are allocated per call."""
-    if n > _SCRATCH_KEPT or torch._C._cuda_isCurrentStreamCapturing():
+    capture (whose replays would share them with later calls), are allocated per call; so are those of
+    another device than the current one, the one whose stream can be asked whether it captures."""
+    if n > _SCRATCH_KEPT or torch._C._cuda_getDevice() != dev or torch._C._cuda_isCurrentStreamCapturing():
         return torch.empty(n, dtype=torch.uint8, device=dev)
     key = (dev, torch._C._cuda_getCurrentRawStream(dev), threading.get_ident())
     ws = _scratch.get(key)

@@ -23,8 +23,8 @@
 // are computed as defined and the choice is made again from those.
 //
 // Bound by the warps' instructions, about 850 per token of 256 experts in 8 groups (scores, a sort of
-// eight keys per lane, rounds of maxima), not by HBM: 16384 tokens 20.7 us with counts (18.1 without
-// groups, 19.0 softmax) where the logits alone would take 2.7; 512 experts 41 us, 64 experts 11.  Few
+// eight keys per lane, rounds of maxima), not by HBM: 16384 tokens 20.7 us with counts (18.4 without
+// groups, 18.5 softmax) where the logits alone would take 2.7; 512 experts 41 us, 64 experts 11.  Few
 // tokens are bound by the one token's chain of operations: 16 tokens 4.6 us.
 #include <type_traits>
 
@@ -239,6 +239,27 @@ __device__ __forceinline__ double softmax_sum(const float* x, float top) {
   return warp_sum_d(sum);
 }
 
+// The scores from those exponentials, each rounded once; returns that of the largest logit (*top).
+template <int V>
+__device__ __forceinline__ float softmax_scores(const float* x, float lowest, float* s, float* top) {
+  float m = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < V; ++i) m = fmaxf(m, x[i]);
+  *top = m = redux_max(m);
+  double e[V], sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const float d = x[i] - m;
+    e[i] = x[i] <= lowest ? 0.0 : d > -690.f ? exp_to_33_bits(static_cast<double>(x[i]) - static_cast<double>(m)) : d != d ? d : 0.0;
+    sum += e[i];
+  }
+  sum = warp_sum_d(sum);
+  const double inv = sum > 0.0 ? 1.0 / sum : sum;   // (NaN stays)
+#pragma unroll
+  for (int i = 0; i < V; ++i) s[i] = static_cast<float>(e[i] * inv);
+  return static_cast<float>(inv);
+}
+
 // Two sides of a decision are told apart by the 32-bit scores if they differ by more than this
 // share of the sizes involved, M = max(size, both sides).  In units of 2^-18: an expert's score is off by
 // 5/8 of the row's size and its key by 1 of itself (the lane in the low five bits); for two experts that
@@ -451,8 +472,9 @@ __device__ __forceinline__ uint32_t choose_fast(const SelectArgs& a, float* sel,
 // score as defined.  A softmax's exponentials are taken in double and rounded once; renormalised, the row's
 // sum stands beside the chosen ones' only in the 1e-20, which counts for less than 2^-28 where the best of
 // them is within e^-20 of the row's first: a share of e^-20 / 512 of the sum at least.  (Weights of the 32-bit
-// scores were off by |x - m| units, on average 5.8e-8.)  16384 x 256 softmax 19.0 us renormalised; 22.6 not,
-// for which every exponential is taken in double for the row's sum.
+// scores were off by |x - m| units, on average 5.8e-8.)  16384 x 256 softmax 18.5 us renormalised; 20.8 not,
+// for which every exponential is taken in double for the row's sum, and is then the score as well (22.4
+// when the sum was taken beside 32-bit scores).
 constexpr float kNoneBeside = 20.f;
 
 // Registers: 64 a thread for up to 256 experts (more CTAs on an SM with less gain nothing: 16384 x 256
@@ -490,7 +512,11 @@ __global__ void __launch_bounds__(kSelWarps * 32, V == 16 ? 3 : 4) select_kernel
     if (t < a.T - step && first < a.E)   // the next token's, toward L2
       prefetch_l2(static_cast<const uint8_t*>(a.logits) + ((t + step) * a.ld + first) * (a.type == MOE_B200_FP32 ? 4 : 2));
     float top = 0.f;
-    const float size = scores<V, SOFTMAX, false>(x, lowest, s, &top);
+    // weights that are a softmax's scores themselves are computed with them (512 experts leave no registers for it)
+    const bool ready = SOFTMAX && V <= 8 && !a.renorm;
+    float size;
+    if (ready) size = softmax_scores<V <= 8 ? V : 1>(x, lowest, s, &top);
+    else size = scores<V, SOFTMAX, false>(x, lowest, s, &top);
     float nan = 0.f;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -509,7 +535,7 @@ __global__ void __launch_bounds__(kSelWarps * 32, V == 16 ? 3 : 4) select_kernel
     }
     // the chosen, by ascending id, to one lane each: those compute and store the weights
 #pragma unroll
-    for (int i = 0; i < V; ++i) s_row[first + i] = x[i];
+    for (int i = 0; i < V; ++i) s_row[first + i] = ready ? s[i] : x[i];
     const int mine = __popc(taken);
     int pos = mine;
 #pragma unroll
@@ -529,6 +555,8 @@ __global__ void __launch_bounds__(kSelWarps * 32, V == 16 ? 3 : 4) select_kernel
       w = have ? __frcp_rn(1.0f + exp_to_f32(-static_cast<double>(logit))) : 0.f;
       const float denom = warp_sum(w) + 1e-20f;
       w = a.renorm ? w / denom : w;
+    } else if (ready) {
+      w = have ? logit : 0.f;   // the score
     } else if (total > 0) {
       const float best = redux_max(logit);
       if (a.renorm && top - best <= kNoneBeside) {

@@ -23,8 +23,8 @@
 // are computed as defined and the choice is made again from those.
 //
 // Bound by the warps' instructions, about 850 per token of 256 experts in 8 groups (scores, a sort of
-// eight keys per lane, rounds of maxima), not by HBM: 16384 tokens 20.7 us with counts (18.4 without
-// groups, 18.5 softmax) where the logits alone would take 2.7; 512 experts 41 us, 64 experts 11.  Few
+// eight keys per lane, rounds of maxima), not by HBM: 16384 tokens 20.7 us with counts (17.9 without
+// groups, 18.0 softmax) where the logits alone would take 2.7; 512 experts 41 us, 64 experts 11.  Few
 // tokens are bound by the one token's chain of operations: 16 tokens 4.6 us.
 #include <type_traits>
 
@@ -472,7 +472,7 @@ __device__ __forceinline__ uint32_t choose_fast(const SelectArgs& a, float* sel,
 // score as defined.  A softmax's exponentials are taken in double and rounded once; renormalised, the row's
 // sum stands beside the chosen ones' only in the 1e-20, which counts for less than 2^-28 where the best of
 // them is within e^-20 of the row's first: a share of e^-20 / 512 of the sum at least.  (Weights of the 32-bit
-// scores were off by |x - m| units, on average 5.8e-8.)  16384 x 256 softmax 18.5 us renormalised; 20.8 not,
+// scores were off by |x - m| units, on average 5.8e-8.)  16384 x 256 softmax 18.0 us renormalised; 21.3 not,
 // for which every exponential is taken in double for the row's sum, and is then the score as well (22.4
 // when the sum was taken beside 32-bit scores).
 constexpr float kNoneBeside = 20.f;
@@ -548,20 +548,19 @@ __global__ void __launch_bounds__(kSelWarps * 32, V == 16 ? 3 : 4) select_kernel
     __syncwarp();
     const bool have = lane < total;
     const int id = have ? s_id[warp][lane] : -1;
-    const float logit = have ? s_row[id] : -INFINITY;
+    const float logit = have ? s_row[id] : SOFTMAX ? -INFINITY : 0.f;
     __syncwarp();
-    float w = 0.f;
+    float w = 0.f, denom = 1.f;   // (the division is left to the lanes that have an expert)
     if constexpr (!SOFTMAX) {
       w = have ? __frcp_rn(1.0f + exp_to_f32(-static_cast<double>(logit))) : 0.f;
-      const float denom = warp_sum(w) + 1e-20f;
-      w = a.renorm ? w / denom : w;
+      denom = warp_sum(w) + 1e-20f;
     } else if (ready) {
       w = have ? logit : 0.f;   // the score
     } else if (total > 0) {
       const float best = redux_max(logit);
       if (a.renorm && top - best <= kNoneBeside) {
         w = logit - best > -110.f ? static_cast<float>(exp_to_33_bits(static_cast<double>(logit) - static_cast<double>(best))) : 0.f;
-        w /= warp_sum(w);
+        denom = warp_sum(w);
       } else {
         const double e = logit - top > -690.f ? exp_to_33_bits(static_cast<double>(logit) - static_cast<double>(top)) : 0.0;
         double sum = softmax_sum<V>(x, top);
@@ -572,7 +571,7 @@ __global__ void __launch_bounds__(kSelWarps * 32, V == 16 ? 3 : 4) select_kernel
     if (lane < a.K) {
       const int64_t o = static_cast<int64_t>(t) * a.K + lane;
       a.idx[o] = id;
-      a.w[o] = bad ? __uint_as_float(0x7fc00000u) : w * a.scale;
+      a.w[o] = bad ? __uint_as_float(0x7fc00000u) : (a.renorm ? w / denom : w) * a.scale;
     }
     if (a.counts && have) atomicAdd(s_cnt + id, 1);
   }

@@ -487,7 +487,8 @@ cudaError_t with_y_type(int type, F&& f) {
 cudaError_t int8_wide_launch(const int8_t* q, int64_t q_ld, const int8_t* w, int64_t w_ld, const LinearArgs& a,
                              int sms, cudaStream_t st) {
   // (Tiles of 256 x 128 for twice the SMs at work gain nothing: an MMA of half the width takes nearly
-  // as long.  512 x 4096 x 7168: 21.9 us with 256 x 256, 20.5 with 256 x 128, 14 split over K.)
+  // as long.  512 x 4096 x 7168: 21.9 us with 256 x 256, 20.5 with 256 x 128; 18.9 in the streaming kernel,
+  // which splits K.)
   const int pairs = sms / 2, tiles = ((a.T + 255) / 256) * ((a.N + 255) / 256);
   CUtensorMap mq, mw;
   if (!encode_rows_u8(&mq, q, a.K, a.T, q_ld, kIWBox) || !encode_rows_u8(&mw, w, a.K, a.N, w_ld, kIWBox))

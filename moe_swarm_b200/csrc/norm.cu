@@ -26,9 +26,10 @@ struct NormArgs {
 };
 
 // e4m3 codes are those of the 32-bit quotients v / scale.  v times the scale's rounded reciprocal alone falls
-// on the other side of some rounding boundaries (the outputs' error 2.98e-4 against 2.86e-4), so the
-// product is corrected once by its exact remainder, which gives the rounded quotient (Markstein, Computation
-// of elementary functions on the IBM RISC System/6000 processor, 1990): 4096 x 7168 36.4 us against 35.2 without.  An infinite scale takes no
+// on the other side of some rounding boundaries (of 235 million codes 1920 differ from those of 64-bit
+// arithmetic throughout, of the quotients' 1839), so the product is corrected once by its exact remainder,
+// which gives the rounded quotient (Markstein, Computation of elementary functions on the IBM RISC
+// System/6000 processor, 1990): 4096 x 7168 36.3 us against 35.2 without.  An infinite scale takes no
 // remainder: what is finite becomes 0, an infinity NaN.
 struct BlockScale {
   float inv, minus;   // reciprocal, negative divisor
@@ -119,7 +120,9 @@ __device__ __forceinline__ void store_x(const NormArgs& a, int row, int cols, Ro
 // (kPacked).  Rows beyond the last are the last one again, without a store: what a layout promises of
 // its elements (exists()) holds for rows that exist only.  Bound by latency where rows are few (one row
 // of 7168: 2.6 us), by HBM where many: 592 rows 6.4 us, 16384 x 512 11.6 us (5.8 TB/s), 901 x 5001
-// with both norms 15.5 us (3.5 TB/s: odd rows are read and written two bytes at a time).
+// with both norms and a 32-bit residual 15.4 to 16.9 us (3.2 to 3.5 TB/s: odd rows are read and written two
+// bytes at a time, and their threads spill).  Beyond 8192 columns, where no ring is: 2048 x 16384 60.0 us to
+// 16 bits (4.5 TB/s), 61.6 to e4m3, 74.4 with a 32-bit residual (5.4).
 template <class YT, class RT, int LAY, int MAXT>
 __global__ void __launch_bounds__(MAXT, 1024 / MAXT) norm_fwd_kernel(NormArgs a) {
   __shared__ float buf[2][8 * 32];
@@ -172,7 +175,7 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) norm_fwd_kernel(NormArgs a)
 // to shared memory as bulk copies while a row is computed, so that the row's barriers and latencies
 // leave the memory busy.  Weights and a gate per column come from L1.  A stage is refilled after
 // the row's last barrier, when every thread holds its part.  1024 threads of an SM, whose rows in flight
-// are about 200 KB; 4096 x 7168 from bf16 to e4m3 36.4 us (5.7 TB/s, HBM), to bf16 40.4, with both
+// are about 200 KB; 4096 x 7168 from bf16 to e4m3 36.3 us (5.7 TB/s, HBM), to bf16 40.3, with both
 // norms and a gate per element 54 (5.4 TB/s).
 // POST: 0, 1: without and with post_weight; kNoBlock: there is no y.
 constexpr int kNoBlock = 2;
@@ -336,7 +339,7 @@ MOE_B200_API int moe_b200_block_norm(const moe_b200_norm_args* a, void* stream) 
   const bool packed = vec && a->cols <= 256 && !(a->pre_weight && a->x_type == MOE_B200_E4M3);
   // The ring: aligned rows of two warps or more, at least four per SM, and two or more of them in
   // a CTA's share of shared memory.  7168 columns, bf16 in, e4m3 out, ring against direct: 592 rows
-  // 6.0 us against 6.4, 4096 rows 36.4 (5.7 TB/s) against 51.9; at 148 and 296 rows the ring is 0.1
+  // 6.0 us against 6.4, 4096 rows 36.3 (5.7 TB/s) against 51.9; at 148 and 296 rows the ring is 0.1
   // to 0.2 us behind.  The norm alone of 4096 x 7168 in 16 bits: 24.8 us against 33.7.
   // A 32-bit residual with nothing but the sum and its norm to compute has wide loads that keep the memory
   // busy without a ring.  In us, ring against direct:
@@ -387,8 +390,9 @@ MOE_B200_API int moe_b200_block_norm(const moe_b200_norm_args* a, void* stream) 
   dispatch_types(a->y_type, a->residual_type, [&](auto yt, auto rt) {
     using YT = decltype(yt);
     using RT = decltype(rt);
-    // rows of up to 8192 columns take at most 512 threads, which may then use twice the registers; odd
-    // ones of up to 256 have no loads for elements that they do not hold (30000 x 99: 10.4 us against 33.8)
+    // rows of up to 8192 columns take at most 512 threads, so that two CTAs fit an SM; a thread has 64 registers
+    // either way, which odd rows exceed by some (kTail and kScattered spill 108 and 80 bytes).  Odd rows of up
+    // to 256 columns have no loads for elements that they do not hold (30000 x 99: 10.4 us against 33.8)
     auto sized = [&](auto t) {
       constexpr int MAXT = decltype(t)::value;
       if constexpr (MAXT == 1024) return vec ? norm_fwd_kernel<YT, RT, kVec, MAXT> : norm_fwd_kernel<YT, RT, kTail, MAXT>;

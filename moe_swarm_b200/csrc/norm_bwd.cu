@@ -255,7 +255,8 @@ __global__ void __launch_bounds__(MAXT, 1) norm_bwd_kernel(NormBwdArgs a) {
 // leaves its ring too little room, and they are read in place.  Rows of one warp go eight to a CTA,
 // each warp with a ring of its own and no CTA barrier until the sums are written.  4096 x 7168 with
 // both norms and a gate per column: 66.5 us with its column sums (5.3 TB/s) against 176 straight from
-// memory; 64 rows 9.0 against 10.1, so there is no lower limit of rows.
+// memory; 64 rows 9.0 against 10.1, so there is no lower limit of rows.  With a 32-bit residual 4096 x 7168
+// 111 us (4.8 TB/s), 8192 x 4096 116 (5.2).
 template <class YT, class RT, int LAY, int POST, int GATE>
 __global__ void __launch_bounds__(512, 1) norm_bwd_ring_kernel(NormBwdArgs a, RingPlan g) {
   extern __shared__ __align__(128) uint8_t ring[];

@@ -614,7 +614,8 @@ MOE_B200_API int moe_b200_block_norm_backward(const moe_b200_norm_backward_args*
       const dim3 block(packed ? shape.lanes : n.warps * 32, side);
       const int quads = !thin ? 8 : a->cols <= 32 * 128 ? 2 : 4;   // factors of a thread
       const size_t smem = sizeof(float4) * quads * block.x + (side > 1 ? sizeof(float) * side * a->cols : 0);
-      if (smem > 48 * 1024)
+      // 48 KB are what a launch may have unasked, the 6 KB of the kernel's own buffers among them
+      if (smem + sizeof(float) * 2 * kBwdSide * 3 * 32 > 48 * 1024)
         e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem);
       if (e == cudaSuccess) e = launch_pdl(kernel, dim3(n.parts), block, smem, st, n);
     }

@@ -278,3 +278,18 @@ def test_gradient_of_an_expert_that_is_off(score, renorm, dtype):
     without[:, 1] = -1
     assert (got[:, 5] == 0).all()
     assert torch.equal(got, M.select_experts_backward(dw, x, without, score=score, renormalize=renorm))
+
+
+# factors per column of 42 to 48 KB, beside 6 KB of other shared memory: odd rows, and aligned ones without dx
+@pytest.mark.parametrize("T,H", [(9, 5376), (9, 5377), (160, 5501), (3, 5889), (9, 6001), (9, 6144), (9, 6145), (9, 5120), (9, 5632), (2, 6136)])
+@pytest.mark.parametrize("pad", [0, 1])
+@pytest.mark.parametrize("with_dx", [False, True])
+def test_gradients_at_the_limit_of_shared_memory(T, H, pad, with_dx):
+    y, dr, dx = (randn(i, T, H + pad, dtype=BF)[:, :H] for i in range(3))
+    w = (1 + randn(9, H, std=0.2)).to(BF)
+    kw = dict(post_weight=w, pre_weight=w if with_dx else None)
+    b = M.block_norm_backward(dx if with_dx else None, dr, y, y, **kw)
+    ref = R.block_norm_backward(dx if with_dx else None, dr, y, y, **kw)
+    R.close(b.residual, *ref["residual"])
+    R.close(b.y, *ref["y"], steps=3 * R.STEPS)
+    R.close(b.post_weight, *ref["post_weight"], steps=3 * R.STEPS + T // 148 + 64)
